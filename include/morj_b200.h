@@ -183,6 +183,56 @@ int morj_label_head(const void* x, long long ld_x, const int* seq_row, const int
 /* Reference-layout GeGLU (unfused path): out[i, j] = bf16(gelu_tanh(gu[i, j]) * gu[i, F + j]), gu: [n, 2F]. */
 int morj_geglu(const void* gu, int n, int F, void* out, void* stream);
 
+/* ---- 8-bit K/V cache (no counterpart in the reference, whose pools are BF16) -----------------------------------------
+ *
+ * K and V pools of e4m3 codes, [pool_slots, hk, d] bytes each, with one FP32 scale per block of 64 consecutive slots and
+ * head, [ceil(pool_slots / 64), hk]: a value is code * scale. Scales are powers of two, 2^-100 at least; 0 (or NaN)
+ * marks a block nothing was stored in. A pool starts with zero scales; its codes need no initial value.
+ *
+ * morj_kv8_store_work (host function, no device access): the store's work list for rows 0..n-1 written to pool slots
+ * slots_host[0..n-1], grouped by block: work_host gets 3 ints per touched block (block, first, count), a pad int when
+ * their number is odd, then n (slot, row) pairs; at most 5 n + 1 ints. Returns the number of touched blocks, -1 on a
+ * slot outside [0, pool_slots), a slot given twice, or a too small cap. One list serves every layer of a step.
+ *
+ * morj_kv8_store: writes the rows k[i], v[i] (BF16, [hk, d], rows ld_k / ld_v elements apart) to their slots. For each
+ * touched block and head, with a = the largest magnitude of the rows written there: scale = max(old scale, smallest
+ * power of two s with a <= 448 s); if it grew, the block's other codes are rounded to the new scale (exact unless they
+ * become e4m3 subnormals); the rows are rounded to nearest even. The result does not depend on the order of the rows.
+ * A non-finite element sets the device error word (0x303) and is stored as 0 (NaN) or the largest value (infinity); it
+ * does not count in a. Slots no row names keep their value. `work`: the device copy of the list, 8-byte aligned;
+ * d in {64, 128}; rows and codes 16-byte aligned, ld multiples of 8.
+ *
+ * morj_kv8_gather: out[i] = bf16(code * scale), saturated, of pool row slots[i], all hk heads (rows ld_out elements
+ * apart), from one pool (K or V). A slot outside the pool sets the device error word (0x301) and its row is not written. */
+int morj_kv8_store_work(const int* slots_host, int n, int pool_slots, int* work_host, int cap);
+int morj_kv8_store(const void* k, long long ld_k, const void* v, long long ld_v, int n, int hk, int d, const int* work,
+                   int n_blocks, void* k_codes, float* k_scale, void* v_codes, float* v_scale, int pool_slots,
+                   void* stream);
+int morj_kv8_gather(const void* codes, const float* scale, int pool_slots, const int* slots, int n, int hk, int d,
+                    void* out, long long ld_out, void* stream);
+
+/* morj_tree_attention over an 8-bit cache: the same segments, key lists, masks and head groups, K and V read as
+ * code * scale. q, out: [n_q, hq, d] BF16. A query that sees no key gets 0. Any hq / hk; d in {64, 128}; the last page
+ * of a segment with no pages is ignored. Keys outside every query's view are not read; a listed key's codes must be
+ * finite (as morj_kv8_store leaves them) where some query of the same tile does not see it. A slot outside the pool
+ * sets the device error word (0x301).
+ *
+ * morj_tree_attention_kv8_work (host function, no device access): the call's work list from host copies of its segment
+ * tables. Writes up to `cap` ints to work_host and counts[8]: counts[0..2] = row tiles, joins, partial units,
+ * counts[3] = rows per tile, counts[4] = ints written. With cap = 0 it writes only the counts. Long key lists of few
+ * tiles are cut into parts, whose partial results go through `workspace` (counts[2] * hk * 16 * (d + 2) * 4 bytes, the
+ * caller's, 16-byte aligned; calls that may overlap on the device must not share it) and are joined in a fixed order.
+ * `work`: the device copy of the list (16-byte aligned); `counts`: the host array. */
+int morj_tree_attention_kv8_work(const int* qo_indptr_host, const int* kv_indptr_host,
+                                 const int* kv_last_page_len_host, int n_segments, int n_bidir, int hq, int hk,
+                                 int page_size, int window, int* work_host, int cap, int* counts);
+int morj_tree_attention_kv8(const void* q, int n_q, const void* k_codes, const float* k_scale, const void* v_codes,
+                            const float* v_scale, int pool_slots, void* out, const int* qo_indptr,
+                            const int* kv_indptr, const int* kv_indices, const int* kv_last_page_len, int n_segments,
+                            int n_bidir, int hq, int hk, int d, int page_size, int window, float sm_scale,
+                            const int* work, const int* counts, void* workspace, unsigned long long workspace_bytes,
+                            void* stream);
+
 /* ---- tensor parallelism over peer memory (no counterpart in the reference, which runs one GPU per model; this
  * replaces the NCCL all-reduce after the row-parallel O and down projections of a T-way sharded model) ----------
  *

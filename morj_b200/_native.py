@@ -43,6 +43,12 @@ SIGNATURES = {
     'morj_mlp_epilogue': [P, P, P, P, P, P, I, I, F, I, P],
     'morj_gather_rows': [P, LL, P, I, I, P, LL, P],
     'morj_scatter_rows': [P, LL, P, I, I, P, LL, P],
+    'morj_kv8_store_work': [IP, I, I, IP, I],
+    'morj_kv8_store': [P, LL, P, LL, I, I, I, P, I, P, P, P, P, I, P],
+    'morj_kv8_gather': [P, P, I, P, I, I, I, P, LL, P],
+    'morj_tree_attention_kv8_work': [IP, IP, IP, I, I, I, I, I, I, IP, I, IP],
+    'morj_tree_attention_kv8': [P, I, P, P, P, P, I, P, P, P, P, P, I, I, I, I, I, I, I, F, P, IP, P,
+                                ctypes.c_ulonglong, P],
     'morj_label_head': [P, LL, P, P, P, I, P, P, I, F, F, P, P],
     'morj_geglu': [P, I, I, P, P],
     'morj_ipc_export': [P, P],
@@ -136,6 +142,45 @@ def attention_work(qo_indptr, kv_indptr, n_bidir, hq, hk, window, page_size=1, k
     if got < 0:
         check(ERR_ARG, 'morj_tree_attention_work')
     return buf[:2 * got]
+
+
+def kv8_store_work(slots, pool_slots):
+    """(work list, number of touched 64-slot blocks) of an 8-bit cache store of rows 0..n-1 to `slots` (host int32;
+    `morj_kv8_store_work`). ValueError for a slot outside the pool or given twice."""
+    import numpy as np
+    s = np.ascontiguousarray(slots, dtype=np.int32).reshape(-1)
+    buf = np.zeros(5 * len(s) + 2, dtype=np.int32)
+    n = lib().morj_kv8_store_work(s.ctypes.data_as(IP), len(s), pool_slots, buf.ctypes.data_as(IP), len(buf))
+    if n < 0:
+        check(ERR_ARG, 'morj_kv8_store_work')
+    return buf[:3 * n + (n & 1) + 2 * len(s)], n
+
+
+KV8_COUNTS = I * 8
+
+
+def kv8_attention_work(qo_indptr, kv_indptr, n_bidir, hq, hk, window, page_size=1, kv_last_page_len=None):
+    """(work list, counts) of an attention call over an 8-bit cache, from host copies of its segment tables
+    (`morj_tree_attention_kv8_work`). `counts` is the ctypes array the call takes."""
+    import numpy as np
+    qo = np.ascontiguousarray(qo_indptr, dtype=np.int32)
+    kv = np.ascontiguousarray(kv_indptr, dtype=np.int32)
+    last = None if kv_last_page_len is None else np.ascontiguousarray(kv_last_page_len, dtype=np.int32)
+    counts = KV8_COUNTS()
+    cap = 0
+    while True:  # (the list's length is known after the first call)
+        buf = np.zeros(max(cap, 1), dtype=np.int32)
+        call('morj_tree_attention_kv8_work', qo.ctypes.data_as(IP), kv.ctypes.data_as(IP),
+             last.ctypes.data_as(IP) if last is not None else None, len(qo) - 1, n_bidir, hq, hk, page_size, window,
+             buf.ctypes.data_as(IP), cap, counts)
+        if counts[4] <= cap:
+            return buf[:counts[4]], counts
+        cap = counts[4]
+
+
+def kv8_attention_workspace(counts, hk, d):
+    """Workspace bytes of an attention call over an 8-bit cache with these counts."""
+    return counts[2] * hk * 16 * (d + 2) * 4
 
 
 def device_error(stream, clear=True):

@@ -32,6 +32,7 @@ enum DeviceError : int {
   kErrTimeoutAttention = 0x201,
   kErrBadIndex = 0x301,
   kErrBadAlignment = 0x302,
+  kErrNotFinite = 0x303,
 };
 
 // a wait that has not completed after this long is treated as a hang
