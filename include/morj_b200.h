@@ -180,6 +180,23 @@ int morj_label_head(const void* x, long long ld_x, const int* seq_row, const int
                     const int* label_ids, int n_seq, const void* norm_w, const void* embed, int H, float eps,
                     float softcap, float* probs, void* stream);
 
+/* Log-probabilities under the whole vocabulary (no counterpart in the reference, whose readout is label-restricted), for
+ * n normed rows h (BF16 [n, H], ld_h; morj_rmsnorm_rows) against w (BF16 [vocab, H], ld_w: the tied embedding):
+ * l = h . w_v (FP32 sums), z = softcap * tanh(l / softcap) (softcap 0: z = l), lse[i] = log sum_v exp z,
+ * logprobs[i, j] = z at targets[i, j] - lse[i] ([n, n_targets]; target -1: 0), entropy[i] = -sum_v p log p, and the
+ * `top` largest logits' ids and log-probabilities ([n, top], larger first, the lower id first among equal logits; at
+ * most MORJ_MAX_TOP). All outputs FP32 / int32; lse and entropy may be NULL. The [n, vocab] logits are never stored.
+ * A target outside [-1, vocab) sets the device error word (0x301) and gives NaN. A row with a NaN gives NaN (top id -1
+ * where no logit can be ranked). H % 8 == 0, ld % 8 == 0; h, w and workspace 16-byte aligned.
+ * workspace: morj_token_logprobs_workspace bytes of the caller's, overwritten; calls that may overlap on the device must
+ * not share it. Rows are taken 2048 at a time, w is read once for each such group. */
+#define MORJ_MAX_TOP 32
+int morj_token_logprobs_workspace(int n, int top, unsigned long long* bytes);
+int morj_token_logprobs(const void* h, long long ld_h, int n, const void* w, long long ld_w, int vocab, int H,
+                        float softcap, const int* targets, int n_targets, float* logprobs, float* lse, float* entropy,
+                        int top, int* top_ids, float* top_logprobs, void* workspace,
+                        unsigned long long workspace_bytes, void* stream);
+
 /* Reference-layout GeGLU (unfused path): out[i, j] = bf16(gelu_tanh(gu[i, j]) * gu[i, F + j]), gu: [n, 2F]. */
 int morj_geglu(const void* gu, int n, int F, void* out, void* stream);
 

@@ -50,6 +50,8 @@ SIGNATURES = {
     'morj_tree_attention_kv8': [P, I, P, P, P, P, I, P, P, P, P, P, I, I, I, I, I, I, I, F, P, IP, P,
                                 ctypes.c_ulonglong, P],
     'morj_label_head': [P, LL, P, P, P, I, P, P, I, F, F, P, P],
+    'morj_token_logprobs_workspace': [I, I, ctypes.POINTER(ctypes.c_ulonglong)],
+    'morj_token_logprobs': [P, LL, I, P, LL, I, I, F, P, I, P, P, P, I, P, P, P, ctypes.c_ulonglong, P],
     'morj_geglu': [P, I, I, P, P],
     'morj_ipc_export': [P, P],
     'morj_ipc_import': [P, ctypes.POINTER(P)],

@@ -1,0 +1,498 @@
+// Log-probabilities of given tokens over the whole vocabulary, without the [rows, vocab] logits in memory.
+//
+//   l_iv = h_i . w_v,  z = c tanh(l / c) (c = 0: z = l),  lse_i = log sum_v exp z_iv,
+//   logp_it = z_it - lse_i,  entropy_i = lse_i - sum_v p_iv z_iv,  top k by (l descending, id ascending).
+//
+// logits_kernel is a GEMM whose epilogue folds every accumulator row into three running numbers, with m the largest z
+// so far: m, s = sum exp(z - m) and t = sum exp(z - m) (z - m), so that lse = m + log s and entropy = log s - t / s
+// without cancellation. A CTA keeps them per row across the vocabulary tiles it computes, with a sorted list of the
+// row's top candidates; the softcap is monotone, so candidates are compared by the raw logit. finish_kernel joins the
+// CTAs' numbers and lists of a row and adds the given tokens' logits as plain dot products.
+//
+// One CTA per SM: warp 0 TMA producer, warp 1 MMA issuer (tcgen05, M = 128, N = 256, two TMEM accumulators), warps 2-5
+// epilogue (thread = row). Row blocks are the fast tile index: the CTAs in flight share a few vocabulary tiles, so w
+// crosses HBM once per call of up to 2048 rows (larger calls go in chunks of 2048).
+#include <algorithm>
+#include <climits>
+
+#include "common.cuh"
+
+namespace morj {
+namespace logprobs {
+
+constexpr int BM = 128, BN = 256, BK = 64;
+constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;
+constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int STAGES = 4;
+constexpr int MAX_TOP = MORJ_MAX_TOP;
+constexpr int LIST_BYTES = BM * MAX_TOP * 8;
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + LIST_BYTES + 1024 /*align*/ + 256 /*barriers*/;
+static_assert(SMEM_BYTES <= 232448, "shared memory per CTA");
+constexpr int TMEM_COLS = 512;
+constexpr int THREADS = 192;
+constexpr int CHUNK_ROWS = 2048;
+constexpr uint32_t IDESC = idesc_bf16(BM, BN);
+constexpr float LOG2E = 1.4426950408889634f;
+
+// What one CTA knows of one row: [cta][row] stats, [cta][row block][k][128 rows] candidates (logit, id).
+struct Scratch {
+  float4* stats;  // m, s, t, number of candidates
+  uint2* lists;
+  int rows;       // rows of a chunk rounded up to whole row blocks
+  int top;
+};
+
+// z = c tanh(l / c). Near 0 tanh's series, elsewhere 1 - 2 / (1 + e^2x): relative error of a few 2^-24 on both sides.
+MORJ_DEV float cap_near(float l, float c, float inv_c) {  // |l| <= c / 4
+  const float x = l * inv_c, x2 = x * x;
+  const float p = fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+  return l * p;
+}
+MORJ_DEV float cap_far(float l, float c, float inv_c) {
+  float r;
+  const float e = fast_exp2(l * (inv_c * 2.f * LOG2E));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+  return fmaf(-2.f * c, r, c);
+}
+MORJ_DEV float cap(float l, float c, float inv_c) {
+  if (c == 0.f) return l;
+  return fabsf(l) <= 0.25f * c ? cap_near(l, c, inv_c) : cap_far(l, c, inv_c);
+}
+
+// Running numbers of a row moved to a larger maximum.
+MORJ_DEV void raise(float& m, float& s, float& t, float now) {
+  if (m != -INFINITY) {
+    const float f = fast_exp2((m - now) * LOG2E);
+    t = f * (t + s * (m - now));
+    s *= f;
+  }
+  m = now;
+}
+
+template <bool CAP>
+MORJ_DEV void fold(const uint32_t (&r)[32], int valid, float c, float inv_c, float& m, float& s, float& t, float mx) {
+  const float zmx = CAP ? cap(mx, c, inv_c) : mx;
+  if (zmx > m) raise(m, s, t, zmx);
+  const float shift = m == -INFINITY ? 0.f : m;
+  float s4[4] = {0.f, 0.f, 0.f, 0.f}, t4[4] = {0.f, 0.f, 0.f, 0.f};  // (short sums: the total rounds once per 32)
+#pragma unroll
+  for (int i = 0; i < 32; ++i) {
+    const float l = __uint_as_float(r[i]);
+    const float u = (CAP ? cap(l, c, inv_c) : l) - shift;
+    const float e = fast_exp2(u * LOG2E);
+    if (i < valid) {
+      s4[i & 3] += e;
+      t4[i & 3] = fmaf(e, u, t4[i & 3]);
+    }
+  }
+  s += (s4[0] + s4[1]) + (s4[2] + s4[3]);
+  t += (t4[0] + t4[1]) + (t4[2] + t4[3]);
+}
+
+__global__ void __launch_bounds__(THREADS, 1)
+    logits_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w, int M, int V,
+                  int K, int a_bytes, float c, const Scratch sc) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  float* list_val = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES);  // [MAX_TOP][128 rows]
+  int* list_id = reinterpret_cast<int*>(list_val + MAX_TOP * BM);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES + LIST_BYTES);
+  // bars: full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 5);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t full0 = smem_u32(bars), empty0 = smem_u32(bars + STAGES);
+  const uint32_t accf0 = smem_u32(bars + 2 * STAGES), acce0 = smem_u32(bars + 2 * STAGES + 2);
+  const uint32_t done0 = smem_u32(bars + 2 * STAGES + 4);
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < STAGES; ++i) {
+      mbar_init(full0 + 8 * i, 1);
+      mbar_init(empty0 + 8 * i, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(accf0 + 8 * b, 1);
+      mbar_init(acce0 + 8 * b, 128);
+    }
+    mbar_init(done0, 1);
+    *abort = 0;
+    fence_mbar_init();
+    tma_prefetch(&map_h);
+    tma_prefetch(&map_w);
+  }
+  if (warp == 1) {
+    tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  pdl_wait();  // (set-up above touches no global memory) the previous kernel on the stream has completed
+  pdl_trigger();
+
+  const int num_m = (M + BM - 1) / BM, num_n = (V + BN - 1) / BN;
+  const int tiles = num_m * num_n, kblocks = (K + BK - 1) / BK;
+  const uint32_t smem_base = smem_u32(smem);
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint64_t pol_h = policy_evict_last();
+      const uint64_t pol_w = num_m == 1 ? policy_evict_first() : policy_evict_normal();
+      int stage = 0, issued = 0;
+      uint32_t phase = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles && ok && !*abort; t += gridDim.x) {
+        const int m = t % num_m, n = t / num_m;
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!mbar_wait(empty0 + 8 * stage, phase ^ 1, abort, kErrTimeoutGemmProducer)) {
+            ok = false;
+            break;
+          }
+          const uint32_t sa = smem_base + stage * STAGE_BYTES;
+          mbar_arrive_expect_tx(full0 + 8 * stage, a_bytes + B_BYTES);
+          tma_load_2d(sa, &map_h, full0 + 8 * stage, kb * BK, m * BM, pol_h);
+          tma_load_2d(sa + A_BYTES, &map_w, full0 + 8 * stage, kb * BK, n * BN, pol_w);
+          ++issued;
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+      }
+      // no copy may still be in flight when the CTA exits: wait for the last fills to land
+      const int pending = issued < STAGES ? issued : STAGES;
+      for (int j = 1; j <= pending; ++j) {
+        const int s = (stage - j + STAGES) % STAGES;
+        const uint32_t ph = (stage - j >= 0) ? phase : (phase ^ 1);
+        mbar_wait_landed(full0 + 8 * s, ph);
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      int stage = 0, acc = 0;
+      uint32_t phase = 0, acc_phase = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+        if (!mbar_wait(acce0 + 8 * acc, acc_phase ^ 1, abort, kErrTimeoutGemmMma)) break;
+        tc_fence_after();
+        const uint32_t d_tmem = tmem_base + acc * BN;
+        for (int kb = 0; kb < kblocks; ++kb) {
+          if (!mbar_wait(full0 + 8 * stage, phase, abort, kErrTimeoutGemmMma)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_base + stage * STAGE_BYTES, sb = sa + A_BYTES;
+#pragma unroll
+          for (int k = 0; k < BK / 16; ++k)
+            umma_bf16(d_tmem, sw128_desc(sa + 32 * k), sw128_desc(sb + 32 * k), IDESC, (kb | k) != 0);
+          umma_commit(empty0 + 8 * stage);
+          if (++stage == STAGES) {
+            stage = 0;
+            phase ^= 1;
+          }
+        }
+        if (!ok) break;
+        umma_commit(accf0 + 8 * acc);
+        if (++acc == 2) {
+          acc = 0;
+          acc_phase ^= 1;
+        }
+      }
+      // TMEM is freed below only after every MMA issued here has completed
+      umma_commit(done0);
+      mbar_wait_landed(done0, 0);
+    }
+  } else {
+    const int quarter = warp & 3;
+    const int r128 = quarter * 32 + lane;
+    const int top = sc.top;
+    const float inv_c = c > 0.f ? 1.f / c : 0.f;
+    float4* stats = sc.stats + (size_t)blockIdx.x * sc.rows + r128;
+    uint2* lists = sc.lists + (size_t)blockIdx.x * sc.rows * top + r128;
+    for (int m = 0; m < num_m; ++m) stats[m * BM] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    int acc = 0;
+    uint32_t acc_phase = 0;
+    int held = -1;  // the row block whose list is in shared memory
+    float4 st = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    int count = 0;
+    float tau = INFINITY;  // candidates must exceed it
+    for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
+      const int m = t % num_m, n = t / num_m;
+      if (m != held) {
+        if (held >= 0) {
+          st.w = __int_as_float(count);
+          stats[held * BM] = st;
+          for (int k = 0; k < count; ++k)
+            lists[(size_t)(held * top + k) * BM] =
+                make_uint2(__float_as_uint(list_val[k * BM + r128]), (uint32_t)list_id[k * BM + r128]);
+        }
+        st = stats[m * BM];
+        count = __float_as_int(st.w);
+        for (int k = 0; k < count; ++k) {
+          const uint2 e = lists[(size_t)(m * top + k) * BM];
+          list_val[k * BM + r128] = __uint_as_float(e.x);
+          list_id[k * BM + r128] = (int)e.y;
+        }
+        tau = top == 0 ? INFINITY : count < top ? -INFINITY : list_val[(top - 1) * BM + r128];
+        held = m;
+      }
+      int ok = lane == 0 ? (int)mbar_wait(accf0 + 8 * acc, acc_phase, abort, kErrTimeoutGemmEpilogue) : 0;
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok) break;
+      tc_fence_after();
+      const bool row_ok = m * BM + r128 < M;
+      const uint32_t tacc = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * BN;
+#pragma unroll 1
+      for (int col = 0; col < BN; col += 32) {
+        const int id0 = n * BN + col, valid = min(32, V - id0);
+        if (valid <= 0) break;  // (warp-uniform)
+        uint32_t r[32];
+        tmem_ld32(tacc + col, r);
+        tmem_wait_ld();
+        float mx = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, i < valid ? __uint_as_float(r[i]) : -INFINITY);
+        if (c > 0.f)
+          fold<true>(r, valid, c, inv_c, st.x, st.y, st.z, mx);
+        else
+          fold<false>(r, valid, c, inv_c, st.x, st.y, st.z, mx);
+        if (row_ok && (mx > tau || (count < top && mx == -INFINITY))) {
+          float v[32];
+#pragma unroll
+          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+          for (int i = 0; i < valid; ++i) {
+            const float x = v[i];
+            if (!(x > tau || (count < top && x >= -INFINITY))) continue;
+            int at = count < top ? count++ : top - 1;
+            for (; at > 0 && list_val[(at - 1) * BM + r128] < x; --at) {
+              list_val[at * BM + r128] = list_val[(at - 1) * BM + r128];
+              list_id[at * BM + r128] = list_id[(at - 1) * BM + r128];
+            }
+            list_val[at * BM + r128] = x;
+            list_id[at * BM + r128] = id0 + i;
+            if (count == top) tau = list_val[(top - 1) * BM + r128];
+          }
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(acce0 + 8 * acc);
+      if (++acc == 2) {
+        acc = 0;
+        acc_phase ^= 1;
+      }
+    }
+    if (held >= 0) {
+      st.w = __int_as_float(count);
+      stats[held * BM] = st;
+      for (int k = 0; k < count; ++k)
+        lists[(size_t)(held * top + k) * BM] =
+            make_uint2(__float_as_uint(list_val[k * BM + r128]), (uint32_t)list_id[k * BM + r128]);
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, TMEM_COLS);
+  }
+}
+
+// ---- finish: one CTA per row ----------------------------------------------------------------------------------------
+constexpr int F_THREADS = 256;
+
+// (logit, id) order of candidates: larger logit first, then the lower id; id < 0: none
+MORJ_DEV bool before(float v, int id, float w, int jd) { return id >= 0 && (jd < 0 || v > w || (v == w && id < jd)); }
+
+struct Outputs {
+  const int* targets;
+  int n_targets;
+  float* logprobs;
+  float* lse;
+  float* entropy;
+  int* top_ids;
+  float* top_logprobs;
+};
+
+MORJ_DEV float cap_exact(float l, float c) { return c > 0.f ? c * tanhf(l / c) : l; }
+
+__global__ void __launch_bounds__(F_THREADS)
+    finish_kernel(const __nv_bfloat16* __restrict__ h, long long ld_h, const __nv_bfloat16* __restrict__ w,
+                  long long ld_w, int V, int K, float c, int ctas, const Scratch sc, const Outputs o, int row0) {
+  pdl_wait();  // the previous kernel on the stream has completed
+  pdl_trigger();
+  __shared__ float red[32], red_v[F_THREADS / 32];
+  __shared__ int red_i[F_THREADS / 32], red_c[F_THREADS / 32];
+  const int local = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const size_t row = (size_t)row0 + local;
+  float4 st = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+  if (threadIdx.x < ctas) st = sc.stats[(size_t)threadIdx.x * sc.rows + local];
+  float m = st.x;
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
+  if (lane == 0) red_v[warp] = m;
+  __syncthreads();
+  for (int i = 0; i < F_THREADS / 32; ++i) m = fmaxf(m, red_v[i]);
+  float s = st.y, t = st.z;
+  if (st.x != -INFINITY) raise(st.x, s, t, m);
+  s = block_sum(s, red);
+  t = block_sum(t, red);
+  const float ls = logf(s), lse = (m == -INFINITY ? 0.f : m) + ls;
+  if (threadIdx.x == 0) {
+    if (o.lse) o.lse[row] = lse;
+    if (o.entropy) o.entropy[row] = ls - t / s;
+  }
+  // the lists' heads compete: thread i walks CTA i's sorted list
+  if (sc.top) {
+    const uint2* list = sc.lists + ((size_t)threadIdx.x * sc.rows + (local / BM) * BM) * sc.top + local % BM;
+    const int count = threadIdx.x < ctas ? __float_as_int(st.w) : 0;
+    int at = 0, id = -1;
+    float v = 0.f;
+    auto load = [&] {
+      id = -1;
+      if (at < count) {
+        const uint2 e = list[(size_t)at * BM];
+        v = __uint_as_float(e.x);
+        id = (int)e.y;
+      }
+    };
+    load();
+    for (int k = 0; k < sc.top; ++k) {
+      float bv = v;
+      int bi = id, bc = threadIdx.x;
+#pragma unroll
+      for (int x = 16; x > 0; x >>= 1) {
+        const float ov = __shfl_xor_sync(0xffffffffu, bv, x);
+        const int oi = __shfl_xor_sync(0xffffffffu, bi, x), oc = __shfl_xor_sync(0xffffffffu, bc, x);
+        if (before(ov, oi, bv, bi)) bv = ov, bi = oi, bc = oc;
+      }
+      __syncthreads();
+      if (lane == 0) red_v[warp] = bv, red_i[warp] = bi, red_c[warp] = bc;
+      __syncthreads();
+      bv = red_v[0], bi = red_i[0], bc = red_c[0];
+      for (int i = 1; i < F_THREADS / 32; ++i)
+        if (before(red_v[i], red_i[i], bv, bi)) bv = red_v[i], bi = red_i[i], bc = red_c[i];
+      if (threadIdx.x == 0) {
+        o.top_ids[row * sc.top + k] = bi;
+        o.top_logprobs[row * sc.top + k] = bi < 0 ? NAN : cap_exact(bv, c) - lse;
+      }
+      if (bi >= 0 && bc == (int)threadIdx.x) {
+        ++at;
+        load();
+      }
+    }
+  }
+  for (int j = warp; j < o.n_targets; j += F_THREADS / 32) {
+    const int id = o.targets[row * o.n_targets + j];
+    float lp = 0.f;
+    if (id != -1) {
+      if (id < 0 || id >= V) {
+        if (lane == 0) report(kErrBadIndex);
+        lp = NAN;
+      } else {
+        const __nv_bfloat16* hr = h + row * ld_h;
+        const __nv_bfloat16* wr = w + (size_t)id * ld_w;
+        float acc = 0.f;
+        for (int k = lane * 8; k < K; k += 256) {
+          float a[8], b[8];
+          load8(hr + k, a);
+          load8(wr + k, b);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc = fmaf(a[e], b[e], acc);
+        }
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, x);
+        lp = cap_exact(acc, c) - lse;
+      }
+    }
+    if (lane == 0) o.logprobs[row * o.n_targets + j] = lp;
+  }
+}
+
+// ---- host -----------------------------------------------------------------------------------------------------------
+static int chunk_rows(int n) { return ((n < CHUNK_ROWS ? n : CHUNK_ROWS) + BM - 1) / BM * BM; }
+
+static unsigned long long workspace(int n, int top) {
+  return (unsigned long long)num_sms() * chunk_rows(n) * (sizeof(float4) + (unsigned long long)top * sizeof(uint2));
+}
+
+static int make_map(CUtensorMap* map, const void* ptr, long long rows, long long cols, long long ld, int box_rows) {
+  const unsigned long long dims[2] = {(unsigned long long)cols, (unsigned long long)rows};
+  const unsigned long long strides[1] = {(unsigned long long)(ld * 2)};
+  const unsigned box[2] = {(unsigned)BK, (unsigned)box_rows};
+  return encode_tiled(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, ptr, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+}
+
+// cudaFuncSetAttribute holds per device
+static int configure() {
+  static bool done[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !done[dev])) {
+    e = cudaFuncSetAttribute(logits_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    if (e == cudaSuccess && dev < 64) done[dev] = true;
+  }
+  return e == cudaSuccess ? MORJ_OK : set_error(MORJ_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+}
+
+}  // namespace logprobs
+}  // namespace morj
+
+extern "C" int morj_token_logprobs_workspace(int n, int top, unsigned long long* bytes) {
+  using namespace morj;
+  if (!bytes || n < 0 || top < 0 || top > logprobs::MAX_TOP)
+    return set_error(MORJ_ERR_ARG, "morj_token_logprobs_workspace: bad arguments (n=%d top=%d)", n, top);
+  *bytes = n ? logprobs::workspace(n, top) : 0;
+  return MORJ_OK;
+}
+
+extern "C" int morj_token_logprobs(const void* h, long long ld_h, int n, const void* w, long long ld_w, int vocab,
+                                   int H, float softcap, const int* targets, int n_targets, float* logprobs_out,
+                                   float* lse, float* entropy, int top, int* top_ids, float* top_logprobs,
+                                   void* workspace, unsigned long long workspace_bytes, void* stream) {
+  using namespace morj;
+  using namespace morj::logprobs;
+  if (n == 0) return MORJ_OK;
+  if (!h || !w || n < 0 || vocab <= 0 || vocab > INT_MAX - BN || H <= 0 || n_targets < 0 ||
+      (n_targets && (!targets || !logprobs_out)) || (top && (!top_ids || !top_logprobs)))
+    return set_error(MORJ_ERR_ARG, "morj_token_logprobs: null pointer or bad size (n=%d vocab=%d H=%d)", n, vocab, H);
+  if (top < 0 || top > MAX_TOP || top > vocab)
+    return set_error(MORJ_ERR_ARG, "morj_token_logprobs: top %d must be in [0, %d] and at most vocab", top, MAX_TOP);
+  if (!(softcap >= 0.f) || softcap > 1e30f || (softcap > 0.f && softcap < 1e-30f))
+    return set_error(MORJ_ERR_ARG, "morj_token_logprobs: softcap must be 0 (none) or in [1e-30, 1e30]");
+  if (H % 8 || ld_h % 8 || ld_w % 8 || ld_h < H || ld_w < H)
+    return set_error(MORJ_ERR_ARG, "morj_token_logprobs: H and leading dimensions must be multiples of 8 (H=%d)", H);
+  if ((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(workspace)) & 15)
+    return set_error(MORJ_ERR_ARG, "morj_token_logprobs: h, w and workspace must be 16-byte aligned");
+  const unsigned long long need = logprobs::workspace(n, top);
+  if (!workspace || workspace_bytes < need)
+    return set_error(MORJ_ERR_ARG, "morj_token_logprobs: a workspace of %llu bytes given, %llu needed", workspace_bytes,
+                     need);
+  int st = configure();
+  if (st) return st;
+  cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
+  CUtensorMap mw;
+  if ((st = make_map(&mw, w, vocab, H, ld_w, BN))) return st;
+  Scratch sc;
+  sc.rows = chunk_rows(n), sc.top = top;
+  sc.stats = static_cast<float4*>(workspace);
+  sc.lists = reinterpret_cast<uint2*>(sc.stats + (size_t)num_sms() * sc.rows);
+  const Outputs o{targets, n_targets, logprobs_out, lse, entropy, top_ids, top_logprobs};
+  for (int r0 = 0; r0 < n; r0 += CHUNK_ROWS) {
+    const int rows = std::min(n - r0, CHUNK_ROWS);
+    const int box = rows >= BM ? BM : (rows + 7) / 8 * 8;  // few rows: only those are loaded
+    CUtensorMap mh;
+    if ((st = make_map(&mh, static_cast<const __nv_bfloat16*>(h) + (size_t)r0 * ld_h, rows, H, ld_h, box))) return st;
+    const long long tiles = (long long)((rows + BM - 1) / BM) * ((vocab + BN - 1) / BN);
+    const int ctas = (int)std::min<long long>(tiles, std::min(num_sms(), F_THREADS));
+    st = launch_pdl("logits_kernel", logits_kernel, dim3(ctas), dim3(THREADS), SMEM_BYTES, s, mh, mw, rows, vocab, H,
+                    box * BK * 2, softcap, sc);
+    if (st) return st;
+    st = launch_pdl("finish_kernel", finish_kernel, dim3(rows), dim3(F_THREADS), 0, s, (const __nv_bfloat16*)h, ld_h,
+                    (const __nv_bfloat16*)w, ld_w, vocab, H, softcap, ctas, sc, o, r0);
+    if (st) return st;
+  }
+  return MORJ_OK;
+}
