@@ -65,8 +65,8 @@ class KV8Pool:
             raise ValueError(f'unsupported 8-bit pool: {slots} slots, {heads} heads of {head_dim} (64 or 128)')
         shape, blocks = (max(slots, 1), heads, head_dim), (max(slots, 1) + BLOCK - 1) // BLOCK
         make = lambda: torch.empty(shape, dtype=torch.uint8, device=device).view(CODES)
-        self._set(make(), torch.zeros(blocks, heads, device=device), make(),
-                  torch.zeros(blocks, heads, device=device))
+        self.scales = torch.zeros(2, blocks, heads, device=device)  # (K's and V's, one tensor to clear)
+        self._set(make(), self.scales[0], make(), self.scales[1])
 
     @classmethod
     def of(cls, k, k_scale, v, v_scale):
@@ -83,6 +83,7 @@ class KV8Pool:
                                                                                (k, v, k_scale, v_scale)}) != 1:
             raise ValueError('codes and scales must be contiguous and on one device')
         self = cls.__new__(cls)
+        self.scales = None
         self._set(k.view(CODES), k_scale, v.view(CODES), v_scale)
         return self
 
@@ -90,6 +91,21 @@ class KV8Pool:
         self.k, self.k_scale, self.v, self.v_scale = k, k_scale, v, v_scale
         self.slots, self.heads, self.head_dim = k.shape
         self.device = k.device
+
+    def clear(self):
+        """Forget what is stored: every block is empty again."""
+        if self.scales is not None:
+            self.scales.zero_()
+        else:
+            self.k_scale.zero_()
+            self.v_scale.zero_()
+
+    def copy_head(self, other):
+        """The codes and scales of a pool of the same heads into the first slots (this pool is new, or larger)."""
+        n, b = min(self.slots, other.slots), min(len(self.k_scale), len(other.k_scale))
+        for name in ('k', 'v'):
+            getattr(self, name).view(torch.uint8)[:n].copy_(getattr(other, name).view(torch.uint8)[:n])
+            getattr(self, name + '_scale')[:b].copy_(getattr(other, name + '_scale')[:b])
 
     @property
     def nbytes(self):

@@ -14,6 +14,11 @@ Forward per step (one pass may need several steps; see `Tree.plan_pass`):
   the last layer computes K/V for every token and the rest only for readout rows; the label head reads them.
 Numerics follow the reference path: FP32 norms and softmax, BF16 rounding where it rounds, attention scale 1.0,
 V = K projection on full-attention layers, proportional partial RoPE there, BF16 embedding scale.
+
+Two additions without a counterpart in the reference: `kv_cache='e4m3'` keeps every K/V pool in 8 bits
+(`morj_b200.kv8`: the projection writes a step's K/V rows to a BF16 buffer, which is stored into the pool and attended
+to from there), and `label_logprobs` / `token_logprobs` read log-probabilities under the whole vocabulary
+(`morj_b200.logprobs`) instead of the softmax over a few labels.
 """
 import os
 import time
@@ -22,6 +27,7 @@ import numpy as np
 import torch
 
 from . import _native as nat
+from . import kv8
 from .checkpoint import PREFIX, iter_random_state, layer_geometry, open_checkpoint
 from .tree import Tree
 
@@ -32,6 +38,7 @@ POISON = os.environ.get('JUDGE_LEAN_POISON') == '1'
 KINDS = {'sliding_attention': 's', 'full_attention': 'g'}
 GLU_BLOCK = 128  # gate/up rows are interleaved in blocks of this many rows for the fused GeGLU epilogue
 MAX_LABELS = 8192  # labels per sequence the label-head kernel holds in shared memory
+MAX_PRUNED_ROWS = 64  # a scoring pass that reads more rows runs its last layer whole (each pruned row has a key list)
 
 
 class Request:
@@ -157,29 +164,32 @@ class _Tables:
 
 
 class LeanGemma4:
+    kv8 = False  # K/V pools in 8 bits (`kv_cache='e4m3'`)
+
     def __init__(self, model_dir, device='cuda', workspace_mb=512, retain_budget_gb=10.0, single_max=16384,
-                 step_tokens=8192, *, tp_group=None, tp_comm='peer'):
+                 step_tokens=8192, *, tp_group=None, tp_comm='peer', kv_cache='bf16'):
         """Load a safetensors checkpoint (`config.json["text_config"]` + `model.language_model.*` tensors) as the
         reference does (`lean_core.py:340-416`). `workspace_mb` is accepted for interface compatibility; the tree
         attention kernel needs no workspace. `tp_group`: a torch.distributed process group (NCCL) to shard the model
         over for tensor parallelism (`morj_b200.tp`); None runs the whole model on this GPU. `tp_comm`: 'peer'
         reduces the row-parallel projections over peer memory fused with their epilogues (`tp.PeerExchange`),
-        'nccl' with an NCCL all-reduce followed by the replicated epilogues."""
+        'nccl' with an NCCL all-reduce followed by the replicated epilogues. `kv_cache`: 'bf16' as the reference, or
+        'e4m3': pools of 8-bit codes with a scale per 64 slots and head, half the bytes per kept token."""
         top, get = open_checkpoint(model_dir, device)
-        self._setup(top, get, device, retain_budget_gb, single_max, step_tokens, tp_group, tp_comm)
+        self._setup(top, get, device, retain_budget_gb, single_max, step_tokens, tp_group, tp_comm, kv_cache)
 
     @classmethod
     def from_state(cls, top, state, device='cuda', retain_budget_gb=10.0, single_max=16384, step_tokens=8192,
-                   tp_group=None, tp_comm='peer'):
+                   tp_group=None, tp_comm='peer', kv_cache='bf16'):
         """An engine over an in-memory state dict in the checkpoint's key layout (tensors on any device)."""
         self = cls.__new__(cls)
         self._setup(top, lambda k: state[k].to(device), device, retain_budget_gb, single_max, step_tokens, tp_group,
-                    tp_comm)
+                    tp_comm, kv_cache)
         return self
 
     @classmethod
     def random_init(cls, top, seed=0, device='cuda', std=0.02, norm_std=0.1, retain_budget_gb=10.0,
-                    single_max=16384, step_tokens=8192, tp_group=None, tp_comm='peer'):
+                    single_max=16384, step_tokens=8192, tp_group=None, tp_comm='peer', kv_cache='bf16'):
         """An engine over seeded random-init weights generated on `device` (no checkpoint on disk); tensors are drawn
         in checkpoint order and handed over one at a time, so the peak memory is the model plus one layer."""
         gen = iter_random_state(top, seed=seed, std=std, norm_std=norm_std, device=device)
@@ -191,12 +201,16 @@ class LeanGemma4:
                 cache[k] = t
             return cache.pop(key)
         self = cls.__new__(cls)
-        self._setup(top, get, device, retain_budget_gb, single_max, step_tokens, tp_group, tp_comm)
+        self._setup(top, get, device, retain_budget_gb, single_max, step_tokens, tp_group, tp_comm, kv_cache)
         return self
 
-    def _setup(self, top, get, device, retain_budget_gb, single_max, step_tokens, tp_group=None, tp_comm='peer'):
+    def _setup(self, top, get, device, retain_budget_gb, single_max, step_tokens, tp_group=None, tp_comm='peer',
+               kv_cache='bf16'):
         if tp_comm not in ('peer', 'nccl'):
             raise ValueError(f"tp_comm must be 'peer' or 'nccl', not {tp_comm!r}")
+        if kv_cache not in ('bf16', 'e4m3'):
+            raise ValueError(f"kv_cache must be 'bf16' or 'e4m3', not {kv_cache!r}")
+        self.kv8 = kv_cache == 'e4m3'
         self.tp_group, self.tp_world, self.tp_rank = tp_group, 1, 0
         self.peer = None
         if tp_group is not None:
@@ -261,7 +275,9 @@ class LeanGemma4:
         # (`lean_core.py:636-640`), built once and grown with the longest position seen (`_rope`)
         self.rope = {}
         self.prune_last = True
-        self.kv_bytes = sum(2 * 2 * self.geom[k][0] * self.geom[k][1] for k in self.types)
+        # bytes of one kept token over all layers (8-bit pools: its share of a block of 64 slots and their scales)
+        per = kv8.BLOCK if self.kv8 else 1
+        self.kv_bytes = -(-sum(self._pool_bytes(k, per) for k in self.types) // per)
         self.retain_budget = retain_budget_gb * 2**30
         self.shared, self.shared_kv = None, None
         self.single_max, self.step_tokens = single_max, step_tokens
@@ -292,7 +308,7 @@ class LeanGemma4:
         self.run(req, [0])
         offsets = np.concatenate([req.tree.slots(n) for n in req.tree.paths[0]]).astype(np.int32)
         idx = torch.as_tensor(offsets, device=self.device)
-        kv = [(self._gather(k, idx), self._gather(v, idx)) for k, v in req.pools]
+        kv = [pool.rows(idx) if self.kv8 else tuple(self._gather(t, idx) for t in pool) for pool in req.pools]
         torch.cuda.current_stream(self.device).synchronize()
         self.shared, self.shared_kv = np.asarray(tokens, dtype=np.int64), kv
 
@@ -336,9 +352,24 @@ class LeanGemma4:
                 self._copy_head(req.pools, None, np.concatenate([tree.slots(n) for n in req.head_nodes]))
         return req
 
-    def _kv_pool(self, kind, slots):
-        """A (K, V) pair of `slots` rows for one layer of `kind`. With POISON (tests) every row starts as NaN."""
+    def _pool_bytes(self, kind, slots):
+        """Device bytes of one layer's K/V pool of `slots` rows."""
         hk, d = self.geom[kind]
+        if self.kv8:
+            return 2 * (slots * hk * d + -(-slots // kv8.BLOCK) * hk * 4)
+        return 4 * slots * hk * d
+
+    def _kv_pool(self, kind, slots):
+        """One layer's K/V pool of `slots` rows for a layer of `kind`: a (K, V) pair, or a `kv8.KV8Pool`. With POISON
+        (tests) every row starts as NaN."""
+        hk, d = self.geom[kind]
+        if self.kv8:
+            pool = kv8.KV8Pool(slots, hk, d, self.device)
+            if POISON:
+                for codes in (pool.k, pool.v):
+                    codes.view(torch.uint8).fill_(0x7f)
+                pool.scales.fill_(float('nan'))
+            return pool
         shape = (max(slots, 1), hk, d)
         if POISON:
             return tuple(torch.full(shape, float('nan'), dtype=torch.bfloat16, device=self.device) for _ in 'kv')
@@ -352,10 +383,20 @@ class LeanGemma4:
                 width, self._stream())
         return out
 
-    def _copy_head(self, pools, slot_of, head, layers=None):
+    def _copy_head(self, pools, slot_of, head, layers=None, plans=None):
         """The shared head's K/V into the pools of `layers` (default every layer, `pools[j]` for layer `layers[j]`),
         at the head's slots: the tree offsets `head` mapped through `slot_of` (per kind; None when slots are tree
-        offsets) (`lean_core.py:594-597`)."""
+        offsets) (`lean_core.py:594-597`). `plans`: 8-bit store plans of these arguments by kind, kept by a caller that
+        comes back for each layer."""
+        if self.kv8:
+            plans = {} if plans is None else plans
+            for pool, i in zip(pools, layers if layers is not None else range(len(self.types))):
+                kind = self.types[i]
+                if kind not in plans:
+                    slots = head if slot_of is None else slot_of[KINDS[kind]][head]
+                    plans[kind] = kv8.StorePlan(slots, pool.slots, self.device)
+                kv8.store(pool, *self.shared_kv[i], plans[kind])
+            return
         for (k, v), i in zip(pools, layers if layers is not None else range(len(self.types))):
             slots = head if slot_of is None else slot_of[KINDS[self.types[i]]][head]
             idx = torch.as_tensor(np.asarray(slots, dtype=np.int32), device=self.device)
@@ -368,11 +409,15 @@ class LeanGemma4:
         """A pinned request's pools, enlarged to at least `cap` slots per kind when a pass needs more; the rows held so
         far move to the same slots of the new pools (`lean_core.py:578-592`)."""
         old = req.pools
-        short = old is None or any(old[i][0].shape[0] < cap[KINDS[kind]] for i, kind in enumerate(self.types))
+        held = lambda pool: pool.slots if self.kv8 else pool[0].shape[0]
+        short = old is None or any(held(old[i]) < cap[KINDS[kind]] for i, kind in enumerate(self.types))
         if not short:
             return old
         new = [self._kv_pool(kind, cap[KINDS[kind]]) for kind in self.types]
-        if old is not None:
+        if old is not None and self.kv8:
+            for pool, was in zip(new, old):
+                pool.copy_head(was)
+        elif old is not None:
             for (k, v), (ok, ov) in zip(new, old):
                 n = min(ok.shape[0], k.shape[0])
                 idx = torch.arange(n, dtype=torch.int32, device=self.device)
@@ -394,7 +439,7 @@ class LeanGemma4:
         """Device bytes a planned pass needs: its largest step's activations, plus every layer's pools when they live
         for the whole pass (pinned requests, and multi-step passes of requests not kept whole)."""
         largest = max(len(st['tokens']) for st in plan['steps'])
-        pools = sum(plan['cap'][KINDS[t]] * 4 * self.geom[t][0] * self.geom[t][1] for t in self.types)
+        pools = sum(self._pool_bytes(t, plan['cap'][KINDS[t]]) for t in self.types)
         return (pools if persistent else 0) + largest * self.act_bytes
 
     def plan(self, req, seqs, available=None):
@@ -447,10 +492,11 @@ class LeanGemma4:
             self._copy_head(pools, plan['slot_of'], head)
         return pools
 
-    def prepare_pass(self, req, seqs, available=None):
+    def prepare_pass(self, req, seqs, available=None, scored=None):
         """Host half of `run`: plan (with the memory fit), the pools the pass writes, and every step's tables uploaded
         to the device. The result can be executed any number of times (`execute_pass`); each execution recomputes
-        the same nodes into the same slots."""
+        the same nodes into the same slots. `scored` (`token_logprobs`): per sequence its first scored token, or None;
+        the pass then reads the rows that predict them instead of the sequences' last rows."""
         t0 = time.perf_counter()
         need, head, pinned, plan = self.plan(req, seqs, available)
         pools = self._pass_pools(req, plan, head)
@@ -458,15 +504,22 @@ class LeanGemma4:
         if any(len(ids) > MAX_LABELS for ids in labels):
             raise ValueError(f'at most {MAX_LABELS} labels per sequence')
         self.h2d_bytes = 0
-        tables = [self._step_tables(k, st, plan, req) for k, st in enumerate(plan['steps'])]
-        ro = self._readout_tables(plan, labels)
+        if scored is not None:
+            plan = dict(plan, readout=self._scored_rows(req, seqs, plan, scored))
+        # A pass that reads many rows runs its last layer whole, a few rows are pruned to. Rows of an image block are read
+        # whole too: pruned, they would lose the block's bidirectional mask.
+        prune = self.prune_last and (scored is None or (len(set(plan['readout'])) <= MAX_PRUNED_ROWS and not req.bidir))
+        slots = {kk: max(plan['cap'][kk], 1) for kk in 'gs'}
+        if self.kv8 and pools is not None:
+            slots.update((KINDS[kind], pool.slots) for kind, pool in zip(self.types, pools))
+        tables = [self._step_tables(k, st, plan, req, slots, prune) for k, st in enumerate(plan['steps'])]
+        ro = self._readout_tables(plan, labels) if scored is None else None
         return dict(req=req, seqs=list(seqs), need=need, head=head, pinned=pinned, plan=plan, pools=pools,
-                    labels=labels, tables=tables, ro=ro, host_ms=1000 * (time.perf_counter() - t0),
+                    labels=labels, tables=tables, ro=ro, prune=prune, host_ms=1000 * (time.perf_counter() - t0),
                     h2d_bytes=self.h2d_bytes, tokens=sum(len(st['tokens']) for st in plan['steps']))
 
-    def execute_pass(self, p):
-        """Device half of `run`: every step's forward and the label head; returns the FP32 probabilities (device,
-        CSR over the requested sequences' labels). Launches only; nothing waits for the GPU."""
+    def _execute_steps(self, p):
+        """Every step's forward; returns the residual rows of the pass's readout rows (in step order). Launches only."""
         plan = p['plan']
         if self.peer is not None:
             self.peer.begin_pass()
@@ -474,9 +527,15 @@ class LeanGemma4:
         at = 0
         for k, st in enumerate(plan['steps']):
             n_rows = len(p['tables'][k][1])
-            self._step(k, st, plan, p['pools'], p['head'], p['req'], p['tables'][k], reads[at:at + n_rows])
+            self._step(k, st, plan, p['pools'], p['head'], p['req'], p['tables'][k], reads[at:at + n_rows],
+                       p['prune'])
             at += n_rows
-        return self._readout(reads[:at], p['ro'])
+        return reads[:at]
+
+    def execute_pass(self, p):
+        """Device half of `run`: every step's forward and the label head; returns the FP32 probabilities (device,
+        CSR over the requested sequences' labels). Launches only; nothing waits for the GPU."""
+        return self._readout(self._execute_steps(p), p['ro'])
 
     def _finish_pass(self, req, p):
         """What a finished pass leaves in the request: the sequences read, the nodes whose K/V are now kept, and in
@@ -497,24 +556,133 @@ class LeanGemma4:
         """Label probabilities of sequences `seqs` of `req`, computing only the nodes it has not kept yet
         (`lean_core.py:495-576`): one list per sequence, in order, each the softmax over that sequence's labels."""
         p = self.prepare_pass(req, seqs, available)
+        flat, = self._timed_pass(p, lambda: (self.execute_pass(p),))
+        bounds = np.cumsum([0] + [len(ids) for ids in p['labels']])
+        out = [flat[a:b].astype(np.float64).tolist() for a, b in zip(bounds[:-1], bounds[1:])]
+        self._finish_pass(req, p)
+        return out
+
+    def _timed_pass(self, p, execute):
+        """Run `execute` (launches only, returning device tensors) between two events, copy its results to the host and
+        check the device error word; sets the attributes the adapter reads after a pass."""
         self.last_need = p['need']
         self.timing = {'host_setup_ms': p['host_ms'], 'steps': len(p['plan']['steps']), 'tokens': p['tokens']}
         start, end = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
         start.record()
-        probs = self.execute_pass(p)
+        results = execute()
         end.record()
-        self.enqueued = time.perf_counter()  # every launch queued; the copy below waits for the GPU
-        flat = probs.cpu().numpy()
-        self.d2h_bytes = flat.nbytes
+        self.enqueued = time.perf_counter()  # every launch queued; the copies below wait for the GPU
+        host = [t.cpu().numpy() if t is not None else None for t in results]
+        self.d2h_bytes = sum(a.nbytes for a in host if a is not None)
         code = nat.device_error(self._stream())
         if self.peer is not None:
             code = self.peer.end_pass(code)
         if code:
             raise nat.NativeFailure(f'a kernel reported device error 0x{code:x}')
-        bounds = np.cumsum([0] + [len(ids) for ids in p['labels']])
-        out = [flat[a:b].astype(np.float64).tolist() for a, b in zip(bounds[:-1], bounds[1:])]
         self.gpu_ms = self.timing['gpu_ms'] = start.elapsed_time(end)
+        return host
+
+    # ---- log-probabilities under the whole vocabulary (no counterpart in the reference) ------------------------------
+    def _vocab_logprobs(self, reads, index, targets, top):
+        """Log-probabilities (`morj_b200.logprobs`) of the residual rows `reads[index]` after the final norm."""
+        from .logprobs import token_logprobs
+        n, H, s = len(index), self.hidden, self._stream()
+        rows = torch.empty(n, H, dtype=torch.bfloat16, device=self.device)
+        self._k('rows', 'morj_gather_rows', reads.data_ptr(), H, index.data_ptr(), n, H, rows.data_ptr(), H, s)
+        h = torch.empty_like(rows)
+        self._k('rows', 'morj_rmsnorm_rows', rows.data_ptr(), self.norm.data_ptr(), n, H, self.eps, h.data_ptr(), s)
+        self.launches += 2 * -(-n // 2048)
+        return token_logprobs(h, self.embed, targets, top=top, softcap=self.softcap or 0.0)
+
+    def _check_scoring(self, req, seqs, top):
+        if not 0 <= top <= 32:
+            raise ValueError(f'top {top} must be in [0, 32]')
+        if not seqs or any(not 0 <= b < req.n_real for b in seqs):
+            raise ValueError(f'sequences {list(seqs)} of a request of {req.n_real}')
+
+    def _check_ids(self, ids):
+        if len(ids) and (min(ids) < 0 or max(ids) >= self.embed.shape[0]):
+            raise ValueError('a token or label id is outside the vocabulary')
+
+    @torch.inference_mode()
+    def label_logprobs(self, req, seqs, top=0, available=None):
+        """The readout of `run` under the whole vocabulary: for each sequence a dict with `logprob` (of its label ids, in
+        order; the softmax of these is what `run` returns), `lse`, `entropy` (nats) of the next-token distribution and,
+        with `top` > 0 (at most 32), `top_ids` and `top_logprobs`."""
+        self._check_scoring(req, seqs, top)
+        for b in seqs:
+            self._check_ids(req.label_ids[b])
+        p = self.prepare_pass(req, seqs, available)
+        targets = np.full((len(seqs), max(len(ids) for ids in p['labels'])), -1, np.int32)
+        for row, ids in zip(targets, p['labels']):
+            row[:len(ids)] = ids
+        targets = torch.from_numpy(targets).to(self.device)
+        host = self._timed_pass(p, lambda: self._vocab_logprobs(self._execute_steps(p), p['ro']['t']['seq_row'], targets,
+                                                                top))
         self._finish_pass(req, p)
+        out = []
+        for i, ids in enumerate(p['labels']):
+            out.append(dict(logprob=host[0][i, :len(ids)], lse=float(host[1][i]), entropy=float(host[2][i])))
+            if top:
+                out[-1].update(top_ids=host[3][i], top_logprobs=host[4][i])
+        return out
+
+    def _scored_rows(self, req, seqs, plan, scored):
+        """The (step, row) of every row that predicts a scored token, in the order of `seqs` and their tokens; fills
+        `scored` with each sequence's first scored token. The row of token t predicts token t + 1."""
+        place = {}
+        for k, st in enumerate(plan['steps']):
+            place.update((int(o), (k, r)) for r, o in enumerate(st['own']))
+        rows = []
+        for i, b in enumerate(seqs):
+            path = [int(o) for n in req.tree.paths[b] for o in req.tree.slots(n)][:len(req.tree.seqs[b])]
+            first = scored[i]
+            if first is None:  # the first token from which on every predecessor is computed in this pass
+                first = len(path)
+                while first > 1 and path[first - 2] in place:
+                    first -= 1
+            if not 1 <= first <= len(path):
+                raise ValueError(f'sequence {b} has tokens 1..{len(path) - 1} to score, not from {first}')
+            missing = next((t for t in range(first, len(path)) if path[t - 1] not in place), None)
+            if missing is not None:
+                raise ValueError(f'token {missing} of sequence {b} is predicted by a row that an earlier pass computed '
+                                 f'(its K/V are kept, its hidden state is not)')
+            scored[i] = first
+            rows += [place[o] for o in path[first - 1:len(path) - 1]]
+        if not rows:
+            raise ValueError('no token to score')
+        return rows
+
+    @torch.inference_mode()
+    def token_logprobs(self, req, seqs, start=None, top=0, available=None):
+        """Log-probabilities of the sequences' own tokens, each given the ones before it, in one pass over `seqs` of
+        `req` (computing what `run` would compute). `start`: per sequence the first token scored (at least 1; None, or
+        None for a sequence: the first one from which on this pass computes every predecessor). Returns per sequence a
+        dict of arrays over the tokens start..len-1: `tokens`, `logprob`, `lse`, `entropy` and, with `top` > 0,
+        `top_ids`, `top_logprobs`; and `start`. Tokens that sequences share are computed once. ValueError for a token
+        whose predecessor an earlier pass computed (kept K/V hold no hidden states)."""
+        self._check_scoring(req, seqs, top)
+        scored = list(start) if start is not None else [None] * len(seqs)
+        if len(scored) != len(seqs):
+            raise ValueError(f'{len(scored)} starts for {len(seqs)} sequences')
+        for b in seqs:
+            self._check_ids(req.tree.seqs[b])
+        p = self.prepare_pass(req, seqs, available, scored=scored)
+        row_of = {place: j for j, place in enumerate(sorted(set(p['plan']['readout'])))}
+        index = np.asarray([row_of[place] for place in p['plan']['readout']], np.int32)
+        tokens = [np.asarray(req.tree.seqs[b])[first:] for b, first in zip(seqs, scored)]
+        index, targets = (torch.from_numpy(a).to(self.device) for a in
+                          (index, np.concatenate(tokens).astype(np.int32)[:, None]))
+        host = self._timed_pass(p, lambda: self._vocab_logprobs(self._execute_steps(p), index, targets, top))
+        self._finish_pass(req, p)
+        out, at = [], 0
+        for first, toks in zip(scored, tokens):
+            rows = slice(at, at + len(toks))
+            at += len(toks)
+            got = dict(start=first, tokens=toks, logprob=host[0][rows, 0], lse=host[1][rows], entropy=host[2][rows])
+            if top:
+                got.update(top_ids=host[3][rows], top_logprobs=host[4][rows])
+            out.append(got)
         return out
 
     def _readout_tables(self, plan, labels):
@@ -557,7 +725,9 @@ class LeanGemma4:
         self.trace.append((kind, flops, e0, e1))
 
     # ---- forward over one step ------------------------------------------------------------------------------------
-    def _step_tables(self, k, st, plan, req):
+    def _step_tables(self, k, st, plan, req, pool_slots, prune=True):
+        """A step's device tables, its readout rows, and what the launches need of the host: per kind (and 'ro', the
+        readout rows) the number of attention work items (8-bit pools: the call's counts and the store's blocks)."""
         t = _Tables(self.device)
         n = len(st['tokens'])
         t.add('tokens', st['tokens'])
@@ -571,17 +741,22 @@ class LeanGemma4:
         n_work = {}
         for kk, kind in (('s', 'sliding_attention'), ('g', 'full_attention')):
             sliding = kind == 'sliding_attention'
-            w = nat.attention_work(qo, st['kv_indptr_' + kk], int(st['n_bidir']) if sliding else 0, self.hq,
-                                   self.geom[kind][0], self.window if sliding else 0)
+            w, n_work[kk] = self._attention_work(qo, st['kv_indptr_' + kk], int(st['n_bidir']) if sliding else 0, kind)
             t.add('work_' + kk, w)
-            n_work[kk] = len(w) // 2
+            if self.kv8:
+                w, n_work['store_' + kk] = nat.kv8_store_work(st['slots'][kk], pool_slots[kk])
+                t.add('store_' + kk, w)
+        if self.kv8:
+            t.add('rows', np.arange(n))
         if req.features is not None:
             t.add('feature_row', req.blocks.feature_rows(st['tokens'], st['positions'], self.image_id))
         # readout rows of this step and the last layer's tables for them: each row attends to its segment's path up
         # to and including itself (reference `lean_core.py:713-727`)
         rows = sorted({r for kk, r in plan['readout'] if kk == k})
         last_kind = KINDS[self.types[-1]]
-        if rows:
+        if rows and not prune:
+            t.add('ro_rows', rows)
+        elif rows:
             seg = np.searchsorted(st['qo_indptr'], rows, side='right') - 1
             ind, ptr = [], [0]
             for row, sg in zip(rows, seg):
@@ -594,14 +769,19 @@ class LeanGemma4:
             t.add('ro_qo', np.arange(len(rows) + 1))
             t.add('ro_kv_indptr', ptr)
             t.add('ro_kv_indices', np.concatenate(ind))
-            last_sliding = self.types[-1] == 'sliding_attention'
-            ro_work = nat.attention_work(np.arange(len(rows) + 1), ptr, 0, self.hq, self.geom[self.types[-1]][0],
-                                         self.window if last_sliding else 0)
+            ro_work, n_work['ro'] = self._attention_work(np.arange(len(rows) + 1), ptr, 0, self.types[-1])
             t.add('ro_work', ro_work)
-            n_work['ro'] = len(ro_work) // 2
         t.upload()
         self.h2d_bytes += t.nbytes
         return t, rows, n_work
+
+    def _attention_work(self, qo, kv_indptr, n_bidir, kind):
+        """(work list, number of items, or the counts an 8-bit call takes) of one layer kind's attention call."""
+        window = self.window if kind == 'sliding_attention' else 0
+        if self.kv8:
+            return nat.kv8_attention_work(qo, kv_indptr, n_bidir, self.hq, self.geom[kind][0], window)
+        w = nat.attention_work(qo, kv_indptr, n_bidir, self.hq, self.geom[kind][0], window)
+        return w, len(w) // 2
 
     def _gemm(self, a, w, out, epi=nat.EPI_STORE, w_rows=None, w_offset_rows=0):
         M, K = a.shape
@@ -684,10 +864,28 @@ class LeanGemma4:
                 k_pool.shape[0], out.data_ptr(), t.ptr(qo), t.ptr(kv_indptr), t.ptr(kv_indices), None, n_seg, n_bidir,
                 self.hq, hk, d, 1, window, 1.0, t.ptr(work), n_work, self._stream())
 
-    def _step(self, k, st, plan, pools, head, req, tables, out):
+    def _store8(self, pool, staged, t, n_work, kk):
+        """A step's staged BF16 K/V rows into the layer's 8-bit pool."""
+        (k, v), hk, d = staged, pool.heads, pool.head_dim
+        self._k('rows', 'morj_kv8_store', k.data_ptr(), hk * d, v.data_ptr(), hk * d, k.shape[0], hk, d,
+                t.ptr('store_' + kk), n_work['store_' + kk], pool.k.data_ptr(), pool.k_scale.data_ptr(),
+                pool.v.data_ptr(), pool.v_scale.data_ptr(), pool.slots, self._stream())
+
+    def _attention8(self, q, pool, out, t, qo, kv_indptr, kv_indices, n_seg, n_bidir, kind, work, counts):
+        """`_attention` over an 8-bit pool."""
+        window = self.window if kind == 'sliding_attention' else 0
+        nbytes = nat.kv8_attention_workspace(counts, pool.heads, pool.head_dim)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
+        self._k('attention', 'morj_tree_attention_kv8', q.data_ptr(), q.shape[0], pool.k.data_ptr(),
+                pool.k_scale.data_ptr(), pool.v.data_ptr(), pool.v_scale.data_ptr(), pool.slots, out.data_ptr(),
+                t.ptr(qo), t.ptr(kv_indptr), t.ptr(kv_indices), None, n_seg, n_bidir, self.hq, pool.heads,
+                pool.head_dim, 1, window, 1.0, t.ptr(work), counts, _ptr(ws), nbytes, self._stream())
+
+    def _step(self, k, st, plan, pools, head, req, tables, out, prune=None):
         """One forward over a planned step (`lean_core.py:599-694`): embedding and first norm, every full layer, the
         pruned last layer; the residual rows of the step's readout tokens go to `out` (rows in step-row order)."""
         t, rows, n_work = tables
+        prune = self.prune_last if prune is None else prune
         n = len(st['tokens'])
         H, hq = self.hidden, self.hq
         dev, bf = self.device, torch.bfloat16
@@ -706,7 +904,11 @@ class LeanGemma4:
         bufs = dict(x=x, h=h, q=torch.empty(n, hq * d_max, dtype=bf, device=dev),
                     attn=torch.empty(n, hq * d_max, dtype=bf, device=dev), o=torch.empty(n, H, dtype=bf, device=dev),
                     act=torch.empty(n, self.layers[0]['gu'].shape[0] // 2, dtype=bf, device=dev),
-                    nb=int(st['n_bidir']), n_seg=len(st['qo_indptr']) - 1)
+                    nb=int(st['n_bidir']), n_seg=len(st['qo_indptr']) - 1, prune=prune)
+        if self.kv8:  # the K/V rows on their way into an 8-bit pool
+            wide = max(hk * dd for hk, dd in self.geom.values())
+            bufs['staged'] = tuple(torch.empty(n, wide, dtype=bf, device=dev) for _ in 'kv')
+        head_plans = {}
         # one step without kept pools: one temporary pool per layer kind, rewritten by every layer of that kind
         temp = {} if pools is not None else {kind: self._kv_pool(kind, plan['cap'][KINDS[kind]])
                                              for kind in set(self.types)}
@@ -717,10 +919,12 @@ class LeanGemma4:
                 kv = pools[i]
             else:
                 kv = temp[kind]
+                if self.kv8:
+                    kv.clear()  # the previous layer's blocks are forgotten
                 if len(head):
-                    self._copy_head([kv], plan['slot_of'], head, layers=[i])
-            if i == last and self.prune_last:
-                self._last_layer(t, rows, n_work, self.layers[i], h, x, kv, out)
+                    self._copy_head([kv], plan['slot_of'], head, layers=[i], plans=head_plans)
+            if i == last and prune:
+                self._last_layer(t, rows, n_work, self.layers[i], h, x, kv, out, bufs.get('staged'))
                 return
             self._layer(i, t, n_work, kv, bufs)
         if rows:  # (no pruning) the readout rows' residual stream
@@ -734,20 +938,25 @@ class LeanGemma4:
         layer, kind = self.layers[i], self.types[i]
         hk, d = self.geom[kind]
         kk = KINDS[kind]
-        k_pool, v_pool = kv
         x, h, o, act = bufs['x'], bufs['h'], bufs['o'], bufs['act']
         n, H, hq, eps, s = x.shape[0], self.hidden, self.hq, self.eps, self._stream()
         sliding = kind == 'sliding_attention'
         q, attn = bufs['q'][:, :hq * d], bufs['attn'][:, :hq * d]
-        self._qkv(h, layer, 0, n, hq, hk, int(sliding), d, kind, t.ptr('positions'), t.ptr('slots_' + kk), q,
-                  k_pool, v_pool)
-        self._attention(q, k_pool, v_pool, attn, t, 'qo', 'kv_indptr_' + kk, 'kv_indices_' + kk, bufs['n_seg'],
-                        bufs['nb'] if sliding else 0, kind, 'work_' + kk, n_work[kk])
+        tables = (t, 'qo', 'kv_indptr_' + kk, 'kv_indices_' + kk, bufs['n_seg'], bufs['nb'] if sliding else 0, kind,
+                  'work_' + kk, n_work[kk])
+        if self.kv8:
+            self._qkv(h, layer, 0, n, hq, hk, int(sliding), d, kind, t.ptr('positions'), t.ptr('rows'), q,
+                      *bufs['staged'])
+            self._store8(kv, bufs['staged'], t, n_work, kk)
+            self._attention8(q, kv, attn, *tables)
+        else:
+            self._qkv(h, layer, 0, n, hq, hk, int(sliding), d, kind, t.ptr('positions'), t.ptr('slots_' + kk), q, *kv)
+            self._attention(q, *kv, attn, *tables)
         last = len(self.layers) - 1
         nxt = self.layers[i + 1]['in_ln'] if i < last else layer['in_ln']
         if self.peer is not None:
             # x rows go back to every rank once, after the last full layer (the readout gathers them)
-            final = i == last - 1 if self.prune_last else i == last
+            final = i == last - 1 if bufs.get('prune', self.prune_last) else i == last
             self._peer_site(attn, layer['o'], 0, n, layer['post_attn'], None, layer['pre_ff'], 1, 0)
             self._gemm(h, layer['gu'], act, nat.EPI_GEGLU)
             self._peer_site(act, layer['down'], 1, n, layer['post_ff'], layer['scalar'], nxt, int(i < last),
@@ -763,7 +972,7 @@ class LeanGemma4:
         self._k('rows', 'morj_mlp_epilogue', o.data_ptr(), x.data_ptr(), h.data_ptr(), layer['post_ff'].data_ptr(),
                 layer['scalar'].data_ptr(), nxt.data_ptr(), n, H, eps, int(i < last), s)
 
-    def _last_layer(self, t, rows, n_work, layer, h, x, kv, xr):
+    def _last_layer(self, t, rows, n_work, layer, h, x, kv, xr, staged=None):
         """Last layer (`lean_core.py:696-737`): K/V of every token (later readouts attend to them), then q,
         attention, O and MLP for the readout rows only; their residual rows end in `xr`."""
         s = self._stream()
@@ -772,12 +981,13 @@ class LeanGemma4:
         kind = self.types[-1]
         hk, d = self.geom[kind]
         kk = KINDS[kind]
-        k_pool, v_pool = kv
         has_v = int(kind == 'sliding_attention')
         dev, bf = self.device, torch.bfloat16
         qd = hq * d
-        self._qkv(h, layer, qd, n, 0, hk, has_v, d, kind, t.ptr('positions'), t.ptr('slots_' + kk), None, k_pool,
-                  v_pool)
+        self._qkv(h, layer, qd, n, 0, hk, has_v, d, kind, t.ptr('positions'),
+                  t.ptr('rows' if self.kv8 else 'slots_' + kk), None, *(staged if self.kv8 else kv))
+        if self.kv8:
+            self._store8(kv, staged, t, n_work, kk)
         if not rows:
             return
         R = len(rows)
@@ -786,8 +996,11 @@ class LeanGemma4:
         q = torch.empty(R, qd, dtype=bf, device=dev)
         self._qkv(hr, layer, 0, R, hq, 0, has_v, d, kind, t.ptr('ro_positions'), None, q, None, None)
         attn = torch.empty(R, qd, dtype=bf, device=dev)
-        self._attention(q, k_pool, v_pool, attn, t, 'ro_qo', 'ro_kv_indptr', 'ro_kv_indices', R, 0, kind, 'ro_work',
-                        n_work['ro'])
+        tables = (t, 'ro_qo', 'ro_kv_indptr', 'ro_kv_indices', R, 0, kind, 'ro_work', n_work['ro'])
+        if self.kv8:
+            self._attention8(q, kv, attn, *tables)
+        else:
+            self._attention(q, *kv, attn, *tables)
         o = torch.empty(R, H, dtype=bf, device=dev)
         self._gemm(attn, layer['o'], o)
         self._reduce(o)
