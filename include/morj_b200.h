@@ -229,14 +229,14 @@ int morj_kv8_gather(const void* codes, const float* scale, int pool_slots, const
                     void* out, long long ld_out, void* stream);
 
 /* morj_tree_attention over an 8-bit cache: the same segments, key lists, masks and head groups, K and V read as
- * code * scale. q, out: [n_q, hq, d] BF16. A query that sees no key gets 0. Any hq / hk; d in {64, 128}; the last page
+ * code * scale. q, out: [n_q, hq, d] BF16; sm_scale > 0. A query that sees no key gets 0. Any hq / hk; d in {64, 128}; the last page
  * of a segment with no pages is ignored. Keys outside every query's view are not read; a listed key's codes must be
  * finite (as morj_kv8_store leaves them) where some query of the same tile does not see it. A slot outside the pool
  * sets the device error word (0x301).
  *
  * morj_tree_attention_kv8_work (host function, no device access): the call's work list from host copies of its segment
- * tables. Writes up to `cap` ints to work_host and counts[8]: counts[0..2] = row tiles, joins, partial units,
- * counts[3] = rows per tile, counts[4] = ints written. With cap = 0 it writes only the counts. Long key lists of few
+ * tables. Writes up to `cap` ints to work_host and counts[8]: counts[0..3] = tiles of few rows, joins, partial units,
+ * rows per such tile, counts[4] = ints written, counts[5] = 128-row tiles. With cap = 0 it writes only the counts. Long key lists of few
  * tiles are cut into parts, whose partial results go through `workspace` (counts[2] * hk * 16 * (d + 2) * 4 bytes, the
  * caller's, 16-byte aligned; calls that may overlap on the device must not share it) and are joined in a fixed order.
  * `work`: the device copy of the list (16-byte aligned); `counts`: the host array. */

@@ -14,7 +14,7 @@ constexpr int BLOCK = 64;            // slots that share a scale
 constexpr int BLOCK_SHIFT = 6;
 constexpr int MIN_EXP = -100;        // the smallest scale is 2^-100
 
-// two e4m3 codes (low byte first) as FP16 values; exact (e4m3's range and precision lie inside FP16's)
+// the two e4m3 codes in the low half of `two` (low byte first) as FP16 values; exact (e4m3's range and precision lie inside FP16's)
 MORJ_DEV uint32_t codes2_f16(uint32_t two) {
   uint32_t r;
   asm("{\n\t.reg .b16 t;\n\tcvt.u16.u32 t, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, t;\n\t}" : "=r"(r) : "r"(two));

@@ -10,7 +10,11 @@
 // [1, 2) by a power of two before it is rounded to FP16, which keeps every bit of a BF16 row that matters at 2^-25 of
 // its largest element.
 //
-// rows_kernel: tiles of 8 or 16 rows (a segment's (query, head) pairs of one KV head), for the single-token form. Every
+// A segment's rows are its (query, head of the group) pairs of one KV head. tile_kernel takes 128 rows at a time on
+// tcgen05; rows_kernel takes 8 or 16, for the single-token form (segments of at most 16 rows), where the codes' bytes
+// bound the call and 128-row tiles would be almost empty.
+//
+// rows_kernel: every
 // warp walks its own groups of 32 keys with mma.m16n8k16, operands straight from global memory: the fragment layouts
 // leave the order of the head dimension (QK) and of the output columns (PV) free, so each lane reads 16 or 32
 // consecutive codes of a key. The host cuts the keys of a tile into parts until the SMs are filled; parts leave
@@ -28,6 +32,9 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int UNIT = 16;             // rows of a partial unit in the workspace
 constexpr int WARPS = 4;
 constexpr int STEP = 32;             // keys a warp takes at a time
+constexpr int FEW_ROWS = 16;         // segments of at most this many rows go to rows_kernel
+constexpr int T_CTAS = 2, T_MIN_KEYS = 256;  // resident CTAs per SM and keys of a part worth one: tile_kernel
+constexpr int R_CTAS = 4, R_MIN_KEYS = 256;  // ... rows_kernel
 constexpr float P_SCALE = 1024.0f;   // probabilities are rounded to FP16 as 1024 p: 2^-34 is their smallest step
 
 struct Item {
@@ -49,7 +56,7 @@ struct Args {
   const int* kv_indptr;
   const int* kv_indices;
   const int* kv_last_page_len;
-  int n_bidir, hq, hk, page_size, window, pool_slots;
+  int n_bidir, hq, hk, page_size, page_shift, window, pool_slots;  // page_shift: log2 of the page size, -1: none
   float scale_log2;
   float* ws;
 };
@@ -82,10 +89,16 @@ __host__ __device__ inline void visible(int q_len, int kv_len, bool bidir, int w
   if (*lo < 0) *lo = 0;
 }
 
+// pages of a segment's keys; division only where the page size is no power of two
+MORJ_DEV int page_of(const Args& a, int t) { return a.page_shift >= 0 ? t >> a.page_shift : t / a.page_size; }
+MORJ_DEV long long slot_of(const Args& a, int entry, int t) {
+  return a.page_shift >= 0 ? ((long long)entry << a.page_shift) + (t & (a.page_size - 1))
+                           : (long long)entry * a.page_size + t % a.page_size;
+}
+
 // pool slot of key t of a segment, -1 (device error recorded) outside the pool
 MORJ_DEV int key_slot(const Args& a, int kv_base, int t) {
-  const long long page = __ldg(a.kv_indices + kv_base + (a.page_size == 1 ? t : t / a.page_size));
-  const long long slot = a.page_size == 1 ? page : page * a.page_size + t % a.page_size;
+  const long long slot = slot_of(a, __ldg(a.kv_indices + kv_base + page_of(a, t)), t);
   if (slot < 0 || slot >= a.pool_slots) {
     report(kErrBadIndex);
     return -1;
@@ -362,6 +375,525 @@ __global__ void __launch_bounds__(WARPS * 32) rows_kernel(const Args a, const It
   }
 }
 
+// ---------------------------------------------------------------------------------------------------------------
+// tile_kernel: 128 rows of a segment and KV head against 64 keys at a time, on tcgen05 (FP16 x FP16, FP32 in TMEM).
+//   warps 0-3   softmax (thread = row): prologue (Q row to FP16 and shared memory), mask, online maximum and sum, P as
+//               FP16 over its own scores in TMEM, the final O / l or the part's (maximum, sum, O)
+//   warp 4      MMA issuer (one thread): S_c = Q K_c^T into TMEM buffer c % 2, O += P_c V_c with P read from TMEM
+//   warps 5-6   K: a chunk's codes from global memory to registers one chunk ahead, converted to FP16 into the
+//               swizzled operand tile, with the keys' scales for the softmax
+//   warps 7-8   the same for V
+// The pipeline is tree_attention_kernel's (S and P double-buffered in TMEM, K buffer free once its S is complete, V
+// buffer once its P V is); its loaders issued TMA copies, these convert. The conversion is one instruction for two
+// codes and runs on warps of its own: 16,384 codes a chunk are about 260 conversions and 200 loads and stores per
+// CTA beside the softmax's 2,000 instructions.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int T_ROWS = 128;
+constexpr int BN = 64;
+constexpr int T_THREADS = 288;
+constexpr int T_TMEM_COLS = 256;      // S/P buffers at columns [0, 64) and [64, 128), O at [128, 128 + D)
+constexpr float T_RESCALE_LOG2 = 4.0f;  // O is rescaled when a row's maximum grows by more than 2^4, so that
+constexpr float T_P_SCALE = 2048.0f;    // 2^11 p <= 2^15 stays inside FP16
+
+template <int D>
+struct TSmem {
+  static constexpr int Q_BYTES = T_ROWS * D * 2;
+  static constexpr int KV_BYTES = BN * D * 2;
+  static constexpr int K_OFF = Q_BYTES;               // 2 buffers
+  static constexpr int V_OFF = K_OFF + 2 * KV_BYTES;  // 2 buffers
+  static constexpr int META_OFF = V_OFF + 2 * KV_BYTES;
+  // scales of a chunk's keys: K [4][64] (chunk c + 4's are written once S_{c+2} is complete, after softmax c), V [2][64];
+  // then per half chunk (32 keys) K [4][2] the common scale or -1, V [2][2] the same and [2][2] the largest
+  static constexpr int KF = 0, VF = 4 * 64, KU = VF + 2 * 64, VU = KU + 8, VM = VU + 4, META_FLOATS = VM + 4;
+  static constexpr int BAR_OFF = META_OFF + META_FLOATS * 4 + 16;
+  // barriers: q_full, k_full[2], v_full[2], meta_full[4], s_full[2], p_full[2], pv_done[2], done; TMEM slot, abort flag
+  static constexpr int TOTAL = (BAR_OFF + 16 * 8 + 16 + 15) / 16 * 16;
+  static_assert(BAR_OFF % 8 == 0 && META_OFF % 16 == 0, "alignment");
+};
+
+__host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn_major = false) {
+  return (1u << 4)  // D: FP32; A and B: FP16 (0)
+         | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
+}
+
+// 32 lanes x 16 consecutive 32-bit columns from registers into TMEM
+MORJ_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+MORJ_DEV uint64_t f2_pack(float lo, float hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+  return r;
+}
+MORJ_DEV uint64_t f2_bits(uint32_t lo, uint32_t hi) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+  return r;
+}
+MORJ_DEV void f2_unpack(uint64_t v, float& lo, float& hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+MORJ_DEV uint64_t f2_fma(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+MORJ_DEV uint64_t f2_add(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+MORJ_DEV float max3f(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+MORJ_DEV void sts16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// warp-level wait: lane 0 polls the barrier, the warp follows its verdict (and sees what lane 0 sees)
+MORJ_DEV bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+  int ok = (threadIdx.x & 31) == 0 ? (int)mbar_wait(bar, parity, abort, kErrTimeoutAttention) : 0;
+  ok = __shfl_sync(0xffffffffu, ok, 0);
+  __syncwarp();
+  return ok != 0;
+}
+
+// One loader warp: keys [32 * part, + 32) of every chunk of one pool (K or V). A lane looks one key's page entry up two
+// chunks ahead and loads its scale one ahead, with its share of the codes: 16 of them from every fourth row (D = 128),
+// so no load waits on another. Lanes are dealt to (row, piece) such that eight consecutive ones store to eight
+// different 16-byte units of the swizzled tile.
+template <int D, bool IS_K>
+MORJ_DEV void load_side(const Args& a, const Seg& sg, const Item& it, int h, int t_begin, int n_chunks, int part,
+                        uint32_t tiles, uint32_t full, uint32_t empty, uint32_t meta_full, float* meta, volatile int* abort) {
+  using L = TSmem<D>;
+  constexpr int LPR = D / 16;        // lanes per row, 16 codes each
+  constexpr int RPI = 32 / LPR;      // rows per load instruction
+  constexpr int NI = 32 / RPI;       // load instructions per chunk
+  const int lane = threadIdx.x & 31;
+  // D = 128: lane bits (half of the row, row, row 2, piece, piece) -> row 0..3, piece 0..7
+  const int piece = LPR == 8 ? (lane & 3) | ((lane >> 3) & 1) << 2 : lane & 3;
+  const int sub = LPR == 8 ? ((lane >> 2) & 1) | (lane >> 4) << 1 : lane >> 2;
+  const uint8_t* codes = (IS_K ? a.k : a.v) + (size_t)h * D + piece * 16;
+  const float* scales = (IS_K ? a.ks : a.vs) + h;
+  const size_t row_bytes = (size_t)a.hk * D;
+  const int t_end = min(it.t1, sg.kv_len);
+  const int* list = a.kv_indices + sg.kv_base;
+  const int t_lane = t_begin + part * 32 + lane;
+  auto entry = [&](int c) {  // (a key outside the part reads the entry of the nearest key inside it)
+    return __ldg(list + page_of(a, max(it.t0, min(t_lane + c * BN, t_end - 1))));
+  };
+  int slot;  // this lane's key of a chunk: pool slot, -1: none
+  float sc;
+  uint4 w[NI];
+  auto fetch = [&](int c, int e) {
+    const int t = t_lane + c * BN;
+    const long long s64 = slot_of(a, e, max(it.t0, min(t, t_end - 1)));
+    const bool in_pool = s64 >= 0 && s64 < a.pool_slots;
+    if (!in_pool) report(kErrBadIndex);
+    const int from = in_pool ? (int)s64 : 0;
+    slot = t >= it.t0 && t < t_end && in_pool ? from : -1;
+    sc = __ldg(scales + (size_t)(from >> BLOCK_SHIFT) * a.hk);
+#pragma unroll
+    for (int i = 0; i < NI; ++i)
+      w[i] = __ldg(reinterpret_cast<const uint4*>(
+          codes + (size_t)__shfl_sync(0xffffffffu, from, i * RPI + sub) * row_bytes));
+  };
+  if (n_chunks == 0) return;
+  fetch(0, entry(0));
+  int e_next = entry(1);
+  for (int c = 0; c < n_chunks; ++c) {
+    const int b = c & 1;
+    // a K buffer is free once the scores of the chunk two back are complete, a V buffer once its P V is
+    if (c >= 2 && !warp_wait(empty + 8 * b, ((c >> 1) - 1) & 1, abort)) return;
+    // the keys' scales: all of them, and the common one when the valid keys agree
+    const unsigned valid = __ballot_sync(0xffffffffu, slot >= 0);
+    if (slot < 0) sc = 0.f;
+    const float first = __shfl_sync(0xffffffffu, sc, valid ? __ffs(valid) - 1 : 0);
+    const bool same = __all_sync(0xffffffffu, slot < 0 || sc == first);
+    if constexpr (IS_K) {
+      meta[L::KF + (c & 3) * 64 + part * 32 + lane] = sc;
+      if (lane == 0) meta[L::KU + (c & 3) * 2 + part] = same ? first : -1.f;
+    } else {
+      float big = same ? first : sc;
+      if (!same) {
+#pragma unroll
+        for (int x = 16; x > 0; x >>= 1) big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, x));
+      }
+      meta[L::VF + b * 64 + part * 32 + lane] = sc;
+      if (lane == 0) meta[L::VU + b * 2 + part] = same ? first : -1.f, meta[L::VM + b * 2 + part] = big;
+    }
+    if (valid != 0xffffffffu) {  // a key that is not there is zeros
+#pragma unroll
+      for (int i = 0; i < NI; ++i)
+        if (!((valid >> (i * RPI + sub)) & 1)) w[i] = make_uint4(0, 0, 0, 0);
+    }
+    const uint32_t base = tiles + b * L::KV_BYTES + (piece >> 2) * (BN * 128);
+    const int u0 = (piece & 3) * 2;
+#pragma unroll
+    for (int i = 0; i < NI; ++i) {
+      const int r = part * 32 + i * RPI + sub;
+      sts16(base + sw128_offset(r, u0), codes2_f16(w[i].x), codes2_f16(w[i].x >> 16), codes2_f16(w[i].y),
+            codes2_f16(w[i].y >> 16));
+      sts16(base + sw128_offset(r, u0 + 1), codes2_f16(w[i].z), codes2_f16(w[i].z >> 16), codes2_f16(w[i].w),
+            codes2_f16(w[i].w >> 16));
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      mbar_arrive(full + 8 * b);
+      if constexpr (IS_K) mbar_arrive(meta_full + 8 * (c & 3));
+    }
+    if (c + 1 < n_chunks) {
+      fetch(c + 1, e_next);  // in flight while the next buffer is waited for
+      e_next = entry(c + 2);
+    }
+  }
+}
+
+template <int D>
+__global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const Item* __restrict__ items) {
+  pdl_wait();  // the previous kernel on the stream has completed
+  pdl_trigger();
+  using L = TSmem<D>;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t sbase = smem_u32(smem);
+  if (sbase & 1023) {  // the swizzled operand tiles need 1024-byte alignment
+    if (threadIdx.x == 0) report(kErrBadAlignment);
+    return;
+  }
+  const uint32_t bar0 = sbase + L::BAR_OFF;
+  const uint32_t q_full = bar0, k_full = bar0 + 8, v_full = bar0 + 24, meta_full = bar0 + 40;
+  const uint32_t s_full = bar0 + 72, p_full = bar0 + 88, pv_done = bar0 + 104, done = bar0 + 120;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::BAR_OFF + 128);
+  volatile int* abort = reinterpret_cast<volatile int*>(smem + L::BAR_OFF + 132);
+  float* meta = reinterpret_cast<float*>(smem + L::META_OFF);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const Item it = items[blockIdx.x / a.hk];
+  const int h = blockIdx.x % a.hk;
+  const Seg sg = load_segment(a, it.seg);
+  const int G = a.hq / a.hk, n_rows = sg.q_len * G;
+  const bool bidir = it.seg < a.n_bidir;
+  const int t_begin = it.t0 - it.t0 % BN;  // chunks line up with 64-slot pages
+  const int t_stop = min(it.t1, sg.kv_len);
+  const int n_chunks = t_stop > it.t0 ? (t_stop - t_begin + BN - 1) / BN : 0;
+
+  if (threadIdx.x == 0) {
+    mbar_init(q_full, 4);
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(k_full + 8 * b, 2);  // one arrival per loader warp
+      mbar_init(v_full + 8 * b, 2);
+      mbar_init(s_full + 8 * b, 1);
+      mbar_init(p_full + 8 * b, 4);  // one arrival per softmax warp
+      mbar_init(pv_done + 8 * b, 1);
+    }
+    for (int b = 0; b < 4; ++b) mbar_init(meta_full + 8 * b, 2);
+    mbar_init(done, 1);
+    *abort = 0;
+    fence_mbar_init();
+  }
+  if (warp == 4) {
+    tmem_alloc(smem_u32(tmem_slot), T_TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp >= 7) {
+    load_side<D, false>(a, sg, it, h, t_begin, n_chunks, warp - 7, sbase + L::V_OFF, v_full, pv_done, 0, meta, abort);
+  } else if (warp >= 5) {
+    load_side<D, true>(a, sg, it, h, t_begin, n_chunks, warp - 5, sbase + L::K_OFF, k_full, s_full, meta_full, meta,
+                       abort);
+  } else if (warp == 4) {
+    if (lane == 0) {
+      constexpr uint32_t IDESC_S = idesc_f16(T_ROWS, BN);
+      constexpr uint32_t IDESC_O = idesc_f16(T_ROWS, D, /*b_mn_major=*/true);
+      bool ok = n_chunks > 0 && mbar_wait(q_full, 0, abort, kErrTimeoutAttention);
+      // operand descriptors: one per buffer, advanced per 16-deep K step by the byte offset (>> 4)
+      const uint64_t q_desc = sw128_desc(sbase);
+      const uint64_t k_desc0 = sw128_desc(sbase + L::K_OFF), v_desc0 = sw128_desc(sbase + L::V_OFF, BN * 128);
+      constexpr uint64_t KV_STEP = L::KV_BYTES >> 4;
+      auto issue_qk = [&](int c) -> bool {
+        const int b = c & 1;
+        if (!mbar_wait(k_full + 8 * b, (c >> 1) & 1, abort, kErrTimeoutAttention)) return false;
+        tc_fence_after();
+        const uint64_t k_desc = k_desc0 + b * KV_STEP;
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t qa = ((kk >> 2) * (T_ROWS * 128) + (kk & 3) * 32) >> 4;
+          const uint32_t kb = ((kk >> 2) * (BN * 128) + (kk & 3) * 32) >> 4;
+          umma_bf16(tmem + b * BN, q_desc + qa, k_desc + kb, IDESC_S, kk > 0);  // (kind::f16: the types are in IDESC)
+        }
+        umma_commit(s_full + 8 * b);
+        return true;
+      };
+      if (ok) ok = issue_qk(0);
+      if (ok && n_chunks > 1) ok = issue_qk(1);
+      for (int c = 0; c < n_chunks && ok; ++c) {
+        const int b = c & 1;
+        // O += P_c V_c, P_c from TMEM buffer b (packed FP16 pairs, 8 columns per 16 keys)
+        if (!mbar_wait(p_full + 8 * b, (c >> 1) & 1, abort, kErrTimeoutAttention) ||
+            !mbar_wait(v_full + 8 * b, (c >> 1) & 1, abort, kErrTimeoutAttention)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint64_t v_desc = v_desc0 + b * KV_STEP;
+#pragma unroll
+        for (int kk = 0; kk < BN / 16; ++kk)
+          umma_bf16_tmem_a(tmem + 128, tmem + b * BN + kk * 8, v_desc + kk * (2048 >> 4), IDESC_O, (c | kk) != 0);
+        umma_commit(pv_done + 8 * b);
+        if (c + 2 < n_chunks) ok = issue_qk(c + 2);  // in issue order after this PV, which reads P_c first
+      }
+      // TMEM is freed only after every MMA issued here has completed
+      umma_commit(done);
+      mbar_wait_landed(done, 0);
+    }
+  } else if (warp < 4) {
+    // ---------------- softmax warpgroup ----------------
+    const int r = warp * 32 + lane;
+    const uint32_t t_lane = tmem + ((uint32_t)(warp * 32) << 16);
+    const int row = it.r0 + r, qi = row / G;
+    const bool row_ok = row < n_rows;
+    const size_t row_at = ((size_t)(sg.q_start + qi) * a.hq + h * G + row % G) * D;
+    // Q row: its largest magnitude, then FP16 of q / qs into the swizzled tile
+    float qs;
+    {
+      // (read twice, the second time from L1: the row in registers would be 64 of them)
+      const uint4* src = reinterpret_cast<const uint4*>(a.q + row_at);
+      const uint4 zero = make_uint4(0, 0, 0, 0);
+      float amax = 0.f;
+#pragma unroll 4
+      for (int i = 0; i < D / 8; ++i) {
+        float x[8];
+        unpack8(row_ok ? __ldg(src + i) : zero, x);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
+      }
+      qs = row_scale(amax);
+      const float inv = 1.f / qs;
+#pragma unroll 4
+      for (int i = 0; i < D / 8; ++i) {
+        float x[8];
+        unpack8(row_ok ? __ldg(src + i) : zero, x);
+        sts16(sbase + (i >> 3) * (T_ROWS * 128) + sw128_offset(r, i & 7), pack_f16x2(x[0] * inv, x[1] * inv),
+              pack_f16x2(x[2] * inv, x[3] * inv), pack_f16x2(x[4] * inv, x[5] * inv),
+              pack_f16x2(x[6] * inv, x[7] * inv));
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(q_full);
+      qs *= a.scale_log2;
+    }
+    int lo = 1, hi = 0;  // visible key positions [lo, hi] of this part
+    if (row_ok) {
+      visible(sg.q_len, sg.kv_len, bidir, a.window, qi, &lo, &hi);
+      lo = max(lo, it.t0), hi = min(hi, it.t1 - 1);
+    }
+    float m_used = -INFINITY, l_run = 0.f;
+    float vref = 0.f, inv_v = 0.f;  // the largest V scale met (O is in units of vref / T_P_SCALE), T_P_SCALE / vref
+    bool ok = true;
+    for (int c = 0; c < n_chunks; ++c) {
+      const int b = c & 1;
+      int here = lane == 0 ? (int)(mbar_wait(meta_full + 8 * (c & 3), (c >> 2) & 1, abort, kErrTimeoutAttention) &&
+                                   mbar_wait(v_full + 8 * b, (c >> 1) & 1, abort, kErrTimeoutAttention) &&
+                                   mbar_wait(s_full + 8 * b, (c >> 1) & 1, abort, kErrTimeoutAttention))
+                           : 0;
+      here = __shfl_sync(0xffffffffu, here, 0);
+      __syncwarp();
+      if (!here) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      // scales of the two half chunks: K's multiply the scores, V's the probabilities
+      const float* kf = meta + L::KF + (c & 3) * 64;
+      const float* vf = meta + L::VF + b * 64;
+      const float2 ku = *reinterpret_cast<const float2*>(meta + L::KU + (c & 3) * 2);
+      const float2 vu = *reinterpret_cast<const float2*>(meta + L::VU + b * 2);
+      const float2 vm = *reinterpret_cast<const float2*>(meta + L::VM + b * 2);
+      const float vmax = max_nan(vm.x, vm.y);
+      float unit = 1.f;
+      if (!(vmax <= vref)) {
+        unit = vref / vmax;
+        vref = vmax;
+        inv_v = T_P_SCALE / vmax;
+      }
+      const int t0 = t_begin + c * BN;
+      const bool full = __all_sync(0xffffffffu, t0 >= lo && t0 + BN - 1 <= hi);
+      float cs[2] = {ku.x >= 0.f ? ku.x * qs : qs, ku.y >= 0.f ? ku.y * qs : qs};
+      cs[0] = cs[0] < 1.2e-38f ? 1.2e-38f : cs[0];  // (a masked score stays -inf times it)
+      cs[1] = cs[1] < 1.2e-38f ? 1.2e-38f : cs[1];
+      // Half a chunk's scores at a time, the first half read twice instead of kept (96 registers a thread): masked, and
+      // times their keys' scales where those differ. Scores times cs are in the log2 domain; cs > 0.
+      uint32_t sr[32];
+      auto scores = [&](int half) {
+        tmem_ld32(t_lane + b * BN + half * 32, sr);
+        tmem_wait_ld();
+        if ((half ? ku.y : ku.x) < 0.f) {
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(kf + half * 32 + j);
+            sr[j] = __float_as_uint(__uint_as_float(sr[j]) * f.x);
+            sr[j + 1] = __float_as_uint(__uint_as_float(sr[j + 1]) * f.y);
+            sr[j + 2] = __float_as_uint(__uint_as_float(sr[j + 2]) * f.z);
+            sr[j + 3] = __float_as_uint(__uint_as_float(sr[j + 3]) * f.w);
+          }
+        }
+        if (!full) {
+          const int first = lo - t0 - half * 32, last = hi - t0 - half * 32;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (j < first || j > last) sr[j] = 0xff800000u;  // -inf
+        }
+      };
+      auto largest = [&] {  // (over independent partials: short dependency chains)
+        float m4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) m4[i] = fmaxf(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1]));
+#pragma unroll
+        for (int j = 8; j < 32; j += 2)
+          m4[(j >> 1) & 3] = max3f(m4[(j >> 1) & 3], __uint_as_float(sr[j]), __uint_as_float(sr[j + 1]));
+        return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+      };
+      scores(1);
+      float mx = largest() * cs[1];
+      scores(0);
+      mx = fmaxf(mx, largest() * cs[0]);
+      float alpha = 1.f;
+      if (mx > m_used + T_RESCALE_LOG2 || m_used == -INFINITY) {
+        if (m_used != -INFINITY) alpha = fast_exp2(m_used - mx);
+        if (mx != -INFINITY) m_used = mx;
+      }
+      l_run *= alpha;
+      alpha *= unit;
+      // exp2(-inf) = 0 for masked keys; a row with no visible key yet keeps m_used = -inf and p = 0
+      const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        // probabilities go to TMEM times f = T_P_SCALE * scale / vref: as part of the exponent where the half chunk
+        // has one scale (the sum is divided by it again), else key by key
+        if (half == 1) scores(1);
+        const float f = (half ? vu.y : vu.x) * inv_v;
+        const bool fold = f >= 9.3e-10f;  // 2^-30: p f stays a normal FP32 number
+        const float lf = fold ? __log2f(f) : 0.f;
+        const uint64_t scale2 = f2_pack(cs[half], cs[half]), shift2 = f2_pack(neg_m + lf, neg_m + lf);
+        uint64_t s4[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s4[i] = f2_pack(0.f, 0.f);
+        uint32_t pk[16];
+        if (fold) {  // (the same for the whole CTA)
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            float x0, x1;
+            f2_unpack(f2_fma(f2_bits(sr[j], sr[j + 1]), scale2, shift2), x0, x1);
+            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+            s4[(j >> 1) & 3] = f2_add(s4[(j >> 1) & 3], f2_pack(p0, p1));
+            pk[j / 2] = pack_f16x2(p0, p1);
+          }
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            float x0, x1;
+            f2_unpack(f2_fma(f2_bits(sr[j], sr[j + 1]), scale2, shift2), x0, x1);
+            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+            s4[(j >> 1) & 3] = f2_add(s4[(j >> 1) & 3], f2_pack(p0, p1));
+            const float2 g = *reinterpret_cast<const float2*>(vf + half * 32 + j);
+            pk[j / 2] = pack_f16x2(p0 * (g.x * inv_v), p1 * (g.y * inv_v));
+          }
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          float x, y;
+          f2_unpack(s4[i], x, y);
+          sum += x + y;
+        }
+        l_run = fmaf(sum, fold ? fast_exp2(-lf) : 1.f, l_run);
+        tmem_st16(t_lane + b * BN + half * 16, pk);  // P_c over the first 32 columns of S_c (read already)
+      }
+      // a rescale of O waits until the previous chunk's PV has completed (the next one needs this chunk's P)
+      if (c >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
+        if (!warp_wait(pv_done + 8 * (b ^ 1), ((c - 1) >> 1) & 1, abort)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll 1
+        for (int col = 0; col < D; col += 32) {
+          uint32_t o[32];
+          tmem_ld32(t_lane + 128 + col, o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+          tmem_st32(t_lane + 128 + col, o);
+        }
+      }
+      tmem_wait_st();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full + 8 * b);
+    }
+    if (ok && (n_chunks == 0 || warp_wait(pv_done + 8 * ((n_chunks - 1) & 1), ((n_chunks - 1) >> 1) & 1, abort))) {
+      tc_fence_after();
+      const float back = vref * (1.f / T_P_SCALE);
+      if (it.unit < 0) {
+        const float inv = l_run == 0.f ? 0.f : back / l_run;
+#pragma unroll 1
+        for (int col = 0; col < D; col += 32) {
+          uint32_t o[32];
+          if (n_chunks) {
+            tmem_ld32(t_lane + 128 + col, o);
+            tmem_wait_ld();
+          }
+          if (row_ok) {
+#pragma unroll
+            for (int v8 = 0; v8 < 4; ++v8) {
+              float x[8];
+#pragma unroll
+              for (int e = 0; e < 8; ++e) x[e] = inv == 0.f ? 0.f : __uint_as_float(o[v8 * 8 + e]) * inv;
+              store8(a.out + row_at + col + v8 * 8, x);
+            }
+          }
+        }
+      } else {
+        float* part = a.ws + ((size_t)(it.unit + r / UNIT) * a.hk + h) * (UNIT * (D + 2));
+        if (row_ok) part[r % UNIT] = m_used, part[UNIT + r % UNIT] = l_run;
+        float4* dst = reinterpret_cast<float4*>(part + 2 * UNIT + (r % UNIT) * D);
+#pragma unroll 1
+        for (int col = 0; col < D; col += 32) {
+          uint32_t o[32];
+          if (n_chunks) {
+            tmem_ld32(t_lane + 128 + col, o);
+            tmem_wait_ld();
+          }
+          if (row_ok) {
+#pragma unroll
+            for (int v = 0; v < 8; ++v) {
+              float x[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) x[e] = back == 0.f ? 0.f : __uint_as_float(o[4 * v + e]) * back;
+              dst[col / 4 + v] = make_float4(x[0], x[1], x[2], x[3]);
+            }
+          }
+        }
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 4) {
+    tc_fence_after();
+    tmem_dealloc(tmem, T_TMEM_COLS);
+  }
+}
+
 // Joins the parts of one 16-row unit: o = sum_p 2^(m_p - m) O_p / sum_p 2^(m_p - m) l_p.
 template <int D>
 __global__ void __launch_bounds__(D) combine_kernel(const Args a, const Item* __restrict__ items) {
@@ -390,12 +922,31 @@ __global__ void __launch_bounds__(D) combine_kernel(const Args a, const Item* __
   }
 }
 
+// cudaFuncSetAttribute holds per device
+template <int D>
+static int configure_tile() {
+  static bool done[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev >= 64 || !done[dev])) {
+    e = cudaFuncSetAttribute(tile_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, TSmem<D>::TOTAL);
+    if (e == cudaSuccess && dev < 64) done[dev] = true;
+  }
+  return e == cudaSuccess ? MORJ_OK : set_error(MORJ_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
+}
+
 template <int D>
 static int launch(const Args& a, const int* counts, const int* work, cudaStream_t s) {
   const Item* items = reinterpret_cast<const Item*>(work);
-  const int n_rows = counts[0], n_combine = counts[1];
+  const int n_rows = counts[0], n_combine = counts[1], n_tiles = counts[5];
   int st = MORJ_OK;
-  if (n_rows) {
+  if (n_tiles) {
+    if ((st = configure_tile<D>())) return st;
+    st = launch_pdl("tile_kernel", tile_kernel<D>, dim3((unsigned)n_tiles * a.hk), dim3(T_THREADS), TSmem<D>::TOTAL, s,
+                    a, items);
+    items += n_tiles;
+  }
+  if (st == MORJ_OK && n_rows) {
     const dim3 grid((unsigned)n_rows * a.hk);
     st = counts[3] == 8
              ? launch_pdl("rows_kernel", rows_kernel<D, 8>, grid, dim3(WARPS * 32), 0, s, a, items)
@@ -405,6 +956,45 @@ static int launch(const Args& a, const int* counts, const int* work, cudaStream_
     st = launch_pdl("combine_kernel", combine_kernel<D>, dim3((unsigned)n_combine * a.hk, 4), dim3(D), 0, s, a,
                     items + n_rows);
   return st;
+}
+
+// The tiles' key ranges cut into parts so that together they fill `slots` resident CTAs once: a part holds an equal
+// share of all keys, at least min_keys, and a tile is cut only into whole shares (a further part would start a second
+// round of CTAs). Parts write units of 16 rows to the workspace; `joins` gets one entry per 16 rows of a cut tile.
+static std::vector<Item> cut(const std::vector<Item>& tiles, int hk, int slots, int min_keys, int& units,
+                             std::vector<Item>& joins) {
+  long long total = 0;
+  for (const Item& it : tiles) total += it.t1 - it.t0;
+  const long long share = std::max<long long>(min_keys, (total * hk + slots - 1) / slots);
+  std::vector<Item> out;
+  for (const Item& it : tiles) {
+    const int keys = it.t1 - it.t0;
+    const int parts = (int)std::max<long long>(1, keys / share);
+    if (parts == 1) {
+      out.push_back(it);
+      continue;
+    }
+    // (whole 64-key chunks, counted from a 64-key boundary)
+    const int first = it.t0 - it.t0 % BN, chunks = (it.t1 - first + BN - 1) / BN;
+    const int step = (chunks + parts - 1) / parts * BN, per = (it.tile + UNIT - 1) / UNIT;
+    Item join = it;
+    join.parts = 0, join.stride = per;
+    for (int t = first; t < it.t1; t += step) {
+      Item part = it;
+      part.t0 = std::max(it.t0, t), part.t1 = std::min(it.t1, t + step);
+      part.unit = units + per * join.parts++;
+      out.push_back(part);
+    }
+    for (int u = 0; u < per; ++u) {
+      Item j = join;
+      j.r0 += u * UNIT, j.unit = units + u, j.tile = std::min(UNIT, it.tile);
+      joins.push_back(j);
+    }
+    units += per * join.parts;
+  }
+  // longest first: the last CTAs to start are the short ones
+  std::stable_sort(out.begin(), out.end(), [](const Item& x, const Item& y) { return x.t1 - x.t0 > y.t1 - y.t0; });
+  return out;
 }
 
 }  // namespace kv8
@@ -421,16 +1011,18 @@ extern "C" int morj_tree_attention_kv8_work(const int* qo_indptr_host, const int
   }
   const int G = hq / hk;
   try {
-    std::vector<Item> items, joins;
-    int rows_max = 0;
-    long long total = 0;  // keys over all tiles
     for (int s = 0; s < n_segments; ++s) {
       const long long rows = (long long)(qo_indptr_host[s + 1] - qo_indptr_host[s]) * G;
       if (rows < 0 || rows > (1 << 30) || kv_indptr_host[s + 1] < kv_indptr_host[s])
         return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8_work: segment %d's tables are out of order", s);
-      rows_max = std::max(rows_max, (int)rows);
     }
-    const int tile = rows_max <= 8 ? 8 : 16;
+    std::vector<Item> tiles, rows, joins;
+    int few_max = 0;  // the largest segment that rows_kernel takes
+    for (int s = 0; s < n_segments; ++s) {
+      const int n = (qo_indptr_host[s + 1] - qo_indptr_host[s]) * G;
+      if (n <= kv8::FEW_ROWS) few_max = std::max(few_max, n);
+    }
+    const int few = few_max <= 8 ? 8 : 16;
     for (int s = 0; s < n_segments; ++s) {
       const int q_len = qo_indptr_host[s + 1] - qo_indptr_host[s];
       const int pages = kv_indptr_host[s + 1] - kv_indptr_host[s];
@@ -440,55 +1032,36 @@ extern "C" int morj_tree_attention_kv8_work(const int* qo_indptr_host, const int
               : (long long)(pages - 1) * page_size + (kv_last_page_len_host ? kv_last_page_len_host[s] : page_size);
       if (kv < 0 || kv > INT_MAX)
         return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8_work: segment %d has %lld keys", s, kv);
+      const bool many = q_len * G > kv8::FEW_ROWS;
+      const int tile = many ? kv8::T_ROWS : few;
       for (int r0 = 0; r0 < q_len * G; r0 += tile) {
         int lo, hi, x;  // what the tile's first query sees from, its last query to
         kv8::visible(q_len, (int)kv, s < n_bidir, window, r0 / G, &lo, &x);
         kv8::visible(q_len, (int)kv, s < n_bidir, window, (std::min(r0 + tile, q_len * G) - 1) / G, &x, &hi);
         Item it{s, r0, 0, 0, -1, 1, 1, tile};
         if (hi >= lo) it.t0 = lo, it.t1 = hi + 1;
-        total += it.t1 - it.t0;
-        items.push_back(it);
+        (many ? tiles : rows).push_back(it);
       }
     }
-    // parts: about four CTAs' worth of warps per SM, at least 256 keys each
-    const long long slots = (long long)num_sms() * 4;
-    long long len = (total * hk + slots - 1) / slots;
-    len = std::max(256LL, (len + 127) / 128 * 128);
-    std::vector<Item> cut;
     int units = 0;
-    for (const Item& it : items) {
-      const int keys = it.t1 - it.t0;
-      const int parts = keys > len ? (int)((keys + len - 1) / len) : 1;
-      if (parts == 1) {
-        cut.push_back(it);
-        continue;
-      }
-      const int step = ((keys + parts - 1) / parts + 127) / 128 * 128;
-      Item join = it;
-      join.unit = units, join.parts = 0;
-      for (int t = it.t0; t < it.t1; t += step) {
-        Item part = it;
-        part.t0 = t, part.t1 = std::min(it.t1, t + step);
-        part.unit = units++;
-        ++join.parts;
-        cut.push_back(part);
-      }
-      joins.push_back(join);
-    }
-    // longest first: the last CTAs to start are the short ones
-    std::stable_sort(cut.begin(), cut.end(), [](const Item& x, const Item& y) { return x.t1 - x.t0 > y.t1 - y.t0; });
-    counts[0] = (int)cut.size();
+    const std::vector<Item> cut_tiles = kv8::cut(tiles, hk, num_sms() * kv8::T_CTAS, kv8::T_MIN_KEYS, units, joins);
+    const std::vector<Item> cut_rows = kv8::cut(rows, hk, num_sms() * kv8::R_CTAS, kv8::R_MIN_KEYS, units, joins);
+    const size_t n_items = cut_tiles.size() + cut_rows.size() + joins.size();
+    counts[0] = (int)cut_rows.size();
     counts[1] = (int)joins.size();
     counts[2] = units;
-    counts[3] = tile;
-    counts[4] = (int)((cut.size() + joins.size()) * (sizeof(Item) / sizeof(int)));
-    const size_t need = (cut.size() + joins.size()) * (sizeof(Item) / sizeof(int));
-    if (need > (size_t)cap) {
+    counts[3] = few;
+    counts[4] = (int)(n_items * (sizeof(Item) / sizeof(int)));
+    counts[5] = (int)cut_tiles.size();
+    counts[6] = counts[7] = 0;
+    if (counts[4] > cap) {
       if (cap == 0) return MORJ_OK;  // (a call that only asks for the counts)
-      return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8_work: %zu ints exceed capacity %d", need, cap);
+      return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8_work: %d ints exceed capacity %d", counts[4], cap);
     }
-    std::copy(cut.begin(), cut.end(), reinterpret_cast<Item*>(work_host));
-    std::copy(joins.begin(), joins.end(), reinterpret_cast<Item*>(work_host) + cut.size());
+    Item* out = reinterpret_cast<Item*>(work_host);
+    out = std::copy(cut_tiles.begin(), cut_tiles.end(), out);
+    out = std::copy(cut_rows.begin(), cut_rows.end(), out);
+    std::copy(joins.begin(), joins.end(), out);
     return MORJ_OK;
   } catch (...) {
     return set_error(MORJ_ERR_OOM, "morj_tree_attention_kv8_work: out of host memory");
@@ -503,12 +1076,14 @@ extern "C" int morj_tree_attention_kv8(const void* q, int n_q, const void* k_cod
                                        void* workspace, unsigned long long workspace_bytes, void* stream) {
   using namespace morj;
   if (!counts) return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8: null counts");
-  if (counts[0] == 0 || n_segments == 0) return MORJ_OK;
+  if ((counts[0] == 0 && counts[5] == 0) || n_segments == 0) return MORJ_OK;
   if (!q || !k_codes || !k_scale || !v_codes || !v_scale || !out || !qo_indptr || !kv_indptr || !kv_indices || !work ||
-      n_q <= 0 || pool_slots <= 0 || counts[0] < 0 || counts[1] < 0 || counts[2] < 0)
+      n_q <= 0 || pool_slots <= 0 || counts[0] < 0 || counts[1] < 0 || counts[2] < 0 || counts[5] < 0)
     return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8: null pointer or bad size");
   if (hq <= 0 || hk <= 0 || hq % hk)
     return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8: hq=%d is not a multiple of hk=%d", hq, hk);
+  if (!(sm_scale > 0.f))
+    return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8: sm_scale must be positive");
   if (page_size <= 0 || n_bidir < 0 || n_bidir > n_segments)
     return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8: bad page_size %d or n_bidir %d", page_size, n_bidir);
   if (d != 64 && d != 128)
@@ -521,9 +1096,12 @@ extern "C" int morj_tree_attention_kv8(const void* q, int n_q, const void* k_cod
   if (workspace_bytes < need || (need && !workspace))
     return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8: a workspace of %llu bytes given, %llu needed",
                      workspace_bytes, need);
+  int page_shift = -1;
+  if ((page_size & (page_size - 1)) == 0)
+    for (page_shift = 0; (1 << page_shift) < page_size;) ++page_shift;
   const kv8::Args a{(const __nv_bfloat16*)q, (const uint8_t*)k_codes, k_scale, (const uint8_t*)v_codes, v_scale,
                     (__nv_bfloat16*)out, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, n_bidir, hq, hk, page_size,
-                    window, pool_slots, sm_scale * kv8::LOG2E, (float*)workspace};
+                    page_shift, window, pool_slots, sm_scale * kv8::LOG2E, (float*)workspace};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return d == 128 ? kv8::launch<128>(a, counts, work, s) : kv8::launch<64>(a, counts, work, s);
 }

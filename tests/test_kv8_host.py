@@ -83,41 +83,51 @@ def test_attention_work_covers_every_row_and_key_once(spec, hq, hk, window, n_bi
 
 
 def check_work(work, counts, spec, G, window, n_bidir):
-    n_items, n_joins, units, tile = counts[0], counts[1], counts[2], counts[3]
-    items = work[:n_items * ITEM].reshape(-1, ITEM).tolist()
-    joins = work[n_items * ITEM:].reshape(-1, ITEM).tolist()
-    assert len(joins) == n_joins
-    parts = {}
-    for seg, r0, t0, t1, unit, _, _, rows in items:
-        assert rows == tile and r0 % tile == 0 and t0 <= t1
+    n_rows, n_joins, units, few, ints, n_tiles = list(counts)[:6]
+    items = work.reshape(-1, ITEM).tolist()
+    assert len(work) == ints and len(items) == n_tiles + n_rows + n_joins
+    parts, rows_of = {}, {}
+    for i, (seg, r0, t0, t1, unit, _, _, rows) in enumerate(items[:n_tiles + n_rows]):
+        # segments of more than 16 rows in 128-row tiles, the others in small ones
+        assert rows == (128 if i < n_tiles else few) and (spec[seg][0] * G > 16) == (i < n_tiles)
+        assert r0 % rows == 0 and t0 <= t1
         parts.setdefault((seg, r0), []).append((t0, t1, unit))
-    seen_units = set()
-    want = {(s, r0) for s, (n, _) in enumerate(spec) for r0 in range(0, n * G, tile)}
-    assert set(parts) == want
-    joined = {(j[0], j[1]): j for j in joins}
+        rows_of[seg] = rows
+    assert few in (8, 16) and (few == 16 or all(n * G <= 8 or n * G > 16 for n, _ in spec))
+    assert set(parts) == {(s, r0) for s, (n, _) in enumerate(spec) if n for r0 in range(0, n * G, rows_of[s])}
+    joined = {(j[0], j[1]): j for j in items[n_tiles + n_rows:]}
+    assert len(joined) == n_joins
+    used = set()
     for (seg, r0), got in parts.items():
         n, keys = spec[seg]
-        rows = range(r0, min(r0 + tile, n * G))
+        rows = range(r0, min(r0 + rows_of[seg], n * G))
         los, his = zip(*(view(n, keys, seg < n_bidir, window, r // G) for r in rows))
         got.sort()
         if max(his) < min(los):
             assert len(got) == 1 and got[0][0] == got[0][1]
         else:
-            assert got[0][0] <= min(los) and got[-1][1] == max(his) + 1 <= keys
-            assert all(a[1] == b[0] for a, b in zip(got, got[1:]))
+            assert got[0][0] == min(los) and got[-1][1] == max(his) + 1 <= keys
+            assert all(a[1] == b[0] and a[1] % 64 == 0 for a, b in zip(got, got[1:]))
+            assert all(a < b for a, b, _ in got)
+        per = (rows_of[seg] + 15) // 16
         if len(got) == 1:
             assert got[0][2] == -1 and (seg, r0) not in joined
-        else:
-            j = joined[(seg, r0)]
-            assert j[5] == len(got) and [u for _, _, u in got] == [j[4] + i * j[6] for i in range(len(got))]
-            assert not seen_units & {u for _, _, u in got}
-            seen_units |= {u for _, _, u in got}
-    assert len(seen_units) == units and (not units or max(seen_units) < units)
+            continue
+        for u in range(per):
+            j = joined.pop((seg, r0 + 16 * u))
+            assert j[5] == len(got) and [x[2] + u for x in got] == [j[4] + i * j[6] for i in range(len(got))]
+            assert j[7] == min(16, rows_of[seg])
+        for _, _, first in got:
+            assert not used & set(range(first, first + per))
+            used |= set(range(first, first + per))
+    assert not joined and used == set(range(units))
 
 
 def test_long_single_rows_are_cut_and_short_ones_are_not():
     _, long = nat.kv8_attention_work([0, 1], [0, 20000], 0, 32, 16, 0)
     assert long[1] == 1 and long[2] > 8
+    _, long = nat.kv8_attention_work([0, 64], [0, 20000], 0, 32, 16, 0)
+    assert long[5] > 1 and long[1] == 8 and long[2] == 8 * long[5]
     _, short = nat.kv8_attention_work([0, 1], [0, 200], 0, 32, 16, 0)
     assert short[1] == 0 and short[2] == 0
 
@@ -186,7 +196,7 @@ def attention_args(**kw):
     (dict(v=None), 'null pointer'), (dict(vs=None), 'null pointer'), (dict(out=None), 'null pointer'),
     (dict(idx=None), 'null pointer'), (dict(work=None), 'null pointer'), (dict(n_q=0), 'bad size'),
     (dict(pool_slots=0), 'bad size'), (dict(hq=3), 'multiple'), (dict(hk=0), 'multiple'), (dict(page=0), 'page_size'),
-    (dict(n_bidir=2), 'n_bidir'), (dict(q=24), '16-byte'), (dict(work=24), '16-byte'),
+    (dict(n_bidir=2), 'n_bidir'), (dict(scale=0.0), 'sm_scale'), (dict(scale=-1.0), 'sm_scale'), (dict(q=24), '16-byte'), (dict(work=24), '16-byte'),
     (dict(counts=(1, 1, 2, 8, 16, 0, 0, 0)), 'workspace of 0 bytes'),
     (dict(counts=(1, 1, 2, 8, 16, 0, 0, 0), ws=16, ws_bytes=33279), '33280 needed')])
 def test_attention_refusals(kw, match):
