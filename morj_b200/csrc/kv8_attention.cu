@@ -56,7 +56,9 @@ struct Args {
   const int* kv_indptr;
   const int* kv_indices;
   const int* kv_last_page_len;
-  int n_bidir, hq, hk, page_size, page_shift, window, pool_slots;  // page_shift: log2 of the page size, -1: none
+  int n_bidir, hq, hk, page_size;
+  unsigned page_magic;  // t / page_size = umulhi(t, page_magic) >> page_shift (page_size > 1)
+  int page_shift, window, pool_slots;
   float scale_log2;
   float* ws;
 };
@@ -89,11 +91,13 @@ __host__ __device__ inline void visible(int q_len, int kv_len, bool bidir, int w
   if (*lo < 0) *lo = 0;
 }
 
-// pages of a segment's keys; division only where the page size is no power of two
-MORJ_DEV int page_of(const Args& a, int t) { return a.page_shift >= 0 ? t >> a.page_shift : t / a.page_size; }
+// Page of key t: t / page_size by a 32-bit reciprocal from the host (exact for 0 <= t < 2^31), since a hardware-free
+// division is some 30 instructions in every loader's loop. Slot of key t in the page with list entry `entry`.
+MORJ_DEV int page_of(const Args& a, int t) {
+  return a.page_size == 1 ? t : (int)(__umulhi((unsigned)t, a.page_magic) >> a.page_shift);
+}
 MORJ_DEV long long slot_of(const Args& a, int entry, int t) {
-  return a.page_shift >= 0 ? ((long long)entry << a.page_shift) + (t & (a.page_size - 1))
-                           : (long long)entry * a.page_size + t % a.page_size;
+  return (long long)entry * a.page_size + (t - page_of(a, t) * a.page_size);
 }
 
 // pool slot of key t of a segment, -1 (device error recorded) outside the pool
@@ -380,9 +384,10 @@ __global__ void __launch_bounds__(WARPS * 32) rows_kernel(const Args a, const It
 //   warps 0-3   softmax (thread = row): prologue (Q row to FP16 and shared memory), mask, online maximum and sum, P as
 //               FP16 over its own scores in TMEM, the final O / l or the part's (maximum, sum, O)
 //   warp 4      MMA issuer (one thread): S_c = Q K_c^T into TMEM buffer c % 2, O += P_c V_c with P read from TMEM
-//   warps 5-6   K: a chunk's codes from global memory to registers one chunk ahead, converted to FP16 into the
+//   warp 5      K: a chunk's codes from global memory to registers one chunk ahead, converted to FP16 into the
 //               swizzled operand tile, with the keys' scales for the softmax
-//   warps 7-8   the same for V
+//   warp 6      the same for V
+//   (warp 7 has no role: a ninth warp would leave 96 registers a thread, a score row read in halves and 1.8x the time)
 // The pipeline is tree_attention_kernel's (S and P double-buffered in TMEM, K buffer free once its S is complete, V
 // buffer once its P V is); its loaders issued TMA copies, these convert. The conversion is one instruction for two
 // codes and runs on warps of its own: 16,384 codes a chunk are about 260 conversions and 200 loads and stores per
@@ -390,7 +395,7 @@ __global__ void __launch_bounds__(WARPS * 32) rows_kernel(const Args a, const It
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int T_ROWS = 128;
 constexpr int BN = 64;
-constexpr int T_THREADS = 288;
+constexpr int T_THREADS = 256;
 constexpr int T_TMEM_COLS = 256;      // S/P buffers at columns [0, 64) and [64, 128), O at [128, 128 + D)
 constexpr float T_RESCALE_LOG2 = 4.0f;  // O is rescaled when a row's maximum grows by more than 2^4, so that
 constexpr float T_P_SCALE = 2048.0f;    // 2^11 p <= 2^15 stays inside FP16
@@ -461,84 +466,114 @@ MORJ_DEV bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
   return ok != 0;
 }
 
-// One loader warp: keys [32 * part, + 32) of every chunk of one pool (K or V). A lane looks one key's page entry up two
-// chunks ahead and loads its scale one ahead, with its share of the codes: 16 of them from every fourth row (D = 128),
-// so no load waits on another. Lanes are dealt to (row, piece) such that eight consecutive ones store to eight
-// different 16-byte units of the swizzled tile.
+// Loads that are issued where they stand: a plain __ldg may be moved down to its first use, past the waits that are
+// meant to hide it.
+MORJ_DEV uint4 load_now(const uint8_t* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "l"(p));
+  return v;
+}
+MORJ_DEV int load_now(const int* p) {
+  int v;
+  asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(v) : "l"(p));
+  return v;
+}
+MORJ_DEV float load_now(const float* p) {
+  float v;
+  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
+  return v;
+}
+
+// The loader warp of one pool (K or V). A lane looks two keys' page entries up two chunks ahead and loads their scales
+// one ahead, with its share of the codes: 16 of them from every fourth row (D = 128), so no load waits on another.
+// Lanes are dealt to (row, piece) such that eight consecutive ones store to eight different 16-byte units of the
+// swizzled tile.
 template <int D, bool IS_K>
-MORJ_DEV void load_side(const Args& a, const Seg& sg, const Item& it, int h, int t_begin, int n_chunks, int part,
-                        uint32_t tiles, uint32_t full, uint32_t empty, uint32_t meta_full, float* meta, volatile int* abort) {
+MORJ_DEV void load_side(const Args& a, const Seg& sg, const Item& it, int h, int t_begin, int n_chunks, uint32_t tiles,
+                        uint32_t full, uint32_t empty, uint32_t meta_full, float* meta, volatile int* abort) {
   using L = TSmem<D>;
   constexpr int LPR = D / 16;        // lanes per row, 16 codes each
   constexpr int RPI = 32 / LPR;      // rows per load instruction
-  constexpr int NI = 32 / RPI;       // load instructions per chunk
+  constexpr int NI = BN / RPI;       // load instructions per chunk
   const int lane = threadIdx.x & 31;
-  // D = 128: lane bits (half of the row, row, row 2, piece, piece) -> row 0..3, piece 0..7
+  // D = 128: lane bits (row 2, half of the row, row 1, piece, piece) -> row 0..3, piece 0..7
   const int piece = LPR == 8 ? (lane & 3) | ((lane >> 3) & 1) << 2 : lane & 3;
   const int sub = LPR == 8 ? ((lane >> 2) & 1) | (lane >> 4) << 1 : lane >> 2;
   const uint8_t* codes = (IS_K ? a.k : a.v) + (size_t)h * D + piece * 16;
   const float* scales = (IS_K ? a.ks : a.vs) + h;
-  const size_t row_bytes = (size_t)a.hk * D;
+  const unsigned row_bytes = (unsigned)a.hk * D;
   const int t_end = min(it.t1, sg.kv_len);
   const int* list = a.kv_indices + sg.kv_base;
-  const int t_lane = t_begin + part * 32 + lane;
-  auto entry = [&](int c) {  // (a key outside the part reads the entry of the nearest key inside it)
-    return __ldg(list + page_of(a, max(it.t0, min(t_lane + c * BN, t_end - 1))));
-  };
-  int slot;  // this lane's key of a chunk: pool slot, -1: none
-  float sc;
+  const int t_lane = t_begin + lane;
+  auto inside = [&](int t) { return max(it.t0, min(t, t_end - 1)); };  // (a key outside the part: the nearest inside)
+  auto entry = [&](int c, int half) { return load_now(list + page_of(a, inside(t_lane + c * BN + half * 32))); };
+  unsigned valid[2];  // which of this lane's half chunk's keys are there
+  float sc[2];
   uint4 w[NI];
-  auto fetch = [&](int c, int e) {
-    const int t = t_lane + c * BN;
-    const long long s64 = slot_of(a, e, max(it.t0, min(t, t_end - 1)));
-    const bool in_pool = s64 >= 0 && s64 < a.pool_slots;
-    if (!in_pool) report(kErrBadIndex);
-    const int from = in_pool ? (int)s64 : 0;
-    slot = t >= it.t0 && t < t_end && in_pool ? from : -1;
-    sc = __ldg(scales + (size_t)(from >> BLOCK_SHIFT) * a.hk);
+  auto fetch = [&](int c, int e0, int e1) {
+    unsigned from[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int t = t_lane + c * BN + half * 32;
+      const long long slot = slot_of(a, half ? e1 : e0, inside(t));
+      const bool in_pool = slot >= 0 && slot < a.pool_slots;
+      if (!in_pool) report(kErrBadIndex);
+      from[half] = in_pool ? (unsigned)slot : 0u;
+      valid[half] = __ballot_sync(0xffffffffu, t >= it.t0 && t < t_end && in_pool);
+    }
 #pragma unroll
     for (int i = 0; i < NI; ++i)
-      w[i] = __ldg(reinterpret_cast<const uint4*>(
-          codes + (size_t)__shfl_sync(0xffffffffu, from, i * RPI + sub) * row_bytes));
+      w[i] = load_now(codes + (unsigned long long)__shfl_sync(0xffffffffu, from[i / (NI / 2)], (i % (NI / 2)) * RPI + sub) *
+                                  row_bytes);
+#pragma unroll
+    for (int half = 0; half < 2; ++half) sc[half] = load_now(scales + (size_t)(from[half] >> BLOCK_SHIFT) * a.hk);
   };
   if (n_chunks == 0) return;
-  fetch(0, entry(0));
-  int e_next = entry(1);
+  int e0 = entry(0, 0), e1 = entry(0, 1);
+  fetch(0, e0, e1);
+  e0 = entry(1, 0), e1 = entry(1, 1);
   for (int c = 0; c < n_chunks; ++c) {
     const int b = c & 1;
     // a K buffer is free once the scores of the chunk two back are complete, a V buffer once its P V is
     if (c >= 2 && !warp_wait(empty + 8 * b, ((c >> 1) - 1) & 1, abort)) return;
-    // the keys' scales: all of them, and the common one when the valid keys agree
-    const unsigned valid = __ballot_sync(0xffffffffu, slot >= 0);
-    if (slot < 0) sc = 0.f;
-    const float first = __shfl_sync(0xffffffffu, sc, valid ? __ffs(valid) - 1 : 0);
-    const bool same = __all_sync(0xffffffffu, slot < 0 || sc == first);
-    if constexpr (IS_K) {
-      meta[L::KF + (c & 3) * 64 + part * 32 + lane] = sc;
-      if (lane == 0) meta[L::KU + (c & 3) * 2 + part] = same ? first : -1.f;
-    } else {
-      float big = same ? first : sc;
-      if (!same) {
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, x));
-      }
-      meta[L::VF + b * 64 + part * 32 + lane] = sc;
-      if (lane == 0) meta[L::VU + b * 2 + part] = same ? first : -1.f, meta[L::VM + b * 2 + part] = big;
-    }
-    if (valid != 0xffffffffu) {  // a key that is not there is zeros
+    if ((valid[0] & valid[1]) != 0xffffffffu) {  // a key that is not there is zeros
 #pragma unroll
       for (int i = 0; i < NI; ++i)
-        if (!((valid >> (i * RPI + sub)) & 1)) w[i] = make_uint4(0, 0, 0, 0);
+        if (!((valid[i / (NI / 2)] >> ((i % (NI / 2)) * RPI + sub)) & 1)) w[i] = make_uint4(0, 0, 0, 0);
     }
     const uint32_t base = tiles + b * L::KV_BYTES + (piece >> 2) * (BN * 128);
     const int u0 = (piece & 3) * 2;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const int r = part * 32 + i * RPI + sub;
+      const int r = i * RPI + sub;
       sts16(base + sw128_offset(r, u0), codes2_f16(w[i].x), codes2_f16(w[i].x >> 16), codes2_f16(w[i].y),
             codes2_f16(w[i].y >> 16));
       sts16(base + sw128_offset(r, u0 + 1), codes2_f16(w[i].z), codes2_f16(w[i].z >> 16), codes2_f16(w[i].w),
             codes2_f16(w[i].w >> 16));
+    }
+    // the keys' scales: all of them, and per half chunk the common one when the valid keys agree
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const unsigned there = valid[half];
+      const bool mine = (there >> lane) & 1;
+      const float x = mine ? sc[half] : 0.f;
+      const float first = __shfl_sync(0xffffffffu, x, there ? __ffs(there) - 1 : 0);
+      const bool same = __all_sync(0xffffffffu, !mine || x == first);
+      if constexpr (IS_K) {
+        meta[L::KF + (c & 3) * 64 + half * 32 + lane] = x;
+        if (lane == 0) meta[L::KU + (c & 3) * 2 + half] = same ? first : -1.f;
+      } else {
+        float big = first;
+        if (!same) {
+          big = x;
+#pragma unroll
+          for (int y = 16; y > 0; y >>= 1) big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, y));
+        }
+        meta[L::VF + b * 64 + half * 32 + lane] = x;
+        if (lane == 0) meta[L::VU + b * 2 + half] = same ? first : -1.f, meta[L::VM + b * 2 + half] = big;
+      }
     }
     fence_proxy_async_smem();
     __syncwarp();
@@ -547,8 +582,8 @@ MORJ_DEV void load_side(const Args& a, const Seg& sg, const Item& it, int h, int
       if constexpr (IS_K) mbar_arrive(meta_full + 8 * (c & 3));
     }
     if (c + 1 < n_chunks) {
-      fetch(c + 1, e_next);  // in flight while the next buffer is waited for
-      e_next = entry(c + 2);
+      fetch(c + 1, e0, e1);  // in flight while the next buffer is waited for
+      e0 = entry(c + 2, 0), e1 = entry(c + 2, 1);
     }
   }
 }
@@ -584,13 +619,13 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
   if (threadIdx.x == 0) {
     mbar_init(q_full, 4);
     for (int b = 0; b < 2; ++b) {
-      mbar_init(k_full + 8 * b, 2);  // one arrival per loader warp
-      mbar_init(v_full + 8 * b, 2);
+      mbar_init(k_full + 8 * b, 1);
+      mbar_init(v_full + 8 * b, 1);
       mbar_init(s_full + 8 * b, 1);
       mbar_init(p_full + 8 * b, 4);  // one arrival per softmax warp
       mbar_init(pv_done + 8 * b, 1);
     }
-    for (int b = 0; b < 4; ++b) mbar_init(meta_full + 8 * b, 2);
+    for (int b = 0; b < 4; ++b) mbar_init(meta_full + 8 * b, 1);
     mbar_init(done, 1);
     *abort = 0;
     fence_mbar_init();
@@ -604,11 +639,10 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp >= 7) {
-    load_side<D, false>(a, sg, it, h, t_begin, n_chunks, warp - 7, sbase + L::V_OFF, v_full, pv_done, 0, meta, abort);
-  } else if (warp >= 5) {
-    load_side<D, true>(a, sg, it, h, t_begin, n_chunks, warp - 5, sbase + L::K_OFF, k_full, s_full, meta_full, meta,
-                       abort);
+  if (warp == 5) {
+    load_side<D, true>(a, sg, it, h, t_begin, n_chunks, sbase + L::K_OFF, k_full, s_full, meta_full, meta, abort);
+  } else if (warp == 6) {
+    load_side<D, false>(a, sg, it, h, t_begin, n_chunks, sbase + L::V_OFF, v_full, pv_done, 0, meta, abort);
   } else if (warp == 4) {
     if (lane == 0) {
       constexpr uint32_t IDESC_S = idesc_f16(T_ROWS, BN);
@@ -729,42 +763,41 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
       float cs[2] = {ku.x >= 0.f ? ku.x * qs : qs, ku.y >= 0.f ? ku.y * qs : qs};
       cs[0] = cs[0] < 1.2e-38f ? 1.2e-38f : cs[0];  // (a masked score stays -inf times it)
       cs[1] = cs[1] < 1.2e-38f ? 1.2e-38f : cs[1];
-      // Half a chunk's scores at a time, the first half read twice instead of kept (96 registers a thread): masked, and
-      // times their keys' scales where those differ. Scores times cs are in the log2 domain; cs > 0.
-      uint32_t sr[32];
-      auto scores = [&](int half) {
-        tmem_ld32(t_lane + b * BN + half * 32, sr);
-        tmem_wait_ld();
+      // Scores, masked, and times their keys' scales where those differ; times cs they are in the log2 domain (cs > 0).
+      uint32_t sr[2][32];
+      tmem_ld32(t_lane + b * BN, sr[0]);
+      tmem_ld32(t_lane + b * BN + 32, sr[1]);
+      tmem_wait_ld();
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
         if ((half ? ku.y : ku.x) < 0.f) {
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             const float4 f = *reinterpret_cast<const float4*>(kf + half * 32 + j);
-            sr[j] = __float_as_uint(__uint_as_float(sr[j]) * f.x);
-            sr[j + 1] = __float_as_uint(__uint_as_float(sr[j + 1]) * f.y);
-            sr[j + 2] = __float_as_uint(__uint_as_float(sr[j + 2]) * f.z);
-            sr[j + 3] = __float_as_uint(__uint_as_float(sr[j + 3]) * f.w);
+            sr[half][j] = __float_as_uint(__uint_as_float(sr[half][j]) * f.x);
+            sr[half][j + 1] = __float_as_uint(__uint_as_float(sr[half][j + 1]) * f.y);
+            sr[half][j + 2] = __float_as_uint(__uint_as_float(sr[half][j + 2]) * f.z);
+            sr[half][j + 3] = __float_as_uint(__uint_as_float(sr[half][j + 3]) * f.w);
           }
         }
-        if (!full) {
-          const int first = lo - t0 - half * 32, last = hi - t0 - half * 32;
+      }
+      if (!full) {
+        const int first = lo - t0, last = hi - t0;
 #pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (j < first || j > last) sr[j] = 0xff800000u;  // -inf
-        }
-      };
-      auto largest = [&] {  // (over independent partials: short dependency chains)
+        for (int j = 0; j < BN; ++j)
+          if (j < first || j > last) sr[j >> 5][j & 31] = 0xff800000u;  // -inf
+      }
+      float mx = -INFINITY;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {  // (over independent partials: short dependency chains)
         float m4[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) m4[i] = fmaxf(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1]));
+        for (int i = 0; i < 4; ++i) m4[i] = fmaxf(__uint_as_float(sr[half][2 * i]), __uint_as_float(sr[half][2 * i + 1]));
 #pragma unroll
         for (int j = 8; j < 32; j += 2)
-          m4[(j >> 1) & 3] = max3f(m4[(j >> 1) & 3], __uint_as_float(sr[j]), __uint_as_float(sr[j + 1]));
-        return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-      };
-      scores(1);
-      float mx = largest() * cs[1];
-      scores(0);
-      mx = fmaxf(mx, largest() * cs[0]);
+          m4[(j >> 1) & 3] = max3f(m4[(j >> 1) & 3], __uint_as_float(sr[half][j]), __uint_as_float(sr[half][j + 1]));
+        mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * cs[half]);
+      }
       float alpha = 1.f;
       if (mx > m_used + T_RESCALE_LOG2 || m_used == -INFINITY) {
         if (m_used != -INFINITY) alpha = fast_exp2(m_used - mx);
@@ -778,7 +811,6 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
       for (int half = 0; half < 2; ++half) {
         // probabilities go to TMEM times f = T_P_SCALE * scale / vref: as part of the exponent where the half chunk
         // has one scale (the sum is divided by it again), else key by key
-        if (half == 1) scores(1);
         const float f = (half ? vu.y : vu.x) * inv_v;
         const bool fold = f >= 9.3e-10f;  // 2^-30: p f stays a normal FP32 number
         const float lf = fold ? __log2f(f) : 0.f;
@@ -791,7 +823,7 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
             float x0, x1;
-            f2_unpack(f2_fma(f2_bits(sr[j], sr[j + 1]), scale2, shift2), x0, x1);
+            f2_unpack(f2_fma(f2_bits(sr[half][j], sr[half][j + 1]), scale2, shift2), x0, x1);
             const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
             s4[(j >> 1) & 3] = f2_add(s4[(j >> 1) & 3], f2_pack(p0, p1));
             pk[j / 2] = pack_f16x2(p0, p1);
@@ -800,7 +832,7 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
             float x0, x1;
-            f2_unpack(f2_fma(f2_bits(sr[j], sr[j + 1]), scale2, shift2), x0, x1);
+            f2_unpack(f2_fma(f2_bits(sr[half][j], sr[half][j + 1]), scale2, shift2), x0, x1);
             const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
             s4[(j >> 1) & 3] = f2_add(s4[(j >> 1) & 3], f2_pack(p0, p1));
             const float2 g = *reinterpret_cast<const float2*>(vf + half * 32 + j);
@@ -815,7 +847,7 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
           sum += x + y;
         }
         l_run = fmaf(sum, fold ? fast_exp2(-lf) : 1.f, l_run);
-        tmem_st16(t_lane + b * BN + half * 16, pk);  // P_c over the first 32 columns of S_c (read already)
+        tmem_st16(t_lane + b * BN + half * 16, pk);  // P_c over the first 32 columns of S_c
       }
       // a rescale of O waits until the previous chunk's PV has completed (the next one needs this chunk's P)
       if (c >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
@@ -1096,12 +1128,14 @@ extern "C" int morj_tree_attention_kv8(const void* q, int n_q, const void* k_cod
   if (workspace_bytes < need || (need && !workspace))
     return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8: a workspace of %llu bytes given, %llu needed",
                      workspace_bytes, need);
-  int page_shift = -1;
-  if ((page_size & (page_size - 1)) == 0)
-    for (page_shift = 0; (1 << page_shift) < page_size;) ++page_shift;
+  // with l = ceil(log2 d): floor(t / d) = t * (floor(2^(31 + l) / d) + 1) >> (31 + l) for 0 <= t < 2^31, 2 <= d < 2^31
+  int l = 0;
+  while (l < 31 && (1u << l) < (unsigned)page_size) ++l;
+  const unsigned page_magic = page_size > 1 ? (unsigned)((1ull << (31 + l)) / page_size + 1) : 0;
+  const int page_shift = l - 1;
   const kv8::Args a{(const __nv_bfloat16*)q, (const uint8_t*)k_codes, k_scale, (const uint8_t*)v_codes, v_scale,
                     (__nv_bfloat16*)out, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, n_bidir, hq, hk, page_size,
-                    page_shift, window, pool_slots, sm_scale * kv8::LOG2E, (float*)workspace};
+                    page_magic, page_shift, window, pool_slots, sm_scale * kv8::LOG2E, (float*)workspace};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return d == 128 ? kv8::launch<128>(a, counts, work, s) : kv8::launch<64>(a, counts, work, s);
 }
