@@ -387,7 +387,7 @@ __global__ void __launch_bounds__(WARPS * 32) rows_kernel(const Args a, const It
 //   warp 5      K: a chunk's codes from global memory to registers one chunk ahead, converted to FP16 into the
 //               swizzled operand tile, with the keys' scales for the softmax
 //   warp 6      the same for V
-//   (warp 7 has no role: a ninth warp would leave 96 registers a thread, a score row read in halves and 1.8x the time)
+//   (warp 7 has no role)
 // The pipeline is tree_attention_kernel's (S and P double-buffered in TMEM, K buffer free once its S is complete, V
 // buffer once its P V is); its loaders issued TMA copies, these convert. The conversion is one instruction for two
 // codes and runs on warps of its own: 16,384 codes a chunk are about 260 conversions and 200 loads and stores per
@@ -486,13 +486,16 @@ MORJ_DEV float load_now(const float* p) {
   return v;
 }
 
-// The loader warp of one pool (K or V). A lane looks two keys' page entries up two chunks ahead and loads their scales
+// The loader warp of one pool, K or V: one piece of code for both, since the instruction cache is what a larger kernel
+// runs out of (with K's and V's own copies and the softmax unrolled over both halves of a chunk the warps took 2.2x the
+// cycles). A lane looks two keys' page entries up two chunks ahead and loads their scales
 // one ahead, with its share of the codes: 16 of them from every fourth row (D = 128), so no load waits on another.
 // Lanes are dealt to (row, piece) such that eight consecutive ones store to eight different 16-byte units of the
 // swizzled tile.
-template <int D, bool IS_K>
-MORJ_DEV void load_side(const Args& a, const Seg& sg, const Item& it, int h, int t_begin, int n_chunks, uint32_t tiles,
-                        uint32_t full, uint32_t empty, uint32_t meta_full, float* meta, volatile int* abort) {
+template <int D>
+MORJ_DEV void load_side(const Args& a, const Seg& sg, const Item& it, int h, int t_begin, int n_chunks, bool is_k,
+                        uint32_t tiles, uint32_t full, uint32_t empty, uint32_t meta_full, float* meta,
+                        volatile int* abort) {
   using L = TSmem<D>;
   constexpr int LPR = D / 16;        // lanes per row, 16 codes each
   constexpr int RPI = 32 / LPR;      // rows per load instruction
@@ -501,8 +504,8 @@ MORJ_DEV void load_side(const Args& a, const Seg& sg, const Item& it, int h, int
   // D = 128: lane bits (row 2, half of the row, row 1, piece, piece) -> row 0..3, piece 0..7
   const int piece = LPR == 8 ? (lane & 3) | ((lane >> 3) & 1) << 2 : lane & 3;
   const int sub = LPR == 8 ? ((lane >> 2) & 1) | (lane >> 4) << 1 : lane >> 2;
-  const uint8_t* codes = (IS_K ? a.k : a.v) + (size_t)h * D + piece * 16;
-  const float* scales = (IS_K ? a.ks : a.vs) + h;
+  const uint8_t* codes = (is_k ? a.k : a.v) + (size_t)h * D + piece * 16;
+  const float* scales = (is_k ? a.ks : a.vs) + h;
   const unsigned row_bytes = (unsigned)a.hk * D;
   const int t_end = min(it.t1, sg.kv_len);
   const int* list = a.kv_indices + sg.kv_base;
@@ -530,6 +533,8 @@ MORJ_DEV void load_side(const Args& a, const Seg& sg, const Item& it, int h, int
 #pragma unroll
     for (int half = 0; half < 2; ++half) sc[half] = load_now(scales + (size_t)(from[half] >> BLOCK_SHIFT) * a.hk);
   };
+  const uint32_t row0 = (piece >> 2) * (BN * 128) + sub * 128;  // units 2 (piece % 4) and the next of the row, swizzled
+  const uint32_t unit0 = row0 + ((((piece & 3) * 2) ^ sub) << 4), unit1 = row0 + ((((piece & 3) * 2 + 1) ^ sub) << 4);
   if (n_chunks == 0) return;
   int e0 = entry(0, 0), e1 = entry(0, 1);
   fetch(0, e0, e1);
@@ -543,17 +548,19 @@ MORJ_DEV void load_side(const Args& a, const Seg& sg, const Item& it, int h, int
       for (int i = 0; i < NI; ++i)
         if (!((valid[i / (NI / 2)] >> ((i % (NI / 2)) * RPI + sub)) & 1)) w[i] = make_uint4(0, 0, 0, 0);
     }
-    const uint32_t base = tiles + b * L::KV_BYTES + (piece >> 2) * (BN * 128);
-    const int u0 = (piece & 3) * 2;
+    const uint32_t tile = tiles + b * L::KV_BYTES;
 #pragma unroll
-    for (int i = 0; i < NI; ++i) {
-      const int r = i * RPI + sub;
-      sts16(base + sw128_offset(r, u0), codes2_f16(w[i].x), codes2_f16(w[i].x >> 16), codes2_f16(w[i].y),
+    for (int i = 0; i < NI; ++i) {  // row i * RPI + sub: its swizzle follows sub and, for RPI = 4, the parity of i
+      const uint32_t at = tile + i * (RPI * 128), x = RPI == 4 ? (i & 1) << 6 : 0;
+      sts16(at + (unit0 ^ x), codes2_f16(w[i].x), codes2_f16(w[i].x >> 16), codes2_f16(w[i].y),
             codes2_f16(w[i].y >> 16));
-      sts16(base + sw128_offset(r, u0 + 1), codes2_f16(w[i].z), codes2_f16(w[i].z >> 16), codes2_f16(w[i].w),
+      sts16(at + (unit1 ^ x), codes2_f16(w[i].z), codes2_f16(w[i].z >> 16), codes2_f16(w[i].w),
             codes2_f16(w[i].w >> 16));
     }
     // the keys' scales: all of them, and per half chunk the common one when the valid keys agree
+    const int ring = is_k ? c & 3 : b;
+    float* key_scales = meta + (is_k ? L::KF : L::VF) + ring * 64 + lane;
+    float* common = meta + (is_k ? L::KU : L::VU) + ring * 2;
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
       const unsigned there = valid[half];
@@ -561,25 +568,23 @@ MORJ_DEV void load_side(const Args& a, const Seg& sg, const Item& it, int h, int
       const float x = mine ? sc[half] : 0.f;
       const float first = __shfl_sync(0xffffffffu, x, there ? __ffs(there) - 1 : 0);
       const bool same = __all_sync(0xffffffffu, !mine || x == first);
-      if constexpr (IS_K) {
-        meta[L::KF + (c & 3) * 64 + half * 32 + lane] = x;
-        if (lane == 0) meta[L::KU + (c & 3) * 2 + half] = same ? first : -1.f;
-      } else {
-        float big = first;
-        if (!same) {
-          big = x;
-#pragma unroll
-          for (int y = 16; y > 0; y >>= 1) big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, y));
-        }
-        meta[L::VF + b * 64 + half * 32 + lane] = x;
-        if (lane == 0) meta[L::VU + b * 2 + half] = same ? first : -1.f, meta[L::VM + b * 2 + half] = big;
+      key_scales[half * 32] = x;
+      float big = first;
+      if (!same) {
+        big = x;
+#pragma unroll 1
+        for (int y = 16; y > 0; y >>= 1) big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, y));
+      }
+      if (lane == 0) {
+        common[half] = same ? first : -1.f;
+        if (!is_k) meta[L::VM + b * 2 + half] = big;
       }
     }
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
       mbar_arrive(full + 8 * b);
-      if constexpr (IS_K) mbar_arrive(meta_full + 8 * (c & 3));
+      if (is_k) mbar_arrive(meta_full + 8 * (c & 3));
     }
     if (c + 1 < n_chunks) {
       fetch(c + 1, e0, e1);  // in flight while the next buffer is waited for
@@ -639,10 +644,10 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 5) {
-    load_side<D, true>(a, sg, it, h, t_begin, n_chunks, sbase + L::K_OFF, k_full, s_full, meta_full, meta, abort);
-  } else if (warp == 6) {
-    load_side<D, false>(a, sg, it, h, t_begin, n_chunks, sbase + L::V_OFF, v_full, pv_done, 0, meta, abort);
+  if (warp == 5 || warp == 6) {
+    const bool is_k = warp == 5;
+    load_side<D>(a, sg, it, h, t_begin, n_chunks, is_k, sbase + (is_k ? L::K_OFF : L::V_OFF), is_k ? k_full : v_full,
+                 is_k ? s_full : pv_done, meta_full, meta, abort);
   } else if (warp == 4) {
     if (lane == 0) {
       constexpr uint32_t IDESC_S = idesc_f16(T_ROWS, BN);
@@ -670,7 +675,8 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
       if (ok && n_chunks > 1) ok = issue_qk(1);
       for (int c = 0; c < n_chunks && ok; ++c) {
         const int b = c & 1;
-        // O += P_c V_c, P_c from TMEM buffer b (packed FP16 pairs, 8 columns per 16 keys)
+        // O += P_c V_c, P_c from TMEM buffer b (packed FP16 pairs, 8 columns per 16 keys; each half of the keys over the
+        // first columns of its own scores)
         if (!mbar_wait(p_full + 8 * b, (c >> 1) & 1, abort, kErrTimeoutAttention) ||
             !mbar_wait(v_full + 8 * b, (c >> 1) & 1, abort, kErrTimeoutAttention)) {
           ok = false;
@@ -680,7 +686,7 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
         const uint64_t v_desc = v_desc0 + b * KV_STEP;
 #pragma unroll
         for (int kk = 0; kk < BN / 16; ++kk)
-          umma_bf16_tmem_a(tmem + 128, tmem + b * BN + kk * 8, v_desc + kk * (2048 >> 4), IDESC_O, (c | kk) != 0);
+          umma_bf16_tmem_a(tmem + 128, tmem + b * BN + (kk >> 1) * 32 + (kk & 1) * 8, v_desc + kk * (2048 >> 4), IDESC_O, (c | kk) != 0);
         umma_commit(pv_done + 8 * b);
         if (c + 2 < n_chunks) ok = issue_qk(c + 2);  // in issue order after this PV, which reads P_c first
       }
@@ -760,43 +766,42 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
       }
       const int t0 = t_begin + c * BN;
       const bool full = __all_sync(0xffffffffu, t0 >= lo && t0 + BN - 1 <= hi);
-      float cs[2] = {ku.x >= 0.f ? ku.x * qs : qs, ku.y >= 0.f ? ku.y * qs : qs};
-      cs[0] = cs[0] < 1.2e-38f ? 1.2e-38f : cs[0];  // (a masked score stays -inf times it)
-      cs[1] = cs[1] < 1.2e-38f ? 1.2e-38f : cs[1];
-      // Scores, masked, and times their keys' scales where those differ; times cs they are in the log2 domain (cs > 0).
-      uint32_t sr[2][32];
-      tmem_ld32(t_lane + b * BN, sr[0]);
-      tmem_ld32(t_lane + b * BN + 32, sr[1]);
-      tmem_wait_ld();
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        if ((half ? ku.y : ku.x) < 0.f) {
+      // Half a chunk's scores at a time, each read from TMEM twice, in loops that stay rolled (code size, see above):
+      // masked, and times their keys' scales where those differ; times cs they are in the log2 domain (cs > 0).
+      uint32_t sr[32];
+      auto scores = [&](int half, float scale) {
+        tmem_ld32(t_lane + b * BN + half * 32, sr);
+        tmem_wait_ld();
+        if (scale < 0.f) {
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             const float4 f = *reinterpret_cast<const float4*>(kf + half * 32 + j);
-            sr[half][j] = __float_as_uint(__uint_as_float(sr[half][j]) * f.x);
-            sr[half][j + 1] = __float_as_uint(__uint_as_float(sr[half][j + 1]) * f.y);
-            sr[half][j + 2] = __float_as_uint(__uint_as_float(sr[half][j + 2]) * f.z);
-            sr[half][j + 3] = __float_as_uint(__uint_as_float(sr[half][j + 3]) * f.w);
+            sr[j] = __float_as_uint(__uint_as_float(sr[j]) * f.x);
+            sr[j + 1] = __float_as_uint(__uint_as_float(sr[j + 1]) * f.y);
+            sr[j + 2] = __float_as_uint(__uint_as_float(sr[j + 2]) * f.z);
+            sr[j + 3] = __float_as_uint(__uint_as_float(sr[j + 3]) * f.w);
           }
         }
-      }
-      if (!full) {
-        const int first = lo - t0, last = hi - t0;
+        if (!full) {
+          const int first = max(lo - t0 - half * 32, 0), last = min(hi - t0 - half * 32, 31);
+          const unsigned seen = first <= last ? (0xffffffffu << first) & (0xffffffffu >> (31 - last)) : 0u;
 #pragma unroll
-        for (int j = 0; j < BN; ++j)
-          if (j < first || j > last) sr[j >> 5][j & 31] = 0xff800000u;  // -inf
-      }
+          for (int j = 0; j < 32; ++j) sr[j] = seen & (1u << j) ? sr[j] : 0xff800000u;  // -inf
+        }
+        const float c = scale < 0.f ? qs : scale * qs;
+        return c < 1.2e-38f ? 1.2e-38f : c;  // (a masked score stays -inf times it)
+      };
       float mx = -INFINITY;
+#pragma unroll 1
+      for (int half = 0; half < 2; ++half) {
+        const float cs = scores(half, half ? ku.y : ku.x);
+        float m4[4];  // (over independent partials: short dependency chains)
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {  // (over independent partials: short dependency chains)
-        float m4[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) m4[i] = fmaxf(__uint_as_float(sr[half][2 * i]), __uint_as_float(sr[half][2 * i + 1]));
+        for (int i = 0; i < 4; ++i) m4[i] = fmaxf(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1]));
 #pragma unroll
         for (int j = 8; j < 32; j += 2)
-          m4[(j >> 1) & 3] = max3f(m4[(j >> 1) & 3], __uint_as_float(sr[half][j]), __uint_as_float(sr[half][j + 1]));
-        mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * cs[half]);
+          m4[(j >> 1) & 3] = max3f(m4[(j >> 1) & 3], __uint_as_float(sr[j]), __uint_as_float(sr[j + 1]));
+        mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * cs);
       }
       float alpha = 1.f;
       if (mx > m_used + T_RESCALE_LOG2 || m_used == -INFINITY) {
@@ -807,38 +812,39 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
       alpha *= unit;
       // exp2(-inf) = 0 for masked keys; a row with no visible key yet keeps m_used = -inf and p = 0
       const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
-#pragma unroll
+#pragma unroll 1
       for (int half = 0; half < 2; ++half) {
-        // probabilities go to TMEM times f = T_P_SCALE * scale / vref: as part of the exponent where the half chunk
-        // has one scale (the sum is divided by it again), else key by key
+        // Probabilities go to TMEM times f = T_P_SCALE * scale / vref: as part of the exponent where the half chunk
+        // has one scale (the sum is divided by it again), else key by key.
+        const float cs = scores(half, half ? ku.y : ku.x);
         const float f = (half ? vu.y : vu.x) * inv_v;
         const bool fold = f >= 9.3e-10f;  // 2^-30: p f stays a normal FP32 number
         const float lf = fold ? __log2f(f) : 0.f;
-        const uint64_t scale2 = f2_pack(cs[half], cs[half]), shift2 = f2_pack(neg_m + lf, neg_m + lf);
+        const uint64_t scale2 = f2_pack(cs, cs), shift2 = f2_pack(neg_m + lf, neg_m + lf);
         uint64_t s4[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) s4[i] = f2_pack(0.f, 0.f);
-        uint32_t pk[16];
-        if (fold) {  // (the same for the whole CTA)
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            float x0, x1;
-            f2_unpack(f2_fma(f2_bits(sr[half][j], sr[half][j + 1]), scale2, shift2), x0, x1);
-            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-            s4[(j >> 1) & 3] = f2_add(s4[(j >> 1) & 3], f2_pack(p0, p1));
-            pk[j / 2] = pack_f16x2(p0, p1);
-          }
-        } else {
+        for (int j = 0; j < 32; j += 2) {
+          float x0, x1;
+          f2_unpack(f2_fma(f2_bits(sr[j], sr[j + 1]), scale2, shift2), x0, x1);
+          const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+          s4[(j >> 1) & 3] = f2_add(s4[(j >> 1) & 3], f2_pack(p0, p1));
+          sr[j] = __float_as_uint(p0), sr[j + 1] = __float_as_uint(p1);
+        }
+        if (!fold) {  // (the same for the whole CTA)
 #pragma unroll
-          for (int j = 0; j < 32; j += 2) {
-            float x0, x1;
-            f2_unpack(f2_fma(f2_bits(sr[half][j], sr[half][j + 1]), scale2, shift2), x0, x1);
-            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-            s4[(j >> 1) & 3] = f2_add(s4[(j >> 1) & 3], f2_pack(p0, p1));
-            const float2 g = *reinterpret_cast<const float2*>(vf + half * 32 + j);
-            pk[j / 2] = pack_f16x2(p0 * (g.x * inv_v), p1 * (g.y * inv_v));
+          for (int j = 0; j < 32; j += 4) {
+            const float4 g = *reinterpret_cast<const float4*>(vf + half * 32 + j);
+            sr[j] = __float_as_uint(__uint_as_float(sr[j]) * (g.x * inv_v));
+            sr[j + 1] = __float_as_uint(__uint_as_float(sr[j + 1]) * (g.y * inv_v));
+            sr[j + 2] = __float_as_uint(__uint_as_float(sr[j + 2]) * (g.z * inv_v));
+            sr[j + 3] = __float_as_uint(__uint_as_float(sr[j + 3]) * (g.w * inv_v));
           }
         }
+        uint32_t pk[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) pk[j] = pack_f16x2(__uint_as_float(sr[2 * j]), __uint_as_float(sr[2 * j + 1]));
         float sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -847,7 +853,8 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
           sum += x + y;
         }
         l_run = fmaf(sum, fold ? fast_exp2(-lf) : 1.f, l_run);
-        tmem_st16(t_lane + b * BN + half * 16, pk);  // P_c over the first 32 columns of S_c
+        // over the first half of the columns of the scores just read
+        tmem_st16(t_lane + b * BN + (half ? 32 : 0), pk);
       }
       // a rescale of O waits until the previous chunk's PV has completed (the next one needs this chunk's P)
       if (c >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
