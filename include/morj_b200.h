@@ -235,14 +235,19 @@ int morj_kv8_gather(const void* codes, const float* scale, int pool_slots, const
  * sets the device error word (0x301).
  *
  * morj_tree_attention_kv8_work (host function, no device access): the call's work list from host copies of its segment
- * tables. Writes up to `cap` ints to work_host and counts[8]: counts[0..3] = tiles of few rows, joins, partial units,
- * rows per such tile, counts[4] = ints written, counts[5] = 128-row tiles. With cap = 0 it writes only the counts. Long key lists of few
- * tiles are cut into parts, whose partial results go through `workspace` (counts[2] * hk * 16 * (d + 2) * 4 bytes, the
- * caller's, 16-byte aligned; calls that may overlap on the device must not share it) and are joined in a fixed order.
- * `work`: the device copy of the list (16-byte aligned); `counts`: the host array. */
-int morj_tree_attention_kv8_work(const int* qo_indptr_host, const int* kv_indptr_host,
+ * tables. Writes up to `cap` ints to work_host and counts[MORJ_KV8_COUNTS]: 0 tiles of few rows, 1 joins, 2 partial
+ * units, 3 rows per such tile, 4 ints written, 5 tiles of 128 rows, 6 pages and 7 blocks those see, 8 list entries. With
+ * cap = 0 it writes only the counts. Segments of more than 16 rows (queries x hq / hk) run in tiles of 128: the pages they
+ * see are first expanded to FP16 in `workspace`, once per call. Long key lists of few tiles are cut into parts, whose
+ * partial results go through `workspace` and are joined in a fixed order.
+ * morj_tree_attention_kv8_workspace (host function): the bytes a call with these counts needs (4 per code pair of the
+ * expanded pages, plus the parts; the caller's, 256-byte aligned; calls that may overlap on the device must not share
+ * it). `work`: the device copy of the list (16-byte aligned); `counts`: the host array. */
+#define MORJ_KV8_COUNTS 12
+int morj_tree_attention_kv8_work(const int* qo_indptr_host, const int* kv_indptr_host, const int* kv_indices_host,
                                  const int* kv_last_page_len_host, int n_segments, int n_bidir, int hq, int hk,
                                  int page_size, int window, int* work_host, int cap, int* counts);
+int morj_tree_attention_kv8_workspace(const int* counts, int hk, int d, int page_size, unsigned long long* bytes);
 int morj_tree_attention_kv8(const void* q, int n_q, const void* k_codes, const float* k_scale, const void* v_codes,
                             const float* v_scale, int pool_slots, void* out, const int* qo_indptr,
                             const int* kv_indptr, const int* kv_indices, const int* kv_last_page_len, int n_segments,

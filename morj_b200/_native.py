@@ -46,7 +46,8 @@ SIGNATURES = {
     'morj_kv8_store_work': [IP, I, I, IP, I],
     'morj_kv8_store': [P, LL, P, LL, I, I, I, P, I, P, P, P, P, I, P],
     'morj_kv8_gather': [P, P, I, P, I, I, I, P, LL, P],
-    'morj_tree_attention_kv8_work': [IP, IP, IP, I, I, I, I, I, I, IP, I, IP],
+    'morj_tree_attention_kv8_work': [IP, IP, IP, IP, I, I, I, I, I, I, IP, I, IP],
+    'morj_tree_attention_kv8_workspace': [IP, I, I, I, ctypes.POINTER(ctypes.c_ulonglong)],
     'morj_tree_attention_kv8': [P, I, P, P, P, P, I, P, P, P, P, P, I, I, I, I, I, I, I, F, P, IP, P,
                                 ctypes.c_ulonglong, P],
     'morj_label_head': [P, LL, P, P, P, I, P, P, I, F, F, P, P],
@@ -158,31 +159,37 @@ def kv8_store_work(slots, pool_slots):
     return buf[:3 * n + (n & 1) + 2 * len(s)], n
 
 
-KV8_COUNTS = I * 8
+KV8_COUNTS = I * 12
 
 
-def kv8_attention_work(qo_indptr, kv_indptr, n_bidir, hq, hk, window, page_size=1, kv_last_page_len=None):
+def kv8_attention_work(qo_indptr, kv_indptr, kv_indices, n_bidir, hq, hk, window, page_size=1, kv_last_page_len=None):
     """(work list, counts) of an attention call over an 8-bit cache, from host copies of its segment tables
     (`morj_tree_attention_kv8_work`). `counts` is the ctypes array the call takes."""
     import numpy as np
-    qo = np.ascontiguousarray(qo_indptr, dtype=np.int32)
-    kv = np.ascontiguousarray(kv_indptr, dtype=np.int32)
+    qo, kv, idx = (np.ascontiguousarray(a, dtype=np.int32) for a in (qo_indptr, kv_indptr, kv_indices))
     last = None if kv_last_page_len is None else np.ascontiguousarray(kv_last_page_len, dtype=np.int32)
+    if len(idx) < kv[-1]:
+        raise ValueError(f'{len(idx)} list entries, kv_indptr ends at {kv[-1]}')
     counts = KV8_COUNTS()
-    cap = 0
-    while True:  # (the list's length is known after the first call)
-        buf = np.zeros(max(cap, 1), dtype=np.int32)
-        call('morj_tree_attention_kv8_work', qo.ctypes.data_as(IP), kv.ctypes.data_as(IP),
-             last.ctypes.data_as(IP) if last is not None else None, len(qo) - 1, n_bidir, hq, hk, page_size, window,
-             buf.ctypes.data_as(IP), cap, counts)
-        if counts[4] <= cap:
-            return buf[:counts[4]], counts
-        cap = counts[4]
+    cap = 4096 + 3 * len(idx) + int(qo[-1]) * max(hq, 1)
+    while True:  # (a longer list says how long)
+        buf = np.empty(cap, dtype=np.int32)
+        status = lib().morj_tree_attention_kv8_work(
+            qo.ctypes.data_as(IP), kv.ctypes.data_as(IP), idx.ctypes.data_as(IP),
+            last.ctypes.data_as(IP) if last is not None else None, len(qo) - 1, n_bidir, hq, hk, page_size, window,
+            buf.ctypes.data_as(IP), cap, counts)
+        if status == ERR_ARG and counts[4] > cap:
+            cap = counts[4]
+            continue
+        check(status, 'morj_tree_attention_kv8_work')
+        return buf[:counts[4]], counts
 
 
-def kv8_attention_workspace(counts, hk, d):
+def kv8_attention_workspace(counts, hk, d, page_size=1):
     """Workspace bytes of an attention call over an 8-bit cache with these counts."""
-    return counts[2] * hk * 16 * (d + 2) * 4
+    n = ctypes.c_ulonglong(0)
+    call('morj_tree_attention_kv8_workspace', counts, hk, d, page_size, ctypes.byref(n))
+    return n.value
 
 
 def device_error(stream, clear=True):

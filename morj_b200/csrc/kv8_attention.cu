@@ -32,6 +32,8 @@ constexpr float LOG2E = 1.4426950408889634f;
 constexpr int UNIT = 16;             // rows of a partial unit in the workspace
 constexpr int WARPS = 4;
 constexpr int STEP = 32;             // keys a warp takes at a time
+constexpr int T_ROWS = 128;           // rows of a tile_kernel tile
+constexpr int BN = 64;                // keys it takes at a time
 constexpr int FEW_ROWS = 16;         // segments of at most this many rows go to rows_kernel
 constexpr int T_CTAS = 2, T_MIN_KEYS = 256;  // resident CTAs per SM and keys of a part worth one: tile_kernel
 constexpr int R_CTAS = 4, R_MIN_KEYS = 256;  // ... rows_kernel
@@ -380,25 +382,102 @@ __global__ void __launch_bounds__(WARPS * 32) rows_kernel(const Args a, const It
 }
 
 // ---------------------------------------------------------------------------------------------------------------
+// Many rows per segment: the pages these segments list are expanded once to FP16, then attended to on tcgen05.
+//
+// expand_kernel: pool[i] = FP16(code * scale / ref) of every distinct listed slot, K and V, in the order the lists name
+// them; ref is the head's largest scale among them, so a value keeps all its bits down to 2^-15 of it. A key is used by
+// every 128-row tile that sees it: expanding costs 3 bytes of traffic per code once (35.7 M codes, the 8,704 tokens of
+// a 16-head layer, K and V), where converting in the tile loaders (built and measured) cost each tile the conversion,
+// the address arithmetic and the instruction cache: 130 us on the op-level tree (2048 + 8 x 64) against the 62 us of the
+// BF16 kernel with the same pipeline.
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int E_THREADS = 256;
+
+template <int D>
+__global__ void __launch_bounds__(E_THREADS) expand_kernel(const Args a, const int2* __restrict__ pages, int n_slots,
+                                                           const int* __restrict__ blocks, int n_blocks,
+                                                           __half* __restrict__ k_out, __half* __restrict__ v_out,
+                                                           float* __restrict__ refs) {
+  pdl_wait();  // the previous kernel on the stream has completed
+  pdl_trigger();
+  constexpr int LPR = D / 16;                  // lanes per row, 16 codes each
+  constexpr int ROWS = E_THREADS / LPR / 2;    // rows per pass of each half of the CTA (K, V)
+  __shared__ float red[2][E_THREADS / 32];
+  const int h = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+  // this CTA's codes first: nothing below is needed to ask for them
+  const int side = threadIdx.x / (E_THREADS / 2), tid = threadIdx.x % (E_THREADS / 2);
+  const uint8_t* codes = (side ? a.v : a.k) + (size_t)h * D + (tid % LPR) * 16;
+  const float* scales = (side ? a.vs : a.ks) + h;
+  uint4 w[BN / ROWS];
+  float sc[BN / ROWS];
+#pragma unroll
+  for (int i = 0; i < BN / ROWS; ++i) {
+    const int t = blockIdx.x * BN + i * ROWS + tid / LPR;
+    sc[i] = 0.f, w[i] = make_uint4(0, 0, 0, 0);
+    if (t < n_slots) {
+      const int2 page = __ldg(pages + page_of(a, t));  // (page of the pool, its slots that are listed: the rest is zeros)
+      const int at = t - page_of(a, t) * a.page_size;
+      const long long slot = (long long)page.x * a.page_size + at;
+      if (at >= page.y) {
+      } else if (slot < 0 || slot >= a.pool_slots) {
+        if (tid % LPR == 0) report(kErrBadIndex);
+      } else {
+        w[i] = __ldg(reinterpret_cast<const uint4*>(codes + (size_t)slot * a.hk * D));
+        sc[i] = __ldg(scales + (size_t)(slot >> BLOCK_SHIFT) * a.hk);
+      }
+    }
+  }
+  // the head's largest scales (every CTA of the head finds the same)
+  float kr = 0.f, vr = 0.f;
+  for (int i = threadIdx.x; i < n_blocks; i += E_THREADS) {
+    if ((long long)blocks[i] * BLOCK >= a.pool_slots) continue;  // (reported above)
+    const size_t at = (size_t)blocks[i] * a.hk + h;
+    kr = fmaxf(kr, __ldg(a.ks + at));
+    vr = fmaxf(vr, __ldg(a.vs + at));
+  }
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) {
+    kr = fmaxf(kr, __shfl_xor_sync(0xffffffffu, kr, x));
+    vr = fmaxf(vr, __shfl_xor_sync(0xffffffffu, vr, x));
+  }
+  if (lane == 0) red[0][warp] = kr, red[1][warp] = vr;
+  __syncthreads();
+  for (int i = 0; i < E_THREADS / 32; ++i) kr = fmaxf(kr, red[0][i]), vr = fmaxf(vr, red[1][i]);
+  if (blockIdx.x == 0 && threadIdx.x == 0) refs[h] = kr, refs[a.hk + h] = vr;
+  const float ref = side ? vr : kr;
+  __half* out = (side ? v_out : k_out) + (size_t)h * D + (tid % LPR) * 16;
+#pragma unroll
+  for (int i = 0; i < BN / ROWS; ++i) {
+    const int t = blockIdx.x * BN + i * ROWS + tid / LPR;
+    if (t >= n_slots) break;
+    const float f = ref > 0.f ? sc[i] / ref : sc[i];
+    const uint32_t c[8] = {w[i].x & 0xffffu, w[i].x >> 16, w[i].y & 0xffffu, w[i].y >> 16,
+                           w[i].z & 0xffffu, w[i].z >> 16, w[i].w & 0xffffu, w[i].w >> 16};
+    uint32_t p[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float2 x = codes2_f32(c[e]);
+      p[e] = pack_f16x2(x.x * f, x.y * f);
+    }
+    uint4* dst = reinterpret_cast<uint4*>(out + (size_t)t * a.hk * D);
+    dst[0] = make_uint4(p[0], p[1], p[2], p[3]);
+    dst[1] = make_uint4(p[4], p[5], p[6], p[7]);
+  }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
 // tile_kernel: 128 rows of a segment and KV head against 64 keys at a time, on tcgen05 (FP16 x FP16, FP32 in TMEM).
 //   warps 0-3   softmax (thread = row): prologue (Q row to FP16 and shared memory), mask, online maximum and sum, P as
 //               FP16 over its own scores in TMEM, the final O / l or the part's (maximum, sum, O)
 //   warp 4      MMA issuer (one thread): S_c = Q K_c^T into TMEM buffer c % 2, O += P_c V_c with P read from TMEM
-//   warp 5      K: a chunk's codes from global memory to registers one chunk ahead, converted to FP16 into the
-//               swizzled operand tile, with the keys' scales for the softmax
-//   warp 6      the same for V
-//   (warp 7 has no role)
-// The pipeline is tree_attention_kernel's (S and P double-buffered in TMEM, K buffer free once its S is complete, V
-// buffer once its P V is); its loaders issued TMA copies, these convert. The conversion is one instruction for two
-// codes and runs on warps of its own: 16,384 codes a chunk are about 260 conversions and 200 loads and stores per
-// CTA beside the softmax's 2,000 instructions.
+//   warps 5, 6  K and V loaders: a chunk whose 64 expanded slots are consecutive by TMA, others gathered by cp.async
+// The pipeline is tree_attention_kernel's (S and P double-buffered in TMEM, a K buffer free once its S is complete, a V
+// buffer once its P V is, two CTAs per SM); what it lacks there is the parts of a key range and rows that see nothing.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int T_ROWS = 128;
-constexpr int BN = 64;
-constexpr int T_THREADS = 256;
-constexpr int T_TMEM_COLS = 256;      // S/P buffers at columns [0, 64) and [64, 128), O at [128, 128 + D)
+constexpr int T_THREADS = 256;          // (warp 7 has no role)
+constexpr int T_TMEM_COLS = 256;        // S/P buffers at columns [0, 64) and [64, 128), O at [128, 128 + D)
 constexpr float T_RESCALE_LOG2 = 4.0f;  // O is rescaled when a row's maximum grows by more than 2^4, so that
-constexpr float T_P_SCALE = 2048.0f;    // 2^11 p <= 2^15 stays inside FP16
+constexpr float T_P_LOG2 = 11.0f;       // 2^11 p <= 2^15 stays inside FP16
 
 template <int D>
 struct TSmem {
@@ -406,14 +485,9 @@ struct TSmem {
   static constexpr int KV_BYTES = BN * D * 2;
   static constexpr int K_OFF = Q_BYTES;               // 2 buffers
   static constexpr int V_OFF = K_OFF + 2 * KV_BYTES;  // 2 buffers
-  static constexpr int META_OFF = V_OFF + 2 * KV_BYTES;
-  // scales of a chunk's keys: K [4][64] (chunk c + 4's are written once S_{c+2} is complete, after softmax c), V [2][64];
-  // then per half chunk (32 keys) K [4][2] the common scale or -1, V [2][2] the same and [2][2] the largest
-  static constexpr int KF = 0, VF = 4 * 64, KU = VF + 2 * 64, VU = KU + 8, VM = VU + 4, META_FLOATS = VM + 4;
-  static constexpr int BAR_OFF = META_OFF + META_FLOATS * 4 + 16;
-  // barriers: q_full, k_full[2], v_full[2], meta_full[4], s_full[2], p_full[2], pv_done[2], done; TMEM slot, abort flag
-  static constexpr int TOTAL = (BAR_OFF + 16 * 8 + 16 + 15) / 16 * 16;
-  static_assert(BAR_OFF % 8 == 0 && META_OFF % 16 == 0, "alignment");
+  static constexpr int BAR_OFF = V_OFF + 2 * KV_BYTES;
+  // barriers: q_full, k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], done; TMEM slot, abort flag
+  static constexpr int TOTAL = BAR_OFF + 128;
 };
 
 __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn_major = false) {
@@ -421,14 +495,6 @@ __host__ __device__ constexpr uint32_t idesc_f16(int M, int N, bool b_mn_major =
          | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) | ((uint32_t)(M >> 4) << 24);
 }
 
-// 32 lanes x 16 consecutive 32-bit columns from registers into TMEM
-MORJ_DEV void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
 MORJ_DEV uint64_t f2_pack(float lo, float hi) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
@@ -458,6 +524,9 @@ MORJ_DEV float max3f(float a, float b, float c) {
 MORJ_DEV void sts16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+MORJ_DEV void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
 // warp-level wait: lane 0 polls the barrier, the warp follows its verdict (and sees what lane 0 sees)
 MORJ_DEV bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
   int ok = (threadIdx.x & 31) == 0 ? (int)mbar_wait(bar, parity, abort, kErrTimeoutAttention) : 0;
@@ -466,135 +535,43 @@ MORJ_DEV bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
   return ok != 0;
 }
 
-// Loads that are issued where they stand: a plain __ldg may be moved down to its first use, past the waits that are
-// meant to hide it.
-MORJ_DEV uint4 load_now(const uint8_t* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-               : "l"(p));
-  return v;
-}
-MORJ_DEV int load_now(const int* p) {
-  int v;
-  asm volatile("ld.global.nc.s32 %0, [%1];" : "=r"(v) : "l"(p));
-  return v;
-}
-MORJ_DEV float load_now(const float* p) {
-  float v;
-  asm volatile("ld.global.nc.f32 %0, [%1];" : "=f"(v) : "l"(p));
-  return v;
-}
-
-// The loader warp of one pool, K or V: one piece of code for both, since the instruction cache is what a larger kernel
-// runs out of (with K's and V's own copies and the softmax unrolled over both halves of a chunk the warps took 2.2x the
-// cycles). A lane looks two keys' page entries up two chunks ahead and loads their scales
-// one ahead, with its share of the codes: 16 of them from every fourth row (D = 128), so no load waits on another.
-// Lanes are dealt to (row, piece) such that eight consecutive ones store to eight different 16-byte units of the
-// swizzled tile.
+// One loader warp fills buffer `dst` with the expanded rows of keys [t0, t0 + BN) and completes `full`. s0, s1: the
+// expanded slots of this lane's keys t0 + 2 lane and the next, -1 outside the part. Where the slots inside it follow one
+// another, the box around them is loaded: its other rows are masked keys, and finite (listed slots, zeros past a page's
+// listed ones or past the end).
 template <int D>
-MORJ_DEV void load_side(const Args& a, const Seg& sg, const Item& it, int h, int t_begin, int n_chunks, bool is_k,
-                        uint32_t tiles, uint32_t full, uint32_t empty, uint32_t meta_full, float* meta,
-                        volatile int* abort) {
-  using L = TSmem<D>;
-  constexpr int LPR = D / 16;        // lanes per row, 16 codes each
-  constexpr int RPI = 32 / LPR;      // rows per load instruction
-  constexpr int NI = BN / RPI;       // load instructions per chunk
-  const int lane = threadIdx.x & 31;
-  // D = 128: lane bits (row 2, half of the row, row 1, piece, piece) -> row 0..3, piece 0..7
-  const int piece = LPR == 8 ? (lane & 3) | ((lane >> 3) & 1) << 2 : lane & 3;
-  const int sub = LPR == 8 ? ((lane >> 2) & 1) | (lane >> 4) << 1 : lane >> 2;
-  const uint8_t* codes = (is_k ? a.k : a.v) + (size_t)h * D + piece * 16;
-  const float* scales = (is_k ? a.ks : a.vs) + h;
-  const unsigned row_bytes = (unsigned)a.hk * D;
-  const int t_end = min(it.t1, sg.kv_len);
-  const int* list = a.kv_indices + sg.kv_base;
-  const int t_lane = t_begin + lane;
-  auto inside = [&](int t) { return max(it.t0, min(t, t_end - 1)); };  // (a key outside the part: the nearest inside)
-  auto entry = [&](int c, int half) { return load_now(list + page_of(a, inside(t_lane + c * BN + half * 32))); };
-  unsigned valid[2];  // which of this lane's half chunk's keys are there
-  float sc[2];
-  uint4 w[NI];
-  auto fetch = [&](int c, int e0, int e1) {
-    unsigned from[2];
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int t = t_lane + c * BN + half * 32;
-      const long long slot = slot_of(a, half ? e1 : e0, inside(t));
-      const bool in_pool = slot >= 0 && slot < a.pool_slots;
-      if (!in_pool) report(kErrBadIndex);
-      from[half] = in_pool ? (unsigned)slot : 0u;
-      valid[half] = __ballot_sync(0xffffffffu, t >= it.t0 && t < t_end && in_pool);
-    }
-#pragma unroll
-    for (int i = 0; i < NI; ++i)
-      w[i] = load_now(codes + (unsigned long long)__shfl_sync(0xffffffffu, from[i / (NI / 2)], (i % (NI / 2)) * RPI + sub) *
-                                  row_bytes);
-#pragma unroll
-    for (int half = 0; half < 2; ++half) sc[half] = load_now(scales + (size_t)(from[half] >> BLOCK_SHIFT) * a.hk);
-  };
-  const uint32_t row0 = (piece >> 2) * (BN * 128) + sub * 128;  // units 2 (piece % 4) and the next of the row, swizzled
-  const uint32_t unit0 = row0 + ((((piece & 3) * 2) ^ sub) << 4), unit1 = row0 + ((((piece & 3) * 2 + 1) ^ sub) << 4);
-  if (n_chunks == 0) return;
-  int e0 = entry(0, 0), e1 = entry(0, 1);
-  fetch(0, e0, e1);
-  e0 = entry(1, 0), e1 = entry(1, 1);
-  for (int c = 0; c < n_chunks; ++c) {
-    const int b = c & 1;
-    // a K buffer is free once the scores of the chunk two back are complete, a V buffer once its P V is
-    if (c >= 2 && !warp_wait(empty + 8 * b, ((c >> 1) - 1) & 1, abort)) return;
-    if ((valid[0] & valid[1]) != 0xffffffffu) {  // a key that is not there is zeros
-#pragma unroll
-      for (int i = 0; i < NI; ++i)
-        if (!((valid[i / (NI / 2)] >> ((i % (NI / 2)) * RPI + sub)) & 1)) w[i] = make_uint4(0, 0, 0, 0);
-    }
-    const uint32_t tile = tiles + b * L::KV_BYTES;
-#pragma unroll
-    for (int i = 0; i < NI; ++i) {  // row i * RPI + sub: its swizzle follows sub and, for RPI = 4, the parity of i
-      const uint32_t at = tile + i * (RPI * 128), x = RPI == 4 ? (i & 1) << 6 : 0;
-      sts16(at + (unit0 ^ x), codes2_f16(w[i].x), codes2_f16(w[i].x >> 16), codes2_f16(w[i].y),
-            codes2_f16(w[i].y >> 16));
-      sts16(at + (unit1 ^ x), codes2_f16(w[i].z), codes2_f16(w[i].z >> 16), codes2_f16(w[i].w),
-            codes2_f16(w[i].w >> 16));
-    }
-    // the keys' scales: all of them, and per half chunk the common one when the valid keys agree
-    const int ring = is_k ? c & 3 : b;
-    float* key_scales = meta + (is_k ? L::KF : L::VF) + ring * 64 + lane;
-    float* common = meta + (is_k ? L::KU : L::VU) + ring * 2;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const unsigned there = valid[half];
-      const bool mine = (there >> lane) & 1;
-      const float x = mine ? sc[half] : 0.f;
-      const float first = __shfl_sync(0xffffffffu, x, there ? __ffs(there) - 1 : 0);
-      const bool same = __all_sync(0xffffffffu, !mine || x == first);
-      key_scales[half * 32] = x;
-      float big = first;
-      if (!same) {
-        big = x;
-#pragma unroll 1
-        for (int y = 16; y > 0; y >>= 1) big = max_nan(big, __shfl_xor_sync(0xffffffffu, big, y));
-      }
-      if (lane == 0) {
-        common[half] = same ? first : -1.f;
-        if (!is_k) meta[L::VM + b * 2 + half] = big;
-      }
-    }
-    fence_proxy_async_smem();
-    __syncwarp();
+MORJ_DEV void load_chunk(uint32_t dst, uint32_t full, const CUtensorMap* map, const __half* __restrict__ pool, int s0,
+                         int s1, int hk, int h, int lane) {
+  const unsigned any = __ballot_sync(0xffffffffu, s0 >= 0 || s1 >= 0);
+  const int mine = s0 >= 0 ? s0 - 2 * lane : s1 - 2 * lane - 1;  // slot of key t0 if the run holds
+  const int first = __shfl_sync(0xffffffffu, mine, any ? __ffs(any) - 1 : 0);
+  if (__all_sync(0xffffffffu, (s0 < 0 || s0 == first + 2 * lane) && (s1 < 0 || s1 == first + 2 * lane + 1))) {
     if (lane == 0) {
-      mbar_arrive(full + 8 * b);
-      if (is_k) mbar_arrive(meta_full + 8 * (c & 3));
+      mbar_arrive_expect_tx(full, BN * D * 2);
+#pragma unroll
+      for (int half = 0; half < D / 64; ++half) tma_load_3d(dst + half * (BN * 128), map, full, half * 64, h, first);
     }
-    if (c + 1 < n_chunks) {
-      fetch(c + 1, e0, e1);  // in flight while the next buffer is waited for
-      e0 = entry(c + 2, 0), e1 = entry(c + 2, 1);
-    }
+    return;
   }
+#pragma unroll
+  for (int k2 = 0; k2 < 2; ++k2) {
+    const int k = 2 * lane + k2, slot = k2 ? s1 : s0;
+    const __half* src = pool + (slot >= 0 ? ((size_t)slot * hk + h) * D : 0);
+#pragma unroll 4
+    for (int u = 0; u < D / 8; ++u)
+      cp_async16(dst + (uint32_t)((u >> 3) * (BN * 128)) + sw128_offset(k, u & 7), src + u * 8, slot >= 0 ? 16u : 0u);
+  }
+  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+  fence_proxy_async_smem();
+  __syncwarp();
+  if (lane == 0) mbar_arrive(full);
 }
 
 template <int D>
-__global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const Item* __restrict__ items) {
+__global__ void __launch_bounds__(T_THREADS, 2)
+    tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const Args a,
+                const Item* __restrict__ items, const int* __restrict__ list, const __half* __restrict__ k_pool,
+                const __half* __restrict__ v_pool, int n_slots, const float* __restrict__ refs) {
   pdl_wait();  // the previous kernel on the stream has completed
   pdl_trigger();
   using L = TSmem<D>;
@@ -605,15 +582,14 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
     return;
   }
   const uint32_t bar0 = sbase + L::BAR_OFF;
-  const uint32_t q_full = bar0, k_full = bar0 + 8, v_full = bar0 + 24, meta_full = bar0 + 40;
-  const uint32_t s_full = bar0 + 72, p_full = bar0 + 88, pv_done = bar0 + 104, done = bar0 + 120;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::BAR_OFF + 128);
-  volatile int* abort = reinterpret_cast<volatile int*>(smem + L::BAR_OFF + 132);
-  float* meta = reinterpret_cast<float*>(smem + L::META_OFF);
+  const uint32_t q_full = bar0, k_full = bar0 + 8, v_full = bar0 + 24;
+  const uint32_t s_full = bar0 + 40, p_full = bar0 + 56, pv_done = bar0 + 72, done = bar0 + 88;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::BAR_OFF + 96);
+  volatile int* abort = reinterpret_cast<volatile int*>(smem + L::BAR_OFF + 100);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const Item it = items[blockIdx.x / a.hk];
-  const int h = blockIdx.x % a.hk;
+  const int h = blockIdx.x % a.hk;  // (the KV head is the fast index: every head of the longest item starts first)
   const Seg sg = load_segment(a, it.seg);
   const int G = a.hq / a.hk, n_rows = sg.q_len * G;
   const bool bidir = it.seg < a.n_bidir;
@@ -622,15 +598,14 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
   const int n_chunks = t_stop > it.t0 ? (t_stop - t_begin + BN - 1) / BN : 0;
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 4);
+    mbar_init(q_full, 4);  // one arrival per softmax warp
     for (int b = 0; b < 2; ++b) {
       mbar_init(k_full + 8 * b, 1);
       mbar_init(v_full + 8 * b, 1);
       mbar_init(s_full + 8 * b, 1);
-      mbar_init(p_full + 8 * b, 4);  // one arrival per softmax warp
+      mbar_init(p_full + 8 * b, 4);
       mbar_init(pv_done + 8 * b, 1);
     }
-    for (int b = 0; b < 4; ++b) mbar_init(meta_full + 8 * b, 1);
     mbar_init(done, 1);
     *abort = 0;
     fence_mbar_init();
@@ -646,8 +621,29 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
 
   if (warp == 5 || warp == 6) {
     const bool is_k = warp == 5;
-    load_side<D>(a, sg, it, h, t_begin, n_chunks, is_k, sbase + (is_k ? L::K_OFF : L::V_OFF), is_k ? k_full : v_full,
-                 is_k ? s_full : pv_done, meta_full, meta, abort);
+    const CUtensorMap* map = is_k ? &k_map : &v_map;
+    if (lane == 0) tma_prefetch(map);
+    const uint32_t base = sbase + (is_k ? L::K_OFF : L::V_OFF);
+    // a K buffer is free once the scores of the chunk two back are complete, a V buffer once its P V is
+    const uint32_t full = is_k ? k_full : v_full, empty = is_k ? s_full : pv_done;
+    const int* pages = list + sg.kv_base;
+    auto slot = [&](int t) {  // expanded slot of key t, -1 outside the part
+      if (t < it.t0 || t >= t_stop) return -1;
+      const long long s = slot_of(a, __ldg(pages + page_of(a, t)), t);
+      if (s < 0 || s >= n_slots) {
+        report(kErrBadIndex);
+        return -1;
+      }
+      return (int)s;
+    };
+    int s0 = slot(t_begin + 2 * lane), s1 = slot(t_begin + 2 * lane + 1);
+    for (int c = 0; c < n_chunks; ++c) {
+      const int b = c & 1, next = t_begin + (c + 1) * BN + 2 * lane;
+      const int n0 = slot(next), n1 = slot(next + 1);
+      if (c >= 2 && !warp_wait(empty + 8 * b, ((c >> 1) - 1) & 1, abort)) break;
+      load_chunk<D>(base + b * L::KV_BYTES, full + 8 * b, map, is_k ? k_pool : v_pool, s0, s1, a.hk, h, lane);
+      s0 = n0, s1 = n1;
+    }
   } else if (warp == 4) {
     if (lane == 0) {
       constexpr uint32_t IDESC_S = idesc_f16(T_ROWS, BN);
@@ -675,8 +671,7 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
       if (ok && n_chunks > 1) ok = issue_qk(1);
       for (int c = 0; c < n_chunks && ok; ++c) {
         const int b = c & 1;
-        // O += P_c V_c, P_c from TMEM buffer b (packed FP16 pairs, 8 columns per 16 keys; each half of the keys over the
-        // first columns of its own scores)
+        // O += P_c V_c, P_c from TMEM buffer b (packed FP16 pairs, 8 columns per 16 keys)
         if (!mbar_wait(p_full + 8 * b, (c >> 1) & 1, abort, kErrTimeoutAttention) ||
             !mbar_wait(v_full + 8 * b, (c >> 1) & 1, abort, kErrTimeoutAttention)) {
           ok = false;
@@ -686,7 +681,7 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
         const uint64_t v_desc = v_desc0 + b * KV_STEP;
 #pragma unroll
         for (int kk = 0; kk < BN / 16; ++kk)
-          umma_bf16_tmem_a(tmem + 128, tmem + b * BN + (kk >> 1) * 32 + (kk & 1) * 8, v_desc + kk * (2048 >> 4), IDESC_O, (c | kk) != 0);
+          umma_bf16_tmem_a(tmem + 128, tmem + b * BN + kk * 8, v_desc + kk * (2048 >> 4), IDESC_O, (c | kk) != 0);
         umma_commit(pv_done + 8 * b);
         if (c + 2 < n_chunks) ok = issue_qk(c + 2);  // in issue order after this PV, which reads P_c first
       }
@@ -702,7 +697,7 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
     const bool row_ok = row < n_rows;
     const size_t row_at = ((size_t)(sg.q_start + qi) * a.hq + h * G + row % G) * D;
     // Q row: its largest magnitude, then FP16 of q / qs into the swizzled tile
-    float qs;
+    float scale;  // scores times it are in the log2 domain
     {
       // (read twice, the second time from L1: the row in registers would be 64 of them)
       const uint4* src = reinterpret_cast<const uint4*>(a.q + row_at);
@@ -715,8 +710,7 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
 #pragma unroll
         for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
       }
-      qs = row_scale(amax);
-      const float inv = 1.f / qs;
+      const float qs = row_scale(amax), inv = 1.f / qs;
 #pragma unroll 4
       for (int i = 0; i < D / 8; ++i) {
         float x[8];
@@ -728,134 +722,78 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(q_full);
-      qs *= a.scale_log2;
+      scale = qs * (refs ? refs[h] : 0.f) * a.scale_log2;
+      scale = scale < 1.2e-38f ? 1.2e-38f : scale;  // (a masked score stays -inf times it)
     }
     int lo = 1, hi = 0;  // visible key positions [lo, hi] of this part
     if (row_ok) {
       visible(sg.q_len, sg.kv_len, bidir, a.window, qi, &lo, &hi);
-      lo = max(lo, it.t0), hi = min(hi, it.t1 - 1);
+      lo = max(lo, it.t0), hi = min(hi, t_stop - 1);
     }
-    float m_used = -INFINITY, l_run = 0.f;
-    float vref = 0.f, inv_v = 0.f;  // the largest V scale met (O is in units of vref / T_P_SCALE), T_P_SCALE / vref
+    float m_used = -INFINITY, l_run = 0.f;  // l_run in units of 2^-T_P_LOG2, as P and O
     bool ok = true;
     for (int c = 0; c < n_chunks; ++c) {
       const int b = c & 1;
-      int here = lane == 0 ? (int)(mbar_wait(meta_full + 8 * (c & 3), (c >> 2) & 1, abort, kErrTimeoutAttention) &&
-                                   mbar_wait(v_full + 8 * b, (c >> 1) & 1, abort, kErrTimeoutAttention) &&
-                                   mbar_wait(s_full + 8 * b, (c >> 1) & 1, abort, kErrTimeoutAttention))
-                           : 0;
-      here = __shfl_sync(0xffffffffu, here, 0);
-      __syncwarp();
-      if (!here) {
+      if (!warp_wait(s_full + 8 * b, (c >> 1) & 1, abort)) {
         ok = false;
         break;
       }
       tc_fence_after();
-      // scales of the two half chunks: K's multiply the scores, V's the probabilities
-      const float* kf = meta + L::KF + (c & 3) * 64;
-      const float* vf = meta + L::VF + b * 64;
-      const float2 ku = *reinterpret_cast<const float2*>(meta + L::KU + (c & 3) * 2);
-      const float2 vu = *reinterpret_cast<const float2*>(meta + L::VU + b * 2);
-      const float2 vm = *reinterpret_cast<const float2*>(meta + L::VM + b * 2);
-      const float vmax = max_nan(vm.x, vm.y);
-      float unit = 1.f;
-      if (!(vmax <= vref)) {
-        unit = vref / vmax;
-        vref = vmax;
-        inv_v = T_P_SCALE / vmax;
-      }
+      uint32_t sr[2][32];
+      tmem_ld32(t_lane + b * BN, sr[0]);
+      tmem_ld32(t_lane + b * BN + 32, sr[1]);
+      tmem_wait_ld();
       const int t0 = t_begin + c * BN;
-      const bool full = __all_sync(0xffffffffu, t0 >= lo && t0 + BN - 1 <= hi);
-      // Half a chunk's scores at a time, each read from TMEM twice, in loops that stay rolled (code size, see above):
-      // masked, and times their keys' scales where those differ; times cs they are in the log2 domain (cs > 0).
-      uint32_t sr[32];
-      auto scores = [&](int half, float scale) {
-        tmem_ld32(t_lane + b * BN + half * 32, sr);
-        tmem_wait_ld();
-        if (scale < 0.f) {
+      // (the maximum and the sum run over 8 independent partials: short dependency chains)
+      float m8[8];
 #pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(kf + half * 32 + j);
-            sr[j] = __float_as_uint(__uint_as_float(sr[j]) * f.x);
-            sr[j + 1] = __float_as_uint(__uint_as_float(sr[j + 1]) * f.y);
-            sr[j + 2] = __float_as_uint(__uint_as_float(sr[j + 2]) * f.z);
-            sr[j + 3] = __float_as_uint(__uint_as_float(sr[j + 3]) * f.w);
-          }
+      for (int i = 0; i < 8; ++i) m8[i] = -INFINITY;
+      if (__all_sync(0xffffffffu, t0 >= lo && t0 + BN - 1 <= hi)) {
+#pragma unroll
+        for (int j = 0; j < BN; j += 2)
+          m8[(j >> 1) & 7] = max3f(m8[(j >> 1) & 7], __uint_as_float(sr[j >> 5][j & 31]),
+                                   __uint_as_float(sr[(j + 1) >> 5][(j + 1) & 31]));
+      } else {
+#pragma unroll
+        for (int j = 0; j < BN; ++j) {
+          const int t = t0 + j;
+          const float v = (t >= lo && t <= hi) ? __uint_as_float(sr[j >> 5][j & 31]) : -INFINITY;
+          sr[j >> 5][j & 31] = __float_as_uint(v);
+          m8[j & 7] = fmaxf(m8[j & 7], v);
         }
-        if (!full) {
-          const int first = max(lo - t0 - half * 32, 0), last = min(hi - t0 - half * 32, 31);
-          const unsigned seen = first <= last ? (0xffffffffu << first) & (0xffffffffu >> (31 - last)) : 0u;
-#pragma unroll
-          for (int j = 0; j < 32; ++j) sr[j] = seen & (1u << j) ? sr[j] : 0xff800000u;  // -inf
-        }
-        const float c = scale < 0.f ? qs : scale * qs;
-        return c < 1.2e-38f ? 1.2e-38f : c;  // (a masked score stays -inf times it)
-      };
-      float mx = -INFINITY;
-#pragma unroll 1
-      for (int half = 0; half < 2; ++half) {
-        const float cs = scores(half, half ? ku.y : ku.x);
-        float m4[4];  // (over independent partials: short dependency chains)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) m4[i] = fmaxf(__uint_as_float(sr[2 * i]), __uint_as_float(sr[2 * i + 1]));
-#pragma unroll
-        for (int j = 8; j < 32; j += 2)
-          m4[(j >> 1) & 3] = max3f(m4[(j >> 1) & 3], __uint_as_float(sr[j]), __uint_as_float(sr[j + 1]));
-        mx = fmaxf(mx, fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * cs);
       }
+      const float mx = scale * fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
+                                     fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])));
       float alpha = 1.f;
       if (mx > m_used + T_RESCALE_LOG2 || m_used == -INFINITY) {
         if (m_used != -INFINITY) alpha = fast_exp2(m_used - mx);
         if (mx != -INFINITY) m_used = mx;
       }
       l_run *= alpha;
-      alpha *= unit;
       // exp2(-inf) = 0 for masked keys; a row with no visible key yet keeps m_used = -inf and p = 0
-      const float neg_m = m_used == -INFINITY ? 0.f : -m_used;
-#pragma unroll 1
-      for (int half = 0; half < 2; ++half) {
-        // Probabilities go to TMEM times f = T_P_SCALE * scale / vref: as part of the exponent where the half chunk
-        // has one scale (the sum is divided by it again), else key by key.
-        const float cs = scores(half, half ? ku.y : ku.x);
-        const float f = (half ? vu.y : vu.x) * inv_v;
-        const bool fold = f >= 9.3e-10f;  // 2^-30: p f stays a normal FP32 number
-        const float lf = fold ? __log2f(f) : 0.f;
-        const uint64_t scale2 = f2_pack(cs, cs), shift2 = f2_pack(neg_m + lf, neg_m + lf);
-        uint64_t s4[4];
+      const float shift = m_used == -INFINITY ? 0.f : T_P_LOG2 - m_used;
+      // scores in pairs: one packed FMA scales and shifts two of them, one packed add sums two probabilities
+      const uint64_t scale2 = f2_pack(scale, scale), shift2 = f2_pack(shift, shift);
+      uint64_t s4[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s4[i] = f2_pack(0.f, 0.f);
+      for (int i = 0; i < 4; ++i) s4[i] = f2_pack(0.f, 0.f);
+      uint32_t pk[BN / 2];
 #pragma unroll
-        for (int j = 0; j < 32; j += 2) {
-          float x0, x1;
-          f2_unpack(f2_fma(f2_bits(sr[j], sr[j + 1]), scale2, shift2), x0, x1);
-          const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-          s4[(j >> 1) & 3] = f2_add(s4[(j >> 1) & 3], f2_pack(p0, p1));
-          sr[j] = __float_as_uint(p0), sr[j + 1] = __float_as_uint(p1);
-        }
-        if (!fold) {  // (the same for the whole CTA)
-#pragma unroll
-          for (int j = 0; j < 32; j += 4) {
-            const float4 g = *reinterpret_cast<const float4*>(vf + half * 32 + j);
-            sr[j] = __float_as_uint(__uint_as_float(sr[j]) * (g.x * inv_v));
-            sr[j + 1] = __float_as_uint(__uint_as_float(sr[j + 1]) * (g.y * inv_v));
-            sr[j + 2] = __float_as_uint(__uint_as_float(sr[j + 2]) * (g.z * inv_v));
-            sr[j + 3] = __float_as_uint(__uint_as_float(sr[j + 3]) * (g.w * inv_v));
-          }
-        }
-        uint32_t pk[16];
-#pragma unroll
-        for (int j = 0; j < 16; ++j) pk[j] = pack_f16x2(__uint_as_float(sr[2 * j]), __uint_as_float(sr[2 * j + 1]));
-        float sum = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float x, y;
-          f2_unpack(s4[i], x, y);
-          sum += x + y;
-        }
-        l_run = fmaf(sum, fold ? fast_exp2(-lf) : 1.f, l_run);
-        // over the first half of the columns of the scores just read
-        tmem_st16(t_lane + b * BN + (half ? 32 : 0), pk);
+      for (int j = 0; j < BN; j += 2) {
+        float x0, x1;
+        f2_unpack(f2_fma(f2_bits(sr[j >> 5][j & 31], sr[(j + 1) >> 5][(j + 1) & 31]), scale2, shift2), x0, x1);
+        const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+        s4[(j >> 1) & 3] = f2_add(s4[(j >> 1) & 3], f2_pack(p0, p1));
+        pk[j / 2] = pack_f16x2(p0, p1);
       }
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x, y;
+        f2_unpack(s4[i], x, y);
+        sum += x + y;
+      }
+      l_run += sum;
       // a rescale of O waits until the previous chunk's PV has completed (the next one needs this chunk's P)
       if (c >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
         if (!warp_wait(pv_done + 8 * (b ^ 1), ((c - 1) >> 1) & 1, abort)) {
@@ -873,6 +811,7 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
           tmem_st32(t_lane + 128 + col, o);
         }
       }
+      tmem_st32(t_lane + b * BN, pk);  // P_c over the first 32 columns of S_c
       tmem_wait_st();
       tc_fence_before();
       __syncwarp();
@@ -880,45 +819,32 @@ __global__ void __launch_bounds__(T_THREADS, 2) tile_kernel(const Args a, const 
     }
     if (ok && (n_chunks == 0 || warp_wait(pv_done + 8 * ((n_chunks - 1) & 1), ((n_chunks - 1) >> 1) & 1, abort))) {
       tc_fence_after();
-      const float back = vref * (1.f / T_P_SCALE);
-      if (it.unit < 0) {
-        const float inv = l_run == 0.f ? 0.f : back / l_run;
+      // a finished row: O / l times V's reference; a part: (maximum, sum, O in units of the values)
+      const float vr = refs ? refs[a.hk + h] : 0.f;
+      const bool part_of = it.unit >= 0;
+      const float unit = exp2_int(-(int)T_P_LOG2);
+      const float back = l_run == 0.f ? 0.f : part_of ? vr * unit : vr / l_run;
+      float* part = a.ws + ((size_t)(max(it.unit, 0) + r / UNIT) * a.hk + h) * (UNIT * (D + 2));
+      if (part_of && row_ok) part[r % UNIT] = m_used, part[UNIT + r % UNIT] = l_run * unit;
+      float4* dst = reinterpret_cast<float4*>(part + 2 * UNIT + (r % UNIT) * D);
 #pragma unroll 1
-        for (int col = 0; col < D; col += 32) {
-          uint32_t o[32];
-          if (n_chunks) {
-            tmem_ld32(t_lane + 128 + col, o);
-            tmem_wait_ld();
-          }
-          if (row_ok) {
-#pragma unroll
-            for (int v8 = 0; v8 < 4; ++v8) {
-              float x[8];
-#pragma unroll
-              for (int e = 0; e < 8; ++e) x[e] = inv == 0.f ? 0.f : __uint_as_float(o[v8 * 8 + e]) * inv;
-              store8(a.out + row_at + col + v8 * 8, x);
-            }
-          }
+      for (int col = 0; col < D; col += 32) {
+        uint32_t o[32];
+        if (n_chunks) {
+          tmem_ld32(t_lane + 128 + col, o);
+          tmem_wait_ld();
         }
-      } else {
-        float* part = a.ws + ((size_t)(it.unit + r / UNIT) * a.hk + h) * (UNIT * (D + 2));
-        if (row_ok) part[r % UNIT] = m_used, part[UNIT + r % UNIT] = l_run;
-        float4* dst = reinterpret_cast<float4*>(part + 2 * UNIT + (r % UNIT) * D);
-#pragma unroll 1
-        for (int col = 0; col < D; col += 32) {
-          uint32_t o[32];
-          if (n_chunks) {
-            tmem_ld32(t_lane + 128 + col, o);
-            tmem_wait_ld();
-          }
-          if (row_ok) {
+        if (!row_ok) continue;
 #pragma unroll
-            for (int v = 0; v < 8; ++v) {
-              float x[4];
+        for (int v8 = 0; v8 < 4; ++v8) {
+          float x[8];
 #pragma unroll
-              for (int e = 0; e < 4; ++e) x[e] = back == 0.f ? 0.f : __uint_as_float(o[4 * v + e]) * back;
-              dst[col / 4 + v] = make_float4(x[0], x[1], x[2], x[3]);
-            }
+          for (int e = 0; e < 8; ++e) x[e] = back == 0.f ? 0.f : __uint_as_float(o[v8 * 8 + e]) * back;
+          if (part_of) {
+            dst[(col + v8 * 8) / 4] = make_float4(x[0], x[1], x[2], x[3]);
+            dst[(col + v8 * 8) / 4 + 1] = make_float4(x[4], x[5], x[6], x[7]);
+          } else {
+            store8(a.out + row_at + col + v8 * 8, x);
           }
         }
       }
@@ -974,26 +900,66 @@ static int configure_tile() {
   return e == cudaSuccess ? MORJ_OK : set_error(MORJ_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
 }
 
+// Offsets in the caller's workspace: the expanded K and V, the heads' reference scales, the parts.
+struct Space {
+  size_t k, v, refs, parts, bytes;
+  Space(const int* counts, int hk, int d, int page_size) {
+    const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
+    const size_t pool = up((size_t)counts[6] * page_size * hk * d * sizeof(__half));
+    k = 0, v = pool, refs = 2 * pool;
+    parts = refs + (counts[6] ? up((size_t)2 * hk * sizeof(float)) : 0);
+    bytes = parts + (size_t)counts[2] * hk * UNIT * (d + 2) * sizeof(float);
+  }
+};
+
 template <int D>
-static int launch(const Args& a, const int* counts, const int* work, cudaStream_t s) {
+static int launch(Args a, const int* counts, const int* work, char* ws, cudaStream_t s) {
+  const Space at(counts, a.hk, D, a.page_size);
+  a.ws = reinterpret_cast<float*>(ws + at.parts);
+  const int n_rows = counts[0], n_combine = counts[1], n_tiles = counts[5], n_pages = counts[6], n_blocks = counts[7];
   const Item* items = reinterpret_cast<const Item*>(work);
-  const int n_rows = counts[0], n_combine = counts[1], n_tiles = counts[5];
   int st = MORJ_OK;
   if (n_tiles) {
     if ((st = configure_tile<D>())) return st;
+    const int* pages = work + (size_t)(n_tiles + n_rows + n_combine) * (sizeof(Item) / sizeof(int));
+    const int* blocks = pages + 2 * (size_t)n_pages;
+    const int* list = blocks + n_blocks;
+    const int n_slots = n_pages * a.page_size;
+    __half* kx = reinterpret_cast<__half*>(ws + at.k);
+    __half* vx = reinterpret_cast<__half*>(ws + at.v);
+    float* refs = reinterpret_cast<float*>(ws + at.refs);
+    CUtensorMap km, vm;
+    // expanded pools [slots, hk, D]: box = 64 columns x 1 head x 64 slots (one slot and an unused map where none is seen)
+    const unsigned long long dims[3] = {(unsigned long long)D, (unsigned long long)a.hk,
+                                        (unsigned long long)(n_slots ? n_slots : 1)};
+    const unsigned long long strides[2] = {(unsigned long long)D * 2, (unsigned long long)a.hk * D * 2};
+    const unsigned box[3] = {64u, 1u, (unsigned)BN};
+    void* kp = n_slots ? (void*)kx : const_cast<uint8_t*>(a.k);
+    void* vp = n_slots ? (void*)vx : const_cast<uint8_t*>(a.v);
+    if ((st = encode_tiled(&km, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, kp, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)))
+      return st;
+    if ((st = encode_tiled(&vm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, vp, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)))
+      return st;
+    if (n_slots)
+      st = launch_pdl("expand_kernel", expand_kernel<D>, dim3((n_slots + BN - 1) / BN, a.hk), dim3(E_THREADS), 0, s, a,
+                      reinterpret_cast<const int2*>(pages), n_slots, blocks, n_blocks, kx, vx, refs);
+    else
+      refs = nullptr;
+    if (st) return st;
     st = launch_pdl("tile_kernel", tile_kernel<D>, dim3((unsigned)n_tiles * a.hk), dim3(T_THREADS), TSmem<D>::TOTAL, s,
-                    a, items);
+                    km, vm, a, items, list, (const __half*)kx, (const __half*)vx, n_slots, (const float*)refs);
+    if (st) return st;
     items += n_tiles;
   }
-  if (st == MORJ_OK && n_rows) {
+  if (n_rows) {
     const dim3 grid((unsigned)n_rows * a.hk);
     st = counts[3] == 8
              ? launch_pdl("rows_kernel", rows_kernel<D, 8>, grid, dim3(WARPS * 32), 0, s, a, items)
              : launch_pdl("rows_kernel", rows_kernel<D, 16>, grid, dim3(WARPS * 32), 0, s, a, items);
+    items += n_rows;
   }
   if (st == MORJ_OK && n_combine)
-    st = launch_pdl("combine_kernel", combine_kernel<D>, dim3((unsigned)n_combine * a.hk, 4), dim3(D), 0, s, a,
-                    items + n_rows);
+    st = launch_pdl("combine_kernel", combine_kernel<D>, dim3((unsigned)n_combine * a.hk, 4), dim3(D), 0, s, a, items);
   return st;
 }
 
@@ -1040,19 +1006,21 @@ static std::vector<Item> cut(const std::vector<Item>& tiles, int hk, int slots, 
 }  // namespace morj
 
 extern "C" int morj_tree_attention_kv8_work(const int* qo_indptr_host, const int* kv_indptr_host,
-                                            const int* kv_last_page_len_host, int n_segments, int n_bidir, int hq,
-                                            int hk, int page_size, int window, int* work_host, int cap, int* counts) {
+                                            const int* kv_indices_host, const int* kv_last_page_len_host,
+                                            int n_segments, int n_bidir, int hq, int hk, int page_size, int window,
+                                            int* work_host, int cap, int* counts) {
   using namespace morj;
   using kv8::Item;
   if (!qo_indptr_host || !kv_indptr_host || !counts || n_segments < 0 || n_bidir < 0 || n_bidir > n_segments ||
-      hk <= 0 || hq <= 0 || hq % hk || page_size <= 0 || cap < 0 || (cap && !work_host)) {
+      hk <= 0 || hq <= 0 || hq % hk || page_size <= 0 || cap < 0 || (cap && !work_host) ||
+      (n_segments && kv_indptr_host[n_segments] > 0 && !kv_indices_host)) {
     return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8_work: bad arguments");
   }
   const int G = hq / hk;
   try {
     for (int s = 0; s < n_segments; ++s) {
       const long long rows = (long long)(qo_indptr_host[s + 1] - qo_indptr_host[s]) * G;
-      if (rows < 0 || rows > (1 << 30) || kv_indptr_host[s + 1] < kv_indptr_host[s])
+      if (rows < 0 || rows > (1 << 30) || kv_indptr_host[s] < 0 || kv_indptr_host[s + 1] < kv_indptr_host[s])
         return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8_work: segment %d's tables are out of order", s);
     }
     std::vector<Item> tiles, rows, joins;
@@ -1062,37 +1030,63 @@ extern "C" int morj_tree_attention_kv8_work(const int* qo_indptr_host, const int
       if (n <= kv8::FEW_ROWS) few_max = std::max(few_max, n);
     }
     const int few = few_max <= 8 ? 8 : 16;
+    // what the tiled segments see: the distinct pages in the order the lists name them, how many slots of each are
+    // listed, and every list entry's place among them
+    std::vector<int> place, pages, used, list;
     for (int s = 0; s < n_segments; ++s) {
       const int q_len = qo_indptr_host[s + 1] - qo_indptr_host[s];
-      const int pages = kv_indptr_host[s + 1] - kv_indptr_host[s];
-      const long long kv =
-          page_size == 1 || pages == 0
-              ? pages
-              : (long long)(pages - 1) * page_size + (kv_last_page_len_host ? kv_last_page_len_host[s] : page_size);
+      const int n_pages = kv_indptr_host[s + 1] - kv_indptr_host[s];
+      const int last = kv_last_page_len_host ? kv_last_page_len_host[s] : page_size;
+      const long long kv = page_size == 1 || n_pages == 0 ? n_pages : (long long)(n_pages - 1) * page_size + last;
       if (kv < 0 || kv > INT_MAX)
         return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8_work: segment %d has %lld keys", s, kv);
       const bool many = q_len * G > kv8::FEW_ROWS;
       const int tile = many ? kv8::T_ROWS : few;
+      int from = INT_MAX, to = -1;  // keys the segment's queries see
       for (int r0 = 0; r0 < q_len * G; r0 += tile) {
         int lo, hi, x;  // what the tile's first query sees from, its last query to
         kv8::visible(q_len, (int)kv, s < n_bidir, window, r0 / G, &lo, &x);
         kv8::visible(q_len, (int)kv, s < n_bidir, window, (std::min(r0 + tile, q_len * G) - 1) / G, &x, &hi);
         Item it{s, r0, 0, 0, -1, 1, 1, tile};
-        if (hi >= lo) it.t0 = lo, it.t1 = hi + 1;
+        if (hi >= lo) it.t0 = lo, it.t1 = hi + 1, from = std::min(from, lo), to = std::max(to, hi);
         (many ? tiles : rows).push_back(it);
       }
+      if (!many || to < from) continue;
+      if (list.empty()) list.resize(kv_indptr_host[n_segments], 0);
+      for (int p = from / page_size; p <= to / page_size; ++p) {
+        const int at = kv_indptr_host[s] + p, page = kv_indices_host[at];
+        if (page < 0) return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8_work: page %d in segment %d's list", page, s);
+        if ((size_t)page >= place.size()) place.resize(std::max<size_t>(page + 1, 2 * place.size()), -1);
+        if (place[page] < 0) {
+          place[page] = (int)pages.size();
+          pages.push_back(page);
+          used.push_back(0);
+        }
+        list[at] = place[page];
+        const int n = p == to / page_size ? to % page_size + 1 : page_size;
+        used[place[page]] = std::max(used[place[page]], n);
+      }
     }
+    if ((long long)pages.size() * page_size > INT_MAX - 64)
+      return set_error(MORJ_ERR_UNSUPPORTED, "morj_tree_attention_kv8_work: %zu pages of %d slots to expand", pages.size(),
+                       page_size);
+    std::vector<int> blocks;  // 64-slot blocks that hold listed slots
+    for (size_t i = 0; i < pages.size(); ++i) {
+      const long long first = (long long)pages[i] * page_size;
+      for (long long b = first / kv8::BLOCK; b <= (first + used[i] - 1) / kv8::BLOCK; ++b) blocks.push_back((int)b);
+    }
+    std::sort(blocks.begin(), blocks.end());
+    blocks.erase(std::unique(blocks.begin(), blocks.end()), blocks.end());
     int units = 0;
     const std::vector<Item> cut_tiles = kv8::cut(tiles, hk, num_sms() * kv8::T_CTAS, kv8::T_MIN_KEYS, units, joins);
     const std::vector<Item> cut_rows = kv8::cut(rows, hk, num_sms() * kv8::R_CTAS, kv8::R_MIN_KEYS, units, joins);
-    const size_t n_items = cut_tiles.size() + cut_rows.size() + joins.size();
-    counts[0] = (int)cut_rows.size();
-    counts[1] = (int)joins.size();
-    counts[2] = units;
-    counts[3] = few;
-    counts[4] = (int)(n_items * (sizeof(Item) / sizeof(int)));
-    counts[5] = (int)cut_tiles.size();
-    counts[6] = counts[7] = 0;
+    const size_t ints = (cut_tiles.size() + cut_rows.size() + joins.size()) * (sizeof(Item) / sizeof(int)) +
+                        2 * pages.size() + blocks.size() + list.size();
+    if (ints > (size_t)INT_MAX)
+      return set_error(MORJ_ERR_UNSUPPORTED, "morj_tree_attention_kv8_work: a work list of %zu ints", ints);
+    const int got[9] = {(int)cut_rows.size(), (int)joins.size(), units, few, (int)ints, (int)cut_tiles.size(),
+                        (int)pages.size(), (int)blocks.size(), (int)list.size()};
+    std::copy(got, got + 9, counts);
     if (counts[4] > cap) {
       if (cap == 0) return MORJ_OK;  // (a call that only asks for the counts)
       return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8_work: %d ints exceed capacity %d", counts[4], cap);
@@ -1100,11 +1094,24 @@ extern "C" int morj_tree_attention_kv8_work(const int* qo_indptr_host, const int
     Item* out = reinterpret_cast<Item*>(work_host);
     out = std::copy(cut_tiles.begin(), cut_tiles.end(), out);
     out = std::copy(cut_rows.begin(), cut_rows.end(), out);
-    std::copy(joins.begin(), joins.end(), out);
+    out = std::copy(joins.begin(), joins.end(), out);
+    int* rest = reinterpret_cast<int*>(out);
+    for (size_t i = 0; i < pages.size(); ++i) *rest++ = pages[i], *rest++ = used[i];
+    rest = std::copy(blocks.begin(), blocks.end(), rest);
+    std::copy(list.begin(), list.end(), rest);
     return MORJ_OK;
   } catch (...) {
     return set_error(MORJ_ERR_OOM, "morj_tree_attention_kv8_work: out of host memory");
   }
+}
+
+extern "C" int morj_tree_attention_kv8_workspace(const int* counts, int hk, int d, int page_size,
+                                                 unsigned long long* bytes) {
+  using namespace morj;
+  if (!counts || !bytes || hk <= 0 || d <= 0 || page_size <= 0 || counts[2] < 0 || counts[6] < 0)
+    return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8_workspace: bad arguments");
+  *bytes = kv8::Space(counts, hk, d, page_size).bytes;
+  return MORJ_OK;
 }
 
 extern "C" int morj_tree_attention_kv8(const void* q, int n_q, const void* k_codes, const float* k_scale,
@@ -1117,7 +1124,7 @@ extern "C" int morj_tree_attention_kv8(const void* q, int n_q, const void* k_cod
   if (!counts) return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8: null counts");
   if ((counts[0] == 0 && counts[5] == 0) || n_segments == 0) return MORJ_OK;
   if (!q || !k_codes || !k_scale || !v_codes || !v_scale || !out || !qo_indptr || !kv_indptr || !kv_indices || !work ||
-      n_q <= 0 || pool_slots <= 0 || counts[0] < 0 || counts[1] < 0 || counts[2] < 0 || counts[5] < 0)
+      n_q <= 0 || pool_slots <= 0 || counts[0] < 0 || counts[1] < 0 || counts[2] < 0 || counts[5] < 0 || counts[6] < 0 || counts[7] < 0)
     return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8: null pointer or bad size");
   if (hq <= 0 || hk <= 0 || hq % hk)
     return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8: hq=%d is not a multiple of hk=%d", hq, hk);
@@ -1131,7 +1138,7 @@ extern "C" int morj_tree_attention_kv8(const void* q, int n_q, const void* k_cod
        reinterpret_cast<uintptr_t>(out) | reinterpret_cast<uintptr_t>(work) | reinterpret_cast<uintptr_t>(workspace)) &
       15)
     return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8: q, codes, out, work and workspace must be 16-byte aligned");
-  const unsigned long long need = (unsigned long long)counts[2] * hk * kv8::UNIT * (d + 2) * sizeof(float);
+  const unsigned long long need = kv8::Space(counts, hk, d, page_size).bytes;
   if (workspace_bytes < need || (need && !workspace))
     return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8: a workspace of %llu bytes given, %llu needed",
                      workspace_bytes, need);
@@ -1142,7 +1149,8 @@ extern "C" int morj_tree_attention_kv8(const void* q, int n_q, const void* k_cod
   const int page_shift = l - 1;
   const kv8::Args a{(const __nv_bfloat16*)q, (const uint8_t*)k_codes, k_scale, (const uint8_t*)v_codes, v_scale,
                     (__nv_bfloat16*)out, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, n_bidir, hq, hk, page_size,
-                    page_magic, page_shift, window, pool_slots, sm_scale * kv8::LOG2E, (float*)workspace};
+                    page_magic, page_shift, window, pool_slots, sm_scale * kv8::LOG2E, nullptr};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  return d == 128 ? kv8::launch<128>(a, counts, work, s) : kv8::launch<64>(a, counts, work, s);
+  return d == 128 ? kv8::launch<128>(a, counts, work, (char*)workspace, s)
+                  : kv8::launch<64>(a, counts, work, (char*)workspace, s);
 }

@@ -173,10 +173,10 @@ class AttentionPlan:
         last = None if kv_last_page_len is None else np.ascontiguousarray(kv_last_page_len, dtype=np.int32)
         if last is not None and (len(last) != len(qo) - 1 or (last < 0).any() or (last > page_size).any()):
             raise ValueError('kv_last_page_len must have one entry in [0, page_size] per segment')
-        work, self.counts = nat.kv8_attention_work(qo, kv, n_bidir, hq, hk, window, page_size, last)
+        work, self.counts = nat.kv8_attention_work(qo, kv, kv_indices, n_bidir, hq, hk, window, page_size, last)
         self.n_q, self.segments, self.n_bidir = int(qo[-1]), len(qo) - 1, n_bidir
         self.hq, self.hk, self.d, self.page_size, self.window = hq, hk, d, page_size, window
-        self.workspace_bytes = nat.kv8_attention_workspace(self.counts, hk, d)
+        self.workspace_bytes = nat.kv8_attention_workspace(self.counts, hk, d, page_size)
         self.buf, (self.qo, self.kv, self.indices, self.last, self.work) = _upload(
             device, qo, kv, kv_indices, last if last is not None else [], work)
         self._ptrs = tuple(t.data_ptr() for t in (self.qo, self.kv, self.indices)) + (

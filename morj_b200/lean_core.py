@@ -741,7 +741,8 @@ class LeanGemma4:
         n_work = {}
         for kk, kind in (('s', 'sliding_attention'), ('g', 'full_attention')):
             sliding = kind == 'sliding_attention'
-            w, n_work[kk] = self._attention_work(qo, st['kv_indptr_' + kk], int(st['n_bidir']) if sliding else 0, kind)
+            w, n_work[kk] = self._attention_work(qo, st['kv_indptr_' + kk], st['kv_indices_' + kk],
+                                                 int(st['n_bidir']) if sliding else 0, kind)
             t.add('work_' + kk, w)
             if self.kv8:
                 w, n_work['store_' + kk] = nat.kv8_store_work(st['slots'][kk], pool_slots[kk])
@@ -769,17 +770,18 @@ class LeanGemma4:
             t.add('ro_qo', np.arange(len(rows) + 1))
             t.add('ro_kv_indptr', ptr)
             t.add('ro_kv_indices', np.concatenate(ind))
-            ro_work, n_work['ro'] = self._attention_work(np.arange(len(rows) + 1), ptr, 0, self.types[-1])
+            ro_work, n_work['ro'] = self._attention_work(np.arange(len(rows) + 1), ptr, np.concatenate(ind), 0,
+                                                          self.types[-1])
             t.add('ro_work', ro_work)
         t.upload()
         self.h2d_bytes += t.nbytes
         return t, rows, n_work
 
-    def _attention_work(self, qo, kv_indptr, n_bidir, kind):
+    def _attention_work(self, qo, kv_indptr, kv_indices, n_bidir, kind):
         """(work list, number of items, or the counts an 8-bit call takes) of one layer kind's attention call."""
         window = self.window if kind == 'sliding_attention' else 0
         if self.kv8:
-            return nat.kv8_attention_work(qo, kv_indptr, n_bidir, self.hq, self.geom[kind][0], window)
+            return nat.kv8_attention_work(qo, kv_indptr, kv_indices, n_bidir, self.hq, self.geom[kind][0], window)
         w = nat.attention_work(qo, kv_indptr, n_bidir, self.hq, self.geom[kind][0], window)
         return w, len(w) // 2
 

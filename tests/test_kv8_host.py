@@ -78,14 +78,42 @@ def test_attention_work_covers_every_row_and_key_once(spec, hq, hk, window, n_bi
     qo = np.concatenate([[0], np.cumsum([a for a, _ in spec])])
     kv = np.concatenate([[0], np.cumsum(pages)])
     last = [n - (p - 1) * page if p else 0 for (_, n), p in zip(spec, pages)]
-    work, counts = nat.kv8_attention_work(qo, kv, n_bidir, hq, hk, window, page, last)
+    perm = np.random.default_rng(len(spec)).permutation(int(kv[-1]) + 5)[:int(kv[-1])]
+    work, counts = nat.kv8_attention_work(qo, kv, perm, n_bidir, hq, hk, window, page, last)
     check_work(work, counts, spec, G, window, n_bidir)
+    check_pages(work, counts, spec, G, window, n_bidir, page, kv, perm)
+
+
+def check_pages(work, counts, spec, G, window, n_bidir, page, kv, indices):
+    """The pages the 128-row tiles see: each once, with the number of its slots that are listed; the lists point to them;
+    the blocks are the 64-slot blocks of those slots."""
+    n_rows, n_joins, _, _, _, n_tiles, n_pages, n_blocks, n_list = list(counts)[:9]
+    rest = work[(n_tiles + n_rows + n_joins) * ITEM:]
+    pairs, blocks, lists = rest[:2 * n_pages].reshape(-1, 2), rest[2 * n_pages:2 * n_pages + n_blocks], \
+        rest[2 * n_pages + n_blocks:]
+    assert len(lists) == n_list and len(set(pairs[:, 0].tolist())) == n_pages
+    slots = set()
+    for s, (n, keys) in enumerate(spec):
+        if n * G <= 16:
+            continue
+        seen = [view(n, keys, s < n_bidir, window, j) for j in range(n)]
+        seen = [(lo, hi) for lo, hi in seen if lo <= hi]
+        if not seen:
+            continue
+        for t in range(min(lo for lo, _ in seen), max(hi for _, hi in seen) + 1):
+            at = int(kv[s]) + t // page
+            p, used = pairs[lists[at]]
+            assert p == indices[at] and t % page < used
+            slots.add(int(p) * page + t % page)
+    assert sum(u for _, u in pairs) >= len(slots) and (n_list == int(kv[-1]) or not slots)
+    assert blocks.tolist() == sorted({x // 64 for p, u in pairs.tolist() for x in (p * page, p * page + u - 1)}
+                                     | {x // 64 for x in slots})
 
 
 def check_work(work, counts, spec, G, window, n_bidir):
     n_rows, n_joins, units, few, ints, n_tiles = list(counts)[:6]
-    items = work.reshape(-1, ITEM).tolist()
-    assert len(work) == ints and len(items) == n_tiles + n_rows + n_joins
+    items = work[:(n_tiles + n_rows + n_joins) * ITEM].reshape(-1, ITEM).tolist()
+    assert len(work) == ints
     parts, rows_of = {}, {}
     for i, (seg, r0, t0, t1, unit, _, _, rows) in enumerate(items[:n_tiles + n_rows]):
         # segments of more than 16 rows in 128-row tiles, the others in small ones
@@ -124,23 +152,27 @@ def check_work(work, counts, spec, G, window, n_bidir):
 
 
 def test_long_single_rows_are_cut_and_short_ones_are_not():
-    _, long = nat.kv8_attention_work([0, 1], [0, 20000], 0, 32, 16, 0)
+    _, long = nat.kv8_attention_work([0, 1], [0, 20000], np.arange(20000), 0, 32, 16, 0)
     assert long[1] == 1 and long[2] > 8
-    _, long = nat.kv8_attention_work([0, 64], [0, 20000], 0, 32, 16, 0)
+    _, long = nat.kv8_attention_work([0, 64], [0, 20000], np.arange(20000), 0, 32, 16, 0)
     assert long[5] > 1 and long[1] == 8 and long[2] == 8 * long[5]
-    _, short = nat.kv8_attention_work([0, 1], [0, 200], 0, 32, 16, 0)
+    _, short = nat.kv8_attention_work([0, 1], [0, 200], np.arange(200), 0, 32, 16, 0)
     assert short[1] == 0 and short[2] == 0
 
 
 def test_attention_work_refusals():
     for args in [dict(hq=3, hk=2), dict(hq=0, hk=1), dict(page_size=0), dict(n_bidir=2), dict(n_bidir=-1)]:
-        a = dict(qo_indptr=[0, 1], kv_indptr=[0, 4], n_bidir=0, hq=4, hk=2, window=0)
+        a = dict(qo_indptr=[0, 1], kv_indptr=[0, 4], kv_indices=range(4), n_bidir=0, hq=4, hk=2, window=0)
         with pytest.raises(ValueError):
             nat.kv8_attention_work(**{**a, **args})
     with pytest.raises(ValueError, match='out of order'):
-        nat.kv8_attention_work([0, 3, 1], [0, 4, 8], 0, 4, 2, 0)
+        nat.kv8_attention_work([0, 3, 1], [0, 4, 8], range(8), 0, 4, 2, 0)
     with pytest.raises(ValueError, match='out of order'):
-        nat.kv8_attention_work([0, 1, 2], [0, 4, 3], 0, 4, 2, 0)
+        nat.kv8_attention_work([0, 1, 2], [0, 4, 3], range(4), 0, 4, 2, 0)
+    with pytest.raises(ValueError, match='list entries'):
+        nat.kv8_attention_work([0, 1], [0, 4], range(3), 0, 4, 2, 0)
+    with pytest.raises(ValueError, match='page -1'):
+        nat.kv8_attention_work([0, 40], [0, 41], [-1] * 41, 0, 4, 2, 0)
 
 
 # a call's arguments are refused before any device access; 16 stands for an aligned pointer that is never read
@@ -183,7 +215,7 @@ def test_gather_refusals(kw):
 
 
 def attention_args(**kw):
-    counts = nat.KV8_COUNTS(*kw.pop('counts', (1, 0, 0, 8, 8, 0, 0, 0)))
+    counts = nat.KV8_COUNTS(*kw.pop('counts', (1, 0, 0, 8, 8)))
     a = dict(q=16, n_q=1, k=16, ks=16, v=16, vs=16, pool_slots=64, out=16, qo=16, kv=16, idx=16, last=None, n_segments=1,
              n_bidir=0, hq=4, hk=2, d=128, page=1, window=0, scale=1.0, work=16, counts=counts, ws=None, ws_bytes=0,
              stream=None)
@@ -197,8 +229,8 @@ def attention_args(**kw):
     (dict(idx=None), 'null pointer'), (dict(work=None), 'null pointer'), (dict(n_q=0), 'bad size'),
     (dict(pool_slots=0), 'bad size'), (dict(hq=3), 'multiple'), (dict(hk=0), 'multiple'), (dict(page=0), 'page_size'),
     (dict(n_bidir=2), 'n_bidir'), (dict(scale=0.0), 'sm_scale'), (dict(scale=-1.0), 'sm_scale'), (dict(q=24), '16-byte'), (dict(work=24), '16-byte'),
-    (dict(counts=(1, 1, 2, 8, 16, 0, 0, 0)), 'workspace of 0 bytes'),
-    (dict(counts=(1, 1, 2, 8, 16, 0, 0, 0), ws=16, ws_bytes=33279), '33280 needed')])
+    (dict(counts=(1, 1, 2, 8, 16)), 'workspace of 0 bytes'),
+    (dict(counts=(1, 1, 2, 8, 16), ws=16, ws_bytes=33279), '33280 needed')])
 def test_attention_refusals(kw, match):
     with pytest.raises(ValueError, match=match):
         nat.call('morj_tree_attention_kv8', *attention_args(**kw))
@@ -207,7 +239,7 @@ def test_attention_refusals(kw, match):
 def test_attention_refuses_other_head_sizes_and_accepts_nothing_to_do():
     with pytest.raises(nat.NativeFailure, match='head_dim 96'):
         nat.call('morj_tree_attention_kv8', *attention_args(d=96))
-    nat.call('morj_tree_attention_kv8', *attention_args(counts=(0,) * 8))
+    nat.call('morj_tree_attention_kv8', *attention_args(counts=(0,)))
 
 
 def test_pool_and_plan_refusals():
