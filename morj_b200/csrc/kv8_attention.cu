@@ -10,15 +10,9 @@
 // [1, 2) by a power of two before it is rounded to FP16, which keeps every bit of a BF16 row that matters at 2^-25 of
 // its largest element.
 //
-// A segment's rows are its (query, head of the group) pairs of one KV head. tile_kernel takes 128 rows at a time on
-// tcgen05; rows_kernel takes 8 or 16, for the single-token form (segments of at most 16 rows), where the codes' bytes
-// bound the call and 128-row tiles would be almost empty.
-//
-// rows_kernel: every
-// warp walks its own groups of 32 keys with mma.m16n8k16, operands straight from global memory: the fragment layouts
-// leave the order of the head dimension (QK) and of the output columns (PV) free, so each lane reads 16 or 32
-// consecutive codes of a key. The host cuts the keys of a tile into parts until the SMs are filled; parts leave
-// (maximum, sum, O) in a workspace and combine_kernel joins them.
+// A segment's rows are its (query, head of the group) pairs of one KV head. Segments of at most 16 rows go to
+// rows_kernel, larger ones in tiles of 128 to tile_kernel. The host cuts the keys of a tile into parts until the SMs are
+// filled once; parts leave (maximum, sum, O) in a workspace and combine_kernel joins them in a fixed order.
 #include <algorithm>
 #include <climits>
 #include <vector>
@@ -31,7 +25,7 @@ namespace kv8 {
 constexpr float LOG2E = 1.4426950408889634f;
 constexpr int UNIT = 16;             // rows of a partial unit in the workspace
 constexpr int WARPS = 4;
-constexpr int STEP = 32;             // keys a warp takes at a time
+constexpr int STEP = 32;             // keys a warp of rows_kernel takes at a time
 constexpr int T_ROWS = 128;           // rows of a tile_kernel tile
 constexpr int BN = 64;                // keys it takes at a time
 constexpr int FEW_ROWS = 16;         // segments of at most this many rows go to rows_kernel
@@ -102,16 +96,6 @@ MORJ_DEV long long slot_of(const Args& a, int entry, int t) {
   return (long long)entry * a.page_size + (t - page_of(a, t) * a.page_size);
 }
 
-// pool slot of key t of a segment, -1 (device error recorded) outside the pool
-MORJ_DEV int key_slot(const Args& a, int kv_base, int t) {
-  const long long slot = slot_of(a, __ldg(a.kv_indices + kv_base + page_of(a, t)), t);
-  if (slot < 0 || slot >= a.pool_slots) {
-    report(kErrBadIndex);
-    return -1;
-  }
-  return (int)slot;
-}
-
 MORJ_DEV void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
@@ -142,19 +126,53 @@ MORJ_DEV float row_scale(float amax) {
   return e == 0x7f800000u ? 1.f : __uint_as_float(e == 0 ? 0x00800000u : e);
 }
 
-// N consecutive codes of one head of a pool row
-template <int N>
-MORJ_DEV void load_codes(const uint8_t* p, bool ok, uint32_t (&w)[N / 4]) {
-  if constexpr (N == 8) {
-    const uint2 u = ok ? __ldg(reinterpret_cast<const uint2*>(p)) : make_uint2(0, 0);
-    w[0] = u.x, w[1] = u.y;
-  } else {
-#pragma unroll
-    for (int i = 0; i < N / 16; ++i) {
-      const uint4 u = ok ? __ldg(reinterpret_cast<const uint4*>(p) + i) : make_uint4(0, 0, 0, 0);
-      w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
-    }
-  }
+// ---------------------------------------------------------------------------------------------------------------
+// Few rows per segment (at most 16; the single-token form): the codes' bytes bound the call, so a warp keeps two groups
+// of 32 keys in flight (cp.async, 16 KB) while it works on a third, eight warps an SM. Groups are taken in turn by the
+// four warps of a CTA; keys are one lane each for their page entry (two groups ahead) and scales. In a group the rows of
+// K and V lie as they come, 16-byte units XOR-swizzled by the key, so both products read their fragments without bank
+// conflicts: mma.m16n8k16 leaves the order of the head dimension (q . k) and of the output columns (P V) free, and each
+// lane takes 32 (16) consecutive codes of a K row and 16 (8) of a V row for D = 128 (64). The loop is 16 keys long to
+// keep its code small: unrolled over 32 keys it was 16 KB, and a CTA that runs it four times spent most of its time
+// fetching instructions (9 readout rows of 1,560 keys: 41 us).
+// ---------------------------------------------------------------------------------------------------------------
+constexpr int R_STAGES = 3;
+
+template <int D>
+struct RSmem {
+  static constexpr int SIDE = STEP * D;                    // codes of one group, K or V
+  static constexpr int STAGE = 2 * SIDE + 2 * STEP * 4;    // K, V, K scales, V scales
+  static constexpr int RING = R_STAGES * STAGE;            // of one warp
+  static constexpr int TOTAL = WARPS * RING;
+  static_assert(TOTAL >= WARPS * 16 * (D + 2) * 4, "the warps' results are joined in the rings");
+};
+
+MORJ_DEV void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+MORJ_DEV void cp_async4(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+MORJ_DEV uint4 lds16(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+  return v;
+}
+MORJ_DEV uint2 lds8(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+MORJ_DEV float lds4(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr));
+  return v;
+}
+
+// byte offset of 16-byte unit u of key k's row in a group
+template <int D>
+MORJ_DEV uint32_t unit_at(int k, int u) {
+  return D == 128 ? (uint32_t)(k * 128 + ((u ^ (k & 7)) << 4)) : (uint32_t)(k * 64 + ((u ^ ((k >> 1) & 3)) << 4));
 }
 
 // ROWS = 8 or 16 rows per tile. Rows 8..15 of the MMA's 16 are zeros when ROWS = 8 and cost no registers.
@@ -162,13 +180,14 @@ template <int D, int ROWS>
 __global__ void __launch_bounds__(WARPS * 32) rows_kernel(const Args a, const Item* __restrict__ items) {
   pdl_wait();  // the previous kernel on the stream has completed
   pdl_trigger();
+  using L = RSmem<D>;
   constexpr int KS = D / 16;       // MMA depth steps of q . k
   constexpr int NT = D / 8;        // 8-column output tiles
   constexpr int HALVES = ROWS / 8;
   constexpr int KRUN = D / 4;      // consecutive codes of a key one lane reads of K
   constexpr int VRUN = D / 8;      // ... and of V
-  __shared__ float sh_o[WARPS][ROWS][D];
-  __shared__ float sh_m[WARPS][ROWS], sh_l[WARPS][ROWS];
+  constexpr int LPR = D / 16;      // 16-byte units of a row
+  extern __shared__ __align__(128) uint8_t smem[];
 
   const Item it = items[blockIdx.x / a.hk];
   const int h = blockIdx.x % a.hk;
@@ -179,39 +198,84 @@ __global__ void __launch_bounds__(WARPS * 32) rows_kernel(const Args a, const It
   const int G = a.hq / a.hk, n_rows = sg.q_len * G;
   const int t_end = min(it.t1, sg.kv_len);
 
-  // this lane's rows: r0 + g and r0 + g + 8
+  // ---- the warp's groups: keys [it.t0 + 32 (warp + 4 i), + 32)
+  const uint32_t ring = smem_u32(smem) + warp * L::RING;
+  const int t_first = it.t0 + warp * STEP;
+  const int groups = t_first < t_end ? (t_end - t_first + WARPS * STEP - 1) / (WARPS * STEP) : 0;
+  const int* list = a.kv_indices + sg.kv_base;
+  const unsigned row_bytes = (unsigned)a.hk * D;
+  const uint8_t* kc = a.k + (size_t)h * D + (lane % LPR) * 16;
+  const uint8_t* vc = a.v + (size_t)h * D + (lane % LPR) * 16;
+  auto key = [&](int i) { return t_first + i * (WARPS * STEP) + lane; };
+  auto entry = [&](int i) { return i < groups ? __ldg(list + page_of(a, min(key(i), t_end - 1))) : 0; };
+  auto issue = [&](int i, int e) {  // ask for group i; e: the lane's page entry
+    if (i < groups) {
+      const uint32_t st = ring + (i % R_STAGES) * L::STAGE;
+      const int t = key(i);
+      const long long at = slot_of(a, e, min(t, t_end - 1));
+      const bool in_pool = at >= 0 && at < a.pool_slots;
+      if (!in_pool) report(kErrBadIndex);
+      const bool ok = t < t_end && in_pool;
+      const unsigned slot = in_pool ? (unsigned)at : 0u;
+      const unsigned there = __ballot_sync(0xffffffffu, ok);
+      const size_t si = (size_t)(slot >> BLOCK_SHIFT) * a.hk + h;
+      cp_async4(st + 2 * L::SIDE + lane * 4, a.ks + si, ok ? 4u : 0u);
+      cp_async4(st + 2 * L::SIDE + STEP * 4 + lane * 4, a.vs + si, ok ? 4u : 0u);
+#pragma unroll 4
+      for (int k = lane / LPR; k < STEP; k += 32 / LPR) {
+        const unsigned long long off = (unsigned long long)__shfl_sync(0xffffffffu, slot, k) * row_bytes;
+        const uint32_t n = (there >> k) & 1 ? 16u : 0u;
+        cp_async16(st + unit_at<D>(k, lane % LPR), kc + off, n);
+        cp_async16(st + L::SIDE + unit_at<D>(k, lane % LPR), vc + off, n);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  int e_next = entry(0);
+#pragma unroll 1
+  for (int i = 0; i < R_STAGES - 1; ++i) {
+    const int e = e_next;
+    e_next = entry(i + 1);
+    issue(i, e);
+  }
+
+  // ---- this lane's rows: r0 + g and r0 + g + 8
   uint32_t qf[HALVES][KS][2];
   float qs[HALVES];
   int lo[HALVES], hi[HALVES];
 #pragma unroll
   for (int b = 0; b < HALVES; ++b) {
     const int r = it.r0 + g + 8 * b;
-    lo[b] = INT_MAX, hi[b] = -1, qs[b] = 0.f;
-    float v[KRUN];
+    lo[b] = INT_MAX, hi[b] = -1;
+    uint4 raw[KRUN / 8];
 #pragma unroll
-    for (int i = 0; i < KRUN; ++i) v[i] = 0.f;
+    for (int i = 0; i < KRUN / 8; ++i) raw[i] = make_uint4(0, 0, 0, 0);
     if (r < n_rows) {
       visible(sg.q_len, sg.kv_len, bidir, a.window, r / G, &lo[b], &hi[b]);
-      const __nv_bfloat16* src = a.q + ((size_t)(sg.q_start + r / G) * a.hq + h * G + r % G) * D + c4 * KRUN;
+      const uint4* src = reinterpret_cast<const uint4*>(
+          a.q + ((size_t)(sg.q_start + r / G) * a.hq + h * G + r % G) * D + c4 * KRUN);
 #pragma unroll
-      for (int i = 0; i < KRUN; i += 8) {
-        float x[8];
-        load8(src + i, x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[i + e] = x[e];
-      }
+      for (int i = 0; i < KRUN / 8; ++i) raw[i] = __ldg(src + i);
     }
     float amax = 0.f;
 #pragma unroll
-    for (int i = 0; i < KRUN; ++i) amax = fmaxf(amax, fabsf(v[i]));
+    for (int i = 0; i < KRUN / 8; ++i) {
+      float x[8];
+      unpack8(raw[i], x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
+    }
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
     amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
     qs[b] = row_scale(amax);
     const float inv = 1.f / qs[b];
+    qs[b] *= a.scale_log2;
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-      qf[b][s][0] = pack_f16x2(v[4 * s] * inv, v[4 * s + 1] * inv);
-      qf[b][s][1] = pack_f16x2(v[4 * s + 2] * inv, v[4 * s + 3] * inv);
+    for (int i = 0; i < KRUN / 8; ++i) {
+      float x[8];
+      unpack8(raw[i], x);
+      qf[b][2 * i][0] = pack_f16x2(x[0] * inv, x[1] * inv), qf[b][2 * i][1] = pack_f16x2(x[2] * inv, x[3] * inv);
+      qf[b][2 * i + 1][0] = pack_f16x2(x[4] * inv, x[5] * inv), qf[b][2 * i + 1][1] = pack_f16x2(x[6] * inv, x[7] * inv);
     }
   }
 
@@ -223,152 +287,162 @@ __global__ void __launch_bounds__(WARPS * 32) rows_kernel(const Args a, const It
   for (int b = 0; b < HALVES; ++b) m[b] = -INFINITY, l[b] = 0.f;
   float vref = 0.f;  // the largest V scale met: O is in units of vref / P_SCALE
 
-  const size_t head_off = (size_t)h * D;
-  const size_t row_codes = (size_t)a.hk * D;
-  for (int base = it.t0 + warp * STEP; base < t_end; base += WARPS * STEP) {
-    // lane = key: its pool row and scales
-    int slot = -1;
-    float kf = 0.f, vf = 0.f;
-    if (base + lane < t_end) slot = key_slot(a, sg.kv_base, base + lane);
-    if (slot >= 0) {
-      const size_t si = (size_t)(slot >> BLOCK_SHIFT) * a.hk + h;
-      kf = __ldg(a.ks + si) * a.scale_log2;
-      vf = __ldg(a.vs + si);
+#pragma unroll 1
+  for (int i = 0; i < groups; ++i) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(R_STAGES - 2) : "memory");
+    __syncwarp();  // group i has landed for every lane; every lane is done with the group whose place is refilled now
+    {
+      const int e = e_next;
+      e_next = entry(i + R_STAGES);
+      issue(i + R_STAGES - 1, e);
     }
-    uint32_t kw[4][KRUN / 4], vw[2][4][VRUN / 4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int s = __shfl_sync(0xffffffffu, slot, j * 8 + g);
-      load_codes<KRUN>(a.k + (s < 0 ? 0 : (size_t)s * row_codes + head_off + c4 * KRUN), s >= 0, kw[j]);
-    }
-#pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int s = __shfl_sync(0xffffffffu, slot, kk * 16 + (e >> 1) * 8 + c4 * 2 + (e & 1));
-        load_codes<VRUN>(a.v + (s < 0 ? 0 : (size_t)s * row_codes + head_off + g * VRUN), s >= 0, vw[kk][e]);
-      }
-    // V scales: O moves to the new unit when a larger one appears
-    float vmax = vf;
-#pragma unroll
-    for (int x = 16; x > 0; x >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, x));
+    const uint32_t st = ring + (i % R_STAGES) * L::STAGE;
+    const uint32_t kf_at = st + 2 * L::SIDE, vf_at = kf_at + STEP * 4;
+    const int base = t_first + i * (WARPS * STEP);
+    // V scales: O moves to the new unit when a larger one appears (as unsigned bits a NaN is the largest)
+    const float vmax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(lds4(vf_at + lane * 4))));
     float unit = 1.f;  // old unit / new unit
-    if (vmax > vref) {
+    if (!(vmax <= vref)) {
       unit = vref / vmax;
       vref = vmax;
     }
-    vf *= vref > 0.f ? P_SCALE / vref : 0.f;
-
-    // scores of 8 keys per MMA column tile: rows g (and g + 8), keys c4 * 2 + {0, 1}
-    float s[4][4];
+    const float inv_v = vref != 0.f ? P_SCALE / vref : 0.f;
+#pragma unroll 1
+    for (int sub = 0; sub < STEP; sub += 16) {
+      // scores of 8 keys per MMA column tile: rows g (and g + 8), keys c4 * 2 + {0, 1}
+      float s[2][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+      for (int j = 0; j < 2; ++j) {
+        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
+        const int k = sub + j * 8 + g;
+        uint32_t w[KRUN / 4];
 #pragma unroll
-      for (int x = 0; x < KS; ++x) {
-        const uint32_t b0 = codes2_f16(kw[j][x] & 0xffffu), b1 = codes2_f16(kw[j][x] >> 16);
-        if constexpr (HALVES == 2)
-          mma_f16(s[j], qf[0][x][0], qf[1][x][0], qf[0][x][1], qf[1][x][1], b0, b1);
-        else
-          mma_f16_top(s[j], qf[0][x][0], qf[0][x][1], b0, b1);
-      }
-    }
-    float mx[HALVES];
+        for (int u = 0; u < KRUN / 16; ++u) {
+          const uint4 x = lds16(st + unit_at<D>(k, c4 * (KRUN / 16) + u));
+          w[4 * u] = x.x, w[4 * u + 1] = x.y, w[4 * u + 2] = x.z, w[4 * u + 3] = x.w;
+        }
 #pragma unroll
-    for (int b = 0; b < HALVES; ++b) mx[b] = -INFINITY;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int key = j * 8 + c4 * 2 + e, t = base + key;
-        const float f = __shfl_sync(0xffffffffu, kf, key);
-#pragma unroll
-        for (int b = 0; b < HALVES; ++b) {
-          float& x = s[j][2 * b + e];
-          x = (t >= lo[b] && t <= hi[b] && t < t_end) ? x * (f * qs[b]) : -INFINITY;
-          mx[b] = max_nan(mx[b], x);
+        for (int x = 0; x < KS; ++x) {
+          const uint32_t b0 = codes2_f16(w[x]), b1 = codes2_f16(w[x] >> 16);
+          if constexpr (HALVES == 2)
+            mma_f16(s[j], qf[0][x][0], qf[1][x][0], qf[0][x][1], qf[1][x][1], b0, b1);
+          else
+            mma_f16_top(s[j], qf[0][x][0], qf[0][x][1], b0, b1);
         }
       }
-    float alpha[HALVES];
+      float mx[HALVES];
 #pragma unroll
-    for (int b = 0; b < HALVES; ++b) {
-      mx[b] = max_nan(mx[b], __shfl_xor_sync(0xffffffffu, mx[b], 1));
-      mx[b] = max_nan(mx[b], __shfl_xor_sync(0xffffffffu, mx[b], 2));
-      const float now = max_nan(m[b], mx[b]);
-      alpha[b] = m[b] == -INFINITY ? 0.f : exp2f(m[b] - now);
-      m[b] = now;
-      l[b] *= alpha[b];
-      alpha[b] *= unit;
-    }
-    if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[HALVES - 1] != 1.f)) {
+      for (int b = 0; b < HALVES; ++b) mx[b] = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < NT; ++j)
+      for (int j = 0; j < 2; ++j) {
+        const uint2 f2 = lds8(kf_at + (sub + j * 8 + c4 * 2) * 4);
 #pragma unroll
-        for (int b = 0; b < HALVES; ++b) o[j][2 * b] *= alpha[b], o[j][2 * b + 1] *= alpha[b];
-    }
-    uint32_t pf[HALVES][4];
+        for (int e = 0; e < 2; ++e) {
+          const int t = base + sub + j * 8 + c4 * 2 + e;
+          const float f = __uint_as_float(e ? f2.y : f2.x);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float f0 = __shfl_sync(0xffffffffu, vf, j * 8 + c4 * 2), f1 = __shfl_sync(0xffffffffu, vf, j * 8 + c4 * 2 + 1);
+          for (int b = 0; b < HALVES; ++b) {
+            float& x = s[j][2 * b + e];
+            x = (t >= lo[b] && t <= hi[b] && t < t_end) ? x * (f * qs[b]) : -INFINITY;
+            mx[b] = max_nan(mx[b], x);
+          }
+        }
+      }
+      float alpha[HALVES];
 #pragma unroll
       for (int b = 0; b < HALVES; ++b) {
-        const float shift = m[b] == -INFINITY ? 0.f : m[b];
-        const float p0 = exp2f(s[j][2 * b] - shift), p1 = exp2f(s[j][2 * b + 1] - shift);
-        l[b] += p0 + p1;
-        pf[b][j] = pack_f16x2(p0 * f0, p1 * f1);
+        mx[b] = max_nan(mx[b], __shfl_xor_sync(0xffffffffu, mx[b], 1));
+        mx[b] = max_nan(mx[b], __shfl_xor_sync(0xffffffffu, mx[b], 2));
+        const float now = max_nan(m[b], mx[b]);
+        alpha[b] = m[b] == -INFINITY ? 0.f : exp2f(m[b] - now);
+        m[b] = now;
+        l[b] *= alpha[b];
+        alpha[b] *= unit;
       }
-    }
+      unit = 1.f;
+      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[HALVES - 1] != 1.f)) {
 #pragma unroll
-    for (int kk = 0; kk < 2; ++kk)
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int b = 0; b < HALVES; ++b) o[j][2 * b] *= alpha[b], o[j][2 * b + 1] *= alpha[b];
+      }
+      uint32_t pf[HALVES][2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        const uint2 f2 = lds8(vf_at + (sub + j * 8 + c4 * 2) * 4);
+        const float f0 = __uint_as_float(f2.x) * inv_v, f1 = __uint_as_float(f2.y) * inv_v;
+#pragma unroll
+        for (int b = 0; b < HALVES; ++b) {
+          const float shift = m[b] == -INFINITY ? 0.f : m[b];
+          const float p0 = exp2f(s[j][2 * b] - shift), p1 = exp2f(s[j][2 * b + 1] - shift);
+          l[b] += p0 + p1;
+          pf[b][j] = pack_f16x2(p0 * f0, p1 * f1);
+        }
+      }
+      // V of keys c4 * 2 + {0, 1, 8, 9}, output columns g * VRUN ..: four columns a word, paired per column
+      uint32_t vw[4][VRUN / 4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int k = sub + (e >> 1) * 8 + c4 * 2 + (e & 1);
+        if constexpr (VRUN == 16) {
+          const uint4 x = lds16(st + L::SIDE + unit_at<D>(k, g));
+          vw[e][0] = x.x, vw[e][1] = x.y, vw[e][2] = x.z, vw[e][3] = x.w;
+        } else {
+          const uint2 x = lds8(st + L::SIDE + unit_at<D>(k, g >> 1) + (g & 1) * 8);
+          vw[e][0] = x.x, vw[e][1] = x.y;
+        }
+      }
 #pragma unroll
       for (int w = 0; w < VRUN / 4; ++w) {
-        // four output columns: the codes of keys (0, 1) and (8, 9) of the 16-key step, paired per column
-        const uint32_t a01 = prmt(vw[kk][0][w], vw[kk][1][w], 0x5140), a23 = prmt(vw[kk][0][w], vw[kk][1][w], 0x7362);
-        const uint32_t b01 = prmt(vw[kk][2][w], vw[kk][3][w], 0x5140), b23 = prmt(vw[kk][2][w], vw[kk][3][w], 0x7362);
-        const uint32_t av[4] = {a01 & 0xffffu, a01 >> 16, a23 & 0xffffu, a23 >> 16};
-        const uint32_t bv[4] = {b01 & 0xffffu, b01 >> 16, b23 & 0xffffu, b23 >> 16};
+        const uint32_t a01 = prmt(vw[0][w], vw[1][w], 0x5140), a23 = prmt(vw[0][w], vw[1][w], 0x7362);
+        const uint32_t b01 = prmt(vw[2][w], vw[3][w], 0x5140), b23 = prmt(vw[2][w], vw[3][w], 0x7362);
+        const uint32_t av[4] = {a01, a01 >> 16, a23, a23 >> 16}, bv[4] = {b01, b01 >> 16, b23, b23 >> 16};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const uint32_t b0 = codes2_f16(av[e]), b1 = codes2_f16(bv[e]);
           if constexpr (HALVES == 2)
-            mma_f16(o[4 * w + e], pf[0][2 * kk], pf[1][2 * kk], pf[0][2 * kk + 1], pf[1][2 * kk + 1], b0, b1);
+            mma_f16(o[4 * w + e], pf[0][0], pf[1][0], pf[0][1], pf[1][1], b0, b1);
           else
-            mma_f16_top(o[4 * w + e], pf[0][2 * kk], pf[0][2 * kk + 1], b0, b1);
+            mma_f16_top(o[4 * w + e], pf[0][0], pf[0][1], b0, b1);
         }
       }
+    }
   }
 
-  // the four warps' results, joined
+  // the four warps' results, joined in the rings
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  float* sh_o = reinterpret_cast<float*>(smem);        // [warp][row][D]
+  float* sh_m = sh_o + WARPS * ROWS * D;               // [warp][row]
+  float* sh_l = sh_m + WARPS * ROWS;
   const float scale_o = vref / P_SCALE;
 #pragma unroll
   for (int b = 0; b < HALVES; ++b) {
     l[b] += __shfl_xor_sync(0xffffffffu, l[b], 1);
     l[b] += __shfl_xor_sync(0xffffffffu, l[b], 2);
     const int r = g + 8 * b;
-    if (c4 == 0) sh_m[warp][r] = m[b], sh_l[warp][r] = l[b];
+    if (c4 == 0) sh_m[warp * ROWS + r] = m[b], sh_l[warp * ROWS + r] = l[b];
     // column tile j, column n of the MMA is output column n * VRUN + j
+    float* dst = sh_o + (warp * ROWS + r) * D + 2 * c4 * VRUN;
 #pragma unroll
-    for (int j = 0; j < NT; ++j) {
-      sh_o[warp][r][(2 * c4) * VRUN + j] = o[j][2 * b] * scale_o;
-      sh_o[warp][r][(2 * c4 + 1) * VRUN + j] = o[j][2 * b + 1] * scale_o;
-    }
+    for (int j = 0; j < NT; ++j) dst[j] = o[j][2 * b] * scale_o, dst[VRUN + j] = o[j][2 * b + 1] * scale_o;
   }
   __syncthreads();
   float* part = it.unit < 0 ? nullptr : a.ws + ((size_t)it.unit * a.hk + h) * (UNIT * (D + 2));
+#pragma unroll 1
   for (int i = threadIdx.x; i < ROWS * D; i += WARPS * 32) {
     const int r = i / D, d = i % D;
     if (it.r0 + r >= n_rows) break;
     float mm = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      mm = fmaxf(mm, sh_m[w][r]);
-    }
+    for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, sh_m[w * ROWS + r]);
     float ll = 0.f, oo = 0.f;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
-      const float f = sh_m[w][r] == -INFINITY ? 0.f : exp2f(sh_m[w][r] - mm);
-      ll += f * sh_l[w][r];
-      oo += f * sh_o[w][r][d];
+      const float mw = sh_m[w * ROWS + r];
+      const float f = mw == -INFINITY ? 0.f : exp2f(mw - mm);
+      ll += f * sh_l[w * ROWS + r];
+      oo += f * sh_o[(w * ROWS + r) * D + d];
     }
     if (part) {
       if (d == 0) part[r] = mm, part[UNIT + r] = ll;
@@ -476,8 +550,8 @@ __global__ void __launch_bounds__(E_THREADS) expand_kernel(const Args a, const i
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int T_THREADS = 256;          // (warp 7 has no role)
 constexpr int T_TMEM_COLS = 256;        // S/P buffers at columns [0, 64) and [64, 128), O at [128, 128 + D)
-constexpr float T_RESCALE_LOG2 = 4.0f;  // O is rescaled when a row's maximum grows by more than 2^4, so that
-constexpr float T_P_LOG2 = 11.0f;       // 2^11 p <= 2^15 stays inside FP16
+constexpr float T_RESCALE_LOG2 = 8.0f;  // O is rescaled when a row's maximum grows by more than 2^8 (2^4: 3-4% slower),
+constexpr float T_P_LOG2 = 7.0f;        // so that 2^7 p <= 2^15 stays inside FP16: p's smallest step is 2^-31
 
 template <int D>
 struct TSmem {
@@ -486,7 +560,7 @@ struct TSmem {
   static constexpr int K_OFF = Q_BYTES;               // 2 buffers
   static constexpr int V_OFF = K_OFF + 2 * KV_BYTES;  // 2 buffers
   static constexpr int BAR_OFF = V_OFF + 2 * KV_BYTES;
-  // barriers: q_full, k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], done; TMEM slot, abort flag
+  // barriers: (unused), k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], done; TMEM slot, abort flag
   static constexpr int TOTAL = BAR_OFF + 128;
 };
 
@@ -523,9 +597,6 @@ MORJ_DEV float max3f(float a, float b, float c) {
 }
 MORJ_DEV void sts16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-MORJ_DEV void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 // warp-level wait: lane 0 polls the barrier, the warp follows its verdict (and sees what lane 0 sees)
 MORJ_DEV bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
@@ -582,7 +653,7 @@ __global__ void __launch_bounds__(T_THREADS, 2)
     return;
   }
   const uint32_t bar0 = sbase + L::BAR_OFF;
-  const uint32_t q_full = bar0, k_full = bar0 + 8, v_full = bar0 + 24;
+  const uint32_t k_full = bar0 + 8, v_full = bar0 + 24;
   const uint32_t s_full = bar0 + 40, p_full = bar0 + 56, pv_done = bar0 + 72, done = bar0 + 88;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::BAR_OFF + 96);
   volatile int* abort = reinterpret_cast<volatile int*>(smem + L::BAR_OFF + 100);
@@ -598,12 +669,11 @@ __global__ void __launch_bounds__(T_THREADS, 2)
   const int n_chunks = t_stop > it.t0 ? (t_stop - t_begin + BN - 1) / BN : 0;
 
   if (threadIdx.x == 0) {
-    mbar_init(q_full, 4);  // one arrival per softmax warp
     for (int b = 0; b < 2; ++b) {
       mbar_init(k_full + 8 * b, 1);
       mbar_init(v_full + 8 * b, 1);
       mbar_init(s_full + 8 * b, 1);
-      mbar_init(p_full + 8 * b, 4);
+      mbar_init(p_full + 8 * b, 4);  // one arrival per softmax warp
       mbar_init(pv_done + 8 * b, 1);
     }
     mbar_init(done, 1);
@@ -613,6 +683,39 @@ __global__ void __launch_bounds__(T_THREADS, 2)
   if (warp == 4) {
     tmem_alloc(smem_u32(tmem_slot), T_TMEM_COLS);
     tmem_relinquish();
+  }
+  // softmax warps: thread = row
+  const int r = (warp & 3) * 32 + lane, row = it.r0 + r, qi = row / G;
+  const bool row_ok = row < n_rows;
+  const size_t row_at = ((size_t)(sg.q_start + qi) * a.hq + h * G + row % G) * D;
+  float scale = 0.f, vr = 0.f;  // scores times `scale` are in the log2 domain; V's reference
+  if (warp < 4) {
+    // Q row: its largest magnitude, then FP16 of q / qs into the swizzled tile (read twice, the second time from L1: the
+    // row in registers would be 64 of them)
+    const float kr = refs ? __ldg(refs + h) : 0.f;
+    vr = refs ? __ldg(refs + a.hk + h) : 0.f;
+    const uint4* src = reinterpret_cast<const uint4*>(a.q + row_at);
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    float amax = 0.f;
+#pragma unroll 8
+    for (int i = 0; i < D / 8; ++i) {
+      float x[8];
+      unpack8(row_ok ? __ldg(src + i) : zero, x);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
+    }
+    const float qs = row_scale(amax), inv = 1.f / qs;
+#pragma unroll 4
+    for (int i = 0; i < D / 8; ++i) {
+      float x[8];
+      unpack8(row_ok ? __ldg(src + i) : zero, x);
+      sts16(sbase + (i >> 3) * (T_ROWS * 128) + sw128_offset(r, i & 7), pack_f16x2(x[0] * inv, x[1] * inv),
+            pack_f16x2(x[2] * inv, x[3] * inv), pack_f16x2(x[4] * inv, x[5] * inv),
+            pack_f16x2(x[6] * inv, x[7] * inv));
+    }
+    fence_proxy_async_smem();
+    scale = qs * kr * a.scale_log2;
+    scale = scale < 1.2e-38f ? 1.2e-38f : scale;  // (a masked score stays -inf times it)
   }
   tc_fence_before();
   __syncthreads();
@@ -648,7 +751,7 @@ __global__ void __launch_bounds__(T_THREADS, 2)
     if (lane == 0) {
       constexpr uint32_t IDESC_S = idesc_f16(T_ROWS, BN);
       constexpr uint32_t IDESC_O = idesc_f16(T_ROWS, D, /*b_mn_major=*/true);
-      bool ok = n_chunks > 0 && mbar_wait(q_full, 0, abort, kErrTimeoutAttention);
+      bool ok = n_chunks > 0;
       // operand descriptors: one per buffer, advanced per 16-deep K step by the byte offset (>> 4)
       const uint64_t q_desc = sw128_desc(sbase);
       const uint64_t k_desc0 = sw128_desc(sbase + L::K_OFF), v_desc0 = sw128_desc(sbase + L::V_OFF, BN * 128);
@@ -691,40 +794,7 @@ __global__ void __launch_bounds__(T_THREADS, 2)
     }
   } else if (warp < 4) {
     // ---------------- softmax warpgroup ----------------
-    const int r = warp * 32 + lane;
     const uint32_t t_lane = tmem + ((uint32_t)(warp * 32) << 16);
-    const int row = it.r0 + r, qi = row / G;
-    const bool row_ok = row < n_rows;
-    const size_t row_at = ((size_t)(sg.q_start + qi) * a.hq + h * G + row % G) * D;
-    // Q row: its largest magnitude, then FP16 of q / qs into the swizzled tile
-    float scale;  // scores times it are in the log2 domain
-    {
-      // (read twice, the second time from L1: the row in registers would be 64 of them)
-      const uint4* src = reinterpret_cast<const uint4*>(a.q + row_at);
-      const uint4 zero = make_uint4(0, 0, 0, 0);
-      float amax = 0.f;
-#pragma unroll 4
-      for (int i = 0; i < D / 8; ++i) {
-        float x[8];
-        unpack8(row_ok ? __ldg(src + i) : zero, x);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
-      }
-      const float qs = row_scale(amax), inv = 1.f / qs;
-#pragma unroll 4
-      for (int i = 0; i < D / 8; ++i) {
-        float x[8];
-        unpack8(row_ok ? __ldg(src + i) : zero, x);
-        sts16(sbase + (i >> 3) * (T_ROWS * 128) + sw128_offset(r, i & 7), pack_f16x2(x[0] * inv, x[1] * inv),
-              pack_f16x2(x[2] * inv, x[3] * inv), pack_f16x2(x[4] * inv, x[5] * inv),
-              pack_f16x2(x[6] * inv, x[7] * inv));
-      }
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(q_full);
-      scale = qs * (refs ? refs[h] : 0.f) * a.scale_log2;
-      scale = scale < 1.2e-38f ? 1.2e-38f : scale;  // (a masked score stays -inf times it)
-    }
     int lo = 1, hi = 0;  // visible key positions [lo, hi] of this part
     if (row_ok) {
       visible(sg.q_len, sg.kv_len, bidir, a.window, qi, &lo, &hi);
@@ -820,7 +890,6 @@ __global__ void __launch_bounds__(T_THREADS, 2)
     if (ok && (n_chunks == 0 || warp_wait(pv_done + 8 * ((n_chunks - 1) & 1), ((n_chunks - 1) >> 1) & 1, abort))) {
       tc_fence_after();
       // a finished row: O / l times V's reference; a part: (maximum, sum, O in units of the values)
-      const float vr = refs ? refs[a.hk + h] : 0.f;
       const bool part_of = it.unit >= 0;
       const float unit = exp2_int(-(int)T_P_LOG2);
       const float back = l_run == 0.f ? 0.f : part_of ? vr * unit : vr / l_run;
@@ -859,42 +928,76 @@ __global__ void __launch_bounds__(T_THREADS, 2)
   }
 }
 
-// Joins the parts of one 16-row unit: o = sum_p 2^(m_p - m) O_p / sum_p 2^(m_p - m) l_p.
+// Joins the parts of one 16-row unit: o = sum_p 2^(m_p - m) O_p / sum_p 2^(m_p - m) l_p. A warp per row, every part's
+// numbers asked for before the first is used.
+constexpr int C_WARPS = 8;
 template <int D>
-__global__ void __launch_bounds__(D) combine_kernel(const Args a, const Item* __restrict__ items) {
+__global__ void __launch_bounds__(C_WARPS * 32) combine_kernel(const Args a, const Item* __restrict__ items) {
   pdl_wait();  // the previous kernel on the stream has completed
   pdl_trigger();
+  constexpr int V = D / 32;  // columns of a lane
   const Item it = items[blockIdx.x / a.hk];
-  const int h = blockIdx.x % a.hk, d = threadIdx.x;
+  const int h = blockIdx.x % a.hk, lane = threadIdx.x % 32;
+  const int r = blockIdx.y * C_WARPS + threadIdx.x / 32, row = it.r0 + r;
   const Seg sg = load_segment(a, it.seg);
-  const int G = a.hq / a.hk, n_rows = sg.q_len * G;
+  const int G = a.hq / a.hk;
+  if (r >= it.tile || row >= sg.q_len * G) return;
   const size_t step = (size_t)it.stride * a.hk * (UNIT * (D + 2));
   const float* first = a.ws + ((size_t)it.unit * a.hk + h) * (UNIT * (D + 2));
-  for (int r = blockIdx.y; r < UNIT && it.r0 + r < n_rows && r < it.tile; r += gridDim.y) {
-    float mm = -INFINITY;
-    for (int p = 0; p < it.parts; ++p) mm = fmaxf(mm, __ldcg(first + p * step + r));
-    float ll = 0.f, oo = 0.f;
-    for (int p = 0; p < it.parts; ++p) {
-      const float* part = first + p * step;
-      const float mp = __ldcg(part + r);
-      const float f = mp == -INFINITY ? 0.f : exp2f(mp - mm);
-      ll += f * __ldcg(part + UNIT + r);
-      oo += f * __ldcg(part + 2 * UNIT + r * D + d);
+  float mm = -INFINITY, ll = 0.f, o[V];
+#pragma unroll
+  for (int e = 0; e < V; ++e) o[e] = 0.f;
+  for (int p0 = 0; p0 < it.parts; p0 += 32) {  // (a lane's part: its maximum and sum)
+    const int p = p0 + lane;
+    const float m = p < it.parts ? __ldcg(first + p * step + r) : -INFINITY;
+    const float l = p < it.parts ? __ldcg(first + p * step + UNIT + r) : 0.f;
+    float now = max_nan(mm, m);
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) now = max_nan(now, __shfl_xor_sync(0xffffffffu, now, x));
+    const float back = mm == -INFINITY ? 0.f : exp2f(mm - now);
+    const float f = m == -INFINITY ? 0.f : exp2f(m - now);
+    float sum = f * l;
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, x);
+    ll = ll * back + sum;
+#pragma unroll
+    for (int e = 0; e < V; ++e) o[e] *= back;
+    mm = now;
+    const int n = min(32, it.parts - p0);
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float w = __shfl_sync(0xffffffffu, f, i);
+      const float* src = first + (size_t)(p0 + i) * step + 2 * UNIT + r * D + lane * V;
+      float x[V];
+      if constexpr (V == 4) {
+        const float4 u = __ldcg(reinterpret_cast<const float4*>(src));
+        x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w;
+      } else {
+        const float2 u = __ldcg(reinterpret_cast<const float2*>(src));
+        x[0] = u.x, x[1] = u.y;
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) o[e] = fmaf(w, x[e], o[e]);
     }
-    const int row = it.r0 + r;
-    a.out[((size_t)(sg.q_start + row / G) * a.hq + h * G + row % G) * D + d] =
-        __float2bfloat16(ll == 0.f ? 0.f : oo / ll);
   }
+  const float inv = ll == 0.f ? 0.f : 1.f / ll;
+  __nv_bfloat16* dst = a.out + ((size_t)(sg.q_start + row / G) * a.hq + h * G + row % G) * D + lane * V;
+#pragma unroll
+  for (int e = 0; e < V; e += 2)
+    *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16x2(ll == 0.f ? 0.f : o[e] * inv, ll == 0.f ? 0.f : o[e + 1] * inv);
 }
 
 // cudaFuncSetAttribute holds per device
 template <int D>
-static int configure_tile() {
+static int configure() {
   static bool done[64] = {};
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev >= 64 || !done[dev])) {
-    e = cudaFuncSetAttribute(tile_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, TSmem<D>::TOTAL);
+    const auto max_smem = cudaFuncAttributeMaxDynamicSharedMemorySize;
+    e = cudaFuncSetAttribute(tile_kernel<D>, max_smem, TSmem<D>::TOTAL);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(rows_kernel<D, 8>, max_smem, RSmem<D>::TOTAL);
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(rows_kernel<D, 16>, max_smem, RSmem<D>::TOTAL);
     if (e == cudaSuccess && dev < 64) done[dev] = true;
   }
   return e == cudaSuccess ? MORJ_OK : set_error(MORJ_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
@@ -918,9 +1021,9 @@ static int launch(Args a, const int* counts, const int* work, char* ws, cudaStre
   a.ws = reinterpret_cast<float*>(ws + at.parts);
   const int n_rows = counts[0], n_combine = counts[1], n_tiles = counts[5], n_pages = counts[6], n_blocks = counts[7];
   const Item* items = reinterpret_cast<const Item*>(work);
-  int st = MORJ_OK;
+  int st = configure<D>();
+  if (st) return st;
   if (n_tiles) {
-    if ((st = configure_tile<D>())) return st;
     const int* pages = work + (size_t)(n_tiles + n_rows + n_combine) * (sizeof(Item) / sizeof(int));
     const int* blocks = pages + 2 * (size_t)n_pages;
     const int* list = blocks + n_blocks;
@@ -954,12 +1057,13 @@ static int launch(Args a, const int* counts, const int* work, char* ws, cudaStre
   if (n_rows) {
     const dim3 grid((unsigned)n_rows * a.hk);
     st = counts[3] == 8
-             ? launch_pdl("rows_kernel", rows_kernel<D, 8>, grid, dim3(WARPS * 32), 0, s, a, items)
-             : launch_pdl("rows_kernel", rows_kernel<D, 16>, grid, dim3(WARPS * 32), 0, s, a, items);
+             ? launch_pdl("rows_kernel", rows_kernel<D, 8>, grid, dim3(WARPS * 32), RSmem<D>::TOTAL, s, a, items)
+             : launch_pdl("rows_kernel", rows_kernel<D, 16>, grid, dim3(WARPS * 32), RSmem<D>::TOTAL, s, a, items);
     items += n_rows;
   }
   if (st == MORJ_OK && n_combine)
-    st = launch_pdl("combine_kernel", combine_kernel<D>, dim3((unsigned)n_combine * a.hk, 4), dim3(D), 0, s, a, items);
+    st = launch_pdl("combine_kernel", combine_kernel<D>, dim3((unsigned)n_combine * a.hk, UNIT / C_WARPS),
+                    dim3(C_WARPS * 32), 0, s, a, items);
   return st;
 }
 

@@ -63,8 +63,8 @@ def attention_ref(q, k, ks, v, vs, qo, kv, indices, last, page, window, n_bidir,
 
     The bound counts: the output's rounding to BF16 (2^-8 of it); each probability's rounding to FP16 (2^-11) and the
     sum's and exponential's FP32 errors (2^-11 with room); the scores' FP32 sums (d + 2 roundings of 2^-24 of
-    sum |q||k|, as an exponent's absolute error); FP16's smallest step for a probability (2^-35 of the largest V scale
-    per key, times the largest code)."""
+    sum |q||k|, as an exponent's absolute error); FP16's smallest step for a probability: 2^-24 of 2^7 p (tiles) or 2^10 p
+    (few rows), so half of it is at most 2^-32 of a key's largest value (the largest V scale times the largest code)."""
     n_q, hq, d = q.shape
     hk = ks.shape[1]
     G = hq // hk
@@ -102,7 +102,7 @@ def attention_ref(q, k, ks, v, vs, qo, kv, indices, last, page, window, n_bidir,
                 out[a:a + n, h * G + g] = o
                 top = float(vs[slot // BLOCK, h].max()) * 448 if keys else 0.0
                 bound[a:a + n, h * G + g] = (o.abs() * 2.0 ** -8 + (p @ vd.abs()) * (2.0 ** -10 + 2 * (d + 2) * 2.0 ** -24 * mag)
-                                             + keys * 2.0 ** -35 * top + 1e-38)
+                                             + keys * 2.0 ** -32 * top + 1e-38)
     return out, bound
 
 
