@@ -30,7 +30,7 @@ constexpr int T_ROWS = 128;           // rows of a tile_kernel tile
 constexpr int BN = 64;                // keys it takes at a time
 constexpr int FEW_ROWS = 16;         // segments of at most this many rows go to rows_kernel
 constexpr int T_CTAS = 2, T_MIN_KEYS = 256;  // resident CTAs per SM and keys of a part worth one: tile_kernel
-constexpr int R_CTAS = 4, R_MIN_KEYS = 256;  // ... rows_kernel
+constexpr int R_CTAS = 3, R_MIN_KEYS = 256;  // ... rows_kernel
 constexpr float P_SCALE = 1024.0f;   // probabilities are rounded to FP16 as 1024 p: 2^-34 is their smallest step
 
 struct Item {
@@ -127,24 +127,25 @@ MORJ_DEV float row_scale(float amax) {
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Few rows per segment (at most 16; the single-token form): the codes' bytes bound the call, so a warp keeps two groups
-// of 32 keys in flight (cp.async, 16 KB) while it works on a third, eight warps an SM. Groups are taken in turn by the
-// four warps of a CTA; keys are one lane each for their page entry (two groups ahead) and scales. In a group the rows of
-// K and V lie as they come, 16-byte units XOR-swizzled by the key, so both products read their fragments without bank
-// conflicts: mma.m16n8k16 leaves the order of the head dimension (q . k) and of the output columns (P V) free, and each
-// lane takes 32 (16) consecutive codes of a K row and 16 (8) of a V row for D = 128 (64). The loop is 16 keys long to
-// keep its code small: unrolled over 32 keys it was 16 KB, and a CTA that runs it four times spent most of its time
+// Few rows per segment (at most 16; the single-token form): the codes' bytes bound the call, so each of an SM's twelve
+// warps has a group of 32 keys (8 KB) on its way while it works on another. Groups are taken in turn by the four warps of
+// a CTA; keys are one lane each for their page entry (two groups ahead) and scales. A group whose slots follow one
+// another comes by two TMA boxes, others are gathered by cp.async; either way the rows of K and V lie as they come,
+// 16-byte units XOR-swizzled by the key, so both products read their fragments without bank conflicts: mma.m16n8k16 leaves the order of the head dimension (q . k) and of the output columns (P V) free, and each
+// lane takes 32 (16) consecutive codes of a K row and 16 (8) of a V row for D = 128 (64). The code is kept small: unrolled over 32 keys with its loads in registers it was 16 KB, and a CTA that runs it four times spent most of its time
 // fetching instructions (9 readout rows of 1,560 keys: 41 us).
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int R_STAGES = 3;
+constexpr int R_STAGES = 2;
 
 template <int D>
 struct RSmem {
-  static constexpr int SIDE = STEP * D;                    // codes of one group, K or V
-  static constexpr int STAGE = 2 * SIDE + 2 * STEP * 4;    // K, V, K scales, V scales
-  static constexpr int RING = R_STAGES * STAGE;            // of one warp
-  static constexpr int TOTAL = WARPS * RING;
-  static_assert(TOTAL >= WARPS * 16 * (D + 2) * 4, "the warps' results are joined in the rings");
+  static constexpr int SIDE = STEP * D;                     // codes of one group, K or V
+  static constexpr int STAGE = 2 * SIDE;
+  static constexpr int SCALE_OFF = WARPS * R_STAGES * STAGE;           // [warp][stage] K scales, V scales
+  static constexpr int BAR_OFF = SCALE_OFF + WARPS * R_STAGES * 2 * STEP * 4;  // [warp][stage], then the abort flag
+  static constexpr int TOTAL = BAR_OFF + WARPS * R_STAGES * 8 + 16;
+  static_assert(SCALE_OFF >= WARPS * 16 * (D + 2) * 4 || D == 64, "the warps' results are joined in the rings");
+  static_assert(SCALE_OFF + WARPS * R_STAGES * 2 * STEP * 4 >= WARPS * 16 * (D + 2) * 4, "... or in them and the scales");
 };
 
 MORJ_DEV void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
@@ -152,6 +153,20 @@ MORJ_DEV void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
 }
 MORJ_DEV void cp_async4(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+// one arrival of this thread on `bar` once its cp.asyncs so far have landed
+MORJ_DEV void cp_async_arrive(uint32_t bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(bar) : "memory");
+}
+MORJ_DEV void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
+  asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+// warp-level wait: lane 0 polls the barrier, the warp follows its verdict (and sees what lane 0 sees)
+MORJ_DEV bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
+  int ok = (threadIdx.x & 31) == 0 ? (int)mbar_wait(bar, parity, abort, kErrTimeoutAttention) : 0;
+  ok = __shfl_sync(0xffffffffu, ok, 0);
+  __syncwarp();
+  return ok != 0;
 }
 MORJ_DEV uint4 lds16(uint32_t addr) {
   uint4 v;
@@ -169,7 +184,7 @@ MORJ_DEV float lds4(uint32_t addr) {
   return v;
 }
 
-// byte offset of 16-byte unit u of key k's row in a group
+// byte offset of 16-byte unit u of key k's row in a group (the 128-byte, for D = 64 the 64-byte swizzle of TMA)
 template <int D>
 MORJ_DEV uint32_t unit_at(int k, int u) {
   return D == 128 ? (uint32_t)(k * 128 + ((u ^ (k & 7)) << 4)) : (uint32_t)(k * 64 + ((u ^ ((k >> 1) & 3)) << 4));
@@ -177,7 +192,9 @@ MORJ_DEV uint32_t unit_at(int k, int u) {
 
 // ROWS = 8 or 16 rows per tile. Rows 8..15 of the MMA's 16 are zeros when ROWS = 8 and cost no registers.
 template <int D, int ROWS>
-__global__ void __launch_bounds__(WARPS * 32) rows_kernel(const Args a, const Item* __restrict__ items) {
+__global__ void __launch_bounds__(WARPS * 32, 3)
+    rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const Args a,
+                const Item* __restrict__ items) {
   pdl_wait();  // the previous kernel on the stream has completed
   pdl_trigger();
   using L = RSmem<D>;
@@ -187,7 +204,11 @@ __global__ void __launch_bounds__(WARPS * 32) rows_kernel(const Args a, const It
   constexpr int KRUN = D / 4;      // consecutive codes of a key one lane reads of K
   constexpr int VRUN = D / 8;      // ... and of V
   constexpr int LPR = D / 16;      // 16-byte units of a row
-  extern __shared__ __align__(128) uint8_t smem[];
+  extern __shared__ __align__(1024) uint8_t smem[];
+  if (smem_u32(smem) & 1023) {  // the swizzle follows the address
+    if (threadIdx.x == 0) report(kErrBadAlignment);
+    return;
+  }
 
   const Item it = items[blockIdx.x / a.hk];
   const int h = blockIdx.x % a.hk;
@@ -199,37 +220,57 @@ __global__ void __launch_bounds__(WARPS * 32) rows_kernel(const Args a, const It
   const int t_end = min(it.t1, sg.kv_len);
 
   // ---- the warp's groups: keys [it.t0 + 32 (warp + 4 i), + 32)
-  const uint32_t ring = smem_u32(smem) + warp * L::RING;
+  const uint32_t ring = smem_u32(smem) + warp * R_STAGES * L::STAGE;
+  const uint32_t scale_at = smem_u32(smem) + L::SCALE_OFF + warp * R_STAGES * (2 * STEP * 4);
+  const uint32_t bars = smem_u32(smem) + L::BAR_OFF + warp * R_STAGES * 8;
+  volatile int* abort = reinterpret_cast<volatile int*>(smem + L::BAR_OFF + WARPS * R_STAGES * 8);
+  if (lane == 0) {
+    for (int i = 0; i < R_STAGES; ++i) mbar_init(bars + 8 * i, 32);
+    if (warp == 0) *abort = 0;
+    fence_mbar_init();
+    tma_prefetch(&k_map);
+    tma_prefetch(&v_map);
+  }
+  __syncthreads();
   const int t_first = it.t0 + warp * STEP;
   const int groups = t_first < t_end ? (t_end - t_first + WARPS * STEP - 1) / (WARPS * STEP) : 0;
   const int* list = a.kv_indices + sg.kv_base;
   const unsigned row_bytes = (unsigned)a.hk * D;
-  const uint8_t* kc = a.k + (size_t)h * D + (lane % LPR) * 16;
-  const uint8_t* vc = a.v + (size_t)h * D + (lane % LPR) * 16;
   auto key = [&](int i) { return t_first + i * (WARPS * STEP) + lane; };
   auto entry = [&](int i) { return i < groups ? __ldg(list + page_of(a, min(key(i), t_end - 1))) : 0; };
   auto issue = [&](int i, int e) {  // ask for group i; e: the lane's page entry
-    if (i < groups) {
-      const uint32_t st = ring + (i % R_STAGES) * L::STAGE;
-      const int t = key(i);
-      const long long at = slot_of(a, e, min(t, t_end - 1));
-      const bool in_pool = at >= 0 && at < a.pool_slots;
-      if (!in_pool) report(kErrBadIndex);
-      const bool ok = t < t_end && in_pool;
-      const unsigned slot = in_pool ? (unsigned)at : 0u;
+    if (i >= groups) return;
+    const int place = i % R_STAGES;
+    const uint32_t st = ring + place * L::STAGE, bar = bars + 8 * place;
+    const int t = key(i);
+    const long long at = slot_of(a, e, min(t, t_end - 1));
+    const bool in_pool = at >= 0 && at < a.pool_slots;
+    if (!in_pool) report(kErrBadIndex);
+    const bool ok = t < t_end && in_pool;
+    const unsigned slot = in_pool ? (unsigned)at : 0u;
+    const size_t si = (size_t)(slot >> BLOCK_SHIFT) * a.hk + h;
+    const uint32_t sc = scale_at + place * (2 * STEP * 4) + lane * 4;
+    cp_async4(sc, a.ks + si, ok ? 4u : 0u);
+    cp_async4(sc + STEP * 4, a.vs + si, ok ? 4u : 0u);
+    const unsigned first = __shfl_sync(0xffffffffu, slot, 0);
+    if (__all_sync(0xffffffffu, ok && slot == first + lane)) {
+      if (lane == 0) {
+        mbar_expect_tx(bar, L::STAGE);
+        tma_load_3d(st, &k_map, bar, 0, h, (int)first);
+        tma_load_3d(st + L::SIDE, &v_map, bar, 0, h, (int)first);
+      }
+    } else {
       const unsigned there = __ballot_sync(0xffffffffu, ok);
-      const size_t si = (size_t)(slot >> BLOCK_SHIFT) * a.hk + h;
-      cp_async4(st + 2 * L::SIDE + lane * 4, a.ks + si, ok ? 4u : 0u);
-      cp_async4(st + 2 * L::SIDE + STEP * 4 + lane * 4, a.vs + si, ok ? 4u : 0u);
-#pragma unroll 4
+      const size_t unit = (size_t)h * D + (lane % LPR) * 16;
+#pragma unroll 2
       for (int k = lane / LPR; k < STEP; k += 32 / LPR) {
-        const unsigned long long off = (unsigned long long)__shfl_sync(0xffffffffu, slot, k) * row_bytes;
+        const unsigned long long off = (unsigned long long)__shfl_sync(0xffffffffu, slot, k) * row_bytes + unit;
         const uint32_t n = (there >> k) & 1 ? 16u : 0u;
-        cp_async16(st + unit_at<D>(k, lane % LPR), kc + off, n);
-        cp_async16(st + L::SIDE + unit_at<D>(k, lane % LPR), vc + off, n);
+        cp_async16(st + unit_at<D>(k, lane % LPR), a.k + off, n);
+        cp_async16(st + L::SIDE + unit_at<D>(k, lane % LPR), a.v + off, n);
       }
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
+    cp_async_arrive(bar);
   };
   int e_next = entry(0);
 #pragma unroll 1
@@ -289,15 +330,21 @@ __global__ void __launch_bounds__(WARPS * 32) rows_kernel(const Args a, const It
 
 #pragma unroll 1
   for (int i = 0; i < groups; ++i) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(R_STAGES - 2) : "memory");
-    __syncwarp();  // group i has landed for every lane; every lane is done with the group whose place is refilled now
+    __syncwarp();  // every lane is done with the group whose place is refilled now
     {
       const int e = e_next;
       e_next = entry(i + R_STAGES);
       issue(i + R_STAGES - 1, e);
     }
-    const uint32_t st = ring + (i % R_STAGES) * L::STAGE;
-    const uint32_t kf_at = st + 2 * L::SIDE, vf_at = kf_at + STEP * 4;
+    const int place = i % R_STAGES;
+    if (!warp_wait(bars + 8 * place, (i / R_STAGES) & 1, abort)) {
+      // (given up: what this warp asked for must land before the CTA leaves)
+      for (int x = i + 1; x < min(groups, i + R_STAGES); ++x)
+        if (lane == 0) mbar_wait_landed(bars + 8 * (x % R_STAGES), (x / R_STAGES) & 1);
+      break;
+    }
+    const uint32_t st = ring + place * L::STAGE;
+    const uint32_t kf_at = scale_at + place * (2 * STEP * 4), vf_at = kf_at + STEP * 4;
     const int base = t_first + i * (WARPS * STEP);
     // V scales: O moves to the new unit when a larger one appears (as unsigned bits a NaN is the largest)
     const float vmax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(lds4(vf_at + lane * 4))));
@@ -307,7 +354,7 @@ __global__ void __launch_bounds__(WARPS * 32) rows_kernel(const Args a, const It
       vref = vmax;
     }
     const float inv_v = vref != 0.f ? P_SCALE / vref : 0.f;
-#pragma unroll 1
+#pragma unroll
     for (int sub = 0; sub < STEP; sub += 16) {
       // scores of 8 keys per MMA column tile: rows g (and g + 8), keys c4 * 2 + {0, 1}
       float s[2][4];
@@ -354,7 +401,7 @@ __global__ void __launch_bounds__(WARPS * 32) rows_kernel(const Args a, const It
         mx[b] = max_nan(mx[b], __shfl_xor_sync(0xffffffffu, mx[b], 1));
         mx[b] = max_nan(mx[b], __shfl_xor_sync(0xffffffffu, mx[b], 2));
         const float now = max_nan(m[b], mx[b]);
-        alpha[b] = m[b] == -INFINITY ? 0.f : exp2f(m[b] - now);
+        alpha[b] = m[b] == -INFINITY ? 0.f : fast_exp2(m[b] - now);
         m[b] = now;
         l[b] *= alpha[b];
         alpha[b] *= unit;
@@ -374,7 +421,7 @@ __global__ void __launch_bounds__(WARPS * 32) rows_kernel(const Args a, const It
 #pragma unroll
         for (int b = 0; b < HALVES; ++b) {
           const float shift = m[b] == -INFINITY ? 0.f : m[b];
-          const float p0 = exp2f(s[j][2 * b] - shift), p1 = exp2f(s[j][2 * b + 1] - shift);
+          const float p0 = fast_exp2(s[j][2 * b] - shift), p1 = fast_exp2(s[j][2 * b + 1] - shift);
           l[b] += p0 + p1;
           pf[b][j] = pack_f16x2(p0 * f0, p1 * f1);
         }
@@ -410,7 +457,6 @@ __global__ void __launch_bounds__(WARPS * 32) rows_kernel(const Args a, const It
   }
 
   // the four warps' results, joined in the rings
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();
   float* sh_o = reinterpret_cast<float*>(smem);        // [warp][row][D]
   float* sh_m = sh_o + WARPS * ROWS * D;               // [warp][row]
@@ -597,13 +643,6 @@ MORJ_DEV float max3f(float a, float b, float c) {
 }
 MORJ_DEV void sts16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
   asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
-}
-// warp-level wait: lane 0 polls the barrier, the warp follows its verdict (and sees what lane 0 sees)
-MORJ_DEV bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
-  int ok = (threadIdx.x & 31) == 0 ? (int)mbar_wait(bar, parity, abort, kErrTimeoutAttention) : 0;
-  ok = __shfl_sync(0xffffffffu, ok, 0);
-  __syncwarp();
-  return ok != 0;
 }
 
 // One loader warp fills buffer `dst` with the expanded rows of keys [t0, t0 + BN) and completes `full`. s0, s1: the
@@ -1055,10 +1094,18 @@ static int launch(Args a, const int* counts, const int* work, char* ws, cudaStre
     items += n_tiles;
   }
   if (n_rows) {
+    CUtensorMap km, vm;  // code pools [slots, hk, D]: box = a row's codes x 1 head x 32 slots
+    const unsigned long long dims[3] = {(unsigned long long)D, (unsigned long long)a.hk, (unsigned long long)a.pool_slots};
+    const unsigned long long strides[2] = {(unsigned long long)D, (unsigned long long)a.hk * D};
+    const unsigned box[3] = {(unsigned)D, 1u, (unsigned)STEP};
+    const CUtensorMapSwizzle swizzle = D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+    if ((st = encode_tiled(&km, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, a.k, dims, strides, box, swizzle))) return st;
+    if ((st = encode_tiled(&vm, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, a.v, dims, strides, box, swizzle))) return st;
     const dim3 grid((unsigned)n_rows * a.hk);
-    st = counts[3] == 8
-             ? launch_pdl("rows_kernel", rows_kernel<D, 8>, grid, dim3(WARPS * 32), RSmem<D>::TOTAL, s, a, items)
-             : launch_pdl("rows_kernel", rows_kernel<D, 16>, grid, dim3(WARPS * 32), RSmem<D>::TOTAL, s, a, items);
+    st = counts[3] == 8 ? launch_pdl("rows_kernel", rows_kernel<D, 8>, grid, dim3(WARPS * 32), RSmem<D>::TOTAL, s, km,
+                                     vm, a, items)
+                        : launch_pdl("rows_kernel", rows_kernel<D, 16>, grid, dim3(WARPS * 32), RSmem<D>::TOTAL, s, km,
+                                     vm, a, items);
     items += n_rows;
   }
   if (st == MORJ_OK && n_combine)
