@@ -236,24 +236,23 @@ int morj_kv8_gather(const void* codes, const float* scale, int pool_slots, const
  *
  * morj_tree_attention_kv8_work (host function, no device access): the call's work list from host copies of its segment
  * tables. Writes up to `cap` ints to work_host and counts[MORJ_KV8_COUNTS]: 0 tiles of few rows, 1 joins, 2 partial
- * units, 3 rows per such tile, 4 ints written, 5 tiles of 128 rows, 6 pages and 7 blocks those see, 8 list entries. With
- * cap = 0 it writes only the counts. Segments of more than 16 rows (queries x hq / hk) run in tiles of 128: the pages they
+ * units, 3 rows per such tile, 4 ints written, 5 tiles of 128 rows, 6 pages and 7 blocks those see, 8 list entries, 9
+ * queries. With cap = 0 it writes only the counts. Segments of more than 16 rows (queries x hq / hk) run in tiles of 128: the pages they
  * see are first expanded to FP16 in `workspace`, once per call. Long key lists of few tiles are cut into parts, whose
  * partial results go through `workspace` and are joined in a fixed order.
  * morj_tree_attention_kv8_workspace (host function): the bytes a call with these counts needs (4 per code pair of the
  * expanded pages, plus the parts; the caller's, 256-byte aligned; calls that may overlap on the device must not share
- * it). `work`: the device copy of the list (16-byte aligned); `counts`: the host array. */
+ * it). `work`: the device copy of the list (16-byte aligned); `counts`: the host array; kv_indices, n_bidir, hq, hk,
+ * page_size and window as the list was made for. */
 #define MORJ_KV8_COUNTS 12
 int morj_tree_attention_kv8_work(const int* qo_indptr_host, const int* kv_indptr_host, const int* kv_indices_host,
                                  const int* kv_last_page_len_host, int n_segments, int n_bidir, int hq, int hk,
                                  int page_size, int window, int* work_host, int cap, int* counts);
 int morj_tree_attention_kv8_workspace(const int* counts, int hk, int d, int page_size, unsigned long long* bytes);
 int morj_tree_attention_kv8(const void* q, int n_q, const void* k_codes, const float* k_scale, const void* v_codes,
-                            const float* v_scale, int pool_slots, void* out, const int* qo_indptr,
-                            const int* kv_indptr, const int* kv_indices, const int* kv_last_page_len, int n_segments,
-                            int n_bidir, int hq, int hk, int d, int page_size, int window, float sm_scale,
-                            const int* work, const int* counts, void* workspace, unsigned long long workspace_bytes,
-                            void* stream);
+                            const float* v_scale, int pool_slots, void* out, const int* kv_indices, int n_bidir, int hq,
+                            int hk, int d, int page_size, int window, float sm_scale, const int* work,
+                            const int* counts, void* workspace, unsigned long long workspace_bytes, void* stream);
 
 /* ---- tensor parallelism over peer memory (no counterpart in the reference, which runs one GPU per model; this
  * replaces the NCCL all-reduce after the row-parallel O and down projections of a T-way sharded model) ----------

@@ -48,8 +48,7 @@ SIGNATURES = {
     'morj_kv8_gather': [P, P, I, P, I, I, I, P, LL, P],
     'morj_tree_attention_kv8_work': [IP, IP, IP, IP, I, I, I, I, I, I, IP, I, IP],
     'morj_tree_attention_kv8_workspace': [IP, I, I, I, ctypes.POINTER(ctypes.c_ulonglong)],
-    'morj_tree_attention_kv8': [P, I, P, P, P, P, I, P, P, P, P, P, I, I, I, I, I, I, I, F, P, IP, P,
-                                ctypes.c_ulonglong, P],
+    'morj_tree_attention_kv8': [P, I, P, P, P, P, I, P, P, I, I, I, I, I, I, F, P, IP, P, ctypes.c_ulonglong, P],
     'morj_label_head': [P, LL, P, P, P, I, P, P, I, F, F, P, P],
     'morj_token_logprobs_workspace': [I, I, ctypes.POINTER(ctypes.c_ulonglong)],
     'morj_token_logprobs': [P, LL, I, P, LL, I, I, F, P, I, P, P, P, I, P, P, P, ctypes.c_ulonglong, P],

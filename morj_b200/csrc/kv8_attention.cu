@@ -29,16 +29,19 @@ constexpr int STEP = 32;             // keys a warp of rows_kernel takes at a ti
 constexpr int T_ROWS = 128;           // rows of a tile_kernel tile
 constexpr int BN = 64;                // keys it takes at a time
 constexpr int FEW_ROWS = 16;         // segments of at most this many rows go to rows_kernel
-constexpr int T_CTAS = 2, T_MIN_KEYS = 256;  // resident CTAs per SM and keys of a part worth one: tile_kernel
-constexpr int R_CTAS = 3, R_MIN_KEYS = 256;  // ... rows_kernel
+constexpr int T_CTAS = 2, T_MIN_KEYS = 256;  // resident CTAs per SM, and the fewest keys of a part: tiles
+constexpr int R_CTAS = 3, R_MIN_KEYS = 256;  // ... few rows
 constexpr float P_SCALE = 1024.0f;   // probabilities are rounded to FP16 as 1024 p: 2^-34 is their smallest step
 
-struct Item {
+// What a CTA needs to know, in one load: which rows and keys of which segment.
+struct __align__(16) Item {
   int seg, r0;         // segment, its first row (row = query * G + head of the group)
   int t0, t1;          // keys [t0, t1) of the segment's list
   int unit;            // first partial unit, -1: the only part, straight to `out`
-  int parts, stride;   // combine entries: parts, and units between them
+  int parts, stride;   // joins: parts, and units between them
   int tile;            // rows of the tile
+  int q_start, q_len;  // the segment's queries
+  int kv_base, kv_len; // its first list entry and its keys
 };
 
 struct Args {
@@ -48,31 +51,13 @@ struct Args {
   const uint8_t* v;
   const float* vs;
   __nv_bfloat16* out;
-  const int* qo_indptr;
-  const int* kv_indptr;
   const int* kv_indices;
-  const int* kv_last_page_len;
   int n_bidir, hq, hk, page_size;
   unsigned page_magic;  // t / page_size = umulhi(t, page_magic) >> page_shift (page_size > 1)
   int page_shift, window, pool_slots;
   float scale_log2;
   float* ws;
 };
-
-struct Seg {
-  int q_start, q_len, kv_base, kv_len;
-};
-MORJ_DEV Seg load_segment(const Args& a, int seg) {
-  Seg s;
-  s.q_start = a.qo_indptr[seg];
-  s.q_len = a.qo_indptr[seg + 1] - s.q_start;
-  s.kv_base = a.kv_indptr[seg];
-  const int pages = a.kv_indptr[seg + 1] - s.kv_base;
-  s.kv_len = a.page_size == 1 ? pages
-             : pages == 0     ? 0
-                              : (pages - 1) * a.page_size + (a.kv_last_page_len ? a.kv_last_page_len[seg] : a.page_size);
-  return s;
-}
 
 // keys [lo, hi] query j of a segment sees (hi < lo: none)
 __host__ __device__ inline void visible(int q_len, int kv_len, bool bidir, int window, int j, int* lo, int* hi) {
@@ -214,10 +199,9 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
   const int h = blockIdx.x % a.hk;
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const int g = lane / 4, c4 = lane % 4;
-  const Seg sg = load_segment(a, it.seg);
   const bool bidir = it.seg < a.n_bidir;
-  const int G = a.hq / a.hk, n_rows = sg.q_len * G;
-  const int t_end = min(it.t1, sg.kv_len);
+  const int G = a.hq / a.hk, n_rows = it.q_len * G;
+  const int t_end = it.t1;
 
   // ---- the warp's groups: keys [it.t0 + 32 (warp + 4 i), + 32)
   const uint32_t ring = smem_u32(smem) + warp * R_STAGES * L::STAGE;
@@ -234,7 +218,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
   __syncthreads();
   const int t_first = it.t0 + warp * STEP;
   const int groups = t_first < t_end ? (t_end - t_first + WARPS * STEP - 1) / (WARPS * STEP) : 0;
-  const int* list = a.kv_indices + sg.kv_base;
+  const int* list = a.kv_indices + it.kv_base;
   const unsigned row_bytes = (unsigned)a.hk * D;
   auto key = [&](int i) { return t_first + i * (WARPS * STEP) + lane; };
   auto entry = [&](int i) { return i < groups ? __ldg(list + page_of(a, min(key(i), t_end - 1))) : 0; };
@@ -292,9 +276,9 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
 #pragma unroll
     for (int i = 0; i < KRUN / 8; ++i) raw[i] = make_uint4(0, 0, 0, 0);
     if (r < n_rows) {
-      visible(sg.q_len, sg.kv_len, bidir, a.window, r / G, &lo[b], &hi[b]);
+      visible(it.q_len, it.kv_len, bidir, a.window, r / G, &lo[b], &hi[b]);
       const uint4* src = reinterpret_cast<const uint4*>(
-          a.q + ((size_t)(sg.q_start + r / G) * a.hq + h * G + r % G) * D + c4 * KRUN);
+          a.q + ((size_t)(it.q_start + r / G) * a.hq + h * G + r % G) * D + c4 * KRUN);
 #pragma unroll
       for (int i = 0; i < KRUN / 8; ++i) raw[i] = __ldg(src + i);
     }
@@ -495,7 +479,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
       part[2 * UNIT + r * D + d] = oo;
     } else {
       const int row = it.r0 + r;
-      a.out[((size_t)(sg.q_start + row / G) * a.hq + h * G + row % G) * D + d] =
+      a.out[((size_t)(it.q_start + row / G) * a.hq + h * G + row % G) * D + d] =
           __float2bfloat16(ll == 0.f ? 0.f : oo / ll);
     }
   }
@@ -520,29 +504,32 @@ __global__ void __launch_bounds__(E_THREADS) expand_kernel(const Args a, const i
                                                            float* __restrict__ refs) {
   pdl_wait();  // the previous kernel on the stream has completed
   pdl_trigger();
-  constexpr int LPR = D / 16;                  // lanes per row, 16 codes each
-  constexpr int ROWS = E_THREADS / LPR / 2;    // rows per pass of each half of the CTA (K, V)
+  constexpr int LPR = D / 8;                     // lanes per row: 8 codes in, 16 bytes out
+  constexpr int SLOTS = BN / (E_THREADS / 64);   // slots of a warp (half of the warps K, half V)
+  constexpr int N = SLOTS / (32 / LPR);          // loads of a lane
   __shared__ float red[2][E_THREADS / 32];
   const int h = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   // this CTA's codes first: nothing below is needed to ask for them
-  const int side = threadIdx.x / (E_THREADS / 2), tid = threadIdx.x % (E_THREADS / 2);
-  const uint8_t* codes = (side ? a.v : a.k) + (size_t)h * D + (tid % LPR) * 16;
-  const float* scales = (side ? a.vs : a.ks) + h;
-  uint4 w[BN / ROWS];
-  float sc[BN / ROWS];
+  const bool is_v = warp >= E_THREADS / 64;
+  const int t_warp = blockIdx.x * BN + (warp % (E_THREADS / 64)) * SLOTS + lane / LPR;
+  const uint8_t* codes = (is_v ? a.v : a.k) + (size_t)h * D + (lane % LPR) * 8;
+  const float* scales = (is_v ? a.vs : a.ks) + h;
+  const unsigned row_bytes = (unsigned)a.hk * D;
+  uint2 w[N];
+  float sc[N];
 #pragma unroll
-  for (int i = 0; i < BN / ROWS; ++i) {
-    const int t = blockIdx.x * BN + i * ROWS + tid / LPR;
-    sc[i] = 0.f, w[i] = make_uint4(0, 0, 0, 0);
+  for (int i = 0; i < N; ++i) {
+    const int t = t_warp + i * (32 / LPR);
+    sc[i] = 0.f, w[i] = make_uint2(0, 0);
     if (t < n_slots) {
-      const int2 page = __ldg(pages + page_of(a, t));  // (page of the pool, its slots that are listed: the rest is zeros)
-      const int at = t - page_of(a, t) * a.page_size;
+      const int p = page_of(a, t), at = t - p * a.page_size;
+      const int2 page = __ldg(pages + p);  // (page of the pool, its slots that are listed: the rest is zeros)
       const long long slot = (long long)page.x * a.page_size + at;
       if (at >= page.y) {
-      } else if (slot < 0 || slot >= a.pool_slots) {
-        if (tid % LPR == 0) report(kErrBadIndex);
+      } else if (slot >= a.pool_slots) {
+        if (lane % LPR == 0) report(kErrBadIndex);
       } else {
-        w[i] = __ldg(reinterpret_cast<const uint4*>(codes + (size_t)slot * a.hk * D));
+        w[i] = __ldg(reinterpret_cast<const uint2*>(codes + (unsigned long long)slot * row_bytes));
         sc[i] = __ldg(scales + (size_t)(slot >> BLOCK_SHIFT) * a.hk);
       }
     }
@@ -550,10 +537,10 @@ __global__ void __launch_bounds__(E_THREADS) expand_kernel(const Args a, const i
   // the head's largest scales (every CTA of the head finds the same)
   float kr = 0.f, vr = 0.f;
   for (int i = threadIdx.x; i < n_blocks; i += E_THREADS) {
-    if ((long long)blocks[i] * BLOCK >= a.pool_slots) continue;  // (reported above)
-    const size_t at = (size_t)blocks[i] * a.hk + h;
-    kr = fmaxf(kr, __ldg(a.ks + at));
-    vr = fmaxf(vr, __ldg(a.vs + at));
+    const int b = __ldg(blocks + i);
+    if ((long long)b * BLOCK >= a.pool_slots) continue;  // (reported above)
+    kr = fmaxf(kr, __ldg(a.ks + (size_t)b * a.hk + h));
+    vr = fmaxf(vr, __ldg(a.vs + (size_t)b * a.hk + h));
   }
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) {
@@ -562,39 +549,35 @@ __global__ void __launch_bounds__(E_THREADS) expand_kernel(const Args a, const i
   }
   if (lane == 0) red[0][warp] = kr, red[1][warp] = vr;
   __syncthreads();
+#pragma unroll
   for (int i = 0; i < E_THREADS / 32; ++i) kr = fmaxf(kr, red[0][i]), vr = fmaxf(vr, red[1][i]);
   if (blockIdx.x == 0 && threadIdx.x == 0) refs[h] = kr, refs[a.hk + h] = vr;
-  const float ref = side ? vr : kr;
-  __half* out = (side ? v_out : k_out) + (size_t)h * D + (tid % LPR) * 16;
+  const float ref = is_v ? vr : kr;
+  const float inv = ref > 0.f ? 1.f / ref : 1.f;
+  __half* out = (is_v ? v_out : k_out) + (size_t)h * D + (lane % LPR) * 8;
 #pragma unroll
-  for (int i = 0; i < BN / ROWS; ++i) {
-    const int t = blockIdx.x * BN + i * ROWS + tid / LPR;
+  for (int i = 0; i < N; ++i) {
+    const int t = t_warp + i * (32 / LPR);
     if (t >= n_slots) break;
-    const float f = ref > 0.f ? sc[i] / ref : sc[i];
-    const uint32_t c[8] = {w[i].x & 0xffffu, w[i].x >> 16, w[i].y & 0xffffu, w[i].y >> 16,
-                           w[i].z & 0xffffu, w[i].z >> 16, w[i].w & 0xffffu, w[i].w >> 16};
-    uint32_t p[8];
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float2 x = codes2_f32(c[e]);
-      p[e] = pack_f16x2(x.x * f, x.y * f);
-    }
-    uint4* dst = reinterpret_cast<uint4*>(out + (size_t)t * a.hk * D);
-    dst[0] = make_uint4(p[0], p[1], p[2], p[3]);
-    dst[1] = make_uint4(p[4], p[5], p[6], p[7]);
+    const float f = sc[i] * inv;
+    const float2 x0 = codes2_f32(w[i].x & 0xffffu), x1 = codes2_f32(w[i].x >> 16);
+    const float2 x2 = codes2_f32(w[i].y & 0xffffu), x3 = codes2_f32(w[i].y >> 16);
+    *reinterpret_cast<uint4*>(out + (unsigned long long)t * row_bytes) =
+        make_uint4(pack_f16x2(x0.x * f, x0.y * f), pack_f16x2(x1.x * f, x1.y * f), pack_f16x2(x2.x * f, x2.y * f),
+                   pack_f16x2(x3.x * f, x3.y * f));
   }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
 // tile_kernel: 128 rows of a segment and KV head against 64 keys at a time, on tcgen05 (FP16 x FP16, FP32 in TMEM).
-//   warps 0-3   softmax (thread = row): prologue (Q row to FP16 and shared memory), mask, online maximum and sum, P as
+//   warps 0, 2  K and V loaders: a chunk whose 64 expanded slots are consecutive by TMA, others gathered by cp.async
+//   warp 1      MMA issuer (one thread): S_c = Q K_c^T into TMEM buffer c % 2, O += P_c V_c with P read from TMEM
+//   warps 4-7   softmax (thread = row): prologue (Q row to FP16 and shared memory), mask, online maximum and sum, P as
 //               FP16 over its own scores in TMEM, the final O / l or the part's (maximum, sum, O)
-//   warp 4      MMA issuer (one thread): S_c = Q K_c^T into TMEM buffer c % 2, O += P_c V_c with P read from TMEM
-//   warps 5, 6  K and V loaders: a chunk whose 64 expanded slots are consecutive by TMA, others gathered by cp.async
 // The pipeline is tree_attention_kernel's (S and P double-buffered in TMEM, a K buffer free once its S is complete, a V
 // buffer once its P V is, two CTAs per SM); what it lacks there is the parts of a key range and rows that see nothing.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int T_THREADS = 256;          // (warp 7 has no role)
+constexpr int T_THREADS = 256;          // (warp 3 has no role)
 constexpr int T_TMEM_COLS = 256;        // S/P buffers at columns [0, 64) and [64, 128), O at [128, 128 + D)
 constexpr float T_RESCALE_LOG2 = 8.0f;  // O is rescaled when a row's maximum grows by more than 2^8 (2^4: 3-4% slower),
 constexpr float T_P_LOG2 = 7.0f;        // so that 2^7 p <= 2^15 stays inside FP16: p's smallest step is 2^-31
@@ -700,11 +683,10 @@ __global__ void __launch_bounds__(T_THREADS, 2)
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const Item it = items[blockIdx.x / a.hk];
   const int h = blockIdx.x % a.hk;  // (the KV head is the fast index: every head of the longest item starts first)
-  const Seg sg = load_segment(a, it.seg);
-  const int G = a.hq / a.hk, n_rows = sg.q_len * G;
+  const int G = a.hq / a.hk, n_rows = it.q_len * G;
   const bool bidir = it.seg < a.n_bidir;
   const int t_begin = it.t0 - it.t0 % BN;  // chunks line up with 64-slot pages
-  const int t_stop = min(it.t1, sg.kv_len);
+  const int t_stop = it.t1;
   const int n_chunks = t_stop > it.t0 ? (t_stop - t_begin + BN - 1) / BN : 0;
 
   if (threadIdx.x == 0) {
@@ -719,16 +701,16 @@ __global__ void __launch_bounds__(T_THREADS, 2)
     *abort = 0;
     fence_mbar_init();
   }
-  if (warp == 4) {
+  if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), T_TMEM_COLS);
     tmem_relinquish();
   }
   // softmax warps: thread = row
   const int r = (warp & 3) * 32 + lane, row = it.r0 + r, qi = row / G;
   const bool row_ok = row < n_rows;
-  const size_t row_at = ((size_t)(sg.q_start + qi) * a.hq + h * G + row % G) * D;
+  const size_t row_at = ((size_t)(it.q_start + qi) * a.hq + h * G + row % G) * D;
   float scale = 0.f, vr = 0.f;  // scores times `scale` are in the log2 domain; V's reference
-  if (warp < 4) {
+  if (warp >= 4) {
     // Q row: its largest magnitude, then FP16 of q / qs into the swizzled tile (read twice, the second time from L1: the
     // row in registers would be 64 of them)
     const float kr = refs ? __ldg(refs + h) : 0.f;
@@ -761,14 +743,14 @@ __global__ void __launch_bounds__(T_THREADS, 2)
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 5 || warp == 6) {
-    const bool is_k = warp == 5;
+  if (warp == 0 || warp == 2) {
+    const bool is_k = warp == 0;
     const CUtensorMap* map = is_k ? &k_map : &v_map;
     if (lane == 0) tma_prefetch(map);
     const uint32_t base = sbase + (is_k ? L::K_OFF : L::V_OFF);
     // a K buffer is free once the scores of the chunk two back are complete, a V buffer once its P V is
     const uint32_t full = is_k ? k_full : v_full, empty = is_k ? s_full : pv_done;
-    const int* pages = list + sg.kv_base;
+    const int* pages = list + it.kv_base;
     auto slot = [&](int t) {  // expanded slot of key t, -1 outside the part
       if (t < it.t0 || t >= t_stop) return -1;
       const long long s = slot_of(a, __ldg(pages + page_of(a, t)), t);
@@ -786,7 +768,7 @@ __global__ void __launch_bounds__(T_THREADS, 2)
       load_chunk<D>(base + b * L::KV_BYTES, full + 8 * b, map, is_k ? k_pool : v_pool, s0, s1, a.hk, h, lane);
       s0 = n0, s1 = n1;
     }
-  } else if (warp == 4) {
+  } else if (warp == 1) {
     if (lane == 0) {
       constexpr uint32_t IDESC_S = idesc_f16(T_ROWS, BN);
       constexpr uint32_t IDESC_O = idesc_f16(T_ROWS, D, /*b_mn_major=*/true);
@@ -831,12 +813,12 @@ __global__ void __launch_bounds__(T_THREADS, 2)
       umma_commit(done);
       mbar_wait_landed(done, 0);
     }
-  } else if (warp < 4) {
+  } else if (warp >= 4) {
     // ---------------- softmax warpgroup ----------------
-    const uint32_t t_lane = tmem + ((uint32_t)(warp * 32) << 16);
+    const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     int lo = 1, hi = 0;  // visible key positions [lo, hi] of this part
     if (row_ok) {
-      visible(sg.q_len, sg.kv_len, bidir, a.window, qi, &lo, &hi);
+      visible(it.q_len, it.kv_len, bidir, a.window, qi, &lo, &hi);
       lo = max(lo, it.t0), hi = min(hi, t_stop - 1);
     }
     float m_used = -INFINITY, l_run = 0.f;  // l_run in units of 2^-T_P_LOG2, as P and O
@@ -961,7 +943,7 @@ __global__ void __launch_bounds__(T_THREADS, 2)
 
   tc_fence_before();
   __syncthreads();
-  if (warp == 4) {
+  if (warp == 1) {
     tc_fence_after();
     tmem_dealloc(tmem, T_TMEM_COLS);
   }
@@ -978,9 +960,8 @@ __global__ void __launch_bounds__(C_WARPS * 32) combine_kernel(const Args a, con
   const Item it = items[blockIdx.x / a.hk];
   const int h = blockIdx.x % a.hk, lane = threadIdx.x % 32;
   const int r = blockIdx.y * C_WARPS + threadIdx.x / 32, row = it.r0 + r;
-  const Seg sg = load_segment(a, it.seg);
   const int G = a.hq / a.hk;
-  if (r >= it.tile || row >= sg.q_len * G) return;
+  if (r >= it.tile || row >= it.q_len * G) return;
   const size_t step = (size_t)it.stride * a.hk * (UNIT * (D + 2));
   const float* first = a.ws + ((size_t)it.unit * a.hk + h) * (UNIT * (D + 2));
   float mm = -INFINITY, ll = 0.f, o[V];
@@ -1020,7 +1001,7 @@ __global__ void __launch_bounds__(C_WARPS * 32) combine_kernel(const Args a, con
     }
   }
   const float inv = ll == 0.f ? 0.f : 1.f / ll;
-  __nv_bfloat16* dst = a.out + ((size_t)(sg.q_start + row / G) * a.hq + h * G + row % G) * D + lane * V;
+  __nv_bfloat16* dst = a.out + ((size_t)(it.q_start + row / G) * a.hq + h * G + row % G) * D + lane * V;
 #pragma unroll
   for (int e = 0; e < V; e += 2)
     *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16x2(ll == 0.f ? 0.f : o[e] * inv, ll == 0.f ? 0.f : o[e + 1] * inv);
@@ -1115,8 +1096,9 @@ static int launch(Args a, const int* counts, const int* work, char* ws, cudaStre
 }
 
 // The tiles' key ranges cut into parts so that together they fill `slots` resident CTAs once: a part holds an equal
-// share of all keys, at least min_keys, and a tile is cut only into whole shares (a further part would start a second
-// round of CTAs). Parts write units of 16 rows to the workspace; `joins` gets one entry per 16 rows of a cut tile.
+// share of all keys, at least min_keys, and a tile is cut only into whole shares. (Cutting further to even out the lengths
+// was measured slower: an SM's last CTAs run faster by themselves, 161 against 166-171 us for 64 single queries over 1 to
+// 8,048 keys.) Parts write units of 16 rows to the workspace; `joins` gets one entry per 16 rows of a cut tile.
 static std::vector<Item> cut(const std::vector<Item>& tiles, int hk, int slots, int min_keys, int& units,
                              std::vector<Item>& joins) {
   long long total = 0;
@@ -1198,7 +1180,7 @@ extern "C" int morj_tree_attention_kv8_work(const int* qo_indptr_host, const int
         int lo, hi, x;  // what the tile's first query sees from, its last query to
         kv8::visible(q_len, (int)kv, s < n_bidir, window, r0 / G, &lo, &x);
         kv8::visible(q_len, (int)kv, s < n_bidir, window, (std::min(r0 + tile, q_len * G) - 1) / G, &x, &hi);
-        Item it{s, r0, 0, 0, -1, 1, 1, tile};
+        Item it{s, r0, 0, 0, -1, 1, 1, tile, qo_indptr_host[s], q_len, kv_indptr_host[s], (int)kv};
         if (hi >= lo) it.t0 = lo, it.t1 = hi + 1, from = std::min(from, lo), to = std::max(to, hi);
         (many ? tiles : rows).push_back(it);
       }
@@ -1235,9 +1217,10 @@ extern "C" int morj_tree_attention_kv8_work(const int* qo_indptr_host, const int
                         2 * pages.size() + blocks.size() + list.size();
     if (ints > (size_t)INT_MAX)
       return set_error(MORJ_ERR_UNSUPPORTED, "morj_tree_attention_kv8_work: a work list of %zu ints", ints);
-    const int got[9] = {(int)cut_rows.size(), (int)joins.size(), units, few, (int)ints, (int)cut_tiles.size(),
-                        (int)pages.size(), (int)blocks.size(), (int)list.size()};
-    std::copy(got, got + 9, counts);
+    const int got[10] = {(int)cut_rows.size(), (int)joins.size(), units, few, (int)ints, (int)cut_tiles.size(),
+                        (int)pages.size(), (int)blocks.size(), (int)list.size(),
+                         n_segments ? qo_indptr_host[n_segments] : 0};
+    std::copy(got, got + 10, counts);
     if (counts[4] > cap) {
       if (cap == 0) return MORJ_OK;  // (a call that only asks for the counts)
       return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8_work: %d ints exceed capacity %d", counts[4], cap);
@@ -1267,21 +1250,21 @@ extern "C" int morj_tree_attention_kv8_workspace(const int* counts, int hk, int 
 
 extern "C" int morj_tree_attention_kv8(const void* q, int n_q, const void* k_codes, const float* k_scale,
                                        const void* v_codes, const float* v_scale, int pool_slots, void* out,
-                                       const int* qo_indptr, const int* kv_indptr, const int* kv_indices,
-                                       const int* kv_last_page_len, int n_segments, int n_bidir, int hq, int hk, int d,
-                                       int page_size, int window, float sm_scale, const int* work, const int* counts,
+                                       const int* kv_indices, int n_bidir, int hq, int hk, int d, int page_size, int window, float sm_scale, const int* work, const int* counts,
                                        void* workspace, unsigned long long workspace_bytes, void* stream) {
   using namespace morj;
   if (!counts) return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8: null counts");
-  if ((counts[0] == 0 && counts[5] == 0) || n_segments == 0) return MORJ_OK;
-  if (!q || !k_codes || !k_scale || !v_codes || !v_scale || !out || !qo_indptr || !kv_indptr || !kv_indices || !work ||
+  if (counts[0] == 0 && counts[5] == 0) return MORJ_OK;
+  if (!q || !k_codes || !k_scale || !v_codes || !v_scale || !out || !kv_indices || !work ||
       n_q <= 0 || pool_slots <= 0 || counts[0] < 0 || counts[1] < 0 || counts[2] < 0 || counts[5] < 0 || counts[6] < 0 || counts[7] < 0)
     return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8: null pointer or bad size");
   if (hq <= 0 || hk <= 0 || hq % hk)
     return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8: hq=%d is not a multiple of hk=%d", hq, hk);
   if (!(sm_scale > 0.f))
     return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8: sm_scale must be positive");
-  if (page_size <= 0 || n_bidir < 0 || n_bidir > n_segments)
+  if (n_q < counts[9])
+    return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8: %d queries, the work list has %d", n_q, counts[9]);
+  if (page_size <= 0 || n_bidir < 0)
     return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8: bad page_size %d or n_bidir %d", page_size, n_bidir);
   if (d != 64 && d != 128)
     return set_error(MORJ_ERR_UNSUPPORTED, "morj_tree_attention_kv8: head_dim %d unsupported (64, 128)", d);
@@ -1299,7 +1282,7 @@ extern "C" int morj_tree_attention_kv8(const void* q, int n_q, const void* k_cod
   const unsigned page_magic = page_size > 1 ? (unsigned)((1ull << (31 + l)) / page_size + 1) : 0;
   const int page_shift = l - 1;
   const kv8::Args a{(const __nv_bfloat16*)q, (const uint8_t*)k_codes, k_scale, (const uint8_t*)v_codes, v_scale,
-                    (__nv_bfloat16*)out, qo_indptr, kv_indptr, kv_indices, kv_last_page_len, n_bidir, hq, hk, page_size,
+                    (__nv_bfloat16*)out, kv_indices, n_bidir, hq, hk, page_size,
                     page_magic, page_shift, window, pool_slots, sm_scale * kv8::LOG2E, nullptr};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return d == 128 ? kv8::launch<128>(a, counts, work, (char*)workspace, s)

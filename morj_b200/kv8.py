@@ -161,7 +161,7 @@ def store(pool, k, v, plan):
 
 
 class AttentionPlan:
-    """A call's segment tables on the device and its work list (arguments as `morj_tree_attention`: host integers)."""
+    """A call's key lists and work list on the device (arguments as `morj_tree_attention`'s tables: host integers)."""
 
     def __init__(self, qo_indptr, kv_indptr, kv_indices, hq, hk, d, page_size=1, kv_last_page_len=None, window=0,
                  n_bidir=0, device='cuda'):
@@ -174,13 +174,10 @@ class AttentionPlan:
         if last is not None and (len(last) != len(qo) - 1 or (last < 0).any() or (last > page_size).any()):
             raise ValueError('kv_last_page_len must have one entry in [0, page_size] per segment')
         work, self.counts = nat.kv8_attention_work(qo, kv, kv_indices, n_bidir, hq, hk, window, page_size, last)
-        self.n_q, self.segments, self.n_bidir = int(qo[-1]), len(qo) - 1, n_bidir
+        self.n_q, self.n_bidir = int(qo[-1]), n_bidir
         self.hq, self.hk, self.d, self.page_size, self.window = hq, hk, d, page_size, window
         self.workspace_bytes = nat.kv8_attention_workspace(self.counts, hk, d, page_size)
-        self.buf, (self.qo, self.kv, self.indices, self.last, self.work) = _upload(
-            device, qo, kv, kv_indices, last if last is not None else [], work)
-        self._ptrs = tuple(t.data_ptr() for t in (self.qo, self.kv, self.indices)) + (
-            self.last.data_ptr() if last is not None else None,)
+        self.buf, (self.indices, self.work) = _upload(device, kv_indices, work)
 
 
 def tree_attention(q, pool, plan, sm_scale, out=None):
@@ -201,7 +198,7 @@ def tree_attention(q, pool, plan, sm_scale, out=None):
     ws = torch.empty(plan.workspace_bytes, dtype=torch.uint8, device=q.device) if plan.workspace_bytes else None
     with _on(pool.device) as s:
         nat.call('morj_tree_attention_kv8', q.data_ptr(), plan.n_q, pool.k.data_ptr(), pool.k_scale.data_ptr(),
-                 pool.v.data_ptr(), pool.v_scale.data_ptr(), pool.slots, out.data_ptr(), *plan._ptrs, plan.segments,
+                 pool.v.data_ptr(), pool.v_scale.data_ptr(), pool.slots, out.data_ptr(), plan.indices.data_ptr(),
                  plan.n_bidir, plan.hq, plan.hk, plan.d, plan.page_size, plan.window, sm_scale, plan.work.data_ptr(),
                  plan.counts, ws.data_ptr() if ws is not None else None, plan.workspace_bytes, s)
     return out

@@ -874,14 +874,14 @@ class LeanGemma4:
                 pool.v.data_ptr(), pool.v_scale.data_ptr(), pool.slots, self._stream())
 
     def _attention8(self, q, pool, out, t, qo, kv_indptr, kv_indices, n_seg, n_bidir, kind, work, counts):
-        """`_attention` over an 8-bit pool."""
+        """`_attention` over an 8-bit pool (whose work list holds the segments)."""
         window = self.window if kind == 'sliding_attention' else 0
         nbytes = nat.kv8_attention_workspace(counts, pool.heads, pool.head_dim)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
         self._k('attention', 'morj_tree_attention_kv8', q.data_ptr(), q.shape[0], pool.k.data_ptr(),
                 pool.k_scale.data_ptr(), pool.v.data_ptr(), pool.v_scale.data_ptr(), pool.slots, out.data_ptr(),
-                t.ptr(qo), t.ptr(kv_indptr), t.ptr(kv_indices), None, n_seg, n_bidir, self.hq, pool.heads,
-                pool.head_dim, 1, window, 1.0, t.ptr(work), counts, _ptr(ws), nbytes, self._stream())
+                t.ptr(kv_indices), n_bidir, self.hq, pool.heads, pool.head_dim, 1, window, 1.0, t.ptr(work), counts,
+                _ptr(ws), nbytes, self._stream())
 
     def _step(self, k, st, plan, pools, head, req, tables, out, prune=None):
         """One forward over a planned step (`lean_core.py:599-694`): embedding and first norm, every full layer, the

@@ -8,7 +8,7 @@ import torch
 from morj_b200 import _native as nat
 from morj_b200 import kv8
 
-ITEM = 8
+ITEM = 12
 
 
 def groups(work, blocks, n):
@@ -80,7 +80,7 @@ def test_attention_work_covers_every_row_and_key_once(spec, hq, hk, window, n_bi
     last = [n - (p - 1) * page if p else 0 for (_, n), p in zip(spec, pages)]
     perm = np.random.default_rng(len(spec)).permutation(int(kv[-1]) + 5)[:int(kv[-1])]
     work, counts = nat.kv8_attention_work(qo, kv, perm, n_bidir, hq, hk, window, page, last)
-    check_work(work, counts, spec, G, window, n_bidir)
+    check_work(work, counts, spec, G, window, n_bidir, kv)
     check_pages(work, counts, spec, G, window, n_bidir, page, kv, perm)
 
 
@@ -110,12 +110,13 @@ def check_pages(work, counts, spec, G, window, n_bidir, page, kv, indices):
                                      | {x // 64 for x in slots})
 
 
-def check_work(work, counts, spec, G, window, n_bidir):
+def check_work(work, counts, spec, G, window, n_bidir, kv):
     n_rows, n_joins, units, few, ints, n_tiles = list(counts)[:6]
     items = work[:(n_tiles + n_rows + n_joins) * ITEM].reshape(-1, ITEM).tolist()
     assert len(work) == ints
     parts, rows_of = {}, {}
-    for i, (seg, r0, t0, t1, unit, _, _, rows) in enumerate(items[:n_tiles + n_rows]):
+    for i, (seg, r0, t0, t1, unit, _, _, rows, q0, q_len, kv0, keys) in enumerate(items[:n_tiles + n_rows]):
+        assert (q_len, keys) == spec[seg] and q0 == sum(n for n, _ in spec[:seg]) and kv0 == kv[seg]
         # segments of more than 16 rows in 128-row tiles, the others in small ones
         assert rows == (128 if i < n_tiles else few) and (spec[seg][0] * G > 16) == (i < n_tiles)
         assert r0 % rows == 0 and t0 <= t1
@@ -215,12 +216,14 @@ def test_gather_refusals(kw):
 
 
 def attention_args(**kw):
-    counts = nat.KV8_COUNTS(*kw.pop('counts', (1, 0, 0, 8, 8)))
-    a = dict(q=16, n_q=1, k=16, ks=16, v=16, vs=16, pool_slots=64, out=16, qo=16, kv=16, idx=16, last=None, n_segments=1,
-             n_bidir=0, hq=4, hk=2, d=128, page=1, window=0, scale=1.0, work=16, counts=counts, ws=None, ws_bytes=0,
-             stream=None)
+    counts = nat.KV8_COUNTS(*kw.pop('counts', (1, 0, 0, 8, 12, 0, 0, 0, 0, 1)))
+    a = dict(q=16, n_q=1, k=16, ks=16, v=16, vs=16, pool_slots=64, out=16, idx=16, n_bidir=0, hq=4, hk=2, d=128, page=1,
+             window=0, scale=1.0, work=16, counts=counts, ws=None, ws_bytes=0, stream=None)
     a.update(kw)
     return list(a.values())
+
+
+PARTS = (1, 1, 2, 8, 24, 0, 0, 0, 0, 1)
 
 
 @pytest.mark.parametrize('kw,match', [
@@ -228,9 +231,10 @@ def attention_args(**kw):
     (dict(v=None), 'null pointer'), (dict(vs=None), 'null pointer'), (dict(out=None), 'null pointer'),
     (dict(idx=None), 'null pointer'), (dict(work=None), 'null pointer'), (dict(n_q=0), 'bad size'),
     (dict(pool_slots=0), 'bad size'), (dict(hq=3), 'multiple'), (dict(hk=0), 'multiple'), (dict(page=0), 'page_size'),
-    (dict(n_bidir=2), 'n_bidir'), (dict(scale=0.0), 'sm_scale'), (dict(scale=-1.0), 'sm_scale'), (dict(q=24), '16-byte'), (dict(work=24), '16-byte'),
-    (dict(counts=(1, 1, 2, 8, 16)), 'workspace of 0 bytes'),
-    (dict(counts=(1, 1, 2, 8, 16), ws=16, ws_bytes=33279), '33280 needed')])
+    (dict(n_bidir=-1), 'n_bidir'), (dict(scale=0.0), 'sm_scale'), (dict(scale=-1.0), 'sm_scale'), (dict(q=24), '16-byte'),
+    (dict(work=24), '16-byte'), (dict(counts=(1, 0, 0, 8, 12, 0, 0, 0, 0, 2)), 'the work list has 2'),
+    (dict(counts=PARTS), 'workspace of 0 bytes'), (dict(counts=PARTS, ws=16, ws_bytes=33279), '33280 needed'),
+    (dict(counts=(0, 0, 0, 8, 12, 1, 3, 1, 5, 1), ws=16, ws_bytes=100), 'needed')])
 def test_attention_refusals(kw, match):
     with pytest.raises(ValueError, match=match):
         nat.call('morj_tree_attention_kv8', *attention_args(**kw))
