@@ -238,7 +238,7 @@ int morj_kv8_gather(const void* codes, const float* scale, int pool_slots, const
  * tables. Writes up to `cap` ints to work_host and counts[MORJ_KV8_COUNTS]: 0 tiles of few rows, 1 joins, 2 partial
  * units, 3 rows per such tile, 4 ints written, 5 tiles of 128 rows, 6 pages and 7 blocks those see, 8 list entries, 9
  * queries. With cap = 0 it writes only the counts. Segments of more than 16 rows (queries x hq / hk) run in tiles of 128: the pages they
- * see are first expanded to FP16 in `workspace`, once per call. Long key lists of few tiles are cut into parts, whose
+ * see are first expanded to 16 bits in `workspace`, once per call. Long key lists of few tiles are cut into parts, whose
  * partial results go through `workspace` and are joined in a fixed order.
  * morj_tree_attention_kv8_workspace (host function): the bytes a call with these counts needs (4 per code pair of the
  * expanded pages, plus the parts; the caller's, 256-byte aligned; calls that may overlap on the device must not share

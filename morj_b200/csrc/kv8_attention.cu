@@ -44,6 +44,20 @@ struct __align__(16) Item {
   int kv_base, kv_len; // its first list entry and its keys
 };
 
+// Quotients by a number the host knows, from a 32-bit reciprocal (exact for 0 <= t < 2^31): the GPU has no division, and
+// some 30 instructions for one in every loader's and store loop cost up to a third of a call.
+struct Quotient {
+  int d, shift;
+  unsigned magic;  // t / d = umulhi(t, magic) >> shift for d > 1
+  // with l = ceil(log2 d): floor(t / d) = t * (floor(2^(31 + l) / d) + 1) >> (31 + l) for 0 <= t < 2^31, 2 <= d < 2^31
+  explicit Quotient(int d_) : d(d_), shift(0), magic(0) {
+    int l = 0;
+    while (l < 31 && (1u << l) < (unsigned)d) ++l;
+    if (d > 1) magic = (unsigned)((1ull << (31 + l)) / d + 1), shift = l - 1;
+  }
+  MORJ_DEV int of(int t) const { return d == 1 ? t : (int)(__umulhi((unsigned)t, magic) >> shift); }
+};
+
 struct Args {
   const __nv_bfloat16* q;
   const uint8_t* k;
@@ -52,9 +66,8 @@ struct Args {
   const float* vs;
   __nv_bfloat16* out;
   const int* kv_indices;
-  int n_bidir, hq, hk, page_size;
-  unsigned page_magic;  // t / page_size = umulhi(t, page_magic) >> page_shift (page_size > 1)
-  int page_shift, window, pool_slots;
+  int n_bidir, hq, hk, window, pool_slots;
+  Quotient page, group;  // by the page size, by hq / hk
   float scale_log2;
   float* ws;
 };
@@ -72,13 +85,14 @@ __host__ __device__ inline void visible(int q_len, int kv_len, bool bidir, int w
   if (*lo < 0) *lo = 0;
 }
 
-// Page of key t: t / page_size by a 32-bit reciprocal from the host (exact for 0 <= t < 2^31), since a hardware-free
-// division is some 30 instructions in every loader's loop. Slot of key t in the page with list entry `entry`.
-MORJ_DEV int page_of(const Args& a, int t) {
-  return a.page_size == 1 ? t : (int)(__umulhi((unsigned)t, a.page_magic) >> a.page_shift);
-}
+// slot of key t in the page with list entry `entry`
 MORJ_DEV long long slot_of(const Args& a, int entry, int t) {
-  return (long long)entry * a.page_size + (t - page_of(a, t) * a.page_size);
+  return (long long)entry * a.page.d + (t - a.page.of(t) * a.page.d);
+}
+// where row `row` of an item's segment (query * G + head of the group) lies in q and out: its (token, head) index
+MORJ_DEV size_t row_index(const Args& a, const Item& it, int h, int row) {
+  const int query = a.group.of(row);
+  return (size_t)(it.q_start + query) * a.hq + h * a.group.d + (row - query * a.group.d);
 }
 
 MORJ_DEV void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -88,7 +102,7 @@ MORJ_DEV void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint
 }
 // the same with rows 8..15 of A zero: their sums are dropped
 MORJ_DEV void mma_f16_top(float (&c)[4], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
-  float x, y;
+  [[maybe_unused]] float x, y;
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%9,%9};"
                : "+f"(c[0]), "+f"(c[1]), "=f"(x), "=f"(y)
                : "r"(a0), "r"(0u), "r"(a2), "r"(b0), "r"(b1), "f"(0.f));
@@ -221,7 +235,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
   const int* list = a.kv_indices + it.kv_base;
   const unsigned row_bytes = (unsigned)a.hk * D;
   auto key = [&](int i) { return t_first + i * (WARPS * STEP) + lane; };
-  auto entry = [&](int i) { return i < groups ? __ldg(list + page_of(a, min(key(i), t_end - 1))) : 0; };
+  auto entry = [&](int i) { return i < groups ? __ldg(list + a.page.of(min(key(i), t_end - 1))) : 0; };
   auto issue = [&](int i, int e) {  // ask for group i; e: the lane's page entry
     if (i >= groups) return;
     const int place = i % R_STAGES;
@@ -276,9 +290,9 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
 #pragma unroll
     for (int i = 0; i < KRUN / 8; ++i) raw[i] = make_uint4(0, 0, 0, 0);
     if (r < n_rows) {
-      visible(it.q_len, it.kv_len, bidir, a.window, r / G, &lo[b], &hi[b]);
+      visible(it.q_len, it.kv_len, bidir, a.window, a.group.of(r), &lo[b], &hi[b]);
       const uint4* src = reinterpret_cast<const uint4*>(
-          a.q + ((size_t)(it.q_start + r / G) * a.hq + h * G + r % G) * D + c4 * KRUN);
+          a.q + row_index(a, it, h, r) * D + c4 * KRUN);
 #pragma unroll
       for (int i = 0; i < KRUN / 8; ++i) raw[i] = __ldg(src + i);
     }
@@ -479,17 +493,18 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
       part[2 * UNIT + r * D + d] = oo;
     } else {
       const int row = it.r0 + r;
-      a.out[((size_t)(it.q_start + row / G) * a.hq + h * G + row % G) * D + d] =
+      a.out[row_index(a, it, h, row) * D + d] =
           __float2bfloat16(ll == 0.f ? 0.f : oo / ll);
     }
   }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// Many rows per segment: the pages these segments list are expanded once to FP16, then attended to on tcgen05.
+// Many rows per segment: the pages these segments list are expanded once to 16 bits, then attended to on tcgen05.
 //
-// expand_kernel: pool[i] = FP16(code * scale / ref) of every distinct listed slot, K and V, in the order the lists name
-// them; ref is the head's largest scale among them, so a value keeps all its bits down to 2^-15 of it. A key is used by
+// expand_kernel: every distinct listed slot in the order the lists name them, K as BF16 (code * scale is exact there, and
+// queries are BF16), V as FP16(code * scale / ref) with the head's largest scale among them, so that probabilities can be
+// FP16 too (11 bits); a value keeps all its bits down to 2^-15 of ref. A key is used by
 // every 128-row tile that sees it: expanding costs 3 bytes of traffic per code once (35.7 M codes, the 8,704 tokens of
 // a 16-head layer, K and V), where converting in the tile loaders (built and measured) cost each tile the conversion,
 // the address arithmetic and the instruction cache: 130 us on the op-level tree (2048 + 8 x 64) against the 62 us of the
@@ -500,14 +515,14 @@ constexpr int E_THREADS = 256;
 template <int D>
 __global__ void __launch_bounds__(E_THREADS) expand_kernel(const Args a, const int2* __restrict__ pages, int n_slots,
                                                            const int* __restrict__ blocks, int n_blocks,
-                                                           __half* __restrict__ k_out, __half* __restrict__ v_out,
+                                                           uint16_t* __restrict__ k_out, uint16_t* __restrict__ v_out,
                                                            float* __restrict__ refs) {
   pdl_wait();  // the previous kernel on the stream has completed
   pdl_trigger();
   constexpr int LPR = D / 8;                     // lanes per row: 8 codes in, 16 bytes out
   constexpr int SLOTS = BN / (E_THREADS / 64);   // slots of a warp (half of the warps K, half V)
   constexpr int N = SLOTS / (32 / LPR);          // loads of a lane
-  __shared__ float red[2][E_THREADS / 32];
+  __shared__ float red[E_THREADS / 32];
   const int h = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   // this CTA's codes first: nothing below is needed to ask for them
   const bool is_v = warp >= E_THREADS / 64;
@@ -522,9 +537,9 @@ __global__ void __launch_bounds__(E_THREADS) expand_kernel(const Args a, const i
     const int t = t_warp + i * (32 / LPR);
     sc[i] = 0.f, w[i] = make_uint2(0, 0);
     if (t < n_slots) {
-      const int p = page_of(a, t), at = t - p * a.page_size;
+      const int p = a.page.of(t), at = t - p * a.page.d;
       const int2 page = __ldg(pages + p);  // (page of the pool, its slots that are listed: the rest is zeros)
-      const long long slot = (long long)page.x * a.page_size + at;
+      const long long slot = (long long)page.x * a.page.d + at;
       if (at >= page.y) {
       } else if (slot >= a.pool_slots) {
         if (lane % LPR == 0) report(kErrBadIndex);
@@ -534,27 +549,21 @@ __global__ void __launch_bounds__(E_THREADS) expand_kernel(const Args a, const i
       }
     }
   }
-  // the head's largest scales (every CTA of the head finds the same)
-  float kr = 0.f, vr = 0.f;
+  // V's largest scale of the head (every CTA of the head finds the same)
+  float vr = 0.f;
   for (int i = threadIdx.x; i < n_blocks; i += E_THREADS) {
     const int b = __ldg(blocks + i);
-    if ((long long)b * BLOCK >= a.pool_slots) continue;  // (reported above)
-    kr = fmaxf(kr, __ldg(a.ks + (size_t)b * a.hk + h));
-    vr = fmaxf(vr, __ldg(a.vs + (size_t)b * a.hk + h));
+    if ((long long)b * BLOCK < a.pool_slots) vr = fmaxf(vr, __ldg(a.vs + (size_t)b * a.hk + h));  // (else: reported above)
   }
 #pragma unroll
-  for (int x = 16; x > 0; x >>= 1) {
-    kr = fmaxf(kr, __shfl_xor_sync(0xffffffffu, kr, x));
-    vr = fmaxf(vr, __shfl_xor_sync(0xffffffffu, vr, x));
-  }
-  if (lane == 0) red[0][warp] = kr, red[1][warp] = vr;
+  for (int x = 16; x > 0; x >>= 1) vr = fmaxf(vr, __shfl_xor_sync(0xffffffffu, vr, x));
+  if (lane == 0) red[warp] = vr;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < E_THREADS / 32; ++i) kr = fmaxf(kr, red[0][i]), vr = fmaxf(vr, red[1][i]);
-  if (blockIdx.x == 0 && threadIdx.x == 0) refs[h] = kr, refs[a.hk + h] = vr;
-  const float ref = is_v ? vr : kr;
-  const float inv = ref > 0.f ? 1.f / ref : 1.f;
-  __half* out = (is_v ? v_out : k_out) + (size_t)h * D + (lane % LPR) * 8;
+  for (int i = 0; i < E_THREADS / 32; ++i) vr = fmaxf(vr, red[i]);
+  if (blockIdx.x == 0 && threadIdx.x == 0) refs[h] = vr;
+  const float inv = is_v && vr > 0.f ? 1.f / vr : 1.f;
+  uint16_t* out = (is_v ? v_out : k_out) + (size_t)h * D + (lane % LPR) * 8;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const int t = t_warp + i * (32 / LPR);
@@ -562,22 +571,29 @@ __global__ void __launch_bounds__(E_THREADS) expand_kernel(const Args a, const i
     const float f = sc[i] * inv;
     const float2 x0 = codes2_f32(w[i].x & 0xffffu), x1 = codes2_f32(w[i].x >> 16);
     const float2 x2 = codes2_f32(w[i].y & 0xffffu), x3 = codes2_f32(w[i].y >> 16);
-    *reinterpret_cast<uint4*>(out + (unsigned long long)t * row_bytes) =
-        make_uint4(pack_f16x2(x0.x * f, x0.y * f), pack_f16x2(x1.x * f, x1.y * f), pack_f16x2(x2.x * f, x2.y * f),
-                   pack_f16x2(x3.x * f, x3.y * f));
+    uint4 u;
+    if (is_v)
+      u = make_uint4(pack_f16x2(x0.x * f, x0.y * f), pack_f16x2(x1.x * f, x1.y * f), pack_f16x2(x2.x * f, x2.y * f),
+                     pack_f16x2(x3.x * f, x3.y * f));
+    else
+      u = make_uint4(pack_bf16x2(x0.x * f, x0.y * f), pack_bf16x2(x1.x * f, x1.y * f), pack_bf16x2(x2.x * f, x2.y * f),
+                     pack_bf16x2(x3.x * f, x3.y * f));
+    *reinterpret_cast<uint4*>(out + (unsigned long long)t * row_bytes) = u;
   }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
-// tile_kernel: 128 rows of a segment and KV head against 64 keys at a time, on tcgen05 (FP16 x FP16, FP32 in TMEM).
+// tile_kernel: 128 rows of a segment and KV head against 64 keys at a time, on tcgen05 (BF16 scores, FP16 P V, FP32 in
+// TMEM).
 //   warps 0, 2  K and V loaders: a chunk whose 64 expanded slots are consecutive by TMA, others gathered by cp.async
 //   warp 1      MMA issuer (one thread): S_c = Q K_c^T into TMEM buffer c % 2, O += P_c V_c with P read from TMEM
-//   warps 4-7   softmax (thread = row): prologue (Q row to FP16 and shared memory), mask, online maximum and sum, P as
-//               FP16 over its own scores in TMEM, the final O / l or the part's (maximum, sum, O)
+//   warp 3      Q rows by cp.async (any hq / hk)
+//   warps 4-7   softmax (thread = row): mask, online maximum and sum, P as FP16 over its own scores in TMEM, the final
+//               O / l or the part's (maximum, sum, O), staged through shared memory to store whole rows
 // The pipeline is tree_attention_kernel's (S and P double-buffered in TMEM, a K buffer free once its S is complete, a V
 // buffer once its P V is, two CTAs per SM); what it lacks there is the parts of a key range and rows that see nothing.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int T_THREADS = 256;          // (warp 3 has no role)
+constexpr int T_THREADS = 256;
 constexpr int T_TMEM_COLS = 256;        // S/P buffers at columns [0, 64) and [64, 128), O at [128, 128 + D)
 constexpr float T_RESCALE_LOG2 = 8.0f;  // O is rescaled when a row's maximum grows by more than 2^8 (2^4: 3-4% slower),
 constexpr float T_P_LOG2 = 7.0f;        // so that 2^7 p <= 2^15 stays inside FP16: p's smallest step is 2^-31
@@ -589,7 +605,7 @@ struct TSmem {
   static constexpr int K_OFF = Q_BYTES;               // 2 buffers
   static constexpr int V_OFF = K_OFF + 2 * KV_BYTES;  // 2 buffers
   static constexpr int BAR_OFF = V_OFF + 2 * KV_BYTES;
-  // barriers: (unused), k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], done; TMEM slot, abort flag
+  // barriers: q_full, k_full[2], v_full[2], s_full[2], p_full[2], pv_done[2], done; TMEM slot, abort flag
   static constexpr int TOTAL = BAR_OFF + 128;
 };
 
@@ -633,7 +649,7 @@ MORJ_DEV void sts16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t 
 // another, the box around them is loaded: its other rows are masked keys, and finite (listed slots, zeros past a page's
 // listed ones or past the end).
 template <int D>
-MORJ_DEV void load_chunk(uint32_t dst, uint32_t full, const CUtensorMap* map, const __half* __restrict__ pool, int s0,
+MORJ_DEV void load_chunk(uint32_t dst, uint32_t full, const CUtensorMap* map, const uint16_t* __restrict__ pool, int s0,
                          int s1, int hk, int h, int lane) {
   const unsigned any = __ballot_sync(0xffffffffu, s0 >= 0 || s1 >= 0);
   const int mine = s0 >= 0 ? s0 - 2 * lane : s1 - 2 * lane - 1;  // slot of key t0 if the run holds
@@ -649,7 +665,7 @@ MORJ_DEV void load_chunk(uint32_t dst, uint32_t full, const CUtensorMap* map, co
 #pragma unroll
   for (int k2 = 0; k2 < 2; ++k2) {
     const int k = 2 * lane + k2, slot = k2 ? s1 : s0;
-    const __half* src = pool + (slot >= 0 ? ((size_t)slot * hk + h) * D : 0);
+    const uint16_t* src = pool + (slot >= 0 ? ((size_t)slot * hk + h) * D : 0);
 #pragma unroll 4
     for (int u = 0; u < D / 8; ++u)
       cp_async16(dst + (uint32_t)((u >> 3) * (BN * 128)) + sw128_offset(k, u & 7), src + u * 8, slot >= 0 ? 16u : 0u);
@@ -663,8 +679,8 @@ MORJ_DEV void load_chunk(uint32_t dst, uint32_t full, const CUtensorMap* map, co
 template <int D>
 __global__ void __launch_bounds__(T_THREADS, 2)
     tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const Args a,
-                const Item* __restrict__ items, const int* __restrict__ list, const __half* __restrict__ k_pool,
-                const __half* __restrict__ v_pool, int n_slots, const float* __restrict__ refs) {
+                const Item* __restrict__ items, const int* __restrict__ list, const uint16_t* __restrict__ k_pool,
+                const uint16_t* __restrict__ v_pool, int n_slots, const float* __restrict__ refs) {
   pdl_wait();  // the previous kernel on the stream has completed
   pdl_trigger();
   using L = TSmem<D>;
@@ -675,7 +691,7 @@ __global__ void __launch_bounds__(T_THREADS, 2)
     return;
   }
   const uint32_t bar0 = sbase + L::BAR_OFF;
-  const uint32_t k_full = bar0 + 8, v_full = bar0 + 24;
+  const uint32_t q_full = bar0, k_full = bar0 + 8, v_full = bar0 + 24;
   const uint32_t s_full = bar0 + 40, p_full = bar0 + 56, pv_done = bar0 + 72, done = bar0 + 88;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::BAR_OFF + 96);
   volatile int* abort = reinterpret_cast<volatile int*>(smem + L::BAR_OFF + 100);
@@ -690,6 +706,7 @@ __global__ void __launch_bounds__(T_THREADS, 2)
   const int n_chunks = t_stop > it.t0 ? (t_stop - t_begin + BN - 1) / BN : 0;
 
   if (threadIdx.x == 0) {
+    mbar_init(q_full, 1);
     for (int b = 0; b < 2; ++b) {
       mbar_init(k_full + 8 * b, 1);
       mbar_init(v_full + 8 * b, 1);
@@ -704,39 +721,6 @@ __global__ void __launch_bounds__(T_THREADS, 2)
   if (warp == 1) {
     tmem_alloc(smem_u32(tmem_slot), T_TMEM_COLS);
     tmem_relinquish();
-  }
-  // softmax warps: thread = row
-  const int r = (warp & 3) * 32 + lane, row = it.r0 + r, qi = row / G;
-  const bool row_ok = row < n_rows;
-  const size_t row_at = ((size_t)(it.q_start + qi) * a.hq + h * G + row % G) * D;
-  float scale = 0.f, vr = 0.f;  // scores times `scale` are in the log2 domain; V's reference
-  if (warp >= 4) {
-    // Q row: its largest magnitude, then FP16 of q / qs into the swizzled tile (read twice, the second time from L1: the
-    // row in registers would be 64 of them)
-    const float kr = refs ? __ldg(refs + h) : 0.f;
-    vr = refs ? __ldg(refs + a.hk + h) : 0.f;
-    const uint4* src = reinterpret_cast<const uint4*>(a.q + row_at);
-    const uint4 zero = make_uint4(0, 0, 0, 0);
-    float amax = 0.f;
-#pragma unroll 8
-    for (int i = 0; i < D / 8; ++i) {
-      float x[8];
-      unpack8(row_ok ? __ldg(src + i) : zero, x);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) amax = fmaxf(amax, fabsf(x[e]));
-    }
-    const float qs = row_scale(amax), inv = 1.f / qs;
-#pragma unroll 4
-    for (int i = 0; i < D / 8; ++i) {
-      float x[8];
-      unpack8(row_ok ? __ldg(src + i) : zero, x);
-      sts16(sbase + (i >> 3) * (T_ROWS * 128) + sw128_offset(r, i & 7), pack_f16x2(x[0] * inv, x[1] * inv),
-            pack_f16x2(x[2] * inv, x[3] * inv), pack_f16x2(x[4] * inv, x[5] * inv),
-            pack_f16x2(x[6] * inv, x[7] * inv));
-    }
-    fence_proxy_async_smem();
-    scale = qs * kr * a.scale_log2;
-    scale = scale < 1.2e-38f ? 1.2e-38f : scale;  // (a masked score stays -inf times it)
   }
   tc_fence_before();
   __syncthreads();
@@ -753,7 +737,7 @@ __global__ void __launch_bounds__(T_THREADS, 2)
     const int* pages = list + it.kv_base;
     auto slot = [&](int t) {  // expanded slot of key t, -1 outside the part
       if (t < it.t0 || t >= t_stop) return -1;
-      const long long s = slot_of(a, __ldg(pages + page_of(a, t)), t);
+      const long long s = slot_of(a, __ldg(pages + a.page.of(t)), t);
       if (s < 0 || s >= n_slots) {
         report(kErrBadIndex);
         return -1;
@@ -770,9 +754,9 @@ __global__ void __launch_bounds__(T_THREADS, 2)
     }
   } else if (warp == 1) {
     if (lane == 0) {
-      constexpr uint32_t IDESC_S = idesc_f16(T_ROWS, BN);
+      constexpr uint32_t IDESC_S = idesc_bf16(T_ROWS, BN);
       constexpr uint32_t IDESC_O = idesc_f16(T_ROWS, D, /*b_mn_major=*/true);
-      bool ok = n_chunks > 0;
+      bool ok = n_chunks > 0 && mbar_wait(q_full, 0, abort, kErrTimeoutAttention);
       // operand descriptors: one per buffer, advanced per 16-deep K step by the byte offset (>> 4)
       const uint64_t q_desc = sw128_desc(sbase);
       const uint64_t k_desc0 = sw128_desc(sbase + L::K_OFF), v_desc0 = sw128_desc(sbase + L::V_OFF, BN * 128);
@@ -813,9 +797,27 @@ __global__ void __launch_bounds__(T_THREADS, 2)
       umma_commit(done);
       mbar_wait_landed(done, 0);
     }
-  } else if (warp >= 4) {
+  } else if (warp == 3) {
+    // ---------------- Q rows into the swizzled tile: D / 8 lanes share a row ----------------
+    constexpr int LPR = D / 8;
+#pragma unroll 4
+    for (int i = lane / LPR; i < T_ROWS; i += 32 / LPR) {
+      const int x = it.r0 + i, u = lane % LPR;
+      const bool ok = x < n_rows;
+      const __nv_bfloat16* src = a.q + (ok ? row_index(a, it, h, x) * D + u * 8 : 0);
+      cp_async16(sbase + (u >> 3) * (T_ROWS * 128) + sw128_offset(i, u & 7), src, ok ? 16u : 0u);
+    }
+    asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(q_full);
+  } else {
     // ---------------- softmax warpgroup ----------------
+    const int r = (warp & 3) * 32 + lane, row = it.r0 + r, qi = a.group.of(row);
     const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const bool row_ok = row < n_rows;
+    const float vr = refs ? __ldg(refs + h) : 0.f;
+    const float scale = a.scale_log2;  // scores times it are in the log2 domain (> 0)
     int lo = 1, hi = 0;  // visible key positions [lo, hi] of this part
     if (row_ok) {
       visible(it.q_len, it.kv_len, bidir, a.window, qi, &lo, &hi);
@@ -910,13 +912,14 @@ __global__ void __launch_bounds__(T_THREADS, 2)
     }
     if (ok && (n_chunks == 0 || warp_wait(pv_done + 8 * ((n_chunks - 1) & 1), ((n_chunks - 1) >> 1) & 1, abort))) {
       tc_fence_after();
-      // a finished row: O / l times V's reference; a part: (maximum, sum, O in units of the values)
+      // A finished row: O / l times V's reference; a part: (maximum, sum, O in units of the values). The warp's 32 rows
+      // go through its quarter of the K and V buffers, which nothing reads any more, and out as whole rows.
       const bool part_of = it.unit >= 0;
       const float unit = exp2_int(-(int)T_P_LOG2);
       const float back = l_run == 0.f ? 0.f : part_of ? vr * unit : vr / l_run;
       float* part = a.ws + ((size_t)(max(it.unit, 0) + r / UNIT) * a.hk + h) * (UNIT * (D + 2));
       if (part_of && row_ok) part[r % UNIT] = m_used, part[UNIT + r % UNIT] = l_run * unit;
-      float4* dst = reinterpret_cast<float4*>(part + 2 * UNIT + (r % UNIT) * D);
+      const uint32_t stage = sbase + L::K_OFF + (warp & 3) * (32 * D * 4);
 #pragma unroll 1
       for (int col = 0; col < D; col += 32) {
         uint32_t o[32];
@@ -924,18 +927,35 @@ __global__ void __launch_bounds__(T_THREADS, 2)
           tmem_ld32(t_lane + 128 + col, o);
           tmem_wait_ld();
         }
-        if (!row_ok) continue;
 #pragma unroll
         for (int v8 = 0; v8 < 4; ++v8) {
           float x[8];
 #pragma unroll
           for (int e = 0; e < 8; ++e) x[e] = back == 0.f ? 0.f : __uint_as_float(o[v8 * 8 + e]) * back;
+          const int c8 = col / 8 + v8;  // (16-byte units swizzled by the row: free of bank conflicts both ways)
           if (part_of) {
-            dst[(col + v8 * 8) / 4] = make_float4(x[0], x[1], x[2], x[3]);
-            dst[(col + v8 * 8) / 4 + 1] = make_float4(x[4], x[5], x[6], x[7]);
+            sts16(stage + lane * (D * 4) + (((2 * c8) ^ (lane & 7)) << 4), __float_as_uint(x[0]), __float_as_uint(x[1]),
+                  __float_as_uint(x[2]), __float_as_uint(x[3]));
+            sts16(stage + lane * (D * 4) + (((2 * c8 + 1) ^ (lane & 7)) << 4), __float_as_uint(x[4]),
+                  __float_as_uint(x[5]), __float_as_uint(x[6]), __float_as_uint(x[7]));
           } else {
-            store8(a.out + row_at + col + v8 * 8, x);
+            sts16(stage + lane * (D * 2) + ((c8 ^ (lane & 7)) << 4), pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]),
+                  pack_bf16x2(x[4], x[5]), pack_bf16x2(x[6], x[7]));
           }
+        }
+      }
+      __syncwarp();
+      const int units = part_of ? D / 4 : D / 8;  // 16-byte units of a row, a power of two up to 32
+      for (int i = lane / units; i < 32; i += 32 / units) {
+        const int u = lane % units, x = (warp & 3) * 32 + i, rx = it.r0 + x;
+        if (rx >= n_rows) break;
+        const uint4 v = lds16(stage + i * (units * 16) + ((u ^ (i & 7)) << 4));
+        if (part_of) {
+          float* dst = a.ws + ((size_t)(it.unit + x / UNIT) * a.hk + h) * (UNIT * (D + 2)) + 2 * UNIT + (x % UNIT) * D;
+          reinterpret_cast<uint4*>(dst)[u] = v;
+        } else {
+          __nv_bfloat16* dst = a.out + row_index(a, it, h, rx) * D;
+          reinterpret_cast<uint4*>(dst)[u] = v;
         }
       }
     }
@@ -1001,7 +1021,7 @@ __global__ void __launch_bounds__(C_WARPS * 32) combine_kernel(const Args a, con
     }
   }
   const float inv = ll == 0.f ? 0.f : 1.f / ll;
-  __nv_bfloat16* dst = a.out + ((size_t)(it.q_start + row / G) * a.hq + h * G + row % G) * D + lane * V;
+  __nv_bfloat16* dst = a.out + row_index(a, it, h, row) * D + lane * V;
 #pragma unroll
   for (int e = 0; e < V; e += 2)
     *reinterpret_cast<uint32_t*>(dst + e) = pack_bf16x2(ll == 0.f ? 0.f : o[e] * inv, ll == 0.f ? 0.f : o[e + 1] * inv);
@@ -1023,21 +1043,21 @@ static int configure() {
   return e == cudaSuccess ? MORJ_OK : set_error(MORJ_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
 }
 
-// Offsets in the caller's workspace: the expanded K and V, the heads' reference scales, the parts.
+// Offsets in the caller's workspace: the expanded K and V, V's reference scales, the parts.
 struct Space {
   size_t k, v, refs, parts, bytes;
   Space(const int* counts, int hk, int d, int page_size) {
     const auto up = [](size_t n) { return (n + 255) / 256 * 256; };
-    const size_t pool = up((size_t)counts[6] * page_size * hk * d * sizeof(__half));
+    const size_t pool = up((size_t)counts[6] * page_size * hk * d * sizeof(uint16_t));
     k = 0, v = pool, refs = 2 * pool;
-    parts = refs + (counts[6] ? up((size_t)2 * hk * sizeof(float)) : 0);
+    parts = refs + (counts[6] ? up((size_t)hk * sizeof(float)) : 0);
     bytes = parts + (size_t)counts[2] * hk * UNIT * (d + 2) * sizeof(float);
   }
 };
 
 template <int D>
 static int launch(Args a, const int* counts, const int* work, char* ws, cudaStream_t s) {
-  const Space at(counts, a.hk, D, a.page_size);
+  const Space at(counts, a.hk, D, a.page.d);
   a.ws = reinterpret_cast<float*>(ws + at.parts);
   const int n_rows = counts[0], n_combine = counts[1], n_tiles = counts[5], n_pages = counts[6], n_blocks = counts[7];
   const Item* items = reinterpret_cast<const Item*>(work);
@@ -1047,9 +1067,9 @@ static int launch(Args a, const int* counts, const int* work, char* ws, cudaStre
     const int* pages = work + (size_t)(n_tiles + n_rows + n_combine) * (sizeof(Item) / sizeof(int));
     const int* blocks = pages + 2 * (size_t)n_pages;
     const int* list = blocks + n_blocks;
-    const int n_slots = n_pages * a.page_size;
-    __half* kx = reinterpret_cast<__half*>(ws + at.k);
-    __half* vx = reinterpret_cast<__half*>(ws + at.v);
+    const int n_slots = n_pages * a.page.d;
+    uint16_t* kx = reinterpret_cast<uint16_t*>(ws + at.k);
+    uint16_t* vx = reinterpret_cast<uint16_t*>(ws + at.v);
     float* refs = reinterpret_cast<float*>(ws + at.refs);
     CUtensorMap km, vm;
     // expanded pools [slots, hk, D]: box = 64 columns x 1 head x 64 slots (one slot and an unused map where none is seen)
@@ -1059,7 +1079,7 @@ static int launch(Args a, const int* counts, const int* work, char* ws, cudaStre
     const unsigned box[3] = {64u, 1u, (unsigned)BN};
     void* kp = n_slots ? (void*)kx : const_cast<uint8_t*>(a.k);
     void* vp = n_slots ? (void*)vx : const_cast<uint8_t*>(a.v);
-    if ((st = encode_tiled(&km, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, kp, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)))
+    if ((st = encode_tiled(&km, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, kp, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)))
       return st;
     if ((st = encode_tiled(&vm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, vp, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)))
       return st;
@@ -1070,7 +1090,7 @@ static int launch(Args a, const int* counts, const int* work, char* ws, cudaStre
       refs = nullptr;
     if (st) return st;
     st = launch_pdl("tile_kernel", tile_kernel<D>, dim3((unsigned)n_tiles * a.hk), dim3(T_THREADS), TSmem<D>::TOTAL, s,
-                    km, vm, a, items, list, (const __half*)kx, (const __half*)vx, n_slots, (const float*)refs);
+                    km, vm, a, items, list, (const uint16_t*)kx, (const uint16_t*)vx, n_slots, (const float*)refs);
     if (st) return st;
     items += n_tiles;
   }
@@ -1250,7 +1270,8 @@ extern "C" int morj_tree_attention_kv8_workspace(const int* counts, int hk, int 
 
 extern "C" int morj_tree_attention_kv8(const void* q, int n_q, const void* k_codes, const float* k_scale,
                                        const void* v_codes, const float* v_scale, int pool_slots, void* out,
-                                       const int* kv_indices, int n_bidir, int hq, int hk, int d, int page_size, int window, float sm_scale, const int* work, const int* counts,
+                                       const int* kv_indices, int n_bidir, int hq, int hk, int d, int page_size,
+                                       int window, float sm_scale, const int* work, const int* counts,
                                        void* workspace, unsigned long long workspace_bytes, void* stream) {
   using namespace morj;
   if (!counts) return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8: null counts");
@@ -1276,14 +1297,9 @@ extern "C" int morj_tree_attention_kv8(const void* q, int n_q, const void* k_cod
   if (workspace_bytes < need || (need && !workspace))
     return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8: a workspace of %llu bytes given, %llu needed",
                      workspace_bytes, need);
-  // with l = ceil(log2 d): floor(t / d) = t * (floor(2^(31 + l) / d) + 1) >> (31 + l) for 0 <= t < 2^31, 2 <= d < 2^31
-  int l = 0;
-  while (l < 31 && (1u << l) < (unsigned)page_size) ++l;
-  const unsigned page_magic = page_size > 1 ? (unsigned)((1ull << (31 + l)) / page_size + 1) : 0;
-  const int page_shift = l - 1;
   const kv8::Args a{(const __nv_bfloat16*)q, (const uint8_t*)k_codes, k_scale, (const uint8_t*)v_codes, v_scale,
-                    (__nv_bfloat16*)out, kv_indices, n_bidir, hq, hk, page_size,
-                    page_magic, page_shift, window, pool_slots, sm_scale * kv8::LOG2E, nullptr};
+                    (__nv_bfloat16*)out, kv_indices, n_bidir, hq, hk, window, pool_slots, kv8::Quotient(page_size),
+                    kv8::Quotient(hq / hk), sm_scale * kv8::LOG2E, nullptr};
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
   return d == 128 ? kv8::launch<128>(a, counts, work, (char*)workspace, s)
                   : kv8::launch<64>(a, counts, work, (char*)workspace, s);
