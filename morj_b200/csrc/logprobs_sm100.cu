@@ -5,9 +5,15 @@
 //
 // logits_kernel is a GEMM whose epilogue folds every accumulator row into three running numbers, with m the largest z
 // so far: m, s = sum exp(z - m) and t = sum exp(z - m) (z - m), so that lse = m + log s and entropy = log s - t / s
-// without cancellation. A CTA keeps them per row across the vocabulary tiles it computes, with a sorted list of the
-// row's top candidates; the softcap is monotone, so candidates are compared by the raw logit. finish_kernel joins the
-// CTAs' numbers and lists of a row and adds the given tokens' logits as plain dot products.
+// without cancellation. A CTA keeps them per row across the vocabulary tiles it computes. finish_kernel joins the CTAs'
+// numbers of a row and adds the given tokens' logits as plain dot products.
+//
+// Top alternatives: the softcap is monotone, so candidates are compared by the raw logit. A logit is appended, unordered,
+// to the CTA's list of the row when it reaches a bound that at least `top` logits of the row are known to reach: at first
+// the top-th largest of the 32 group maxima of the CTA's first tile, then the largest such bound of any CTA. That leaves
+// about ten candidates a row and CTA and no branch per logit; a list that fills up all the same (equal or rising logits)
+// is cut to its top ones. (A sorted list per row in shared memory cost 1.0 ms of 2.1 on 540 rows with 5 alternatives: one
+// of 32 rows inserting holds up the warp.)
 //
 // One CTA per SM: warp 0 TMA producer, warp 1 MMA issuer (tcgen05, M = 128, N = 256, two TMEM accumulators), warps 2-5
 // epilogue (thread = row). Row blocks are the fast tile index: the CTAs in flight share a few vocabulary tiles, so w
@@ -25,8 +31,9 @@ constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;
 constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
 constexpr int STAGES = 4;
 constexpr int MAX_TOP = MORJ_MAX_TOP;
-constexpr int LIST_BYTES = BM * MAX_TOP * 8;
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + LIST_BYTES + 1024 /*align*/ + 256 /*barriers*/;
+constexpr int CAND = 64;  // candidates a CTA's list of a row holds: top ones (32 at most) and one group of 32 more
+static_assert(CAND >= MAX_TOP + 32, "a cut list takes a whole group of columns");
+constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*align*/ + 256 /*barriers*/;
 static_assert(SMEM_BYTES <= 232448, "shared memory per CTA");
 constexpr int TMEM_COLS = 512;
 constexpr int THREADS = 192;
@@ -34,13 +41,25 @@ constexpr int CHUNK_ROWS = 2048;
 constexpr uint32_t IDESC = idesc_bf16(BM, BN);
 constexpr float LOG2E = 1.4426950408889634f;
 
-// What one CTA knows of one row: [cta][row] stats, [cta][row block][k][128 rows] candidates (logit, id).
+// What the CTAs know of the rows.
 struct Scratch {
-  float4* stats;  // m, s, t, number of candidates
-  uint2* lists;
-  int rows;       // rows of a chunk rounded up to whole row blocks
+  float4* stats;    // [cta][row]: m, s, t, number of candidates
+  float* own;       // [cta][row]: candidates must exceed it (the top-th of a cut list)
+  uint2* lists;     // [cta][row block][CAND][128 rows]: candidates (logit, id)
+  unsigned* bound;  // [row]: at least `top` logits reach it, as an ordered integer; 0: none known
+  int rows;         // rows of a chunk rounded up to whole row blocks
   int top;
 };
+
+// floats as unsigned integers of the same order (never 0 for a number; -0 as +0), and the next float below such a one
+MORJ_DEV unsigned ordered(float f) {
+  const unsigned b = __float_as_uint(f + 0.f);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+MORJ_DEV float below(unsigned o) {
+  const unsigned p = o - (o == 0x80000000u ? 2u : 1u);  // (below +0 comes -0, which is not below it)
+  return __uint_as_float(p & 0x80000000u ? p & 0x7fffffffu : ~p);
+}
 
 // z = c tanh(l / c). Near 0 tanh's series, elsewhere 1 - 2 / (1 + e^2x): relative error of a few 2^-24 on both sides.
 MORJ_DEV float cap_near(float l, float c, float inv_c) {  // |l| <= c / 4
@@ -69,7 +88,8 @@ MORJ_DEV void raise(float& m, float& s, float& t, float now) {
   m = now;
 }
 
-template <bool CAP>
+// 32 logits into a row's numbers. CAP: 0 no softcap, 1 every |l| of the warp's rows is at most c / 4, 2 any.
+template <int CAP>
 MORJ_DEV void fold(const uint32_t (&r)[32], int valid, float c, float inv_c, float& m, float& s, float& t, float mx) {
   const float zmx = CAP ? cap(mx, c, inv_c) : mx;
   if (zmx > m) raise(m, s, t, zmx);
@@ -78,7 +98,7 @@ MORJ_DEV void fold(const uint32_t (&r)[32], int valid, float c, float inv_c, flo
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
     const float l = __uint_as_float(r[i]);
-    const float u = (CAP ? cap(l, c, inv_c) : l) - shift;
+    const float u = (CAP == 0 ? l : CAP == 1 ? cap_near(l, c, inv_c) : cap(l, c, inv_c)) - shift;
     const float e = fast_exp2(u * LOG2E);
     if (i < valid) {
       s4[i & 3] += e;
@@ -89,14 +109,38 @@ MORJ_DEV void fold(const uint32_t (&r)[32], int valid, float c, float inv_c, flo
   t += (t4[0] + t4[1]) + (t4[2] + t4[3]);
 }
 
+// (logit, id) order of candidates: larger logit first, then the lower id; id < 0: none
+MORJ_DEV bool before(float v, int id, float w, int jd) { return id >= 0 && (jd < 0 || v > w || (v == w && id < jd)); }
+
+// Cuts a row's list (entries 128 apart) to its `top` first ones, keeping their order of ids; returns the last one's logit.
+__device__ __noinline__ float cut_list(uint2* list, int count, int top) {
+  float v[CAND];
+  int id[CAND];
+  for (int i = 0; i < count; ++i) {
+    const uint2 e = list[i * BM];
+    v[i] = __uint_as_float(e.x), id[i] = (int)e.y;
+  }
+  float pv = INFINITY;
+  int pid = -1;
+  for (int k = 0; k < top; ++k) {  // the next one after (pv, pid)
+    float bv = 0.f;
+    int bid = -1;
+    for (int i = 0; i < count; ++i)
+      if ((k == 0 || before(pv, pid, v[i], id[i])) && before(v[i], id[i], bv, bid)) bv = v[i], bid = id[i];
+    pv = bv, pid = bid;
+  }
+  int n = 0;
+  for (int i = 0; i < count; ++i)
+    if (!before(pv, pid, v[i], id[i])) list[n++ * BM] = make_uint2(__float_as_uint(v[i]), (unsigned)id[i]);
+  return pv;
+}
+
 __global__ void __launch_bounds__(THREADS, 1)
     logits_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w, int M, int V,
                   int K, int a_bytes, float c, const Scratch sc) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  float* list_val = reinterpret_cast<float*>(smem + STAGES * STAGE_BYTES);  // [MAX_TOP][128 rows]
-  int* list_id = reinterpret_cast<int*>(list_val + MAX_TOP * BM);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES + LIST_BYTES);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
   // bars: full[STAGES], empty[STAGES], acc_full[2], acc_empty[2], done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 5);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -210,40 +254,73 @@ __global__ void __launch_bounds__(THREADS, 1)
     const int top = sc.top;
     const float inv_c = c > 0.f ? 1.f / c : 0.f;
     float4* stats = sc.stats + (size_t)blockIdx.x * sc.rows + r128;
-    uint2* lists = sc.lists + (size_t)blockIdx.x * sc.rows * top + r128;
-    for (int m = 0; m < num_m; ++m) stats[m * BM] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+    float* own_of = sc.own + (size_t)blockIdx.x * sc.rows + r128;
+    uint2* lists = sc.lists + (size_t)blockIdx.x * sc.rows * CAND + r128;
+    for (int m = 0; m < num_m; ++m) {  // (each thread's own entries: nobody else writes them)
+      stats[m * BM] = make_float4(-INFINITY, 0.f, 0.f, 0.f);
+      if (top) own_of[m * BM] = -INFINITY;
+    }
     int acc = 0;
     uint32_t acc_phase = 0;
-    int held = -1;  // the row block whose list is in shared memory
+    int held = -1;  // the row block whose numbers are in registers
     float4 st = make_float4(-INFINITY, 0.f, 0.f, 0.f);
     int count = 0;
-    float tau = INFINITY;  // candidates must exceed it
+    float own = -INFINITY;
     for (int t = blockIdx.x; t < tiles; t += gridDim.x) {
       const int m = t % num_m, n = t / num_m;
+      const bool row_ok = m * BM + r128 < M;
       if (m != held) {
         if (held >= 0) {
           st.w = __int_as_float(count);
           stats[held * BM] = st;
-          for (int k = 0; k < count; ++k)
-            lists[(size_t)(held * top + k) * BM] =
-                make_uint2(__float_as_uint(list_val[k * BM + r128]), (uint32_t)list_id[k * BM + r128]);
+          if (top) own_of[held * BM] = own;
         }
         st = stats[m * BM];
         count = __float_as_int(st.w);
-        for (int k = 0; k < count; ++k) {
-          const uint2 e = lists[(size_t)(m * top + k) * BM];
-          list_val[k * BM + r128] = __uint_as_float(e.x);
-          list_id[k * BM + r128] = (int)e.y;
-        }
-        tau = top == 0 ? INFINITY : count < top ? -INFINITY : list_val[(top - 1) * BM + r128];
+        own = top ? own_of[m * BM] : INFINITY;
         held = m;
       }
+      uint2* list = lists + (size_t)m * CAND * BM;
+      const unsigned known = top && row_ok ? __ldcg(sc.bound + m * BM + r128) : 0u;  // (arrives during the wait below)
       int ok = lane == 0 ? (int)mbar_wait(accf0 + 8 * acc, acc_phase, abort, kErrTimeoutGemmEpilogue) : 0;
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok) break;
       tc_fence_after();
-      const bool row_ok = m * BM + r128 < M;
       const uint32_t tacc = tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * BN;
+      float tau = row_ok ? own : INFINITY;  // candidates must exceed it
+      if (known) tau = fmaxf(tau, below(known));
+      const bool fresh = top && st.x == -INFINITY && known == 0;
+      if (__any_sync(0xffffffffu, fresh)) {  // (the TMEM loads are the whole warp's)
+        // the rows' first tile: the top-th largest of its 32 groups of 8 columns (columns past V are zeros: left out)
+        float g[32];
+#pragma unroll
+        for (int col = 0; col < BN; col += 32) {
+          uint32_t r[32];
+          tmem_ld32(tacc + col, r);
+          tmem_wait_ld();
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            float x = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+              x = fmaxf(x, n * BN + col + q * 8 + i < V ? __uint_as_float(r[q * 8 + i]) : -INFINITY);
+            g[col / 8 + q] = x;
+          }
+        }
+        float first = INFINITY;
+        for (int k = 0; k < top; ++k) {
+          first = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) first = fmaxf(first, g[i]);
+#pragma unroll
+          for (int i = 0; i < 32; ++i) g[i] = g[i] == first ? -INFINITY : g[i];
+        }
+        if (fresh && row_ok && first > -INFINITY) {
+          atomicMax(sc.bound + m * BM + r128, ordered(first));
+          tau = fmaxf(tau, below(ordered(first)));
+        }
+        __syncwarp();
+      }
 #pragma unroll 1
       for (int col = 0; col < BN; col += 32) {
         const int id0 = n * BN + col, valid = min(32, V - id0);
@@ -251,29 +328,31 @@ __global__ void __launch_bounds__(THREADS, 1)
         uint32_t r[32];
         tmem_ld32(tacc + col, r);
         tmem_wait_ld();
-        float mx = -INFINITY;
+        float mx = -INFINITY, far = 0.f;
 #pragma unroll
-        for (int i = 0; i < 32; ++i) mx = fmaxf(mx, i < valid ? __uint_as_float(r[i]) : -INFINITY);
-        if (c > 0.f)
-          fold<true>(r, valid, c, inv_c, st.x, st.y, st.z, mx);
+        for (int i = 0; i < 32; ++i) {
+          mx = fmaxf(mx, i < valid ? __uint_as_float(r[i]) : -INFINITY);
+          far = fmaxf(far, fabsf(__uint_as_float(r[i])));
+        }
+        if (c == 0.f)
+          fold<0>(r, valid, c, inv_c, st.x, st.y, st.z, mx);
+        else if (__all_sync(0xffffffffu, far <= 0.25f * c || !row_ok))
+          fold<1>(r, valid, c, inv_c, st.x, st.y, st.z, mx);
         else
-          fold<false>(r, valid, c, inv_c, st.x, st.y, st.z, mx);
-        if (row_ok && (mx > tau || (count < top && mx == -INFINITY))) {
-          float v[32];
+          fold<2>(r, valid, c, inv_c, st.x, st.y, st.z, mx);
+        if (__any_sync(0xffffffffu, mx > tau)) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-          for (int i = 0; i < valid; ++i) {
-            const float x = v[i];
-            if (!(x > tau || (count < top && x >= -INFINITY))) continue;
-            int at = count < top ? count++ : top - 1;
-            for (; at > 0 && list_val[(at - 1) * BM + r128] < x; --at) {
-              list_val[at * BM + r128] = list_val[(at - 1) * BM + r128];
-              list_id[at * BM + r128] = list_id[(at - 1) * BM + r128];
-            }
-            list_val[at * BM + r128] = x;
-            list_id[at * BM + r128] = id0 + i;
-            if (count == top) tau = list_val[(top - 1) * BM + r128];
+          for (int i = 0; i < 32; ++i) {
+            const float x = __uint_as_float(r[i]);
+            if (i < valid && x > tau) list[count++ * BM] = make_uint2(r[i], (unsigned)(id0 + i));
           }
+          if (count > CAND - 32) {
+            own = cut_list(list, count, top);
+            count = top;
+            atomicMax(sc.bound + m * BM + r128, ordered(own));
+            tau = fmaxf(tau, own);
+          }
+          __syncwarp();
         }
       }
       tc_fence_before();
@@ -286,9 +365,6 @@ __global__ void __launch_bounds__(THREADS, 1)
     if (held >= 0) {
       st.w = __int_as_float(count);
       stats[held * BM] = st;
-      for (int k = 0; k < count; ++k)
-        lists[(size_t)(held * top + k) * BM] =
-            make_uint2(__float_as_uint(list_val[k * BM + r128]), (uint32_t)list_id[k * BM + r128]);
     }
   }
 
@@ -300,11 +376,9 @@ __global__ void __launch_bounds__(THREADS, 1)
   }
 }
 
-// ---- finish: one CTA per row ----------------------------------------------------------------------------------------
+// ---- finish: two CTAs per row, one for its numbers and top alternatives, one for the given tokens -------------------
 constexpr int F_THREADS = 256;
-
-// (logit, id) order of candidates: larger logit first, then the lower id; id < 0: none
-MORJ_DEV bool before(float v, int id, float w, int jd) { return id >= 0 && (jd < 0 || v > w || (v == w && id < jd)); }
+constexpr int POOL = 2048;
 
 struct Outputs {
   const int* targets;
@@ -323,42 +397,111 @@ __global__ void __launch_bounds__(F_THREADS)
                   long long ld_w, int V, int K, float c, int ctas, const Scratch sc, const Outputs o, int row0) {
   pdl_wait();  // the previous kernel on the stream has completed
   pdl_trigger();
-  __shared__ float red[32], red_v[F_THREADS / 32];
-  __shared__ int red_i[F_THREADS / 32], red_c[F_THREADS / 32];
+  __shared__ float red_s[F_THREADS / 32], red_t[F_THREADS / 32], red_v[2][F_THREADS / 32];
+  __shared__ int red_i[2][F_THREADS / 32], red_c[2][F_THREADS / 32];
   const int local = blockIdx.x, warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const size_t row = (size_t)row0 + local;
+  // what does not depend on anything is asked for first
   float4 st = make_float4(-INFINITY, 0.f, 0.f, 0.f);
   if (threadIdx.x < ctas) st = sc.stats[(size_t)threadIdx.x * sc.rows + local];
+  const uint2* list = sc.lists + ((size_t)threadIdx.x * sc.rows + (local / BM) * BM) * CAND + local % BM;
+  constexpr int AHEAD = 8;
+  uint2 head[AHEAD];  // the first entries of this thread's list (left over from another call past its count)
+  unsigned known = 0;
+  if (blockIdx.y == 0 && sc.top) {
+    known = sc.bound[local];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) head[i] = threadIdx.x < ctas ? __ldcg(list + i * BM) : make_uint2(0, 0);
+  }
+  // the given tokens' logits: eight warps share a round of up to eight of them, each target's columns cut evenly
+  __shared__ float dots[F_THREADS / 32];
+  const int round = min(o.n_targets, F_THREADS / 32);
+  const int per = round ? F_THREADS / 32 / round : 1;
+  auto dot = [&](int j) {  // this warp's share of the target it has in the round from j on
+    const int mine = j + warp / per;
+    float acc = 0.f;
+    if (warp / per < round && mine < o.n_targets) {
+      const int id = o.targets[row * o.n_targets + mine];
+      if (id >= 0 && id < V) {
+        const __nv_bfloat16* hr = h + row * ld_h;
+        const __nv_bfloat16* wr = w + (size_t)id * ld_w;
+#pragma unroll 4
+        for (int k = (warp % per * 32 + lane) * 8; k < K; k += per * 256) {
+          float a[8], b[8];
+          load8(hr + k, a);
+          load8(wr + k, b);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) acc = fmaf(a[e], b[e], acc);
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, x);
+    if (lane == 0) dots[warp] = acc;
+  };
+  if (blockIdx.y == 1) dot(0);
   float m = st.x;
 #pragma unroll
   for (int x = 16; x > 0; x >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, x));
-  if (lane == 0) red_v[warp] = m;
+  if (lane == 0) red_v[0][warp] = m;
   __syncthreads();
-  for (int i = 0; i < F_THREADS / 32; ++i) m = fmaxf(m, red_v[i]);
+#pragma unroll
+  for (int i = 0; i < F_THREADS / 32; ++i) m = fmaxf(m, red_v[0][i]);
   float s = st.y, t = st.z;
   if (st.x != -INFINITY) raise(st.x, s, t, m);
-  s = block_sum(s, red);
-  t = block_sum(t, red);
-  const float ls = logf(s), lse = (m == -INFINITY ? 0.f : m) + ls;
-  if (threadIdx.x == 0) {
-    if (o.lse) o.lse[row] = lse;
-    if (o.entropy) o.entropy[row] = ls - t / s;
+#pragma unroll
+  for (int x = 16; x > 0; x >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, x);
+    t += __shfl_xor_sync(0xffffffffu, t, x);
   }
-  // the lists' heads compete: thread i walks CTA i's sorted list
-  if (sc.top) {
-    const uint2* list = sc.lists + ((size_t)threadIdx.x * sc.rows + (local / BM) * BM) * sc.top + local % BM;
+  if (lane == 0) red_s[warp] = s, red_t[warp] = t;
+  __syncthreads();
+  s = t = 0.f;
+#pragma unroll
+  for (int i = 0; i < F_THREADS / 32; ++i) s += red_s[i], t += red_t[i];
+  const float ls = logf(s), lse = (m == -INFINITY ? 0.f : m) + ls;
+
+  if (blockIdx.y == 0) {
+    if (threadIdx.x == 0) {
+      if (o.lse) o.lse[row] = lse;
+      if (o.entropy) o.entropy[row] = ls - t / s;
+    }
+    if (!sc.top) return;
+    // The candidates that reach the final bound, in any order, into shared memory (thread i scans CTA i's list); in each
+    // round a thread offers the first of its share that comes after the one taken last. A row that keeps more than the
+    // pool holds (many equal logits) reads the lists instead.
     const int count = threadIdx.x < ctas ? __float_as_int(st.w) : 0;
-    int at = 0, id = -1;
-    float v = 0.f;
-    auto load = [&] {
-      id = -1;
-      if (at < count) {
-        const uint2 e = list[(size_t)at * BM];
-        v = __uint_as_float(e.x);
-        id = (int)e.y;
+    const float least = known ? below(known) : -INFINITY;  // candidates exceed it
+    __shared__ uint2 pool[POOL];
+    __shared__ int kept;
+    if (threadIdx.x == 0) kept = 0;
+    __syncthreads();
+    auto keep = [&](const uint2& e) {
+      if (__uint_as_float(e.x) > least) {
+        const int at = atomicAdd(&kept, 1);
+        if (at < POOL) pool[at] = e;
       }
     };
-    load();
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (i < count) keep(head[i]);
+    for (int i = AHEAD; i < count; ++i) keep(__ldcg(list + i * BM));
+    __syncthreads();
+    const bool pooled = kept <= POOL;
+    const int from = pooled ? threadIdx.x : 0, to = pooled ? kept : count, step = pooled ? F_THREADS : 1;
+    float v = 0.f;
+    int id = -1;
+    auto next = [&](bool any, float pv, int pid) {  // this thread's first one after (pv, pid)
+      float bv = 0.f;
+      int bid = -1;
+      for (int i = from; i < to; i += step) {
+        const uint2 e = pooled ? pool[i] : __ldcg(list + i * BM);
+        const float x = __uint_as_float(e.x);
+        if ((any || before(pv, pid, x, (int)e.y)) && before(x, (int)e.y, bv, bid)) bv = x, bid = (int)e.y;
+      }
+      v = bv, id = bid;
+    };
+    next(true, 0.f, 0);
     for (int k = 0; k < sc.top; ++k) {
       float bv = v;
       int bi = id, bc = threadIdx.x;
@@ -368,55 +511,55 @@ __global__ void __launch_bounds__(F_THREADS)
         const int oi = __shfl_xor_sync(0xffffffffu, bi, x), oc = __shfl_xor_sync(0xffffffffu, bc, x);
         if (before(ov, oi, bv, bi)) bv = ov, bi = oi, bc = oc;
       }
+      const int b = k & 1;  // (two buffers: one barrier a round)
+      if (lane == 0) red_v[b][warp] = bv, red_i[b][warp] = bi, red_c[b][warp] = bc;
       __syncthreads();
-      if (lane == 0) red_v[warp] = bv, red_i[warp] = bi, red_c[warp] = bc;
-      __syncthreads();
-      bv = red_v[0], bi = red_i[0], bc = red_c[0];
+      bv = red_v[b][0], bi = red_i[b][0], bc = red_c[b][0];
+#pragma unroll
       for (int i = 1; i < F_THREADS / 32; ++i)
-        if (before(red_v[i], red_i[i], bv, bi)) bv = red_v[i], bi = red_i[i], bc = red_c[i];
+        if (before(red_v[b][i], red_i[b][i], bv, bi)) bv = red_v[b][i], bi = red_i[b][i], bc = red_c[b][i];
       if (threadIdx.x == 0) {
         o.top_ids[row * sc.top + k] = bi;
         o.top_logprobs[row * sc.top + k] = bi < 0 ? NAN : cap_exact(bv, c) - lse;
       }
-      if (bi >= 0 && bc == (int)threadIdx.x) {
-        ++at;
-        load();
-      }
+      if (bi >= 0 && bc == (int)threadIdx.x) next(false, bv, bi);
     }
+    return;
   }
-  for (int j = warp; j < o.n_targets; j += F_THREADS / 32) {
-    const int id = o.targets[row * o.n_targets + j];
-    float lp = 0.f;
-    if (id != -1) {
-      if (id < 0 || id >= V) {
-        if (lane == 0) report(kErrBadIndex);
+  for (int j = 0; j < o.n_targets; j += round) {
+    if (j) dot(j);
+    __syncthreads();
+    const int mine = j + threadIdx.x;
+    if (threadIdx.x < round && mine < o.n_targets) {
+      const int id = o.targets[row * o.n_targets + mine];
+      float l = 0.f;
+      for (int i = 0; i < per; ++i) l += dots[threadIdx.x * per + i];
+      float lp = cap_exact(l, c) - lse;
+      if (id == -1) lp = 0.f;
+      if (id < -1 || id >= V) {
+        report(kErrBadIndex);
         lp = NAN;
-      } else {
-        const __nv_bfloat16* hr = h + row * ld_h;
-        const __nv_bfloat16* wr = w + (size_t)id * ld_w;
-        float acc = 0.f;
-        for (int k = lane * 8; k < K; k += 256) {
-          float a[8], b[8];
-          load8(hr + k, a);
-          load8(wr + k, b);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) acc = fmaf(a[e], b[e], acc);
-        }
-#pragma unroll
-        for (int x = 16; x > 0; x >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, x);
-        lp = cap_exact(acc, c) - lse;
       }
+      o.logprobs[row * o.n_targets + mine] = lp;
     }
-    if (lane == 0) o.logprobs[row * o.n_targets + j] = lp;
+    __syncthreads();
   }
 }
 
 // ---- host -----------------------------------------------------------------------------------------------------------
 static int chunk_rows(int n) { return ((n < CHUNK_ROWS ? n : CHUNK_ROWS) + BM - 1) / BM * BM; }
 
-static unsigned long long workspace(int n, int top) {
-  return (unsigned long long)num_sms() * chunk_rows(n) * (sizeof(float4) + (unsigned long long)top * sizeof(uint2));
-}
+// Offsets in the caller's workspace.
+struct Space {
+  size_t own, lists, bound, bytes;
+  Space(int n, int top) {
+    const size_t rows = chunk_rows(n), per_cta = rows * num_sms();
+    own = per_cta * sizeof(float4);
+    lists = own + (top ? per_cta * sizeof(float) : 0);
+    bound = lists + (top ? per_cta * CAND * sizeof(uint2) : 0);
+    bytes = bound + (top ? rows * sizeof(unsigned) : 0);
+  }
+};
 
 static int make_map(CUtensorMap* map, const void* ptr, long long rows, long long cols, long long ld, int box_rows) {
   const unsigned long long dims[2] = {(unsigned long long)cols, (unsigned long long)rows};
@@ -444,7 +587,7 @@ extern "C" int morj_token_logprobs_workspace(int n, int top, unsigned long long*
   using namespace morj;
   if (!bytes || n < 0 || top < 0 || top > logprobs::MAX_TOP)
     return set_error(MORJ_ERR_ARG, "morj_token_logprobs_workspace: bad arguments (n=%d top=%d)", n, top);
-  *bytes = n ? logprobs::workspace(n, top) : 0;
+  *bytes = n ? logprobs::Space(n, top).bytes : 0;
   return MORJ_OK;
 }
 
@@ -466,7 +609,8 @@ extern "C" int morj_token_logprobs(const void* h, long long ld_h, int n, const v
     return set_error(MORJ_ERR_ARG, "morj_token_logprobs: H and leading dimensions must be multiples of 8 (H=%d)", H);
   if ((reinterpret_cast<uintptr_t>(h) | reinterpret_cast<uintptr_t>(w) | reinterpret_cast<uintptr_t>(workspace)) & 15)
     return set_error(MORJ_ERR_ARG, "morj_token_logprobs: h, w and workspace must be 16-byte aligned");
-  const unsigned long long need = logprobs::workspace(n, top);
+  const Space at(n, top);
+  const unsigned long long need = at.bytes;
   if (!workspace || workspace_bytes < need)
     return set_error(MORJ_ERR_ARG, "morj_token_logprobs: a workspace of %llu bytes given, %llu needed", workspace_bytes,
                      need);
@@ -477,8 +621,11 @@ extern "C" int morj_token_logprobs(const void* h, long long ld_h, int n, const v
   if ((st = make_map(&mw, w, vocab, H, ld_w, BN))) return st;
   Scratch sc;
   sc.rows = chunk_rows(n), sc.top = top;
-  sc.stats = static_cast<float4*>(workspace);
-  sc.lists = reinterpret_cast<uint2*>(sc.stats + (size_t)num_sms() * sc.rows);
+  char* ws = static_cast<char*>(workspace);
+  sc.stats = reinterpret_cast<float4*>(ws);
+  sc.own = reinterpret_cast<float*>(ws + at.own);
+  sc.lists = reinterpret_cast<uint2*>(ws + at.lists);
+  sc.bound = reinterpret_cast<unsigned*>(ws + at.bound);
   const Outputs o{targets, n_targets, logprobs_out, lse, entropy, top_ids, top_logprobs};
   for (int r0 = 0; r0 < n; r0 += CHUNK_ROWS) {
     const int rows = std::min(n - r0, CHUNK_ROWS);
@@ -487,10 +634,14 @@ extern "C" int morj_token_logprobs(const void* h, long long ld_h, int n, const v
     if ((st = make_map(&mh, static_cast<const __nv_bfloat16*>(h) + (size_t)r0 * ld_h, rows, H, ld_h, box))) return st;
     const long long tiles = (long long)((rows + BM - 1) / BM) * ((vocab + BN - 1) / BN);
     const int ctas = (int)std::min<long long>(tiles, std::min(num_sms(), F_THREADS));
+    if (top) {
+      const cudaError_t e = cudaMemsetAsync(sc.bound, 0, sc.rows * sizeof(unsigned), s);
+      if (e != cudaSuccess) return set_error(MORJ_ERR_CUDA, "cudaMemsetAsync: %s", cudaGetErrorString(e));
+    }
     st = launch_pdl("logits_kernel", logits_kernel, dim3(ctas), dim3(THREADS), SMEM_BYTES, s, mh, mw, rows, vocab, H,
                     box * BK * 2, softcap, sc);
     if (st) return st;
-    st = launch_pdl("finish_kernel", finish_kernel, dim3(rows), dim3(F_THREADS), 0, s, (const __nv_bfloat16*)h, ld_h,
+    st = launch_pdl("finish_kernel", finish_kernel, dim3(rows, n_targets ? 2 : 1), dim3(F_THREADS), 0, s, (const __nv_bfloat16*)h, ld_h,
                     (const __nv_bfloat16*)w, ld_w, vocab, H, softcap, ctas, sc, o, r0);
     if (st) return st;
   }
