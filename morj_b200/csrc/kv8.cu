@@ -6,7 +6,7 @@
 // are rescaled exactly unless they become subnormal.
 //
 // One CTA owns one (block, head) of K or V: it reads the block's new rows once into registers (all loads issued up
-// front), reduces their largest magnitude, moves the block's other codes if the scale grew, and writes the new codes.
+// front, eight CTAs an SM), reduces their largest magnitude, moves the block's other codes if the scale grew, and writes the new codes.
 // No atomics and no second pass over memory; the result does not depend on the order of the rows.
 #include <algorithm>
 #include <vector>
@@ -26,21 +26,35 @@ struct Side {  // K or V
   float* scale;
 };
 
+// The largest magnitude in 8 BF16 values as bits of a BF16 (0x7f80 and above: not finite), pairs at a time.
+MORJ_DEV unsigned amax_bits(unsigned m, const uint4& u) {
+  m = __vmaxu2(m, u.x & 0x7fff7fffu);
+  m = __vmaxu2(m, u.y & 0x7fff7fffu);
+  m = __vmaxu2(m, u.z & 0x7fff7fffu);
+  return __vmaxu2(m, u.w & 0x7fff7fffu);
+}
+MORJ_DEV uint32_t finite2(uint32_t two) {  // infinities and NaN as 0
+  if ((two & 0x7f80u) == 0x7f80u) two &= 0xffff0000u;
+  if ((two & 0x7f800000u) == 0x7f800000u) two &= 0x0000ffffu;
+  return two;
+}
+
 template <int D>
-__global__ void __launch_bounds__(THREADS) store_kernel(const Side k, const Side v, int n, int hk, const int* __restrict__ work,
-                                                        int n_blocks, int pool_slots) {
+__global__ void __launch_bounds__(THREADS, 8) store_kernel(const Side k, const Side v, int n, int hk,
+                                                           const int* __restrict__ work, int n_blocks,
+                                                           int pool_slots) {
   pdl_wait();  // the previous kernel on the stream has completed
   pdl_trigger();
   constexpr int LPR = D / 8;                       // lanes per row, 8 values each
   constexpr int ROWS = THREADS / LPR;              // rows per iteration of the CTA
   constexpr int ITERS = BLOCK / ROWS;
-  __shared__ float red[THREADS / 32];
+  __shared__ int2 pair[BLOCK];                     // (slot, row) of the rows; slot -1: none
+  __shared__ unsigned red[THREADS / 32];
   __shared__ unsigned written[2];                  // slots of the block this call writes
   const int entry = blockIdx.x, h = blockIdx.y;
   const Side a = blockIdx.z ? v : k;
   const int block = work[3 * entry], first = work[3 * entry + 1], count = work[3 * entry + 2];
-  const int2* pairs = reinterpret_cast<const int2*>(work + 3 * n_blocks + (n_blocks & 1)) + first;
-  const int part = threadIdx.x % LPR, lane = threadIdx.x % 32;
+  const int part = threadIdx.x % LPR, r0 = threadIdx.x / LPR, lane = threadIdx.x % 32;
   const __nv_bfloat16* src = a.rows + (size_t)h * D + part * 8;
   uint8_t* codes = a.codes + (size_t)h * D + part * 8;
   const size_t row_bytes = (size_t)hk * D;
@@ -48,63 +62,61 @@ __global__ void __launch_bounds__(THREADS) store_kernel(const Side k, const Side
     if (threadIdx.x == 0) report(kErrBadIndex);
     return;
   }
-
-  uint4 raw[ITERS];
-  int slot[ITERS];
-#pragma unroll
-  for (int i = 0; i < ITERS; ++i) {
-    const int r = i * ROWS + threadIdx.x / LPR;
-    slot[i] = -1;
-    if (r < count) {
-      const int2 p = pairs[r];  // (slot, row)
-      if ((p.x >> BLOCK_SHIFT) != block || p.x >= pool_slots || (unsigned)p.y >= (unsigned)n) {
-        if (part == 0) report(kErrBadIndex);
-      } else {
-        slot[i] = p.x;
-        raw[i] = *reinterpret_cast<const uint4*>(src + (size_t)p.y * a.ld);
-      }
-    }
-  }
   float* scale = a.scale + (size_t)block * hk + h;
   const float stored = *scale;
+  if (threadIdx.x < BLOCK) {
+    int2 p = make_int2(-1, 0);
+    if (threadIdx.x < count) {
+      p = reinterpret_cast<const int2*>(work + 3 * n_blocks + (n_blocks & 1))[first + threadIdx.x];
+      if ((p.x >> BLOCK_SHIFT) != block || p.x >= pool_slots || (unsigned)p.y >= (unsigned)n) {
+        report(kErrBadIndex);
+        p = make_int2(-1, 0);
+      }
+    }
+    pair[threadIdx.x] = p;
+  }
   if (threadIdx.x < 2) written[threadIdx.x] = 0;
+  __syncthreads();
 
-  float amax = 0.f;
-  bool bad = false;
+  uint4 raw[ITERS];
 #pragma unroll
   for (int i = 0; i < ITERS; ++i) {
-    if (slot[i] < 0) continue;
-    float x[8];
-    unpack8(raw[i], x);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float m = fabsf(x[e]);
-      if (m <= kBf16Max)
-        amax = fmaxf(amax, m);
-      else
-        bad = true;  // infinite or NaN
-    }
+    const int2 p = pair[i * ROWS + r0];
+    raw[i] = make_uint4(0, 0, 0, 0);
+    if (p.x >= 0) raw[i] = *reinterpret_cast<const uint4*>(src + (size_t)p.y * a.ld);
   }
-  if (bad) report(kErrNotFinite);
+  unsigned m = 0;
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-  if (lane == 0) red[threadIdx.x / 32] = amax;
+  for (int i = 0; i < ITERS; ++i) m = amax_bits(m, raw[i]);
+  m = max(m & 0xffffu, m >> 16);
+  const bool bad = m >= 0x7f80u;
+  if (bad) {  // infinite or NaN: reported, and not counted
+    report(kErrNotFinite);
+    m = 0;
+#pragma unroll
+    for (int i = 0; i < ITERS; ++i)
+      m = amax_bits(m, make_uint4(finite2(raw[i].x), finite2(raw[i].y), finite2(raw[i].z), finite2(raw[i].w)));
+    m = max(m & 0xffffu, m >> 16);
+  }
+  m = __reduce_max_sync(0xffffffffu, m);
+  if (lane == 0) red[threadIdx.x / 32] = m;
   __syncthreads();
-  amax = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+  m = max(max(red[0], red[1]), max(red[2], red[3]));
+  const float amax = __uint_as_float(m << 16);
   const float old = stored > 0.f ? stored : 0.f;  // (0 or NaN: no codes yet)
   const float now = fmaxf(old, scale_for(amax));
-  if (threadIdx.x == 0 && now != stored) *scale = now;  // (every thread read `stored` before the barrier above)
+  if (threadIdx.x == 0 && now != stored) *scale = now;  // (every thread read `stored` before the barriers above)
 
   if (old > 0.f && now > old) {
     // the block's scale grew: the codes of the slots this call does not write move to it
-#pragma unroll
-    for (int i = 0; i < ITERS; ++i)
-      if (slot[i] >= 0 && part == 0) atomicOr(&written[(slot[i] & 63) >> 5], 1u << (slot[i] & 31));
+    if (threadIdx.x < count && pair[threadIdx.x].x >= 0) {
+      const int at = pair[threadIdx.x].x & (BLOCK - 1);
+      atomicOr(&written[at >> 5], 1u << (at & 31));
+    }
     __syncthreads();
     const float ratio = old / now;  // (powers of two: exact)
-#pragma unroll
-    for (int i = 0; i < ITERS; ++i) {
-      const int r = i * ROWS + threadIdx.x / LPR;
+#pragma unroll 2
+    for (int r = r0; r < BLOCK; r += ROWS) {
       const long long s = (long long)block * BLOCK + r;
       if (s >= pool_slots || ((written[r >> 5] >> (r & 31)) & 1)) continue;
       uint2* p = reinterpret_cast<uint2*>(codes + (size_t)s * row_bytes);
@@ -119,12 +131,17 @@ __global__ void __launch_bounds__(THREADS) store_kernel(const Side k, const Side
   const float inv = 1.0f / now;  // (a power of two)
 #pragma unroll
   for (int i = 0; i < ITERS; ++i) {
-    if (slot[i] < 0) continue;
+    const int slot = pair[i * ROWS + r0].x;
+    if (slot < 0) continue;
     float x[8];
     unpack8(raw[i], x);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = x[e] == x[e] ? x[e] * inv : 0.f;  // NaN (reported): 0; infinite: saturated
-    *reinterpret_cast<uint2*>(codes + (size_t)slot[i] * row_bytes) =
+    for (int e = 0; e < 8; ++e) x[e] *= inv;
+    if (bad) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = x[e] == x[e] ? x[e] : 0.f;  // NaN: 0; infinite: saturated by the conversion
+    }
+    *reinterpret_cast<uint2*>(codes + (size_t)slot * row_bytes) =
         make_uint2(f32_codes2(x[0], x[1]) | f32_codes2(x[2], x[3]) << 16,
                    f32_codes2(x[4], x[5]) | f32_codes2(x[6], x[7]) << 16);
   }
