@@ -160,12 +160,21 @@ MORJ_DEV void cp_async_arrive(uint32_t bar) {
 MORJ_DEV void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
   asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
-// warp-level wait: lane 0 polls the barrier, the warp follows its verdict (and sees what lane 0 sees)
+// A whole warp waits for a barrier's phase. Every lane polls (one broadcast read) and the warp goes on when all have seen
+// it: a lane polling for the others costs the shuffle that tells them as well.
 MORJ_DEV bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
-  int ok = (threadIdx.x & 31) == 0 ? (int)mbar_wait(bar, parity, abort, kErrTimeoutAttention) : 0;
-  ok = __shfl_sync(0xffffffffu, ok, 0);
-  __syncwarp();
-  return ok != 0;
+  if (__all_sync(0xffffffffu, mbar_test(bar, parity))) return true;
+  unsigned long long t0 = 0;
+  for (uint32_t i = 1;; ++i) {
+    if (__all_sync(0xffffffffu, mbar_test_suspend(bar, parity, 20000))) return true;
+    if ((i & 63) == 0) {
+      const unsigned long long now = global_ns();
+      if (t0 == 0) t0 = now;
+      const bool late = now - t0 > kWaitLimitNs;
+      if (late) *abort = 1, report(kErrTimeoutAttention);
+      if (__any_sync(0xffffffffu, late || *abort)) return false;
+    }
+  }
 }
 MORJ_DEV uint4 lds16(uint32_t addr) {
   uint4 v;
@@ -510,65 +519,78 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
 // the address arithmetic and the instruction cache: 130 us on the op-level tree (2048 + 8 x 64) against the 62 us of the
 // BF16 kernel with the same pipeline.
 // ---------------------------------------------------------------------------------------------------------------
-constexpr int E_THREADS = 256;
+// A CTA takes 64 slots of a head's K or V. Three steps of loads that depend on one another (page, codes, convert), each
+// asked for at once, and many CTAs an SM: one warp's share with the lookups inline took 27 us for those 35.7 M codes.
+constexpr int E_THREADS = 128;
 
 template <int D>
-__global__ void __launch_bounds__(E_THREADS) expand_kernel(const Args a, const int2* __restrict__ pages, int n_slots,
-                                                           const int* __restrict__ blocks, int n_blocks,
-                                                           uint16_t* __restrict__ k_out, uint16_t* __restrict__ v_out,
-                                                           float* __restrict__ refs) {
+__global__ void __launch_bounds__(E_THREADS, 12) expand_kernel(const Args a, const int2* __restrict__ pages,
+                                                               int n_slots, const int* __restrict__ blocks,
+                                                               int n_blocks, uint16_t* __restrict__ k_out,
+                                                               uint16_t* __restrict__ v_out, float* __restrict__ refs) {
   pdl_wait();  // the previous kernel on the stream has completed
   pdl_trigger();
-  constexpr int LPR = D / 8;                     // lanes per row: 8 codes in, 16 bytes out
-  constexpr int SLOTS = BN / (E_THREADS / 64);   // slots of a warp (half of the warps K, half V)
-  constexpr int N = SLOTS / (32 / LPR);          // loads of a lane
+  constexpr int LPR = D / 8;              // lanes per row: 8 codes in, 16 bytes out
+  constexpr int ROWS = E_THREADS / LPR;   // rows per iteration of the CTA
+  constexpr int N = BN / ROWS;
+  __shared__ int slots[BN];               // of the pool; -1: nothing listed (zeros)
+  __shared__ float factor[BN];
   __shared__ float red[E_THREADS / 32];
   const int h = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
-  // this CTA's codes first: nothing below is needed to ask for them
-  const bool is_v = warp >= E_THREADS / 64;
-  const int t_warp = blockIdx.x * BN + (warp % (E_THREADS / 64)) * SLOTS + lane / LPR;
-  const uint8_t* codes = (is_v ? a.v : a.k) + (size_t)h * D + (lane % LPR) * 8;
+  const bool is_v = blockIdx.z;
+  const int t0 = blockIdx.x * BN, part = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
   const float* scales = (is_v ? a.vs : a.ks) + h;
   const unsigned row_bytes = (unsigned)a.hk * D;
-  uint2 w[N];
-  float sc[N];
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int t = t_warp + i * (32 / LPR);
-    sc[i] = 0.f, w[i] = make_uint2(0, 0);
+  float sc = 0.f;
+  if (threadIdx.x < BN) {
+    const int t = t0 + threadIdx.x;
+    int slot = -1;
     if (t < n_slots) {
       const int p = a.page.of(t), at = t - p * a.page.d;
       const int2 page = __ldg(pages + p);  // (page of the pool, its slots that are listed: the rest is zeros)
-      const long long slot = (long long)page.x * a.page.d + at;
-      if (at >= page.y) {
-      } else if (slot >= a.pool_slots) {
-        if (lane % LPR == 0) report(kErrBadIndex);
-      } else {
-        w[i] = __ldg(reinterpret_cast<const uint2*>(codes + (unsigned long long)slot * row_bytes));
-        sc[i] = __ldg(scales + (size_t)(slot >> BLOCK_SHIFT) * a.hk);
+      const long long s = (long long)page.x * a.page.d + at;
+      if (at < page.y) {
+        if (s < a.pool_slots)
+          slot = (int)s;
+        else
+          report(kErrBadIndex);
       }
     }
+    slots[threadIdx.x] = slot;
+    if (slot >= 0) sc = __ldg(scales + (size_t)(slot >> BLOCK_SHIFT) * a.hk);
   }
-  // V's largest scale of the head (every CTA of the head finds the same)
-  float vr = 0.f;
-  for (int i = threadIdx.x; i < n_blocks; i += E_THREADS) {
-    const int b = __ldg(blocks + i);
-    if ((long long)b * BLOCK < a.pool_slots) vr = fmaxf(vr, __ldg(a.vs + (size_t)b * a.hk + h));  // (else: reported above)
-  }
-#pragma unroll
-  for (int x = 16; x > 0; x >>= 1) vr = fmaxf(vr, __shfl_xor_sync(0xffffffffu, vr, x));
-  if (lane == 0) red[warp] = vr;
   __syncthreads();
-#pragma unroll
-  for (int i = 0; i < E_THREADS / 32; ++i) vr = fmaxf(vr, red[i]);
-  if (blockIdx.x == 0 && threadIdx.x == 0) refs[h] = vr;
-  const float inv = is_v && vr > 0.f ? 1.f / vr : 1.f;
-  uint16_t* out = (is_v ? v_out : k_out) + (size_t)h * D + (lane % LPR) * 8;
+  const uint8_t* codes = (is_v ? a.v : a.k) + (size_t)h * D + part * 8;
+  uint2 w[N];
 #pragma unroll
   for (int i = 0; i < N; ++i) {
-    const int t = t_warp + i * (32 / LPR);
-    if (t >= n_slots) break;
-    const float f = sc[i] * inv;
+    const int slot = slots[i * ROWS + r0];
+    w[i] = make_uint2(0, 0);
+    if (slot >= 0) w[i] = __ldg(reinterpret_cast<const uint2*>(codes + (size_t)slot * row_bytes));
+  }
+  float inv = 1.f;
+  if (is_v) {  // V's largest scale of the head (every CTA of the head finds the same)
+    float vr = 0.f;
+    for (int i = threadIdx.x; i < n_blocks; i += E_THREADS) {
+      const int b = __ldg(blocks + i);
+      if ((long long)b * BLOCK < a.pool_slots) vr = fmaxf(vr, __ldg(a.vs + (size_t)b * a.hk + h));  // (else: reported)
+    }
+#pragma unroll
+    for (int x = 16; x > 0; x >>= 1) vr = fmaxf(vr, __shfl_xor_sync(0xffffffffu, vr, x));
+    if (lane == 0) red[warp] = vr;
+    __syncthreads();
+    vr = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    if (blockIdx.x == 0 && threadIdx.x == 0) refs[h] = vr;
+    if (vr > 0.f) inv = 1.f / vr;
+  }
+  if (threadIdx.x < BN) factor[threadIdx.x] = sc * inv;
+  __syncthreads();
+  uint16_t* out = (is_v ? v_out : k_out) + (size_t)h * D + part * 8;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int r = i * ROWS + r0;
+    if (t0 + r >= n_slots) break;
+    const float f = factor[r];
     const float2 x0 = codes2_f32(w[i].x & 0xffffu), x1 = codes2_f32(w[i].x >> 16);
     const float2 x2 = codes2_f32(w[i].y & 0xffffu), x3 = codes2_f32(w[i].y >> 16);
     uint4 u;
@@ -578,7 +600,7 @@ __global__ void __launch_bounds__(E_THREADS) expand_kernel(const Args a, const i
     else
       u = make_uint4(pack_bf16x2(x0.x * f, x0.y * f), pack_bf16x2(x1.x * f, x1.y * f), pack_bf16x2(x2.x * f, x2.y * f),
                      pack_bf16x2(x3.x * f, x3.y * f));
-    *reinterpret_cast<uint4*>(out + (unsigned long long)t * row_bytes) = u;
+    *reinterpret_cast<uint4*>(out + (size_t)(t0 + r) * row_bytes) = u;
   }
 }
 
@@ -761,10 +783,9 @@ __global__ void __launch_bounds__(T_THREADS, 2)
       const uint64_t q_desc = sw128_desc(sbase);
       const uint64_t k_desc0 = sw128_desc(sbase + L::K_OFF), v_desc0 = sw128_desc(sbase + L::V_OFF, BN * 128);
       constexpr uint64_t KV_STEP = L::KV_BYTES >> 4;
-      auto issue_qk = [&](int c) -> bool {
+      auto k_landed = [&](int c) { return mbar_wait(k_full + 8 * (c & 1), (c >> 1) & 1, abort, kErrTimeoutAttention); };
+      auto issue_qk = [&](int c) {
         const int b = c & 1;
-        if (!mbar_wait(k_full + 8 * b, (c >> 1) & 1, abort, kErrTimeoutAttention)) return false;
-        tc_fence_after();
         const uint64_t k_desc = k_desc0 + b * KV_STEP;
 #pragma unroll
         for (int kk = 0; kk < D / 16; ++kk) {
@@ -773,25 +794,27 @@ __global__ void __launch_bounds__(T_THREADS, 2)
           umma_bf16(tmem + b * BN, q_desc + qa, k_desc + kb, IDESC_S, kk > 0);  // (kind::f16: the types are in IDESC)
         }
         umma_commit(s_full + 8 * b);
-        return true;
       };
-      if (ok) ok = issue_qk(0);
-      if (ok && n_chunks > 1) ok = issue_qk(1);
+      for (int c = 0; c < min(n_chunks, 2) && ok; ++c) {
+        ok = k_landed(c);
+        tc_fence_after();
+        if (ok) issue_qk(c);
+      }
       for (int c = 0; c < n_chunks && ok; ++c) {
         const int b = c & 1;
-        // O += P_c V_c, P_c from TMEM buffer b (packed FP16 pairs, 8 columns per 16 keys)
-        if (!mbar_wait(p_full + 8 * b, (c >> 1) & 1, abort, kErrTimeoutAttention) ||
-            !mbar_wait(v_full + 8 * b, (c >> 1) & 1, abort, kErrTimeoutAttention)) {
-          ok = false;
-          break;
-        }
+        // O += P_c V_c, P_c from TMEM buffer b (packed FP16 pairs, 8 columns per 16 keys). The copies are waited for
+        // first: they have landed long before P_c comes, and a wait costs 100 cycles even then.
+        ok = mbar_wait(v_full + 8 * b, (c >> 1) & 1, abort, kErrTimeoutAttention) &&
+             (c + 2 >= n_chunks || k_landed(c + 2)) &&
+             mbar_wait(p_full + 8 * b, (c >> 1) & 1, abort, kErrTimeoutAttention);
+        if (!ok) break;
         tc_fence_after();
         const uint64_t v_desc = v_desc0 + b * KV_STEP;
 #pragma unroll
         for (int kk = 0; kk < BN / 16; ++kk)
           umma_bf16_tmem_a(tmem + 128, tmem + b * BN + kk * 8, v_desc + kk * (2048 >> 4), IDESC_O, (c | kk) != 0);
         umma_commit(pv_done + 8 * b);
-        if (c + 2 < n_chunks) ok = issue_qk(c + 2);  // in issue order after this PV, which reads P_c first
+        if (c + 2 < n_chunks) issue_qk(c + 2);  // in issue order after this PV, which reads P_c first
       }
       // TMEM is freed only after every MMA issued here has completed
       umma_commit(done);
@@ -1084,7 +1107,7 @@ static int launch(Args a, const int* counts, const int* work, char* ws, cudaStre
     if ((st = encode_tiled(&vm, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, vp, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B)))
       return st;
     if (n_slots)
-      st = launch_pdl("expand_kernel", expand_kernel<D>, dim3((n_slots + BN - 1) / BN, a.hk), dim3(E_THREADS), 0, s, a,
+      st = launch_pdl("expand_kernel", expand_kernel<D>, dim3((n_slots + BN - 1) / BN, a.hk, 2), dim3(E_THREADS), 0, s, a,
                       reinterpret_cast<const int2*>(pages), n_slots, blocks, n_blocks, kx, vx, refs);
     else
       refs = nullptr;
