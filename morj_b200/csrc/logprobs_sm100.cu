@@ -26,19 +26,17 @@
 namespace morj {
 namespace logprobs {
 
-constexpr int BM = 128, BN = 256, BK = 64;
-constexpr int A_BYTES = BM * BK * 2, B_BYTES = BN * BK * 2;
-constexpr int STAGE_BYTES = A_BYTES + B_BYTES;
+constexpr int BM = 128, BK = 64;
+constexpr int BN_WIDE = 256, BN_NARROW = 64;  // vocabulary rows of a tile
+constexpr int A_BYTES = BM * BK * 2;
 constexpr int STAGES = 4;
 constexpr int MAX_TOP = MORJ_MAX_TOP;
 constexpr int CAND = 64;  // candidates a CTA's list of a row holds: top ones (32 at most) and one group of 32 more
 static_assert(CAND >= MAX_TOP + 32, "a cut list takes a whole group of columns");
-constexpr int SMEM_BYTES = STAGES * STAGE_BYTES + 1024 /*align*/ + 256 /*barriers*/;
-static_assert(SMEM_BYTES <= 232448, "shared memory per CTA");
-constexpr int TMEM_COLS = 512;
+constexpr int smem_bytes(int bn) { return STAGES * (A_BYTES + bn * BK * 2) + 1024 /*align*/ + 256 /*barriers*/; }
+static_assert(smem_bytes(BN_WIDE) <= 232448, "shared memory per CTA");
 constexpr int THREADS = 192;
 constexpr int CHUNK_ROWS = 2048;
-constexpr uint32_t IDESC = idesc_bf16(BM, BN);
 constexpr float LOG2E = 1.4426950408889634f;
 
 // What the CTAs know of the rows.
@@ -65,7 +63,7 @@ MORJ_DEV float below(unsigned o) {
 MORJ_DEV float cap_near(float l, float c, float inv_c) {  // |l| <= c / 4
   const float x = l * inv_c, x2 = x * x;
   const float p = fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
-  return l * p;
+  return __fmul_rn(l, p);  // (not joined with what is subtracted from it: one value whether or not others are far)
 }
 MORJ_DEV float cap_far(float l, float c, float inv_c) {
   float r;
@@ -135,9 +133,13 @@ __device__ __noinline__ float cut_list(uint2* list, int count, int top) {
   return pv;
 }
 
+template <int BN>
 __global__ void __launch_bounds__(THREADS, 1)
     logits_kernel(const __grid_constant__ CUtensorMap map_h, const __grid_constant__ CUtensorMap map_w, int M, int V,
                   int K, int a_bytes, float c, const Scratch sc) {
+  constexpr int B_BYTES = BN * BK * 2, STAGE_BYTES = A_BYTES + B_BYTES;
+  constexpr uint32_t IDESC = idesc_bf16(BM, BN);
+  constexpr int TMEM_COLS = 2 * BN;  // (two accumulators)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + STAGES * STAGE_BYTES);
@@ -291,7 +293,8 @@ __global__ void __launch_bounds__(THREADS, 1)
       if (known) tau = fmaxf(tau, below(known));
       const bool fresh = top && st.x == -INFINITY && known == 0;
       if (__any_sync(0xffffffffu, fresh)) {  // (the TMEM loads are the whole warp's)
-        // the rows' first tile: the top-th largest of its 32 groups of 8 columns (columns past V are zeros: left out)
+        // the rows' first tile: the top-th largest of its 32 groups of columns (columns past V are zeros: left out)
+        constexpr int GROUP = BN / 32, PER = 32 / GROUP;
         float g[32];
 #pragma unroll
         for (int col = 0; col < BN; col += 32) {
@@ -299,12 +302,12 @@ __global__ void __launch_bounds__(THREADS, 1)
           tmem_ld32(tacc + col, r);
           tmem_wait_ld();
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
+          for (int q = 0; q < PER; ++q) {
             float x = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-              x = fmaxf(x, n * BN + col + q * 8 + i < V ? __uint_as_float(r[q * 8 + i]) : -INFINITY);
-            g[col / 8 + q] = x;
+            for (int i = 0; i < GROUP; ++i)
+              x = fmaxf(x, n * BN + col + q * GROUP + i < V ? __uint_as_float(r[q * GROUP + i]) : -INFINITY);
+            g[col / GROUP + q] = x;
           }
         }
         float first = INFINITY;
@@ -378,7 +381,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 
 // ---- finish: two CTAs per row, one for its numbers and top alternatives, one for the given tokens -------------------
 constexpr int F_THREADS = 256;
-constexpr int POOL = 2048;
+constexpr int POOL = 512;
 
 struct Outputs {
   const int* targets;
@@ -405,7 +408,7 @@ __global__ void __launch_bounds__(F_THREADS)
   float4 st = make_float4(-INFINITY, 0.f, 0.f, 0.f);
   if (threadIdx.x < ctas) st = sc.stats[(size_t)threadIdx.x * sc.rows + local];
   const uint2* list = sc.lists + ((size_t)threadIdx.x * sc.rows + (local / BM) * BM) * CAND + local % BM;
-  constexpr int AHEAD = 8;
+  constexpr int AHEAD = 16;
   uint2 head[AHEAD];  // the first entries of this thread's list (left over from another call past its count)
   unsigned known = 0;
   if (blockIdx.y == 0 && sc.top) {
@@ -467,15 +470,29 @@ __global__ void __launch_bounds__(F_THREADS)
       if (o.entropy) o.entropy[row] = ls - t / s;
     }
     if (!sc.top) return;
-    // The candidates that reach the final bound, in any order, into shared memory (thread i scans CTA i's list); in each
-    // round a thread offers the first of its share that comes after the one taken last. A row that keeps more than the
-    // pool holds (many equal logits) reads the lists instead.
+    // Thread i has CTA i's list. The bound is raised once more: the largest candidates of the CTAs are different logits,
+    // so at least `top` logits reach the top-th largest of them, and few others do. What reaches it goes to shared memory
+    // in any order, and each one's place is the number of those before it. (Rounds that take one alternative each, over
+    // the bound the CTAs had found, took 23 us for 9 rows of 262144 logits.)
     const int count = threadIdx.x < ctas ? __float_as_int(st.w) : 0;
-    const float least = known ? below(known) : -INFINITY;  // candidates exceed it
+    float most = -INFINITY;
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+      if (i < count) most = fmaxf(most, __uint_as_float(head[i].x));
+#pragma unroll 8
+    for (int i = AHEAD; i < count; ++i) most = fmaxf(most, __uint_as_float(__ldcg(list + i * BM).x));
+    __shared__ float mosts[F_THREADS];
     __shared__ uint2 pool[POOL];
+    __shared__ unsigned raised;
     __shared__ int kept;
-    if (threadIdx.x == 0) kept = 0;
+    mosts[threadIdx.x] = most;
+    if (threadIdx.x == 0) kept = 0, raised = known;
     __syncthreads();
+    int rank = 0;
+    for (int i = 0; i < ctas; ++i) rank += mosts[i] > most || (mosts[i] == most && i < (int)threadIdx.x);
+    if (count && rank == sc.top - 1) atomicMax(&raised, ordered(most));
+    __syncthreads();
+    const float least = raised ? below(raised) : -INFINITY;  // candidates exceed it
     auto keep = [&](const uint2& e) {
       if (__uint_as_float(e.x) > least) {
         const int at = atomicAdd(&kept, 1);
@@ -487,15 +504,29 @@ __global__ void __launch_bounds__(F_THREADS)
       if (i < count) keep(head[i]);
     for (int i = AHEAD; i < count; ++i) keep(__ldcg(list + i * BM));
     __syncthreads();
-    const bool pooled = kept <= POOL;
-    const int from = pooled ? threadIdx.x : 0, to = pooled ? kept : count, step = pooled ? F_THREADS : 1;
+    auto take = [&](int k, float v, int id) {  // id < 0: the row has fewer logits that can be compared
+      o.top_ids[row * sc.top + k] = id;
+      o.top_logprobs[row * sc.top + k] = id < 0 ? NAN : cap_exact(v, c) - lse;
+    };
+    const int n = kept;
+    if (n <= POOL) {
+      for (int i = threadIdx.x; i < n; i += F_THREADS) {
+        const uint2 e = pool[i];
+        int place = 0;
+        for (int j = 0; j < n; ++j) place += before(__uint_as_float(pool[j].x), (int)pool[j].y, __uint_as_float(e.x), (int)e.y);
+        if (place < sc.top) take(place, __uint_as_float(e.x), (int)e.y);
+      }
+      for (int k = n + threadIdx.x; k < sc.top; k += F_THREADS) take(k, 0.f, -1);
+      return;
+    }
+    // Many equal logits: in each round a thread offers the first of its list that comes after the one taken last.
     float v = 0.f;
     int id = -1;
     auto next = [&](bool any, float pv, int pid) {  // this thread's first one after (pv, pid)
       float bv = 0.f;
       int bid = -1;
-      for (int i = from; i < to; i += step) {
-        const uint2 e = pooled ? pool[i] : __ldcg(list + i * BM);
+      for (int i = 0; i < count; ++i) {
+        const uint2 e = __ldcg(list + i * BM);
         const float x = __uint_as_float(e.x);
         if ((any || before(pv, pid, x, (int)e.y)) && before(x, (int)e.y, bv, bid)) bv = x, bid = (int)e.y;
       }
@@ -518,10 +549,7 @@ __global__ void __launch_bounds__(F_THREADS)
 #pragma unroll
       for (int i = 1; i < F_THREADS / 32; ++i)
         if (before(red_v[b][i], red_i[b][i], bv, bi)) bv = red_v[b][i], bi = red_i[b][i], bc = red_c[b][i];
-      if (threadIdx.x == 0) {
-        o.top_ids[row * sc.top + k] = bi;
-        o.top_logprobs[row * sc.top + k] = bi < 0 ? NAN : cap_exact(bv, c) - lse;
-      }
+      if (threadIdx.x == 0) take(k, bv, bi);
       if (bi >= 0 && bc == (int)threadIdx.x) next(false, bv, bi);
     }
     return;
@@ -574,7 +602,10 @@ static int configure() {
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e == cudaSuccess && (dev >= 64 || !done[dev])) {
-    e = cudaFuncSetAttribute(logits_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES);
+    e = cudaFuncSetAttribute(logits_kernel<BN_WIDE>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(BN_WIDE));
+    if (e == cudaSuccess)
+      e = cudaFuncSetAttribute(logits_kernel<BN_NARROW>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                               smem_bytes(BN_NARROW));
     if (e == cudaSuccess && dev < 64) done[dev] = true;
   }
   return e == cudaSuccess ? MORJ_OK : set_error(MORJ_ERR_CUDA, "cudaFuncSetAttribute: %s", cudaGetErrorString(e));
@@ -598,7 +629,7 @@ extern "C" int morj_token_logprobs(const void* h, long long ld_h, int n, const v
   using namespace morj;
   using namespace morj::logprobs;
   if (n == 0) return MORJ_OK;
-  if (!h || !w || n < 0 || vocab <= 0 || vocab > INT_MAX - BN || H <= 0 || n_targets < 0 ||
+  if (!h || !w || n < 0 || vocab <= 0 || vocab > INT_MAX - BN_WIDE || H <= 0 || n_targets < 0 ||
       (n_targets && (!targets || !logprobs_out)) || (top && (!top_ids || !top_logprobs)))
     return set_error(MORJ_ERR_ARG, "morj_token_logprobs: null pointer or bad size (n=%d vocab=%d H=%d)", n, vocab, H);
   if (top < 0 || top > MAX_TOP || top > vocab)
@@ -617,8 +648,6 @@ extern "C" int morj_token_logprobs(const void* h, long long ld_h, int n, const v
   int st = configure();
   if (st) return st;
   cudaStream_t s = reinterpret_cast<cudaStream_t>(stream);
-  CUtensorMap mw;
-  if ((st = make_map(&mw, w, vocab, H, ld_w, BN))) return st;
   Scratch sc;
   sc.rows = chunk_rows(n), sc.top = top;
   char* ws = static_cast<char*>(workspace);
@@ -632,17 +661,23 @@ extern "C" int morj_token_logprobs(const void* h, long long ld_h, int n, const v
     const int box = rows >= BM ? BM : (rows + 7) / 8 * 8;  // few rows: only those are loaded
     CUtensorMap mh;
     if ((st = make_map(&mh, static_cast<const __nv_bfloat16*>(h) + (size_t)r0 * ld_h, rows, H, ld_h, box))) return st;
-    const long long tiles = (long long)((rows + BM - 1) / BM) * ((vocab + BN - 1) / BN);
+    // Wide tiles where there are enough of them for most SMs, else four times as many narrow ones: the epilogue's passes
+    // over a tile's columns are what a small call waits for (1 row, 4096 x 256: 18 against 25 us).
+    const int blocks = (rows + BM - 1) / BM, wide = (vocab + BN_WIDE - 1) / BN_WIDE;
+    const int bn = (long long)blocks * wide * 2 > num_sms() ? BN_WIDE : BN_NARROW;
+    const long long tiles = (long long)blocks * ((vocab + bn - 1) / bn);
+    CUtensorMap mw;
+    if ((st = make_map(&mw, w, vocab, H, ld_w, bn))) return st;
     const int ctas = (int)std::min<long long>(tiles, std::min(num_sms(), F_THREADS));
     if (top) {
       const cudaError_t e = cudaMemsetAsync(sc.bound, 0, sc.rows * sizeof(unsigned), s);
       if (e != cudaSuccess) return set_error(MORJ_ERR_CUDA, "cudaMemsetAsync: %s", cudaGetErrorString(e));
     }
-    st = launch_pdl("logits_kernel", logits_kernel, dim3(ctas), dim3(THREADS), SMEM_BYTES, s, mh, mw, rows, vocab, H,
-                    box * BK * 2, softcap, sc);
+    st = launch_pdl("logits_kernel", bn == BN_WIDE ? logits_kernel<BN_WIDE> : logits_kernel<BN_NARROW>, dim3(ctas),
+                    dim3(THREADS), smem_bytes(bn), s, mh, mw, rows, vocab, H, box * BK * 2, softcap, sc);
     if (st) return st;
-    st = launch_pdl("finish_kernel", finish_kernel, dim3(rows, n_targets ? 2 : 1), dim3(F_THREADS), 0, s, (const __nv_bfloat16*)h, ld_h,
-                    (const __nv_bfloat16*)w, ld_w, vocab, H, softcap, ctas, sc, o, r0);
+    st = launch_pdl("finish_kernel", finish_kernel, dim3(rows, n_targets ? 2 : 1), dim3(F_THREADS), 0, s,
+                    (const __nv_bfloat16*)h, ld_h, (const __nv_bfloat16*)w, ld_w, vocab, H, softcap, ctas, sc, o, r0);
     if (st) return st;
   }
   return MORJ_OK;

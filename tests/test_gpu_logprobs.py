@@ -106,6 +106,27 @@ def test_equal_logits_are_ranked_by_id():
     assert got.logprob[2, 0] == 0
 
 
+@pytest.mark.parametrize('V', [40000, 9001])
+def test_more_equal_logits_than_fit_in_shared_memory(V):
+    h, w = torch.ones(3, 64, device=DEV, dtype=torch.bfloat16), torch.zeros(V, 64, device=DEV, dtype=torch.bfloat16)
+    w[:, 0] = 0.5
+    w[V - 1, 0] = 0.75  # the one that comes first
+    got = check(h, w, torch.tensor([[V - 1], [0], [-1]], device=DEV, dtype=torch.int32), 32, 30.0)
+    assert got.top_ids.tolist() == [[V - 1] + list(range(31))] * 3
+
+
+@pytest.mark.parametrize('V', [700, 40000])
+def test_a_row_s_numbers_do_not_depend_on_its_neighbours(V):
+    g = torch.Generator(device=DEV).manual_seed(3)
+    h, w = grid(g, 64, 128, V)
+    targets = torch.randint(V, (64, 2), generator=g, device=DEV, dtype=torch.int32)
+    loud = h.clone()
+    loud[1::2] *= 32  # far beyond a quarter of the softcap, in the same warps
+    a, b = (token_logprobs(x, w, targets, top=4, softcap=20.0) for x in (h, loud))
+    for x, y in zip(a, b):
+        assert torch.equal(x[::2], y[::2])
+
+
 def test_candidates_in_rising_and_falling_order():
     V = 6000
     h = torch.zeros(2, 64, dtype=torch.bfloat16, device=DEV)
