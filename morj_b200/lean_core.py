@@ -669,15 +669,18 @@ class LeanGemma4:
             self._check_ids(req.tree.seqs[b])
         p = self.prepare_pass(req, seqs, available, scored=scored)
         row_of = {place: j for j, place in enumerate(sorted(set(p['plan']['readout'])))}
-        index = np.asarray([row_of[place] for place in p['plan']['readout']], np.int32)
+        index = np.asarray([row_of[place] for place in p['plan']['readout']], np.int64)
         tokens = [np.asarray(req.tree.seqs[b])[first:] for b, first in zip(seqs, scored)]
-        index, targets = (torch.from_numpy(a).to(self.device) for a in
-                          (index, np.concatenate(tokens).astype(np.int32)[:, None]))
+        # a token that sequences share (one row, one target) is scored once
+        vocab = self.embed.shape[0]
+        pairs, place = np.unique(index * vocab + np.concatenate(tokens), return_inverse=True)
+        index, targets = (torch.from_numpy(a.astype(np.int32)).to(self.device) for a in
+                          (pairs // vocab, (pairs % vocab)[:, None]))
         host = self._timed_pass(p, lambda: self._vocab_logprobs(self._execute_steps(p), index, targets, top))
         self._finish_pass(req, p)
         out, at = [], 0
         for first, toks in zip(scored, tokens):
-            rows = slice(at, at + len(toks))
+            rows = place[at:at + len(toks)]
             at += len(toks)
             got = dict(start=first, tokens=toks, logprob=host[0][rows, 0], lse=host[1][rows], entropy=host[2][rows])
             if top:
