@@ -15,6 +15,7 @@
 // filled once; parts leave (maximum, sum, O) in a workspace and combine_kernel joins them in a fixed order.
 #include <algorithm>
 #include <climits>
+#include <unordered_map>
 #include <vector>
 
 #include "kv8.cuh"
@@ -29,6 +30,11 @@ constexpr int STEP = 32;             // keys a warp of rows_kernel takes at a ti
 constexpr int T_ROWS = 128;           // rows of a tile_kernel tile
 constexpr int BN = 64;                // keys it takes at a time
 constexpr int FEW_ROWS = 16;         // segments of at most this many rows go to rows_kernel
+// ... and all segments of a call, 16 rows at a time, whose 16-row tiles see at most this many keys together (times the KV
+// heads) in at most one CTA per resident place: one launch in place of two and no expansion. 1 to 8 segments of 32 to
+// 2,048 rows, heads of 64 and 128, both ways: 6 to 16 us against 9 to 20 below it, level at twice as many, 25 against 20
+// at four times.
+constexpr long long FEW_KEYS = 32768;
 constexpr int T_CTAS = 2, T_MIN_KEYS = 256;  // resident CTAs per SM, and the fewest keys of a part: tiles
 constexpr int R_CTAS = 3, R_MIN_KEYS = 256;  // ... few rows
 constexpr float P_SCALE = 1024.0f;   // probabilities are rounded to FP16 as 1024 p: 2^-34 is their smallest step
@@ -1200,47 +1206,72 @@ extern "C" int morj_tree_attention_kv8_work(const int* qo_indptr_host, const int
         return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8_work: segment %d's tables are out of order", s);
     }
     std::vector<Item> tiles, rows, joins;
-    int few_max = 0;  // the largest segment that rows_kernel takes
-    for (int s = 0; s < n_segments; ++s) {
-      const int n = (qo_indptr_host[s + 1] - qo_indptr_host[s]) * G;
-      if (n <= kv8::FEW_ROWS) few_max = std::max(few_max, n);
-    }
-    const int few = few_max <= 8 ? 8 : 16;
-    // what the tiled segments see: the distinct pages in the order the lists name them, how many slots of each are
-    // listed, and every list entry's place among them
-    std::vector<int> place, pages, used, list;
-    for (int s = 0; s < n_segments; ++s) {
+    std::vector<int> kv_len(n_segments);
+    // the keys that rows [r0, r0 + n) of a segment see: what its first query sees from, its last query to
+    auto seen = [&](int s, int r0, int n, int* lo, int* hi) {
       const int q_len = qo_indptr_host[s + 1] - qo_indptr_host[s];
+      int x;
+      kv8::visible(q_len, kv_len[s], s < n_bidir, window, r0 / G, lo, &x);
+      kv8::visible(q_len, kv_len[s], s < n_bidir, window, (std::min(r0 + n, q_len * G) - 1) / G, &x, hi);
+    };
+    const long long places = (long long)kv8::R_CTAS * num_sms();
+    long long few_tiles = 0, few_keys = 0;  // if rows_kernel took every segment
+    int most = 0, most_few = 0;             // the largest segment, and the largest that it takes anyhow
+    for (int s = 0; s < n_segments; ++s) {
       const int n_pages = kv_indptr_host[s + 1] - kv_indptr_host[s];
       const int last = kv_last_page_len_host ? kv_last_page_len_host[s] : page_size;
       const long long kv = page_size == 1 || n_pages == 0 ? n_pages : (long long)(n_pages - 1) * page_size + last;
       if (kv < 0 || kv > INT_MAX)
         return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8_work: segment %d has %lld keys", s, kv);
-      const bool many = q_len * G > kv8::FEW_ROWS;
+      kv_len[s] = (int)kv;
+      const int n = (qo_indptr_host[s + 1] - qo_indptr_host[s]) * G;
+      most = std::max(most, n);
+      if (n <= kv8::FEW_ROWS) most_few = std::max(most_few, n);
+      for (int r0 = 0; r0 < n && few_tiles * hk <= places; r0 += kv8::FEW_ROWS) {
+        int lo, hi;
+        seen(s, r0, kv8::FEW_ROWS, &lo, &hi);
+        ++few_tiles, few_keys += std::max(hi - lo + 1, 0);
+      }
+    }
+    const bool all_few = few_tiles * hk <= places && few_keys * hk <= kv8::FEW_KEYS;
+    const int few = (all_few ? most : most_few) <= 8 ? 8 : 16;
+    // what the tiled segments see: the distinct pages in the order the lists name them, how many slots of each are
+    // listed, and every list entry's place among them
+    std::vector<int> near, pages, used, list;
+    std::unordered_map<int, int> far;  // (pages past what a table should be made for)
+    auto place = [&](int page) -> int& {  // the page's place, -1 before it has one
+      if (page >= 1 << 24) return far.emplace(page, -1).first->second;
+      if ((size_t)page >= near.size()) near.resize(std::max<size_t>(page + 1, 2 * near.size()), -1);
+      return near[page];
+    };
+    for (int s = 0; s < n_segments; ++s) {
+      const int q_len = qo_indptr_host[s + 1] - qo_indptr_host[s];
+      const int kv = kv_len[s];
+      const bool many = !all_few && q_len * G > kv8::FEW_ROWS;
       const int tile = many ? kv8::T_ROWS : few;
       int from = INT_MAX, to = -1;  // keys the segment's queries see
       for (int r0 = 0; r0 < q_len * G; r0 += tile) {
-        int lo, hi, x;  // what the tile's first query sees from, its last query to
-        kv8::visible(q_len, (int)kv, s < n_bidir, window, r0 / G, &lo, &x);
-        kv8::visible(q_len, (int)kv, s < n_bidir, window, (std::min(r0 + tile, q_len * G) - 1) / G, &x, &hi);
-        Item it{s, r0, 0, 0, -1, 1, 1, tile, qo_indptr_host[s], q_len, kv_indptr_host[s], (int)kv};
+        int lo, hi;
+        seen(s, r0, tile, &lo, &hi);
+        Item it{s, r0, 0, 0, -1, 1, 1, tile, qo_indptr_host[s], q_len, kv_indptr_host[s], kv};
         if (hi >= lo) it.t0 = lo, it.t1 = hi + 1, from = std::min(from, lo), to = std::max(to, hi);
         (many ? tiles : rows).push_back(it);
       }
-      if (!many || to < from) continue;
-      if (list.empty()) list.resize(kv_indptr_host[n_segments], 0);
+      if (q_len * G <= kv8::FEW_ROWS || to < from) continue;
+      if (many && list.empty()) list.resize(kv_indptr_host[n_segments], 0);
       for (int p = from / page_size; p <= to / page_size; ++p) {
         const int at = kv_indptr_host[s] + p, page = kv_indices_host[at];
         if (page < 0) return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8_work: page %d in segment %d's list", page, s);
-        if ((size_t)page >= place.size()) place.resize(std::max<size_t>(page + 1, 2 * place.size()), -1);
-        if (place[page] < 0) {
-          place[page] = (int)pages.size();
+        if (!many) continue;
+        int& index = place(page);
+        if (index < 0) {
+          index = (int)pages.size();
           pages.push_back(page);
           used.push_back(0);
         }
-        list[at] = place[page];
+        list[at] = index;
         const int n = p == to / page_size ? to % page_size + 1 : page_size;
-        used[place[page]] = std::max(used[place[page]], n);
+        used[index] = std::max(used[index], n);
       }
     }
     if ((long long)pages.size() * page_size > INT_MAX - 64)

@@ -354,6 +354,155 @@ def test_a_pool_beyond_32_bit_offsets():
     assert ((got.double() - out).abs() <= bound).all()
 
 
+# ---- attention of calls with many rows (128-row tiles on expanded pages) ----------------------------------------------
+
+MANY = {
+    'nothing to see': [(300, 40), (40, 0), (0, 10), (900, 1500), (3, 1)],
+    'prompts': [(700, 700), (401, 1101), (60, 1130)],
+    'ends inside a tile': [(129, 2049), (640, 1999), (127, 1)],
+    'with few rows': [(800, 1300), (1, 2500), (8, 8), (1, 0)],
+}
+
+
+@pytest.mark.parametrize('name', MANY)
+@pytest.mark.parametrize('hq,hk,d', [(4, 2, 64), (16, 16, 128), (9, 3, 128), (8, 1, 64)])
+@pytest.mark.parametrize('window,page', [(0, 1), (500, 64), (1000, 5)])
+def test_attention_of_many_rows_matches_the_definition(name, hq, hk, d, window, page):
+    spec = MANY[name]
+    rng = np.random.default_rng(len(name) + window)
+    g = torch.Generator(device=DEV).manual_seed(len(name))
+    qo, kv, indices, last, slots = make_segments(rng, spec, page)
+    pool = random_pool(g, slots, hk, d)
+    q = torch.randn(int(qo[-1]), hq, d, generator=g, device=DEV).to(torch.bfloat16)
+    _, plan = check_attention(pool, q, qo, kv, indices, last, page, window, 0, d ** -0.5)
+    assert plan.counts[5] > 0
+
+
+@pytest.mark.parametrize('window', [0, 300, 500])
+def test_attention_of_large_image_blocks(window):
+    rng, g = np.random.default_rng(1), torch.Generator(device=DEV).manual_seed(1)
+    qo, kv, indices, last, slots = make_segments(rng, [(500, 500), (700, 1200), (400, 900)], 1)
+    pool = random_pool(g, slots, 4, 128)
+    q = torch.randn(int(qo[-1]), 8, 128, generator=g, device=DEV).to(torch.bfloat16)
+    _, plan = check_attention(pool, q, qo, kv, indices, None, 1, window, 2, 128 ** -0.5)
+    assert plan.counts[5] > 0
+
+
+def test_attention_of_many_rows_with_scales_far_apart():
+    rng, g = np.random.default_rng(3), torch.Generator(device=DEV).manual_seed(3)
+    qo, kv, indices, last, slots = make_segments(rng, [(500, 2000)], 1)
+    k, v = pool_rows(g, slots, 2, 64, DEV), pool_rows(g, slots, 2, 64, DEV)
+    gain = torch.exp2(torch.randint(-10, 11, ((slots + 63) // 64, 1, 1), generator=g, device=DEV).float())
+    v = (v.float() * gain.repeat_interleave(64, 0)[:slots]).to(torch.bfloat16)
+    gain = torch.exp2(torch.randint(-6, 1, ((slots + 63) // 64, 1, 1), generator=g, device=DEV).float())
+    k = (k.float() * gain.repeat_interleave(64, 0)[:slots]).to(torch.bfloat16)
+    pool = kv8.KV8Pool(slots, 2, 64, DEV)
+    kv8.store(pool, k, v, kv8.StorePlan(np.arange(slots), slots, DEV))
+    q = torch.randn(int(qo[-1]), 4, 64, generator=g, device=DEV).to(torch.bfloat16)
+    q[0, 0] *= 2.0 ** -60
+    q[0, 2] = 0
+    q[0, 1] *= 100
+    _, plan = check_attention(pool, q, qo, kv, indices, last, 1, 0, 0, 0.125)
+    assert plan.counts[5] > 0
+
+
+@pytest.mark.parametrize('spec,window,page', [([(9, 90), (700, 3000), (1, 500)], 0, 64), ([(6000, 6200)], 64, 1),
+                                              ([(300, 4000), (200, 1111)], 700, 16)])
+def test_attention_of_many_rows_reads_nothing_a_query_may_not_see(spec, window, page):
+    rng, g = np.random.default_rng(4), torch.Generator(device=DEV).manual_seed(4)
+    qo, kv, indices, last, slots = make_segments(rng, spec, page)
+    good = random_pool(g, slots, 2, 64)
+    codes = [torch.full_like(c.view(torch.uint8), 0x7f) for c in (good.k, good.v)]
+    scales = [torch.full_like(s, float('nan')) for s in (good.k_scale, good.v_scale)]
+    for s, (n, keys) in enumerate(spec):
+        pages = indices[kv[s]:kv[s + 1]].astype(np.int64)
+        at = (pages[:, None] * page + np.arange(page)).reshape(-1)[:keys]
+        at = at[max(0, keys - n - (window - 1)) if window else 0:]
+        if window:  # (whole pages are expanded from the first one a query sees on: its unseen slots are the caller's too)
+            first = max(0, keys - n - (window - 1)) // page * page
+            at = (pages[:, None] * page + np.arange(page)).reshape(-1)[first:keys]
+        at = torch.as_tensor(at, device=DEV)
+        for new, old in zip(codes, (good.k, good.v)):
+            new[at] = old.view(torch.uint8)[at]
+        for new, old in zip(scales, (good.k_scale, good.v_scale)):
+            new[at // BLOCK] = old[at // BLOCK]
+    pool = kv8.KV8Pool.of(codes[0], scales[0], codes[1], scales[1])
+    q = torch.randn(int(qo[-1]), 4, 64, generator=g, device=DEV).to(torch.bfloat16)
+    plan = kv8.AttentionPlan(qo, kv, indices, 4, 2, 64, page_size=page, kv_last_page_len=last, window=window, device=DEV)
+    assert plan.counts[5] > 0
+    got = kv8.tree_attention(q, pool, plan, 0.125)
+    want, _ = check_attention(good, q, qo, kv, indices, last, page, window, 0, 0.125)
+    assert torch.equal(got, want)
+
+
+def test_attention_of_many_rows_reports_a_slot_outside_the_pool():
+    g = torch.Generator(device=DEV).manual_seed(7)
+    pool = random_pool(g, 2000, 2, 64)
+    where = np.arange(2000)
+    where[1234] = 2000
+    plan = kv8.AttentionPlan([0, 700], [0, 2000], where, 4, 2, 64, device=DEV)
+    assert plan.counts[5] > 0
+    kv8.tree_attention(torch.zeros(700, 4, 64, dtype=torch.bfloat16, device=DEV), pool, plan, 1.0)
+    assert nat.device_error(torch.cuda.current_stream().cuda_stream) == 0x301
+
+
+def test_attention_of_many_rows_on_streams_in_graphs_and_into_given_outputs():
+    g = torch.Generator(device=DEV).manual_seed(9)
+    qo, kv, indices, last, slots = make_segments(np.random.default_rng(9), [(500, 1500), (1, 900), (20, 100)], 1)
+    pool = random_pool(g, slots, 2, 128)
+    q = torch.randn(int(qo[-1]), 4, 128, generator=g, device=DEV).to(torch.bfloat16)
+    buf = torch.full((q.shape[0] + 2, 4, 128), 5.0, dtype=torch.bfloat16, device=DEV)
+    want, plan = check_attention(pool, q, qo, kv, indices, last, 1, 0, 0, 0.1, out=buf[1:-1])
+    assert plan.counts[5] > 0 and (buf[0] == 5).all() and (buf[-1] == 5).all()
+    side, outs, graphs = torch.cuda.Stream(), [], []
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):  # two calls of one plan at once
+        other = kv8.tree_attention(q, pool, plan, 0.1)
+    here = kv8.tree_attention(q, pool, plan, 0.1)
+    torch.cuda.synchronize()
+    assert torch.equal(other, want) and torch.equal(here, want)
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(kv8.tree_attention(q, pool, plan, 0.1))
+        graphs.append(graph)
+    q.mul_(0.5)
+    with torch.cuda.stream(side):
+        side.wait_stream(torch.cuda.default_stream())
+        graphs[1].replay()
+    graphs[0].replay()
+    torch.cuda.synchronize()
+    assert torch.equal(outs[0], outs[1]) and torch.equal(outs[0], kv8.tree_attention(q, pool, plan, 0.1))
+    assert not torch.equal(outs[0], want)
+
+
+def test_many_rows_over_a_pool_beyond_32_bit_offsets():
+    if torch.cuda.mem_get_info()[0] < 20 << 30:
+        pytest.skip('needs 20 GB')
+    hk, d = 16, 128
+    slots = (1 << 32) // (hk * d) + 200  # more than 2^32 codes in K alone
+    pool = kv8.KV8Pool(slots, hk, d, DEV)
+    g = torch.Generator(device=DEV).manual_seed(10)
+    where = np.concatenate([np.arange(slots - 150, slots), np.arange(20), (1 << 31) // (hk * d) + np.arange(-3, 4)])
+    n = len(where)
+    k, v = pool_rows(g, n, hk, d, DEV), pool_rows(g, n, hk, d, DEV)
+    kv8.store(pool, k, v, kv8.StorePlan(where, slots, DEV))
+    # the same blocks of the large pool, with their codes and scales, one after another in a small one
+    blocks, index = np.unique(where // BLOCK, return_inverse=True)
+    at = index * BLOCK + where % BLOCK
+    near = kv8.KV8Pool(len(blocks) * BLOCK, hk, d, DEV)
+    for big, small, sb, ss in ((pool.k, near.k, pool.k_scale, near.k_scale), (pool.v, near.v, pool.v_scale, near.v_scale)):
+        small.view(torch.uint8)[at] = big.view(torch.uint8)[torch.as_tensor(where, device=DEV)]
+        ss.copy_(sb[torch.as_tensor(blocks, device=DEV)])
+    q = torch.randn(400, 32, d, generator=g, device=DEV).to(torch.bfloat16)
+    out = []
+    for p, slot in ((pool, where), (near, at)):
+        plan = kv8.AttentionPlan([0, 400], [0, n], slot, 32, hk, d, device=DEV)
+        assert plan.counts[5] > 0
+        out.append(kv8.tree_attention(q, p, plan, 0.1))
+    assert torch.equal(out[0], out[1])
+
+
 def test_a_rounded_value_is_the_nearest_code():
     # every e4m3 value and the midpoints between neighbours, against the reference rounding
     bits = torch.arange(256, dtype=torch.uint8, device=DEV).view(torch.float8_e4m3fn).float()

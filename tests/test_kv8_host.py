@@ -67,6 +67,9 @@ CASES = [  # (segments (queries, keys), hq, hk, window, n_bidir)
     ([(2, 9000)], 24, 8, 0, 0),
     ([(1, 20000)], 64, 1, 0, 0),
     ([(700, 1700), (1, 4000), (64, 64)], 32, 16, 1024, 0),
+    ([(130, 130), (5, 200), (3, 1), (900, 2000)], 8, 2, 0, 0),
+    ([(400, 400), (600, 1000)], 4, 4, 160, 1),
+    ([(300, 40), (40, 0), (2, 5), (900, 1500)], 6, 2, 0, 0),
 ]
 
 
@@ -80,7 +83,14 @@ def test_attention_work_covers_every_row_and_key_once(spec, hq, hk, window, n_bi
     last = [n - (p - 1) * page if p else 0 for (_, n), p in zip(spec, pages)]
     perm = np.random.default_rng(len(spec)).permutation(int(kv[-1]) + 5)[:int(kv[-1])]
     work, counts = nat.kv8_attention_work(qo, kv, perm, n_bidir, hq, hk, window, page, last)
-    check_work(work, counts, spec, G, window, n_bidir, kv)
+    # few rows see few keys: everything 16 rows at a time
+    few = [[view(n, keys, s < n_bidir, window, r // G) for r in range(r0, min(r0 + 16, n * G))]
+           for s, (n, keys) in enumerate(spec) for r0 in range(0, n * G, 16)]
+    seen = sum(max(max(hi for _, hi in rows) - min(lo for lo, _ in rows) + 1, 0) for rows in few)
+    all_few = seen * hk <= 32768 and len(few) * hk <= 3 * 148
+    check_work(work, counts, spec, G, window, n_bidir, kv, all_few)
+    if all_few:
+        return
     check_pages(work, counts, spec, G, window, n_bidir, page, kv, perm)
 
 
@@ -110,7 +120,7 @@ def check_pages(work, counts, spec, G, window, n_bidir, page, kv, indices):
                                      | {x // 64 for x in slots})
 
 
-def check_work(work, counts, spec, G, window, n_bidir, kv):
+def check_work(work, counts, spec, G, window, n_bidir, kv, all_few):
     n_rows, n_joins, units, few, ints, n_tiles = list(counts)[:6]
     items = work[:(n_tiles + n_rows + n_joins) * ITEM].reshape(-1, ITEM).tolist()
     assert len(work) == ints
@@ -118,11 +128,11 @@ def check_work(work, counts, spec, G, window, n_bidir, kv):
     for i, (seg, r0, t0, t1, unit, _, _, rows, q0, q_len, kv0, keys) in enumerate(items[:n_tiles + n_rows]):
         assert (q_len, keys) == spec[seg] and q0 == sum(n for n, _ in spec[:seg]) and kv0 == kv[seg]
         # segments of more than 16 rows in 128-row tiles, the others in small ones
-        assert rows == (128 if i < n_tiles else few) and (spec[seg][0] * G > 16) == (i < n_tiles)
+        assert rows == (128 if i < n_tiles else few) and (not all_few and spec[seg][0] * G > 16) == (i < n_tiles)
         assert r0 % rows == 0 and t0 <= t1
         parts.setdefault((seg, r0), []).append((t0, t1, unit))
         rows_of[seg] = rows
-    assert few in (8, 16) and (few == 16 or all(n * G <= 8 or n * G > 16 for n, _ in spec))
+    assert few in (8, 16) and (few == 16 or all(n * G <= 8 or (not all_few and n * G > 16) for n, _ in spec))
     assert set(parts) == {(s, r0) for s, (n, _) in enumerate(spec) if n for r0 in range(0, n * G, rows_of[s])}
     joined = {(j[0], j[1]): j for j in items[n_tiles + n_rows:]}
     assert len(joined) == n_joins
