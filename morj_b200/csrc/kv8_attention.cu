@@ -182,6 +182,9 @@ MORJ_DEV bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort) {
     }
   }
 }
+MORJ_DEV void sts16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
 MORJ_DEV uint4 lds16(uint32_t addr) {
   uint4 v;
   asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
@@ -203,6 +206,9 @@ template <int D>
 MORJ_DEV uint32_t unit_at(int k, int u) {
   return D == 128 ? (uint32_t)(k * 128 + ((u ^ (k & 7)) << 4)) : (uint32_t)(k * 64 + ((u ^ ((k >> 1) & 3)) << 4));
 }
+
+// 16-byte unit u of row r's FP32 results: where eight lanes of two rows and four column runs write, eight bank groups
+MORJ_DEV int spread(int r, int u) { return u ^ ((u >> 3) * 2 + (r & 1)); }
 
 // ROWS = 8 or 16 rows per tile. Rows 8..15 of the MMA's 16 are zeros when ROWS = 8 and cost no registers.
 template <int D, int ROWS>
@@ -481,35 +487,44 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
     l[b] += __shfl_xor_sync(0xffffffffu, l[b], 2);
     const int r = g + 8 * b;
     if (c4 == 0) sh_m[warp * ROWS + r] = m[b], sh_l[warp * ROWS + r] = l[b];
-    // column tile j, column n of the MMA is output column n * VRUN + j
-    float* dst = sh_o + (warp * ROWS + r) * D + 2 * c4 * VRUN;
+    // column tile j, column n of the MMA is output column n * VRUN + j: the lane's are 2 VRUN consecutive ones
+    const uint32_t row_at = smem_u32(sh_o) + (warp * ROWS + r) * (D * 4);
 #pragma unroll
-    for (int j = 0; j < NT; ++j) dst[j] = o[j][2 * b] * scale_o, dst[VRUN + j] = o[j][2 * b + 1] * scale_o;
+    for (int q = 0; q < VRUN / 2; ++q) {
+      constexpr int Q = VRUN / 4;
+      const int e = q / Q, j = q % Q * 4;
+      sts16(row_at + spread(r, c4 * (VRUN / 2) + q) * 16, __float_as_uint(o[j][2 * b + e] * scale_o),
+            __float_as_uint(o[j + 1][2 * b + e] * scale_o), __float_as_uint(o[j + 2][2 * b + e] * scale_o),
+            __float_as_uint(o[j + 3][2 * b + e] * scale_o));
+    }
   }
   __syncthreads();
   float* part = it.unit < 0 ? nullptr : a.ws + ((size_t)it.unit * a.hk + h) * (UNIT * (D + 2));
 #pragma unroll 1
-  for (int i = threadIdx.x; i < ROWS * D; i += WARPS * 32) {
-    const int r = i / D, d = i % D;
+  for (int i = threadIdx.x; i < ROWS * (D / 4); i += WARPS * 32) {
+    const int r = i / (D / 4), u = i % (D / 4);
     if (it.r0 + r >= n_rows) break;
     float mm = -INFINITY;
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) mm = fmaxf(mm, sh_m[w * ROWS + r]);
-    float ll = 0.f, oo = 0.f;
+    float ll = 0.f, x[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < WARPS; ++w) {
       const float mw = sh_m[w * ROWS + r];
       const float f = mw == -INFINITY ? 0.f : exp2f(mw - mm);
       ll += f * sh_l[w * ROWS + r];
-      oo += f * sh_o[(w * ROWS + r) * D + d];
+      const uint4 v = lds16(smem_u32(sh_o) + (w * ROWS + r) * (D * 4) + spread(r, u) * 16);
+      x[0] += f * __uint_as_float(v.x), x[1] += f * __uint_as_float(v.y);
+      x[2] += f * __uint_as_float(v.z), x[3] += f * __uint_as_float(v.w);
     }
     if (part) {
-      if (d == 0) part[r] = mm, part[UNIT + r] = ll;
-      part[2 * UNIT + r * D + d] = oo;
+      if (u == 0) part[r] = mm, part[UNIT + r] = ll;
+      reinterpret_cast<float4*>(part + 2 * UNIT + r * D)[u] = make_float4(x[0], x[1], x[2], x[3]);
     } else {
-      const int row = it.r0 + r;
-      a.out[row_index(a, it, h, row) * D + d] =
-          __float2bfloat16(ll == 0.f ? 0.f : oo / ll);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[e] = ll == 0.f ? 0.f : x[e] / ll;
+      *reinterpret_cast<uint2*>(a.out + row_index(a, it, h, it.r0 + r) * D + 4 * u) =
+          make_uint2(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]));
     }
   }
 }
@@ -667,9 +682,6 @@ MORJ_DEV float max3f(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
   return d;
-}
-MORJ_DEV void sts16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
 
 // One loader warp fills buffer `dst` with the expanded rows of keys [t0, t0 + BN) and completes `full`. s0, s1: the
