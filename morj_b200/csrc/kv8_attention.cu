@@ -106,12 +106,11 @@ MORJ_DEV void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-// the same with rows 8..15 of A zero: their sums are dropped
-MORJ_DEV void mma_f16_top(float (&c)[4], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
-  [[maybe_unused]] float x, y;
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%5}, {%7,%8}, {%0,%1,%9,%9};"
-               : "+f"(c[0]), "+f"(c[1]), "=f"(x), "=f"(y)
-               : "r"(a0), "r"(0u), "r"(a2), "r"(b0), "r"(b1), "f"(0.f));
+// an 8 x 8 matrix of 16-bit elements, lane 4 i + j with elements (i, 2 j) and (i, 2 j + 1), transposed
+MORJ_DEV uint32_t transposed(uint32_t x) {
+  uint32_t d;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+  return d;
 }
 // maximum that keeps a NaN
 MORJ_DEV float max_nan(float a, float b) {
@@ -207,10 +206,16 @@ MORJ_DEV uint32_t unit_at(int k, int u) {
   return D == 128 ? (uint32_t)(k * 128 + ((u ^ (k & 7)) << 4)) : (uint32_t)(k * 64 + ((u ^ ((k >> 1) & 3)) << 4));
 }
 
-// 16-byte unit u of row r's FP32 results: where eight lanes of two rows and four column runs write, eight bank groups
-MORJ_DEV int spread(int r, int u) { return u ^ ((u >> 3) * 2 + (r & 1)); }
+// 16-byte unit u of row r's FP32 results: where eight lanes of two column runs and four rows write, eight bank groups
+template <int D>
+MORJ_DEV int spread(int r, int u) {
+  const int x = (r >> 1) & 3;
+  return u ^ (D == 128 ? x : (x & 1) * 4 + (x >> 1));
+}
 
-// ROWS = 8 or 16 rows per tile. Rows 8..15 of the MMA's 16 are zeros when ROWS = 8 and cost no registers.
+// ROWS = 8 or 16 rows per tile. Both products are taken transposed, S^T = K Q^T and O^T = V^T P^T: the MMA's 16 rows are
+// keys and output columns, of which there are always enough, and its 8 columns the tile's rows (two MMAs for 16). With
+// the rows on the 16 side half of every MMA and of its sums was empty for 8 of them: 148 us for 64 single queries.
 template <int D, int ROWS>
 __global__ void __launch_bounds__(WARPS * 32, 3)
     rows_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const Args a,
@@ -219,7 +224,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
   pdl_trigger();
   using L = RSmem<D>;
   constexpr int KS = D / 16;       // MMA depth steps of q . k
-  constexpr int NT = D / 8;        // 8-column output tiles
+  constexpr int NT = D / 16;       // 16-column output tiles
   constexpr int HALVES = ROWS / 8;
   constexpr int KRUN = D / 4;      // consecutive codes of a key one lane reads of K
   constexpr int VRUN = D / 8;      // ... and of V
@@ -299,19 +304,16 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
     issue(i, e);
   }
 
-  // ---- this lane's rows: r0 + g and r0 + g + 8
+  // ---- Q^T fragments: rows r0 + g (+ 8), this lane's run of the head dimension
   uint32_t qf[HALVES][KS][2];
   float qs[HALVES];
-  int lo[HALVES], hi[HALVES];
 #pragma unroll
   for (int b = 0; b < HALVES; ++b) {
     const int r = it.r0 + g + 8 * b;
-    lo[b] = INT_MAX, hi[b] = -1;
     uint4 raw[KRUN / 8];
 #pragma unroll
     for (int i = 0; i < KRUN / 8; ++i) raw[i] = make_uint4(0, 0, 0, 0);
     if (r < n_rows) {
-      visible(it.q_len, it.kv_len, bidir, a.window, a.group.of(r), &lo[b], &hi[b]);
       const uint4* src = reinterpret_cast<const uint4*>(
           a.q + row_index(a, it, h, r) * D + c4 * KRUN);
 #pragma unroll
@@ -339,12 +341,27 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
     }
   }
 
-  float o[NT][4];
+  // ---- this lane's rows of the results: r0 + 2 c4, the next one (+ 8)
+  float row_qs[HALVES][2];
+  int lo[HALVES][2], hi[HALVES][2];
+  float o[HALVES][NT][4];  // (column g VRUN + 2 tile, row 0), (.., row 1), (the next column, row 0), (.., row 1)
+  float m[HALVES][2], l[HALVES][2];
 #pragma unroll
-  for (int j = 0; j < NT; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-  float m[HALVES], l[HALVES];
+  for (int b = 0; b < HALVES; ++b) {
 #pragma unroll
-  for (int b = 0; b < HALVES; ++b) m[b] = -INFINITY, l[b] = 0.f;
+    for (int e = 0; e < 2; ++e) {
+      const int r = it.r0 + 2 * c4 + e + 8 * b;
+      row_qs[b][e] = __shfl_sync(0xffffffffu, qs[b], 4 * (2 * c4 + e));
+      lo[b][e] = INT_MAX, hi[b][e] = -1;
+      if (r < n_rows) {
+        visible(it.q_len, it.kv_len, bidir, a.window, a.group.of(r), &lo[b][e], &hi[b][e]);
+        hi[b][e] = min(hi[b][e], t_end - 1);
+      }
+      m[b][e] = -INFINITY, l[b][e] = 0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < NT; ++j) o[b][j][0] = o[b][j][1] = o[b][j][2] = o[b][j][3] = 0.f;
+  }
   float vref = 0.f;  // the largest V scale met: O is in units of vref / P_SCALE
 
 #pragma unroll 1
@@ -373,83 +390,92 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
       vref = vmax;
     }
     const float inv_v = vref != 0.f ? P_SCALE / vref : 0.f;
+    // scores of keys base + 16 half + g (+ 8), this lane's rows
+    float s[2][HALVES][4];
 #pragma unroll
-    for (int sub = 0; sub < STEP; sub += 16) {
-      // scores of 8 keys per MMA column tile: rows g (and g + 8), keys c4 * 2 + {0, 1}
-      float s[2][4];
+    for (int half = 0; half < 2; ++half) {
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.f;
-        const int k = sub + j * 8 + g;
-        uint32_t w[KRUN / 4];
+      for (int b = 0; b < HALVES; ++b) s[half][b][0] = s[half][b][1] = s[half][b][2] = s[half][b][3] = 0.f;
+      uint32_t w[2][KRUN / 4];
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
 #pragma unroll
         for (int u = 0; u < KRUN / 16; ++u) {
-          const uint4 x = lds16(st + unit_at<D>(k, c4 * (KRUN / 16) + u));
-          w[4 * u] = x.x, w[4 * u + 1] = x.y, w[4 * u + 2] = x.z, w[4 * u + 3] = x.w;
+          const uint4 x = lds16(st + unit_at<D>(half * 16 + e * 8 + g, c4 * (KRUN / 16) + u));
+          w[e][4 * u] = x.x, w[e][4 * u + 1] = x.y, w[e][4 * u + 2] = x.z, w[e][4 * u + 3] = x.w;
         }
 #pragma unroll
-        for (int x = 0; x < KS; ++x) {
-          const uint32_t b0 = codes2_f16(w[x]), b1 = codes2_f16(w[x] >> 16);
-          if constexpr (HALVES == 2)
-            mma_f16(s[j], qf[0][x][0], qf[1][x][0], qf[0][x][1], qf[1][x][1], b0, b1);
-          else
-            mma_f16_top(s[j], qf[0][x][0], qf[0][x][1], b0, b1);
-        }
+      for (int x = 0; x < KS; ++x) {
+        const uint32_t a0 = codes2_f16(w[0][x]), a1 = codes2_f16(w[1][x]);
+        const uint32_t a2 = codes2_f16(w[0][x] >> 16), a3 = codes2_f16(w[1][x] >> 16);
+#pragma unroll
+        for (int b = 0; b < HALVES; ++b) mma_f16(s[half][b], a0, a1, a2, a3, qf[b][x][0], qf[b][x][1]);
       }
-      float mx[HALVES];
+    }
+    float mx[HALVES][2];
 #pragma unroll
-      for (int b = 0; b < HALVES; ++b) mx[b] = -INFINITY;
+    for (int b = 0; b < HALVES; ++b) mx[b][0] = mx[b][1] = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint2 f2 = lds8(kf_at + (sub + j * 8 + c4 * 2) * 4);
+    for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int t = base + sub + j * 8 + c4 * 2 + e;
-          const float f = __uint_as_float(e ? f2.y : f2.x);
+      for (int k8 = 0; k8 < 2; ++k8) {
+        const int k = half * 16 + k8 * 8 + g, t = base + k;
+        const float f = lds4(kf_at + k * 4);
 #pragma unroll
-          for (int b = 0; b < HALVES; ++b) {
-            float& x = s[j][2 * b + e];
-            x = (t >= lo[b] && t <= hi[b] && t < t_end) ? x * (f * qs[b]) : -INFINITY;
-            mx[b] = max_nan(mx[b], x);
+        for (int b = 0; b < HALVES; ++b)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            float& x = s[half][b][2 * k8 + e];
+            x = t >= lo[b][e] && t <= hi[b][e] ? x * (f * row_qs[b][e]) : -INFINITY;
+            mx[b][e] = max_nan(mx[b][e], x);
           }
+      }
+    float alpha[HALVES][2];
+    bool same = true;
+#pragma unroll
+    for (int b = 0; b < HALVES; ++b)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+#pragma unroll
+        for (int x = 4; x < 32; x <<= 1) mx[b][e] = max_nan(mx[b][e], __shfl_xor_sync(0xffffffffu, mx[b][e], x));
+        const float now = max_nan(m[b][e], mx[b][e]);
+        alpha[b][e] = m[b][e] == -INFINITY ? 0.f : fast_exp2(m[b][e] - now);
+        m[b][e] = now;
+        l[b][e] *= alpha[b][e];
+        alpha[b][e] *= unit;
+        same = same && alpha[b][e] == 1.f;
+      }
+    if (!__all_sync(0xffffffffu, same)) {
+#pragma unroll
+      for (int b = 0; b < HALVES; ++b)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+          o[b][j][0] *= alpha[b][0], o[b][j][1] *= alpha[b][1];
+          o[b][j][2] *= alpha[b][0], o[b][j][3] *= alpha[b][1];
         }
-      }
-      float alpha[HALVES];
+    }
 #pragma unroll
-      for (int b = 0; b < HALVES; ++b) {
-        mx[b] = max_nan(mx[b], __shfl_xor_sync(0xffffffffu, mx[b], 1));
-        mx[b] = max_nan(mx[b], __shfl_xor_sync(0xffffffffu, mx[b], 2));
-        const float now = max_nan(m[b], mx[b]);
-        alpha[b] = m[b] == -INFINITY ? 0.f : fast_exp2(m[b] - now);
-        m[b] = now;
-        l[b] *= alpha[b];
-        alpha[b] *= unit;
-      }
-      unit = 1.f;
-      if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[HALVES - 1] != 1.f)) {
-#pragma unroll
-        for (int j = 0; j < NT; ++j)
-#pragma unroll
-          for (int b = 0; b < HALVES; ++b) o[j][2 * b] *= alpha[b], o[j][2 * b + 1] *= alpha[b];
-      }
+    for (int half = 0; half < 2; ++half) {
       uint32_t pf[HALVES][2];
 #pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        const uint2 f2 = lds8(vf_at + (sub + j * 8 + c4 * 2) * 4);
-        const float f0 = __uint_as_float(f2.x) * inv_v, f1 = __uint_as_float(f2.y) * inv_v;
+      for (int k8 = 0; k8 < 2; ++k8) {
+        const float f = lds4(vf_at + (half * 16 + k8 * 8 + g) * 4) * inv_v;
 #pragma unroll
         for (int b = 0; b < HALVES; ++b) {
-          const float shift = m[b] == -INFINITY ? 0.f : m[b];
-          const float p0 = fast_exp2(s[j][2 * b] - shift), p1 = fast_exp2(s[j][2 * b + 1] - shift);
-          l[b] += p0 + p1;
-          pf[b][j] = pack_f16x2(p0 * f0, p1 * f1);
+          float p[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            p[e] = fast_exp2(s[half][b][2 * k8 + e] - (m[b][e] == -INFINITY ? 0.f : m[b][e]));
+            l[b][e] += p[e];
+          }
+          pf[b][k8] = transposed(pack_f16x2(p[0] * f, p[1] * f));
         }
       }
       // V of keys c4 * 2 + {0, 1, 8, 9}, output columns g * VRUN ..: four columns a word, paired per column
       uint32_t vw[4][VRUN / 4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int k = sub + (e >> 1) * 8 + c4 * 2 + (e & 1);
+        const int k = half * 16 + (e >> 1) * 8 + c4 * 2 + (e & 1);
         if constexpr (VRUN == 16) {
           const uint4 x = lds16(st + L::SIDE + unit_at<D>(k, g));
           vw[e][0] = x.x, vw[e][1] = x.y, vw[e][2] = x.z, vw[e][3] = x.w;
@@ -459,19 +485,16 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
         }
       }
 #pragma unroll
-      for (int w = 0; w < VRUN / 4; ++w) {
-        const uint32_t a01 = prmt(vw[0][w], vw[1][w], 0x5140), a23 = prmt(vw[0][w], vw[1][w], 0x7362);
-        const uint32_t b01 = prmt(vw[2][w], vw[3][w], 0x5140), b23 = prmt(vw[2][w], vw[3][w], 0x7362);
-        const uint32_t av[4] = {a01, a01 >> 16, a23, a23 >> 16}, bv[4] = {b01, b01 >> 16, b23, b23 >> 16};
+      for (int w = 0; w < VRUN / 4; ++w)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const uint32_t b0 = codes2_f16(av[e]), b1 = codes2_f16(bv[e]);
-          if constexpr (HALVES == 2)
-            mma_f16(o[4 * w + e], pf[0][0], pf[1][0], pf[0][1], pf[1][1], b0, b1);
-          else
-            mma_f16_top(o[4 * w + e], pf[0][0], pf[0][1], b0, b1);
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t lo2 = prmt(vw[0][w], vw[1][w], e ? 0x7362 : 0x5140);
+          const uint32_t hi2 = prmt(vw[2][w], vw[3][w], e ? 0x7362 : 0x5140);
+          const uint32_t a0 = codes2_f16(lo2), a1 = codes2_f16(lo2 >> 16);
+          const uint32_t a2 = codes2_f16(hi2), a3 = codes2_f16(hi2 >> 16);
+#pragma unroll
+          for (int b = 0; b < HALVES; ++b) mma_f16(o[b][2 * w + e], a0, a1, a2, a3, pf[b][0], pf[b][1]);
         }
-      }
     }
   }
 
@@ -482,22 +505,20 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
   float* sh_l = sh_m + WARPS * ROWS;
   const float scale_o = vref / P_SCALE;
 #pragma unroll
-  for (int b = 0; b < HALVES; ++b) {
-    l[b] += __shfl_xor_sync(0xffffffffu, l[b], 1);
-    l[b] += __shfl_xor_sync(0xffffffffu, l[b], 2);
-    const int r = g + 8 * b;
-    if (c4 == 0) sh_m[warp * ROWS + r] = m[b], sh_l[warp * ROWS + r] = l[b];
-    // column tile j, column n of the MMA is output column n * VRUN + j: the lane's are 2 VRUN consecutive ones
-    const uint32_t row_at = smem_u32(sh_o) + (warp * ROWS + r) * (D * 4);
+  for (int b = 0; b < HALVES; ++b)
 #pragma unroll
-    for (int q = 0; q < VRUN / 2; ++q) {
-      constexpr int Q = VRUN / 4;
-      const int e = q / Q, j = q % Q * 4;
-      sts16(row_at + spread(r, c4 * (VRUN / 2) + q) * 16, __float_as_uint(o[j][2 * b + e] * scale_o),
-            __float_as_uint(o[j + 1][2 * b + e] * scale_o), __float_as_uint(o[j + 2][2 * b + e] * scale_o),
-            __float_as_uint(o[j + 3][2 * b + e] * scale_o));
+    for (int e = 0; e < 2; ++e) {
+#pragma unroll
+      for (int x = 4; x < 32; x <<= 1) l[b][e] += __shfl_xor_sync(0xffffffffu, l[b][e], x);
+      const int r = 2 * c4 + e + 8 * b;
+      if (g == 0) sh_m[warp * ROWS + r] = m[b][e], sh_l[warp * ROWS + r] = l[b][e];
+      const uint32_t row_at = smem_u32(sh_o) + (warp * ROWS + r) * (D * 4);
+#pragma unroll
+      for (int q = 0; q < VRUN / 4; ++q)
+        sts16(row_at + spread<D>(r, g * (VRUN / 4) + q) * 16, __float_as_uint(o[b][2 * q][e] * scale_o),
+              __float_as_uint(o[b][2 * q][2 + e] * scale_o), __float_as_uint(o[b][2 * q + 1][e] * scale_o),
+              __float_as_uint(o[b][2 * q + 1][2 + e] * scale_o));
     }
-  }
   __syncthreads();
   float* part = it.unit < 0 ? nullptr : a.ws + ((size_t)it.unit * a.hk + h) * (UNIT * (D + 2));
 #pragma unroll 1
@@ -513,7 +534,7 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
       const float mw = sh_m[w * ROWS + r];
       const float f = mw == -INFINITY ? 0.f : exp2f(mw - mm);
       ll += f * sh_l[w * ROWS + r];
-      const uint4 v = lds16(smem_u32(sh_o) + (w * ROWS + r) * (D * 4) + spread(r, u) * 16);
+      const uint4 v = lds16(smem_u32(sh_o) + (w * ROWS + r) * (D * 4) + spread<D>(r, u) * 16);
       x[0] += f * __uint_as_float(v.x), x[1] += f * __uint_as_float(v.y);
       x[2] += f * __uint_as_float(v.z), x[3] += f * __uint_as_float(v.w);
     }
