@@ -44,7 +44,7 @@ struct Scratch {
   float4* stats;    // [cta][row]: m, s, t, number of candidates
   float* own;       // [cta][row]: candidates must exceed it (the top-th of a cut list)
   uint2* lists;     // [cta][row block][CAND][128 rows]: candidates (logit, id)
-  unsigned* bound;  // [row]: at least `top` logits reach it, as an ordered integer; 0: none known
+  unsigned* bound;  // [row]: at least `top` logits reach it, as an ordered integer; 0: none known. Null: one tile per CTA
   int rows;         // rows of a chunk rounded up to whole row blocks
   int top;
 };
@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(THREADS, 1)
         held = m;
       }
       uint2* list = lists + (size_t)m * CAND * BM;
-      const unsigned known = top && row_ok ? __ldcg(sc.bound + m * BM + r128) : 0u;  // (arrives during the wait below)
+      const unsigned known = sc.bound && row_ok ? __ldcg(sc.bound + m * BM + r128) : 0u;  // (arrives during the wait below)
       int ok = lane == 0 ? (int)mbar_wait(accf0 + 8 * acc, acc_phase, abort, kErrTimeoutGemmEpilogue) : 0;
       ok = __shfl_sync(0xffffffffu, ok, 0);
       if (!ok) break;
@@ -319,7 +319,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           for (int i = 0; i < 32; ++i) g[i] = g[i] == first ? -INFINITY : g[i];
         }
         if (fresh && row_ok && first > -INFINITY) {
-          atomicMax(sc.bound + m * BM + r128, ordered(first));
+          if (sc.bound) atomicMax(sc.bound + m * BM + r128, ordered(first));
           tau = fmaxf(tau, below(ordered(first)));
         }
         __syncwarp();
@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           if (count > CAND - 32) {
             own = cut_list(list, count, top);
             count = top;
-            atomicMax(sc.bound + m * BM + r128, ordered(own));
+            if (sc.bound) atomicMax(sc.bound + m * BM + r128, ordered(own));
             tau = fmaxf(tau, own);
           }
           __syncwarp();
@@ -412,7 +412,7 @@ __global__ void __launch_bounds__(F_THREADS)
   uint2 head[AHEAD];  // the first entries of this thread's list (left over from another call past its count)
   unsigned known = 0;
   if (blockIdx.y == 0 && sc.top) {
-    known = sc.bound[local];
+    known = sc.bound ? sc.bound[local] : 0u;
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i) head[i] = threadIdx.x < ctas ? __ldcg(list + i * BM) : make_uint2(0, 0);
   }
@@ -654,7 +654,6 @@ extern "C" int morj_token_logprobs(const void* h, long long ld_h, int n, const v
   sc.stats = reinterpret_cast<float4*>(ws);
   sc.own = reinterpret_cast<float*>(ws + at.own);
   sc.lists = reinterpret_cast<uint2*>(ws + at.lists);
-  sc.bound = reinterpret_cast<unsigned*>(ws + at.bound);
   const Outputs o{targets, n_targets, logprobs_out, lse, entropy, top_ids, top_logprobs};
   for (int r0 = 0; r0 < n; r0 += CHUNK_ROWS) {
     const int rows = std::min(n - r0, CHUNK_ROWS);
@@ -669,7 +668,9 @@ extern "C" int morj_token_logprobs(const void* h, long long ld_h, int n, const v
     CUtensorMap mw;
     if ((st = make_map(&mw, w, vocab, H, ld_w, bn))) return st;
     const int ctas = (int)std::min<long long>(tiles, std::min(num_sms(), F_THREADS));
-    if (top) {
+    // (CTAs with one tile each have no later tile to use a bound for: nothing to clear)
+    sc.bound = top && tiles > ctas ? reinterpret_cast<unsigned*>(ws + at.bound) : nullptr;
+    if (sc.bound) {
       const cudaError_t e = cudaMemsetAsync(sc.bound, 0, sc.rows * sizeof(unsigned), s);
       if (e != cudaSuccess) return set_error(MORJ_ERR_CUDA, "cudaMemsetAsync: %s", cudaGetErrorString(e));
     }

@@ -55,17 +55,15 @@ def token_logprobs(h, w, targets, top=0, softcap=0.0):
     if (n and h.stride(1) != 1) or w.stride(1) != 1:
         raise ValueError('the elements of a row must be contiguous')
     T = targets.shape[1]
-    # one allocation: logprob, lse, entropy, top_logprobs, then the ids
-    out = torch.empty(n * (T + 2 + 2 * top), dtype=torch.float32, device=dev)
-    logprob, lse, entropy = out[:n * T].view(n, T), out[n * T:n * (T + 1)], out[n * (T + 1):n * (T + 2)]
-    lps = out[n * (T + 2):n * (T + 2 + top)].view(n, top)
-    ids = out[n * (T + 2 + top):].view(torch.int32).view(n, top)
+    make = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=dev)
+    logprob, lse, entropy = make(n, T), make(n), make(n)
+    ids, lps = (make(n, top, dtype=torch.int32), make(n, top)) if top else (None, None)
     if n:
         nbytes = workspace_bytes(n, top)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        ws = make(nbytes, dtype=torch.uint8)
         with _on(dev) as s:
             nat.call('morj_token_logprobs', h.data_ptr(), h.stride(0) if n > 1 else H, n, w.data_ptr(),
                      w.stride(0) if w.shape[0] > 1 else H, w.shape[0], H, softcap, targets.data_ptr() if T else None, T,
                      logprob.data_ptr() if T else None, lse.data_ptr(), entropy.data_ptr(), top,
                      ids.data_ptr() if top else None, lps.data_ptr() if top else None, ws.data_ptr(), nbytes, s)
-    return TokenLogprobs(logprob, lse, entropy, ids, lps) if top else TokenLogprobs(logprob, lse, entropy)
+    return TokenLogprobs(logprob, lse, entropy, ids, lps)
