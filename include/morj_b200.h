@@ -187,7 +187,8 @@ int morj_label_head(const void* x, long long ld_x, const int* seq_row, const int
  * `top` largest logits' ids and log-probabilities ([n, top], larger first, the lower id first among equal logits; at
  * most MORJ_MAX_TOP). All outputs FP32 / int32; lse and entropy may be NULL. The [n, vocab] logits are never stored.
  * A target outside [-1, vocab) sets the device error word (0x301) and gives NaN. A row with a NaN gives NaN; NaN and
- * -infinity are no alternatives (top id -1 and NaN where none is left). H % 8 == 0, ld % 8 == 0; h, w and workspace 16-byte aligned.
+ * -infinity are no alternatives (top id -1 and NaN where none is left). H % 8 == 0, ld % 8 == 0; h, w and workspace
+ * 16-byte aligned.
  * workspace: morj_token_logprobs_workspace bytes of the caller's, overwritten; calls that may overlap on the device must
  * not share it. Rows are taken 2048 at a time, w is read once for each such group. */
 #define MORJ_MAX_TOP 32
@@ -229,16 +230,17 @@ int morj_kv8_gather(const void* codes, const float* scale, int pool_slots, const
                     void* out, long long ld_out, void* stream);
 
 /* morj_tree_attention over an 8-bit cache: the same segments, key lists, masks and head groups, K and V read as
- * code * scale. q, out: [n_q, hq, d] BF16; sm_scale > 0. A query that sees no key gets 0. Any hq / hk; d in {64, 128}; the last page
- * of a segment with no pages is ignored. Keys outside every query's view are not read; a listed key's codes must be
+ * code * scale. q, out: [n_q, hq, d] BF16; sm_scale > 0. A query that sees no key gets 0. Any hq / hk; d in {64, 128};
+ * the last page of a segment with no pages is ignored. Keys outside every query's view are not read; a listed key's codes must be
  * finite (as morj_kv8_store leaves them) where some query of the same tile does not see it. A slot outside the pool
  * sets the device error word (0x301).
  *
  * morj_tree_attention_kv8_work (host function, no device access): the call's work list from host copies of its segment
  * tables. Writes up to `cap` ints to work_host and counts[MORJ_KV8_COUNTS]: 0 tiles of few rows, 1 joins, 2 partial
  * units, 3 rows per such tile, 4 ints written, 5 tiles of 128 rows, 6 pages and 7 blocks those see, 8 list entries, 9
- * queries. With cap = 0 it writes only the counts. Segments of more than 16 rows (queries x hq / hk) run in tiles of 128: the pages they
- * see are first expanded to 16 bits in `workspace`, once per call. Long key lists of few tiles are cut into parts, whose
+ * queries. With cap = 0 it writes only the counts. Segments of at most 16 rows (queries x hq / hk), and every segment of
+ * a call whose rows see few keys together, run in tiles of 8 or 16 rows; the others in tiles of 128: the pages they see
+ * are first expanded to 16 bits in `workspace`, once per call. Long key lists of few tiles are cut into parts, whose
  * partial results go through `workspace` and are joined in a fixed order.
  * morj_tree_attention_kv8_workspace (host function): the bytes a call with these counts needs (4 per code pair of the
  * expanded pages, plus the parts; the caller's, 256-byte aligned; calls that may overlap on the device must not share

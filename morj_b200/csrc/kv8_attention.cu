@@ -4,15 +4,16 @@
 //   s_ij = sm_scale * (q_i . code_k[j]) * scale_k[block(j)],  p = softmax over the visible j,
 //   o_i  = sum_j p_ij * scale_v[block(j)] * code_v[j],        a row that sees nothing is 0.
 //
-// Codes become FP16 by one conversion for two of them (exact), so both products run as FP16 x FP16 with FP32 sums and
-// the scales stay out of the operands: K's multiplies the scores, V's the probabilities (relative to the largest V
-// scale met so far, so the products stay inside FP16 and O is kept in units of that scale). A query row is brought to
-// [1, 2) by a power of two before it is rounded to FP16, which keeps every bit of a BF16 row that matters at 2^-25 of
-// its largest element.
+// A segment's rows are its (query, head of the group) pairs of one KV head. The host sends segments of few rows to
+// rows_kernel, which converts codes where it uses them, and the others in tiles of 128 to tile_kernel, for which
+// expand_kernel converts the listed pages once. It cuts the keys of a tile into parts until the SMs are filled once; parts
+// leave (maximum, sum, O) in a workspace and combine_kernel joins them in a fixed order.
 //
-// A segment's rows are its (query, head of the group) pairs of one KV head. Segments of at most 16 rows go to
-// rows_kernel, larger ones in tiles of 128 to tile_kernel. The host cuts the keys of a tile into parts until the SMs are
-// filled once; parts leave (maximum, sum, O) in a workspace and combine_kernel joins them in a fixed order.
+// rows_kernel: codes become FP16 by one conversion for two of them (exact), so both products run as FP16 x FP16 with FP32
+// sums and the scales stay out of the operands: K's multiplies the scores, V's the probabilities (relative to the
+// largest V scale met so far, so the products stay inside FP16 and O is kept in units of that scale). A query row is
+// brought to [1, 2) by a power of two before it is rounded to FP16, which keeps every bit of a BF16 row that matters at
+// 2^-25 of its largest element. tile_kernel: K as BF16 (exact) against the queries as they are, P and V as FP16.
 #include <algorithm>
 #include <climits>
 #include <unordered_map>
@@ -135,9 +136,12 @@ MORJ_DEV float row_scale(float amax) {
 // warps has a group of 32 keys (8 KB) on its way while it works on another. Groups are taken in turn by the four warps of
 // a CTA; keys are one lane each for their page entry (two groups ahead) and scales. A group whose slots follow one
 // another comes by two TMA boxes, others are gathered by cp.async; either way the rows of K and V lie as they come,
-// 16-byte units XOR-swizzled by the key, so both products read their fragments without bank conflicts: mma.m16n8k16 leaves the order of the head dimension (q . k) and of the output columns (P V) free, and each
-// lane takes 32 (16) consecutive codes of a K row and 16 (8) of a V row for D = 128 (64). The code is kept small: unrolled over 32 keys with its loads in registers it was 16 KB, and a CTA that runs it four times spent most of its time
-// fetching instructions (9 readout rows of 1,560 keys: 41 us).
+// 16-byte units XOR-swizzled by the key, so both products read their fragments without bank conflicts: mma.m16n8k16
+// leaves the order of the head dimension (q . k) and of the output columns (P V) free, and each lane takes 32 (16)
+// consecutive codes of a K row and 16 (8) of a V row for D = 128 (64).
+// Measured: 64 single queries over 1 to 8,048 keys of 16 heads of 128, 786 MB, 130 us = 6.05 TB/s (0.92 of the measured
+// copy), 9 readout rows of 1,560 keys 19 us (latency: page entry -> codes -> five groups a warp -> join). Not kept: the
+// codes of K straight into an e4m3 mma against queries split in two codes (167 against 148 us at the time).
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int R_STAGES = 2;
 
@@ -555,11 +559,10 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
 //
 // expand_kernel: every distinct listed slot in the order the lists name them, K as BF16 (code * scale is exact there, and
 // queries are BF16), V as FP16(code * scale / ref) with the head's largest scale among them, so that probabilities can be
-// FP16 too (11 bits); a value keeps all its bits down to 2^-15 of ref. A key is used by
-// every 128-row tile that sees it: expanding costs 3 bytes of traffic per code once (35.7 M codes, the 8,704 tokens of
-// a 16-head layer, K and V), where converting in the tile loaders (built and measured) cost each tile the conversion,
-// the address arithmetic and the instruction cache: 130 us on the op-level tree (2048 + 8 x 64) against the 62 us of the
-// BF16 kernel with the same pipeline.
+// FP16 too (11 bits); a value keeps all its bits down to 2^-15 of ref. A key is used by every 128-row tile that sees it:
+// expanding costs 3 bytes of traffic per code once (35.7 M codes, the 8,704 tokens of a 16-head layer, K and V), where
+// converting in the tile loaders (built and measured) cost each tile the conversion, the address arithmetic and the
+// instruction cache: 130 us on the op-level tree (2048 + 8 x 64) against 73 now.
 // ---------------------------------------------------------------------------------------------------------------
 // A CTA takes 64 slots of a head's K or V. Three steps of loads that depend on one another (page, codes, convert), each
 // asked for at once, and many CTAs an SM: one warp's share with the lookups inline took 27 us for those 35.7 M codes.
@@ -656,6 +659,11 @@ __global__ void __launch_bounds__(E_THREADS, 12) expand_kernel(const Args a, con
 //               O / l or the part's (maximum, sum, O), staged through shared memory to store whole rows
 // The pipeline is tree_attention_kernel's (S and P double-buffered in TMEM, a K buffer free once its S is complete, a V
 // buffer once its P V is, two CTAs per SM); what it lacks there is the parts of a key range and rows that see nothing.
+// Bound by the chain of a 64-key chunk, P stored -> P V and the next S issued -> S seen -> softmax, 1,600 cycles of which
+// two are under way per CTA: 51.8 GFLOP (2048 + 8 x 64 rows, 32 heads of 128) in 63 of the call's 73 us = 820 TFLOP/s.
+// The MMAs themselves need 640 cycles a chunk (N = 64 reads shared memory for 48 of them per 16-deep step, not 32).
+// Measured and not kept: the MMAs by a whole warp with one lane's predicate, or elected (30-60% slower), P handed over in
+// halves (1-3% slower), keys cut further to even out the CTAs (5% slower, the joins cost more).
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int T_THREADS = 256;
 constexpr int T_TMEM_COLS = 256;        // S/P buffers at columns [0, 64) and [64, 128), O at [128, 128 + D)

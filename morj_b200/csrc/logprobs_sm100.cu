@@ -15,6 +15,10 @@
 // is cut to its top ones. (A sorted list per row in shared memory cost 1.0 ms of 2.1 on 540 rows with 5 alternatives: one
 // of 32 rows inserting holds up the warp.)
 //
+// Bound by the tensor cores or, for few rows, by reading w: 2,040 x 262,144 x 5,376 (5.75 TFLOP) 4.45-4.6 ms = 1,250-1,290
+// TFLOP/s under the power cap, 540 rows (five row blocks of 128, the last with 28) 1.30 ms = 1,170, 9 rows (2.82 GB)
+// 0.457 ms = 6.2 TB/s. 1 row of 4,096 logits, 17 us, is latency: three dependent steps in two launches.
+//
 // One CTA per SM: warp 0 TMA producer, warp 1 MMA issuer (tcgen05, M = 128, N = 256, two TMEM accumulators), warps 2-5
 // epilogue (thread = row). Row blocks are the fast tile index: the CTAs in flight share a few vocabulary tiles, so w
 // crosses HBM once per call of up to 2048 rows (larger calls go in chunks of 2048).
