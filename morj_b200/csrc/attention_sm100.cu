@@ -155,7 +155,6 @@ __global__ void __launch_bounds__(THREADS, 2)
                           const int* __restrict__ kv_indices, const int* __restrict__ kv_last_page_len, int n_bidir,
                           int hq, int hk, int page_size, int window, float scale_log2, const int* __restrict__ work) {
   pdl_wait();  // the previous kernel on the stream has completed
-  pdl_trigger();
   using L = Smem<D>;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = smem_u32(smem);
@@ -219,6 +218,7 @@ __global__ void __launch_bounds__(THREADS, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();  // (behind the allocation: no CTA of the next kernel may take the columns this one is waiting for)
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0 || warp == 2) {

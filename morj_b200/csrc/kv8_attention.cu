@@ -751,7 +751,6 @@ __global__ void __launch_bounds__(T_THREADS, 2)
                 const Item* __restrict__ items, const int* __restrict__ list, const uint16_t* __restrict__ k_pool,
                 const uint16_t* __restrict__ v_pool, int n_slots, const float* __restrict__ refs) {
   pdl_wait();  // the previous kernel on the stream has completed
-  pdl_trigger();
   using L = TSmem<D>;
   extern __shared__ __align__(1024) uint8_t smem[];
   const uint32_t sbase = smem_u32(smem);
@@ -794,6 +793,7 @@ __global__ void __launch_bounds__(T_THREADS, 2)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();  // (behind the allocation: no CTA of the next kernel may take the columns this one is waiting for)
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0 || warp == 2) {
