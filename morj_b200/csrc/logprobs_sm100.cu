@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(THREADS, 1)
 
 // ---- finish: two CTAs per row, one for its numbers and top alternatives, one for the given tokens -------------------
 constexpr int F_THREADS = 256;
-constexpr int POOL = 512;
+constexpr int POOL = 1024;
 
 struct Outputs {
   const int* targets;
