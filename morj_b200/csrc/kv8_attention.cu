@@ -618,7 +618,7 @@ __global__ void __launch_bounds__(E_THREADS, 12) expand_kernel(const Args a, con
     float vr = 0.f;
     for (int i = threadIdx.x; i < n_blocks; i += E_THREADS) {
       const int b = __ldg(blocks + i);
-      if ((long long)b * BLOCK < a.pool_slots) vr = fmaxf(vr, __ldg(a.vs + (size_t)b * a.hk + h));  // (else: reported)
+      if (b >= 0 && (long long)b * BLOCK < a.pool_slots) vr = fmaxf(vr, __ldg(a.vs + (size_t)b * a.hk + h));  // (else: reported)
     }
 #pragma unroll
     for (int x = 16; x > 0; x >>= 1) vr = fmaxf(vr, __shfl_xor_sync(0xffffffffu, vr, x));
@@ -1321,7 +1321,8 @@ extern "C" int morj_tree_attention_kv8_work(const int* qo_indptr_host, const int
     std::vector<int> blocks;  // 64-slot blocks that hold listed slots
     for (size_t i = 0; i < pages.size(); ++i) {
       const long long first = (long long)pages[i] * page_size;
-      for (long long b = first / kv8::BLOCK; b <= (first + used[i] - 1) / kv8::BLOCK; ++b) blocks.push_back((int)b);
+      for (long long b = first / kv8::BLOCK; b <= (first + used[i] - 1) / kv8::BLOCK; ++b)
+        blocks.push_back((int)std::min<long long>(b, INT_MAX));  // (past every pool: the kernel looks at none there)
     }
     std::sort(blocks.begin(), blocks.end());
     blocks.erase(std::unique(blocks.begin(), blocks.end()), blocks.end());

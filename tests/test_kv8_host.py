@@ -171,6 +171,17 @@ def test_long_single_rows_are_cut_and_short_ones_are_not():
     assert short[1] == 0 and short[2] == 0
 
 
+def test_a_page_far_outside_any_pool_names_no_block_inside_one():
+    # (page * page size passes 2^31 blocks: the device is to find the block outside the pool, not a wrapped one inside)
+    work, counts = nat.kv8_attention_work([0, 300], [0, 2], [3, 2**31 - 1], 0, 4, 2, 0, 4096, [904])
+    n_tiles, n_pages, n_blocks = counts[5], counts[6], counts[7]
+    assert n_tiles > 0 and n_pages == 2
+    at = (counts[0] + counts[1] + n_tiles) * ITEM + 2 * n_pages
+    blocks = work[at:at + n_blocks].astype(np.int64)
+    near = blocks[blocks < 2**25]
+    assert (blocks >= 0).all() and near.tolist() == list(range(3 * 64, 4 * 64)) and n_blocks > len(near)
+
+
 def test_attention_work_refusals():
     for args in [dict(hq=3, hk=2), dict(hq=0, hk=1), dict(page_size=0), dict(n_bidir=2), dict(n_bidir=-1)]:
         a = dict(qo_indptr=[0, 1], kv_indptr=[0, 4], kv_indices=range(4), n_bidir=0, hq=4, hk=2, window=0)
