@@ -187,6 +187,16 @@ def test_answers_scored_against_a_kept_prompt(state, kv_cache):  # noqa: F811
         m.token_logprobs(req, later, start=[1] * len(later))
 
 
+@pytest.mark.parametrize('kv_cache', ['bf16', 'e4m3'])
+def test_a_sequence_may_be_asked_for_twice(state, kv_cache):  # noqa: F811
+    c = CASES['tiny-nested']
+    m = engine(state, kv_cache=kv_cache)
+    a, b, again = m.token_logprobs(m.prepare(c['seqs'], c['label_ids']), [1, 0, 1], start=[None, None, 3], top=2)
+    assert np.array_equal(a['logprob'][2:], again['logprob']) and np.array_equal(a['top_ids'][2:], again['top_ids'])
+    x, y = m.label_logprobs(m.prepare(c['seqs'], c['label_ids']), [1, 1], top=2)
+    assert np.array_equal(x['logprob'], y['logprob']) and x['lse'] == y['lse']
+
+
 def test_scoring_refusals(state):  # noqa: F811
     c = CASES['tiny']
     m = engine(state)
