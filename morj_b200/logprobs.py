@@ -55,12 +55,14 @@ def token_logprobs(h, w, targets, top=0, softcap=0.0):
     if (n and h.stride(1) != 1) or w.stride(1) != 1:
         raise ValueError('the elements of a row must be contiguous')
     T = targets.shape[1]
-    make = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device=dev)
-    logprob, lse, entropy = make(n, T), make(n), make(n)
-    ids, lps = (make(n, top, dtype=torch.int32), make(n, top)) if top else (None, None)
+    # one allocation for the outputs (several cost a small call more than its kernels)
+    flat = torch.empty(n * (T + 2 + 2 * top), dtype=torch.float32, device=dev)
+    logprob, lse, entropy, lps, ids = flat.split_with_sizes((n * T, n, n, n * top, n * top))
+    logprob = logprob.view(n, T)
+    ids, lps = (ids.view(torch.int32).view(n, top), lps.view(n, top)) if top else (None, None)
     if n:
         nbytes = workspace_bytes(n, top)
-        ws = make(nbytes, dtype=torch.uint8)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
         with _on(dev) as s:
             nat.call('morj_token_logprobs', h.data_ptr(), h.stride(0) if n > 1 else H, n, w.data_ptr(),
                      w.stride(0) if w.shape[0] > 1 else H, w.shape[0], H, softcap, targets.data_ptr() if T else None, T,
