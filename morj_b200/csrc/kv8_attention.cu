@@ -33,9 +33,9 @@ constexpr int BN = 64;                // keys it takes at a time
 constexpr int FEW_ROWS = 16;         // segments of at most this many rows go to rows_kernel
 // ... and all segments of a call, 16 rows at a time, whose 16-row tiles see at most this many keys together (times the KV
 // heads) in at most one CTA per resident place: one launch in place of two and no expansion. 1 to 8 segments of 32 to
-// 2,048 rows, heads of 64 and 128, both ways: 6 to 16 us against 9 to 20 below it, level at twice as many, 25 against 20
-// at four times.
-constexpr long long FEW_KEYS = 32768;
+// 2,048 rows, heads of 64 and 128, both ways: 6 to 16 us against 9 to 22 up to it, level on the whole at twice as many,
+// up to 27 against 21 at four times.
+constexpr long long FEW_KEYS = 65536;
 constexpr int T_CTAS = 2, T_MIN_KEYS = 256;  // resident CTAs per SM, and the fewest keys of a part: tiles
 constexpr int R_CTAS = 3, R_MIN_KEYS = 256;  // ... few rows
 constexpr float P_SCALE = 1024.0f;   // probabilities are rounded to FP16 as 1024 p: 2^-34 is their smallest step

@@ -87,7 +87,7 @@ def test_attention_work_covers_every_row_and_key_once(spec, hq, hk, window, n_bi
     few = [[view(n, keys, s < n_bidir, window, r // G) for r in range(r0, min(r0 + 16, n * G))]
            for s, (n, keys) in enumerate(spec) for r0 in range(0, n * G, 16)]
     seen = sum(max(max(hi for _, hi in rows) - min(lo for lo, _ in rows) + 1, 0) for rows in few)
-    all_few = seen * hk <= 32768 and len(few) * hk <= 3 * 148
+    all_few = seen * hk <= 65536 and len(few) * hk <= 3 * 148
     check_work(work, counts, spec, G, window, n_bidir, kv, all_few)
     if all_few:
         return
