@@ -21,16 +21,14 @@ BLOCK = 64
 CODES = torch.float8_e4m3fn
 
 
-def _index(device):
-    device = torch.device(device)
-    return device.index if device.index is not None else torch.cuda.current_device()
-
-
 class _on:
-    """The device of a call made the current one while it launches (nothing when it already is)."""
+    """The device of a call made the current one while it launches (nothing when it already is). ValueError for tensors
+    that are not on a CUDA device: a kernel given their addresses would fault the GPU."""
 
     def __init__(self, device):
-        self.index, self.back = _index(device), None
+        if device.type != 'cuda':
+            raise ValueError(f'the tensors of a launch must be on a CUDA device, not on {device}')
+        self.index, self.back = device.index, None
 
     def __enter__(self):
         now = torch.cuda.current_device()

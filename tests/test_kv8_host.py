@@ -316,3 +316,15 @@ def test_pool_and_plan_refusals():
         kv8.tree_attention(q, pool, plan, 1.0, out=q.float())
     empty = kv8.AttentionPlan([0, 0], [0, 2], [0, 1], 4, 2, 64, device='cpu')
     assert kv8.tree_attention(q[:0], pool, empty, 1.0).shape == (0, 4, 64)
+
+
+def test_tensors_that_are_not_on_a_cuda_device_are_refused():
+    # (launched, the kernels would read host addresses)
+    pool = kv8.KV8Pool(70, 2, 64, 'cpu')
+    rows = torch.zeros(2, 2, 64, dtype=torch.bfloat16)
+    plan = kv8.AttentionPlan([0, 1], [0, 2], [0, 1], 4, 2, 64, device='cpu')
+    for bad in (lambda: kv8.store(pool, rows, rows, kv8.StorePlan([1, 2], 70, 'cpu')),
+                lambda: pool.rows(torch.zeros(3, dtype=torch.int32)),
+                lambda: kv8.tree_attention(torch.zeros(1, 4, 64, dtype=torch.bfloat16), pool, plan, 1.0)):
+        with pytest.raises(ValueError, match='must be on a CUDA device, not on cpu'):
+            bad()

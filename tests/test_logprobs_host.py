@@ -3,8 +3,10 @@ access (16 stands for an aligned pointer that is never read)."""
 import ctypes
 
 import pytest
+import torch
 
 from morj_b200 import _native as nat
+from morj_b200.logprobs import token_logprobs
 
 
 def args(**kw):
@@ -41,3 +43,10 @@ def test_nothing_to_do_and_workspace_sizes():
             nat.call('morj_token_logprobs_workspace', *bad, ctypes.byref(b))
     with pytest.raises(ValueError):
         nat.call('morj_token_logprobs_workspace', 1, 0, None)
+
+
+def test_tensors_that_are_not_on_a_cuda_device_are_refused():
+    # (launched, the kernels would read host addresses)
+    h, w = torch.zeros(2, 64, dtype=torch.bfloat16), torch.zeros(100, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match='must be on a CUDA device, not on cpu'):
+        token_logprobs(h, w, torch.zeros(2, 1, dtype=torch.int32))
