@@ -378,8 +378,9 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
     }
     const int place = i % R_STAGES;
     if (!warp_wait(bars + 8 * place, (i / R_STAGES) & 1, abort)) {
-      // (given up: what this warp asked for must land before the CTA leaves)
-      for (int x = i + 1; x < min(groups, i + R_STAGES); ++x)
+      // (given up, perhaps because another warp did: what this warp asked for, group i too, must land before the CTA
+      // writes over the rings and leaves)
+      for (int x = i; x < min(groups, i + R_STAGES); ++x)
         if (lane == 0) mbar_wait_landed(bars + 8 * (x % R_STAGES), (x / R_STAGES) & 1);
       break;
     }
@@ -813,14 +814,17 @@ __global__ void __launch_bounds__(T_THREADS, 2)
       }
       return (int)s;
     };
-    int s0 = slot(t_begin + 2 * lane), s1 = slot(t_begin + 2 * lane + 1);
-    for (int c = 0; c < n_chunks; ++c) {
+    int s0 = slot(t_begin + 2 * lane), s1 = slot(t_begin + 2 * lane + 1), c = 0;
+    for (; c < n_chunks; ++c) {
       const int b = c & 1, next = t_begin + (c + 1) * BN + 2 * lane;
       const int n0 = slot(next), n1 = slot(next + 1);
       if (c >= 2 && !warp_wait(empty + 8 * b, ((c >> 1) - 1) & 1, abort)) break;
       load_chunk<D>(base + b * L::KV_BYTES, full + 8 * b, map, is_k ? k_pool : v_pool, s0, s1, a.hk, h, lane);
       s0 = n0, s1 = n1;
     }
+    // no copy may still be in flight when the CTA exits (after a wait that ran out nobody else has seen the last ones land)
+    if (lane == 0)
+      for (int x = max(c - 2, 0); x < c; ++x) mbar_wait_landed(full + 8 * (x & 1), (x >> 1) & 1);
   } else if (warp == 1) {
     if (lane == 0) {
       constexpr uint32_t IDESC_S = idesc_bf16(T_ROWS, BN);
