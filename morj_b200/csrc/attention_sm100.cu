@@ -237,11 +237,17 @@ __global__ void __launch_bounds__(THREADS, 2)
     const uint32_t base = sbase + (is_k ? L::K_OFF : L::V_OFF);
     // a K buffer is free once the scores of the chunk two back are complete, a V buffer once its PV is
     const uint32_t full = is_k ? k_full : v_full, empty = is_k ? s_full : pv_done;
-    for (int c = 0; c < n_chunks; ++c) {
+    int c = 0;
+    for (; c < n_chunks; ++c) {
       const int b = c & 1;
       if (c >= 2 && !warp_wait(empty + 8 * b, ((c >> 1) - 1) & 1, abort)) break;
       load_chunk<D>(base + b * L::KV_BYTES, full + 8 * b, is_k ? &k_map : &v_map, is_k ? k_pool : v_pool,
                     kv_indices, sg, t_begin + c * BN, t_end, hk, h, page_size, lane);
+    }
+    // no copy may still be in flight when the CTA exits (after a wait that ran out nobody else has seen the last ones land)
+    if (lane == 0) {
+      for (int x = max(c - 2, 0); x < c; ++x) mbar_wait_landed(full + 8 * (x & 1), (x >> 1) & 1);
+      if (is_k) mbar_wait_landed(q_full, 0);
     }
   } else if (warp == 1) {
     // ---------------- MMA issuer ----------------
