@@ -146,11 +146,27 @@ def attention_work(qo_indptr, kv_indptr, n_bidir, hq, hk, window, page_size=1, k
     return buf[:2 * got]
 
 
+def host_int32(name, values):
+    """`values` as a contiguous int32 vector. ValueError where that would change one: not whole numbers, or outside int32
+    (a plain cast would turn slot 2^32 + 5 into slot 5)."""
+    import numpy as np
+    a = np.asarray(values).reshape(-1)
+    if not a.size:
+        return np.zeros(0, np.int32)
+    if a.dtype.kind not in 'iu':
+        raise ValueError(f'{name} must be integers, not {a.dtype}')
+    if a.dtype.itemsize >= 4 and a.dtype != np.int32:
+        lo, hi = int(a.min()), int(a.max())
+        if lo < -2**31 or hi >= 2**31:
+            raise ValueError(f'{name} must fit 32 bits: {lo if lo < -2**31 else hi}')
+    return np.ascontiguousarray(a, dtype=np.int32)
+
+
 def kv8_store_work(slots, pool_slots):
-    """(work list, number of touched 64-slot blocks) of an 8-bit cache store of rows 0..n-1 to `slots` (host int32;
+    """(work list, number of touched 64-slot blocks) of an 8-bit cache store of rows 0..n-1 to `slots` (host integers;
     `morj_kv8_store_work`). ValueError for a slot outside the pool or given twice."""
     import numpy as np
-    s = np.ascontiguousarray(slots, dtype=np.int32).reshape(-1)
+    s = host_int32('slots', slots)
     buf = np.zeros(5 * len(s) + 2, dtype=np.int32)
     n = lib().morj_kv8_store_work(s.ctypes.data_as(IP), len(s), pool_slots, buf.ctypes.data_as(IP), len(buf))
     if n < 0:
@@ -165,8 +181,9 @@ def kv8_attention_work(qo_indptr, kv_indptr, kv_indices, n_bidir, hq, hk, window
     """(work list, counts) of an attention call over an 8-bit cache, from host copies of its segment tables
     (`morj_tree_attention_kv8_work`). `counts` is the ctypes array the call takes."""
     import numpy as np
-    qo, kv, idx = (np.ascontiguousarray(a, dtype=np.int32) for a in (qo_indptr, kv_indptr, kv_indices))
-    last = None if kv_last_page_len is None else np.ascontiguousarray(kv_last_page_len, dtype=np.int32)
+    qo, kv, idx = (host_int32(name, a) for name, a in (('qo_indptr', qo_indptr), ('kv_indptr', kv_indptr),
+                                                   ('kv_indices', kv_indices)))
+    last = None if kv_last_page_len is None else host_int32('kv_last_page_len', kv_last_page_len)
     if len(idx) < kv[-1]:
         raise ValueError(f'{len(idx)} list entries, kv_indptr ends at {kv[-1]}')
     counts = KV8_COUNTS()

@@ -163,12 +163,13 @@ class AttentionPlan:
 
     def __init__(self, qo_indptr, kv_indptr, kv_indices, hq, hk, d, page_size=1, kv_last_page_len=None, window=0,
                  n_bidir=0, device='cuda'):
-        qo, kv = (np.ascontiguousarray(x, dtype=np.int32).reshape(-1) for x in (qo_indptr, kv_indptr))
-        if len(qo) < 1 or len(qo) != len(kv) or qo[0] != 0 or kv[0] < 0 or len(np.asarray(kv_indices)) < kv[-1]:
+        qo, kv = nat.host_int32('qo_indptr', qo_indptr), nat.host_int32('kv_indptr', kv_indptr)
+        kv_indices = nat.host_int32('kv_indices', kv_indices)
+        if len(qo) < 1 or len(qo) != len(kv) or qo[0] != 0 or kv[0] < 0 or len(kv_indices) < kv[-1]:
             raise ValueError('qo_indptr and kv_indptr must have one entry per segment and one more, within kv_indices')
         if d not in (64, 128):
             raise ValueError(f'head_dim {d} unsupported (64, 128)')
-        last = None if kv_last_page_len is None else np.ascontiguousarray(kv_last_page_len, dtype=np.int32)
+        last = None if kv_last_page_len is None else nat.host_int32('kv_last_page_len', kv_last_page_len)
         if last is not None and (len(last) != len(qo) - 1 or (last < 0).any() or (last > page_size).any()):
             raise ValueError('kv_last_page_len must have one entry in [0, page_size] per segment')
         work, self.counts = nat.kv8_attention_work(qo, kv, kv_indices, n_bidir, hq, hk, window, page_size, last)

@@ -328,3 +328,29 @@ def test_tensors_that_are_not_on_a_cuda_device_are_refused():
                 lambda: kv8.tree_attention(torch.zeros(1, 4, 64, dtype=torch.bfloat16), pool, plan, 1.0)):
         with pytest.raises(ValueError, match='must be on a CUDA device, not on cpu'):
             bad()
+
+
+@pytest.mark.parametrize('bad', [2**32 + 5, -2**32 + 5, 2**31])
+def test_host_indices_past_32_bits_are_refused(bad):
+    # (cast, 2^32 + 5 would be slot 5: another token's K/V overwritten, or read)
+    for slots in (np.array([1, bad]), [1, bad]):
+        with pytest.raises(ValueError, match='fit 32 bits'):
+            nat.kv8_store_work(slots, 64)
+        with pytest.raises(ValueError, match='fit 32 bits'):
+            kv8.StorePlan(slots, 64, 'cpu')
+    good = dict(qo_indptr=[0, 1], kv_indptr=[0, 2], kv_indices=[0, 1], kv_last_page_len=[1])
+    for name in good:
+        args = {**good, name: np.array(good[name][:-1] + [bad])}
+        with pytest.raises(ValueError, match=f'{name} must fit 32 bits'):
+            kv8.AttentionPlan(**args, hq=4, hk=2, d=64, device='cpu')
+        with pytest.raises(ValueError, match=f'{name} must fit 32 bits'):
+            nat.kv8_attention_work(**args, n_bidir=0, hq=4, hk=2, window=0)
+
+
+def test_host_indices_that_are_not_whole_numbers_are_refused():
+    with pytest.raises(ValueError, match='slots must be integers'):
+        kv8.StorePlan([1.5, 2.0], 64, 'cpu')
+    with pytest.raises(ValueError, match='kv_indices must be integers'):
+        kv8.AttentionPlan([0, 1], [0, 2], np.array([0.0, 1.0]), 4, 2, 64, device='cpu')
+    work, blocks = nat.kv8_store_work(np.array([70, 3], np.uint64), 128)
+    assert blocks == 2 and work[6:].tolist() == [3, 1, 70, 0]
