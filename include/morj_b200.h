@@ -231,8 +231,9 @@ int morj_kv8_gather(const void* codes, const float* scale, int pool_slots, const
 
 /* morj_tree_attention over an 8-bit cache: the same segments, key lists, masks and head groups, K and V read as
  * code * scale. q, out: [n_q, hq, d] BF16; sm_scale > 0. A query that sees no key gets 0. Any hq / hk; d in {64, 128};
- * the last page of a segment with no pages is ignored. Keys outside every query's view are not read; a listed key's codes must be
- * finite (as morj_kv8_store leaves them) where some query of the same tile does not see it. A slot outside the pool
+ * the last page of a segment with no pages is ignored. Slots that no query sees may hold anything (of a page that some
+ * query sees, the slots before and between may be read, and take no part); where a query of a tile of rows sees a key and
+ * another one does not, the key's codes and scales must be finite (as morj_kv8_store leaves them). A slot outside the pool
  * sets the device error word (0x301).
  *
  * morj_tree_attention_kv8_work (host function, no device access): the call's work list from host copies of its segment

@@ -593,7 +593,7 @@ __global__ void __launch_bounds__(E_THREADS, 12) expand_kernel(const Args a, con
     int slot = -1;
     if (t < n_slots) {
       const int p = a.page.of(t), at = t - p * a.page.d;
-      const int2 page = __ldg(pages + p);  // (page of the pool, its slots that are listed: the rest is zeros)
+      const int2 page = __ldg(pages + p);  // (page of the pool, its slots up to the last one seen: the rest is zeros)
       const long long s = (long long)page.x * a.page.d + at;
       if (at < page.y) {
         if (s < a.pool_slots)
@@ -715,16 +715,17 @@ MORJ_DEV float max3f(float a, float b, float c) {
 }
 
 // One loader warp fills buffer `dst` with the expanded rows of keys [t0, t0 + BN) and completes `full`. s0, s1: the
-// expanded slots of this lane's keys t0 + 2 lane and the next, -1 outside the part. Where the slots inside it follow one
-// another, the box around them is loaded: its other rows are masked keys, and finite (listed slots, zeros past a page's
-// listed ones or past the end).
+// expanded slots of this lane's keys t0 + 2 lane and the next, -1 outside the part. Where the slots follow one another the
+// box around them is loaded. Of K also where only those inside the part do: the box's other rows are keys the softmax
+// masks, whatever they hold. Of V only when the whole chunk is inside: the product with a masked key's probability 0 is NaN
+// where its value is, so the first and last chunk of a part are gathered, with zeros outside.
 template <int D>
-MORJ_DEV void load_chunk(uint32_t dst, uint32_t full, const CUtensorMap* map, const uint16_t* __restrict__ pool, int s0,
-                         int s1, int hk, int h, int lane) {
+MORJ_DEV void load_chunk(uint32_t dst, uint32_t full, const CUtensorMap* map, const uint16_t* __restrict__ pool, bool whole,
+                         int s0, int s1, int hk, int h, int lane) {
   const unsigned any = __ballot_sync(0xffffffffu, s0 >= 0 || s1 >= 0);
   const int mine = s0 >= 0 ? s0 - 2 * lane : s1 - 2 * lane - 1;  // slot of key t0 if the run holds
   const int first = __shfl_sync(0xffffffffu, mine, any ? __ffs(any) - 1 : 0);
-  if (__all_sync(0xffffffffu, (s0 < 0 || s0 == first + 2 * lane) && (s1 < 0 || s1 == first + 2 * lane + 1))) {
+  if (__all_sync(0xffffffffu, (s0 < 0 ? !whole : s0 == first + 2 * lane) && (s1 < 0 ? !whole : s1 == first + 2 * lane + 1))) {
     if (lane == 0) {
       mbar_arrive_expect_tx(full, BN * D * 2);
 #pragma unroll
@@ -819,7 +820,8 @@ __global__ void __launch_bounds__(T_THREADS, 2)
       const int b = c & 1, next = t_begin + (c + 1) * BN + 2 * lane;
       const int n0 = slot(next), n1 = slot(next + 1);
       if (c >= 2 && !warp_wait(empty + 8 * b, ((c >> 1) - 1) & 1, abort)) break;
-      load_chunk<D>(base + b * L::KV_BYTES, full + 8 * b, map, is_k ? k_pool : v_pool, s0, s1, a.hk, h, lane);
+      load_chunk<D>(base + b * L::KV_BYTES, full + 8 * b, map, is_k ? k_pool : v_pool, !is_k, s0, s1, a.hk, h,
+                    lane);
       s0 = n0, s1 = n1;
     }
     // no copy may still be in flight when the CTA exits (after a wait that ran out nobody else has seen the last ones land)

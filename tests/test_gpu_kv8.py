@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 import torch
 
-from kv8_cases import (BLOCK, attention_ref, e4m3, make_segments, pool_rows, store_ref)
+from kv8_cases import (BLOCK, attention_ref, e4m3, fill, make_segments, pool_rows, segments, store_ref)
 from morj_b200 import _native as nat
 from morj_b200 import kv8
 
@@ -518,3 +518,57 @@ def test_a_rounded_value_is_the_nearest_code():
     check_store(pool, x, x, np.arange(n) * 64)
     assert (pool.k_scale == 1).all()
     assert torch.equal(pool.k.double()[::64][:, 0], e4m3(x[:, 0].double()))
+
+
+# ---- what no query, or another tile's queries only, may see -----------------------------------------------------------
+
+def hidden_as_nan(good, qo, kv, indices, last, page, window):
+    """A copy of the pool whose codes and scales are NaN except in the slots that some query sees (a block's scale stays
+    where one of its slots does)."""
+    pool = kv8.KV8Pool(good.slots, good.heads, good.head_dim, DEV)
+    for t in (pool.k, pool.v):
+        t.view(torch.uint8).fill_(0x7f)
+    pool.scales.fill_(float('nan'))
+    for s, (_, n, keys) in enumerate(segments(qo, kv, last, page)):
+        pages = indices[kv[s]:kv[s + 1]].astype(np.int64)
+        at = (pages[:, None] * page + np.arange(page)).reshape(-1)[:keys]
+        at = torch.as_tensor(at[max(0, keys - n - (window - 1)) if window else 0:], device=DEV)
+        for new, old in ((pool.k, good.k), (pool.v, good.v)):
+            new.view(torch.uint8)[at] = old.view(torch.uint8)[at]
+        for new, old in ((pool.k_scale, good.k_scale), (pool.v_scale, good.v_scale)):
+            new[at // BLOCK] = old[at // BLOCK]
+    return pool
+
+
+@pytest.mark.parametrize('d', [64, 128])
+@pytest.mark.parametrize('spec,window,page', [([(300, 4000), (200, 1111)], 700, 16), ([(300, 4000), (200, 1111)], 701, 64),
+                                              ([(500, 2000), (1, 900), (400, 3333)], 333, 256), ([(2000, 6200)], 65, 1000),
+                                              ([(300, 4000), (200, 1111)], 700, 1)])
+def test_attention_of_many_rows_ignores_a_window_s_first_page_before_the_window(spec, window, page, d):
+    rng, g = np.random.default_rng(page), torch.Generator(device=DEV).manual_seed(page)
+    qo, kv, indices, last, slots = make_segments(rng, spec, page)
+    good = kv8.KV8Pool(slots, 2, d, DEV)
+    fill(good, pool_rows(g, slots, 2, d, DEV), pool_rows(g, slots, 2, d, DEV), np.arange(slots), kv8.store, kv8.StorePlan)
+    pool = hidden_as_nan(good, qo, kv, indices, last, page, window)
+    q = torch.randn(int(qo[-1]), 4, d, generator=g, device=DEV).to(torch.bfloat16)
+    plan = kv8.AttentionPlan(qo, kv, indices, 4, 2, d, page_size=page, kv_last_page_len=last, window=window, device=DEV)
+    assert plan.counts[5] > 0
+    got = kv8.tree_attention(q, pool, plan, d ** -0.5)
+    want, _ = check_attention(good, q, qo, kv, indices, last, page, window, 0, d ** -0.5)
+    assert torch.equal(got, want)
+
+
+def test_attention_of_many_rows_keeps_another_segment_s_nan_out():
+    # two segments list the same pages; the shorter one ends inside a page whose further slots hold NaN
+    g = torch.Generator(device=DEV).manual_seed(12)
+    good = random_pool(g, 2048, 2, 64)
+    lists = np.random.default_rng(12).permutation(32)
+    qo, kv, indices, last = [0, 400, 900], [0, 24, 48], np.concatenate([lists[:24], lists[:24]]), [10, 64]
+    q = torch.randn(900, 4, 64, generator=g, device=DEV).to(torch.bfloat16)
+    plan = kv8.AttentionPlan(qo, kv, indices, 4, 2, 64, page_size=64, kv_last_page_len=last, device=DEV)
+    assert plan.counts[5] > 0
+    want = kv8.tree_attention(q, good, plan, 0.125)
+    good.k.view(torch.uint8)[int(lists[23]) * 64 + 10:int(lists[23]) * 64 + 64] = 0x7f
+    good.v.view(torch.uint8)[int(lists[23]) * 64 + 10:int(lists[23]) * 64 + 64] = 0x7f
+    got = kv8.tree_attention(q, good, plan, 0.125)
+    assert torch.equal(got[:400], want[:400]) and torch.isnan(got[-1]).all()
