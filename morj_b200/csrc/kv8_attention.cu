@@ -13,7 +13,8 @@
 // sums and the scales stay out of the operands: K's multiplies the scores, V's the probabilities (relative to the
 // largest V scale met so far, so the products stay inside FP16 and O is kept in units of that scale). A query row is
 // brought to [1, 2) by a power of two before it is rounded to FP16, which keeps every bit of a BF16 row that matters at
-// 2^-25 of its largest element. tile_kernel: K as BF16 (exact) against the queries as they are, P and V as FP16.
+// 2^-25 of its largest element. tile_kernel: K as BF16 (exact) against the queries as they are, P and V as FP16, V's scales
+// in V or, where a head's lie far apart, in P.
 #include <algorithm>
 #include <climits>
 #include <unordered_map>
@@ -560,7 +561,10 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
 //
 // expand_kernel: every distinct listed slot in the order the lists name them, K as BF16 (code * scale is exact there, and
 // queries are BF16), V as FP16(code * scale / ref) with the head's largest scale among them, so that probabilities can be
-// FP16 too (11 bits); a value keeps all its bits down to 2^-15 of ref. A key is used by every 128-row tile that sees it:
+// FP16 too (11 bits). That is exact while the head's scales lie within 2^15 of one another (the smallest code is 2^-9, the
+// smallest FP16 2^-24). Where they do not, V is expanded as its codes, and tile_kernel takes each key's scale into its
+// probability, relative to the largest one its tile has met, so that what other segments hold moves no bit of a segment's
+// result. A key is used by every 128-row tile that sees it:
 // expanding costs 3 bytes of traffic per code once (35.7 M codes, the 8,704 tokens of a 16-head layer, K and V), where
 // converting in the tile loaders (built and measured) cost each tile the conversion, the address arithmetic and the
 // instruction cache: 130 us on the op-level tree (2048 + 8 x 64) against 73 now.
@@ -568,6 +572,8 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
 // A CTA takes 64 slots of a head's K or V. Three steps of loads that depend on one another (page, codes, convert), each
 // asked for at once, and many CTAs an SM: one warp's share with the lookups inline took 27 us for those 35.7 M codes.
 constexpr int E_THREADS = 128;
+constexpr float EXACT_SPREAD = 32768.f;  // scales of a head within this factor: V relative to the largest is exact in FP16
+constexpr float SCALES_APART = -1.f;     // a head's reference where they are not: V is its codes
 
 template <int D>
 __global__ void __launch_bounds__(E_THREADS, 12) expand_kernel(const Args a, const int2* __restrict__ pages,
@@ -581,7 +587,7 @@ __global__ void __launch_bounds__(E_THREADS, 12) expand_kernel(const Args a, con
   constexpr int N = BN / ROWS;
   __shared__ int slots[BN];               // of the pool; -1: nothing listed (zeros)
   __shared__ float factor[BN];
-  __shared__ float red[E_THREADS / 32];
+  __shared__ float red[E_THREADS / 32], low[E_THREADS / 32];
   const int h = blockIdx.y, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
   const bool is_v = blockIdx.z;
   const int t0 = blockIdx.x * BN, part = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
@@ -616,18 +622,30 @@ __global__ void __launch_bounds__(E_THREADS, 12) expand_kernel(const Args a, con
   }
   float inv = 1.f;
   if (is_v) {  // V's largest scale of the head (every CTA of the head finds the same)
-    float vr = 0.f;
+    float vr = 0.f, vm = INFINITY;  // ... and its smallest (0 and NaN mark blocks nothing was stored in)
     for (int i = threadIdx.x; i < n_blocks; i += E_THREADS) {
       const int b = __ldg(blocks + i);
-      if (b >= 0 && (long long)b * BLOCK < a.pool_slots) vr = fmaxf(vr, __ldg(a.vs + (size_t)b * a.hk + h));  // (else: reported)
+      if (b >= 0 && (long long)b * BLOCK < a.pool_slots) {  // (else: reported)
+        const float x = __ldg(a.vs + (size_t)b * a.hk + h);
+        vr = fmaxf(vr, x);
+        if (x > 0.f) vm = fminf(vm, x);
+      }
     }
 #pragma unroll
-    for (int x = 16; x > 0; x >>= 1) vr = fmaxf(vr, __shfl_xor_sync(0xffffffffu, vr, x));
-    if (lane == 0) red[warp] = vr;
+    for (int x = 16; x > 0; x >>= 1) {
+      vr = fmaxf(vr, __shfl_xor_sync(0xffffffffu, vr, x));
+      vm = fminf(vm, __shfl_xor_sync(0xffffffffu, vm, x));
+    }
+    if (lane == 0) red[warp] = vr, low[warp] = vm;
     __syncthreads();
     vr = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    if (blockIdx.x == 0 && threadIdx.x == 0) refs[h] = vr;
-    if (vr > 0.f) inv = 1.f / vr;
+    vm = fminf(fminf(low[0], low[1]), fminf(low[2], low[3]));
+    const bool apart = vr > vm * EXACT_SPREAD;
+    if (blockIdx.x == 0 && threadIdx.x == 0) refs[h] = apart ? SCALES_APART : vr;
+    if (apart)
+      sc = 1.f;
+    else if (vr > 0.f)
+      inv = 1.f / vr;
   }
   if (threadIdx.x < BN) factor[threadIdx.x] = sc * inv;
   __syncthreads();
@@ -747,11 +765,148 @@ MORJ_DEV void load_chunk(uint32_t dst, uint32_t full, const CUtensorMap* map, co
   if (lane == 0) mbar_arrive(full);
 }
 
+// The softmax warps' walk over a part's chunks: a thread's row, its visible keys [lo, hi], running maximum m_used and sum
+// l_run (in units of 2^-T_P_LOG2, as P and O). False when a wait ran out.
+// APART: the V scales of the head lie far apart and V is its codes: each probability is multiplied by its key's V scale
+// relative to `vr`, the largest one the part has met so far, in units of which O is.
+struct ChunkSide {
+  uint32_t t_lane, s_full, p_full, pv_done;
+  int t_begin, t0, t_stop, n_chunks, lo, hi;
+  float scale;  // scores times it are in the log2 domain (> 0)
+  volatile int* abort;
+};
+template <int D, bool APART>
+MORJ_DEV bool softmax_chunks(const Args& a, int h, const int2* pages, const int* places, int n_slots, const ChunkSide& x,
+                             float& m_used, float& l_run, float& vr) {
+  const int lane = threadIdx.x % 32;
+  const float scale = x.scale;
+  auto scale_of = [&](int t) {  // V's of key t, 0 outside the part
+    if (t < x.t0 || t >= x.t_stop) return 0.f;
+    const int place = __ldg(places + a.page.of(t));
+    if ((long long)place * a.page.d >= n_slots) return 0.f;  // (reported by the loaders, as is a slot outside the pool)
+    const long long s = slot_of(a, __ldg(pages + place).x, t);
+    return s < a.pool_slots ? __ldg(a.vs + (size_t)(s >> BLOCK_SHIFT) * a.hk + h) : 0.f;
+  };
+  for (int c = 0; c < x.n_chunks; ++c) {
+    const int b = c & 1;
+    if (!warp_wait(x.s_full + 8 * b, (c >> 1) & 1, x.abort)) return false;
+    tc_fence_after();
+    uint32_t sr[2][32];
+    tmem_ld32(x.t_lane + b * BN, sr[0]);
+    tmem_ld32(x.t_lane + b * BN + 32, sr[1]);
+    tmem_wait_ld();
+    const int t0 = x.t_begin + c * BN;
+    // (the maximum and the sum run over 8 independent partials: short dependency chains)
+    float m8[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m8[i] = -INFINITY;
+    if (__all_sync(0xffffffffu, t0 >= x.lo && t0 + BN - 1 <= x.hi)) {
+#pragma unroll
+      for (int j = 0; j < BN; j += 2)
+        m8[(j >> 1) & 7] = max3f(m8[(j >> 1) & 7], __uint_as_float(sr[j >> 5][j & 31]),
+                                 __uint_as_float(sr[(j + 1) >> 5][(j + 1) & 31]));
+    } else {
+#pragma unroll
+      for (int j = 0; j < BN; ++j) {
+        const int t = t0 + j;
+        const float v = (t >= x.lo && t <= x.hi) ? __uint_as_float(sr[j >> 5][j & 31]) : -INFINITY;
+        sr[j >> 5][j & 31] = __float_as_uint(v);
+        m8[j & 7] = fmaxf(m8[j & 7], v);
+      }
+    }
+    const float mx = scale * fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
+                                   fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])));
+    float alpha = 1.f;
+    if (mx > m_used + T_RESCALE_LOG2 || m_used == -INFINITY) {
+      if (m_used != -INFINITY) alpha = fast_exp2(m_used - mx);
+      if (mx != -INFINITY) m_used = mx;
+    }
+    l_run *= alpha;
+    float f0 = 1.f, f1 = 1.f;  // APART: V scales of keys t0 + lane and t0 + 32 + lane relative to vr
+    if constexpr (APART) {
+      f0 = scale_of(t0 + lane), f1 = scale_of(t0 + 32 + lane);
+      // (as unsigned bits a NaN is the largest)
+      const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, max(__float_as_uint(f0), __float_as_uint(f1))));
+      if (!(most <= vr)) {
+        alpha *= vr / most;  // (l_run is past it)
+        vr = most;
+      }
+      const float inv = vr != 0.f ? 1.f / vr : 0.f;
+      f0 *= inv, f1 *= inv;
+    }
+    // exp2(-inf) = 0 for masked keys; a row with no visible key yet keeps m_used = -inf and p = 0
+    const float shift = m_used == -INFINITY ? 0.f : T_P_LOG2 - m_used;
+    // scores in pairs: one packed FMA scales and shifts two of them, one packed add sums two probabilities
+    const uint64_t scale2 = f2_pack(scale, scale), shift2 = f2_pack(shift, shift);
+    uint64_t s4[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s4[i] = f2_pack(0.f, 0.f);
+    uint32_t pk[BN / 2];
+    if constexpr (!APART) {
+#pragma unroll
+      for (int j = 0; j < BN; j += 2) {
+        float y0, y1;
+        f2_unpack(f2_fma(f2_bits(sr[j >> 5][j & 31], sr[(j + 1) >> 5][(j + 1) & 31]), scale2, shift2), y0, y1);
+        const float p0 = fast_exp2(y0), p1 = fast_exp2(y1);
+        s4[(j >> 1) & 3] = f2_add(s4[(j >> 1) & 3], f2_pack(p0, p1));
+        pk[j / 2] = pack_f16x2(p0, p1);
+      }
+    } else {  // (the sum takes p, the product p times its key's scale)
+#pragma unroll
+      for (int j = 0; j < BN; j += 2) {
+        const float p0 = fast_exp2(fmaf(__uint_as_float(sr[j >> 5][j & 31]), scale, shift));
+        const float p1 = fast_exp2(fmaf(__uint_as_float(sr[(j + 1) >> 5][(j + 1) & 31]), scale, shift));
+        s4[(j >> 1) & 3] = f2_add(s4[(j >> 1) & 3], f2_pack(p0, p1));
+        const float f = j < 32 ? f0 : f1;
+        pk[j / 2] = pack_f16x2(p0 * __shfl_sync(0xffffffffu, f, j & 31), p1 * __shfl_sync(0xffffffffu, f, (j + 1) & 31));
+      }
+    }
+    float sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      float u, v;
+      f2_unpack(s4[i], u, v);
+      sum += u + v;
+    }
+    l_run += sum;
+    // a rescale of O waits until the previous chunk's PV has completed (the next one needs this chunk's P)
+    if (c >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
+      if (!warp_wait(x.pv_done + 8 * (b ^ 1), ((c - 1) >> 1) & 1, x.abort)) return false;
+      tc_fence_after();
+#pragma unroll 1
+      for (int col = 0; col < D; col += 32) {
+        uint32_t o[32];
+        tmem_ld32(x.t_lane + 128 + col, o);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+        tmem_st32(x.t_lane + 128 + col, o);
+      }
+    }
+    tmem_st32(x.t_lane + b * BN, pk);  // P_c over the first 32 columns of S_c
+    tmem_wait_st();
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(x.p_full + 8 * b);
+  }
+  return true;
+}
+// (A call of its own costs the usual walk 1.5%; inlined, its code and registers cost it 3-6%. Static, so that it keeps to its
+// callers' 128 registers.)
+template <int D>
+static __device__ __noinline__ bool softmax_chunks_apart(const Args& a, int h, const int2* pages, const int* places,
+                                                         int n_slots, const ChunkSide& x, float& m_used, float& l_run,
+                                                         float& vr) {
+  return softmax_chunks<D, true>(a, h, pages, places, n_slots, x, m_used, l_run, vr);
+}
+
 template <int D>
 __global__ void __launch_bounds__(T_THREADS, 2)
-    tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const Args a,
-                const Item* __restrict__ items, const int* __restrict__ list, const uint16_t* __restrict__ k_pool,
-                const uint16_t* __restrict__ v_pool, int n_slots, const float* __restrict__ refs) {
+    tile_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+                const __grid_constant__ Args a,
+                const Item* __restrict__ items, const int2* __restrict__ pages, const int* __restrict__ list,
+                const uint16_t* __restrict__ k_pool, const uint16_t* __restrict__ v_pool, int n_slots,
+                const float* __restrict__ refs) {
   pdl_wait();  // the previous kernel on the stream has completed
   using L = TSmem<D>;
   extern __shared__ __align__(1024) uint8_t smem[];
@@ -805,10 +960,10 @@ __global__ void __launch_bounds__(T_THREADS, 2)
     const uint32_t base = sbase + (is_k ? L::K_OFF : L::V_OFF);
     // a K buffer is free once the scores of the chunk two back are complete, a V buffer once its P V is
     const uint32_t full = is_k ? k_full : v_full, empty = is_k ? s_full : pv_done;
-    const int* pages = list + it.kv_base;
+    const int* places = list + it.kv_base;
     auto slot = [&](int t) {  // expanded slot of key t, -1 outside the part
       if (t < it.t0 || t >= t_stop) return -1;
-      const long long s = slot_of(a, __ldg(pages + a.page.of(t)), t);
+      const long long s = slot_of(a, __ldg(places + a.page.of(t)), t);
       if (s < 0 || s >= n_slots) {
         report(kErrBadIndex);
         return -1;
@@ -892,100 +1047,18 @@ __global__ void __launch_bounds__(T_THREADS, 2)
     const int r = (warp & 3) * 32 + lane, row = it.r0 + r, qi = a.group.of(row);
     const uint32_t t_lane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const bool row_ok = row < n_rows;
-    const float vr = refs ? __ldg(refs + h) : 0.f;
-    const float scale = a.scale_log2;  // scores times it are in the log2 domain (> 0)
+    float vr = refs ? __ldg(refs + h) : 0.f;
+    const bool apart = vr == SCALES_APART;
+    if (apart) vr = 0.f;  // the largest V scale met so far: O is in units of it
     int lo = 1, hi = 0;  // visible key positions [lo, hi] of this part
     if (row_ok) {
       visible(it.q_len, it.kv_len, bidir, a.window, qi, &lo, &hi);
       lo = max(lo, it.t0), hi = min(hi, t_stop - 1);
     }
-    float m_used = -INFINITY, l_run = 0.f;  // l_run in units of 2^-T_P_LOG2, as P and O
-    bool ok = true;
-    for (int c = 0; c < n_chunks; ++c) {
-      const int b = c & 1;
-      if (!warp_wait(s_full + 8 * b, (c >> 1) & 1, abort)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      uint32_t sr[2][32];
-      tmem_ld32(t_lane + b * BN, sr[0]);
-      tmem_ld32(t_lane + b * BN + 32, sr[1]);
-      tmem_wait_ld();
-      const int t0 = t_begin + c * BN;
-      // (the maximum and the sum run over 8 independent partials: short dependency chains)
-      float m8[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i) m8[i] = -INFINITY;
-      if (__all_sync(0xffffffffu, t0 >= lo && t0 + BN - 1 <= hi)) {
-#pragma unroll
-        for (int j = 0; j < BN; j += 2)
-          m8[(j >> 1) & 7] = max3f(m8[(j >> 1) & 7], __uint_as_float(sr[j >> 5][j & 31]),
-                                   __uint_as_float(sr[(j + 1) >> 5][(j + 1) & 31]));
-      } else {
-#pragma unroll
-        for (int j = 0; j < BN; ++j) {
-          const int t = t0 + j;
-          const float v = (t >= lo && t <= hi) ? __uint_as_float(sr[j >> 5][j & 31]) : -INFINITY;
-          sr[j >> 5][j & 31] = __float_as_uint(v);
-          m8[j & 7] = fmaxf(m8[j & 7], v);
-        }
-      }
-      const float mx = scale * fmaxf(fmaxf(fmaxf(m8[0], m8[1]), fmaxf(m8[2], m8[3])),
-                                     fmaxf(fmaxf(m8[4], m8[5]), fmaxf(m8[6], m8[7])));
-      float alpha = 1.f;
-      if (mx > m_used + T_RESCALE_LOG2 || m_used == -INFINITY) {
-        if (m_used != -INFINITY) alpha = fast_exp2(m_used - mx);
-        if (mx != -INFINITY) m_used = mx;
-      }
-      l_run *= alpha;
-      // exp2(-inf) = 0 for masked keys; a row with no visible key yet keeps m_used = -inf and p = 0
-      const float shift = m_used == -INFINITY ? 0.f : T_P_LOG2 - m_used;
-      // scores in pairs: one packed FMA scales and shifts two of them, one packed add sums two probabilities
-      const uint64_t scale2 = f2_pack(scale, scale), shift2 = f2_pack(shift, shift);
-      uint64_t s4[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s4[i] = f2_pack(0.f, 0.f);
-      uint32_t pk[BN / 2];
-#pragma unroll
-      for (int j = 0; j < BN; j += 2) {
-        float x0, x1;
-        f2_unpack(f2_fma(f2_bits(sr[j >> 5][j & 31], sr[(j + 1) >> 5][(j + 1) & 31]), scale2, shift2), x0, x1);
-        const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-        s4[(j >> 1) & 3] = f2_add(s4[(j >> 1) & 3], f2_pack(p0, p1));
-        pk[j / 2] = pack_f16x2(p0, p1);
-      }
-      float sum = 0.f;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x, y;
-        f2_unpack(s4[i], x, y);
-        sum += x + y;
-      }
-      l_run += sum;
-      // a rescale of O waits until the previous chunk's PV has completed (the next one needs this chunk's P)
-      if (c >= 1 && __any_sync(0xffffffffu, alpha != 1.f)) {
-        if (!warp_wait(pv_done + 8 * (b ^ 1), ((c - 1) >> 1) & 1, abort)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-#pragma unroll 1
-        for (int col = 0; col < D; col += 32) {
-          uint32_t o[32];
-          tmem_ld32(t_lane + 128 + col, o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-          tmem_st32(t_lane + 128 + col, o);
-        }
-      }
-      tmem_st32(t_lane + b * BN, pk);  // P_c over the first 32 columns of S_c
-      tmem_wait_st();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(p_full + 8 * b);
-    }
+    const ChunkSide side{t_lane, s_full, p_full, pv_done, t_begin, it.t0, t_stop, n_chunks, lo, hi, a.scale_log2, abort};
+    float m_used = -INFINITY, l_run = 0.f;
+    const bool ok = apart ? softmax_chunks_apart<D>(a, h, pages, list + it.kv_base, n_slots, side, m_used, l_run, vr)
+                          : softmax_chunks<D, false>(a, h, nullptr, nullptr, 0, side, m_used, l_run, vr);
     if (ok && (n_chunks == 0 || warp_wait(pv_done + 8 * ((n_chunks - 1) & 1), ((n_chunks - 1) >> 1) & 1, abort))) {
       tc_fence_after();
       // A finished row: O / l times V's reference; a part: (maximum, sum, O in units of the values). The warp's 32 rows
@@ -1166,7 +1239,8 @@ static int launch(Args a, const int* counts, const int* work, char* ws, cudaStre
       refs = nullptr;
     if (st) return st;
     st = launch_pdl("tile_kernel", tile_kernel<D>, dim3((unsigned)n_tiles * a.hk), dim3(T_THREADS), TSmem<D>::TOTAL, s,
-                    km, vm, a, items, list, (const uint16_t*)kx, (const uint16_t*)vx, n_slots, (const float*)refs);
+                    km, vm, a, items, reinterpret_cast<const int2*>(pages), list, (const uint16_t*)kx, (const uint16_t*)vx,
+                    n_slots, (const float*)refs);
     if (st) return st;
     items += n_tiles;
   }

@@ -572,3 +572,58 @@ def test_attention_of_many_rows_keeps_another_segment_s_nan_out():
     good.v.view(torch.uint8)[int(lists[23]) * 64 + 10:int(lists[23]) * 64 + 64] = 0x7f
     got = kv8.tree_attention(q, good, plan, 0.125)
     assert torch.equal(got[:400], want[:400]) and torch.isnan(got[-1]).all()
+
+
+# ---- V scales of a call further apart than one FP16 range -------------------------------------------------------------
+
+def scaled_segments(spec, gains, page, d, seed):
+    """Segments over private pages, the V rows of segment s times 2^gains[s] in head 1 (head 0 stays as it is)."""
+    rng, g = np.random.default_rng(seed), torch.Generator(device=DEV).manual_seed(seed)
+    qo, kv, indices, last, slots = make_segments(rng, spec, page)
+    k, v = pool_rows(g, slots, 2, d, DEV), pool_rows(g, slots, 2, d, DEV)
+    for s, gain in enumerate(gains):
+        pages = torch.as_tensor(indices[kv[s]:kv[s + 1]].astype(np.int64), device=DEV)
+        at = (pages[:, None] * page + torch.arange(page, device=DEV)).reshape(-1)
+        v[at, 1] = (v[at, 1].float() * 2.0 ** gain).to(torch.bfloat16)
+    pool = kv8.KV8Pool(slots, 2, d, DEV)
+    fill(pool, k, v, np.arange(slots), kv8.store, kv8.StorePlan)
+    q = torch.randn(int(qo[-1]), 4, d, generator=g, device=DEV).to(torch.bfloat16)
+    return pool, q, qo, kv, indices, last
+
+
+@pytest.mark.parametrize('gains', [(0, -30, 0, 0), (-70, 0, 40, 3), (0, 0, 60, -60), (0, 20, 10, -10)])
+@pytest.mark.parametrize('window,d,page', [(0, 128, 64), (0, 64, 128), (400, 128, 64)])
+def test_attention_of_many_rows_over_segments_whose_v_scales_are_far_apart(gains, window, d, page):
+    # (pages of whole scale blocks; each segment is held to its own largest V, `attention_ref`)
+    spec = [(300, 1500), (500, 3900), (40, 700), (260, 260)]
+    args = scaled_segments(spec, gains, page, d, 21)
+    _, plan = check_attention(*args, page, window, 0, d ** -0.5)
+    assert plan.counts[5] > 0 and (window or plan.counts[1] > 0)
+
+
+def test_attention_of_many_rows_within_a_segment_whose_v_scales_are_far_apart():
+    for d, span in ((64, 30), (128, 60)):
+        rng, g = np.random.default_rng(22), torch.Generator(device=DEV).manual_seed(22)
+        qo, kv, indices, last, slots = make_segments(rng, [(500, 2000), (9, 1500)], 1)
+        k, v = pool_rows(g, slots, 2, d, DEV), pool_rows(g, slots, 2, d, DEV)
+        gain = torch.exp2(torch.randint(-span, span + 1, ((slots + 63) // 64, 2, 1), generator=g, device=DEV).float())
+        v = (v.float() * gain.repeat_interleave(64, 0)[:slots]).to(torch.bfloat16)
+        pool = kv8.KV8Pool(slots, 2, d, DEV)
+        fill(pool, k, v, np.arange(slots), kv8.store, kv8.StorePlan)
+        q = torch.randn(int(qo[-1]), 4, d, generator=g, device=DEV).to(torch.bfloat16)
+        for window in (0, 333):
+            _, plan = check_attention(pool, q, qo, kv, indices, last, 1, window, 0, d ** -0.5)
+            assert plan.counts[5] > 0 or window  # (with the window the call is small enough to go 16 rows at a time)
+
+
+def test_another_segment_s_v_scales_move_no_bit():
+    spec = [(300, 1500), (500, 3900), (260, 260)]
+    got = []
+    for gain in (30, 45, 60):
+        pool, q, qo, kv, indices, last = scaled_segments(spec, (0, gain, 0), 64, 128, 23)
+        plan = kv8.AttentionPlan(qo, kv, indices, 4, 2, 128, page_size=64, kv_last_page_len=last, device=DEV)
+        got.append(kv8.tree_attention(q, pool, plan, 128 ** -0.5))
+    own = torch.ones(q.shape[0], dtype=torch.bool, device=DEV)
+    own[300:800] = False
+    assert torch.equal(got[0][own], got[1][own]) and torch.equal(got[0][own], got[2][own])
+    assert got[0][own].abs().amin((0, 2)).max() > 0 or (got[0][own] != 0).float().mean() > 0.99
