@@ -505,10 +505,11 @@ class LeanGemma4:
             raise ValueError(f'at most {MAX_LABELS} labels per sequence')
         self.h2d_bytes = 0
         if scored is not None:
-            plan = dict(plan, readout=self._scored_rows(req, seqs, plan, scored))
-        # A pass that reads many rows runs its last layer whole, a few rows are pruned to. Rows of an image block are read
-        # whole too: pruned, they would lose the block's bidirectional mask.
-        prune = self.prune_last and (scored is None or (len(set(plan['readout'])) <= MAX_PRUNED_ROWS and not req.bidir))
+            # (the row of the last image block's closing token is the first one that predicts a scored token)
+            earliest = int(req.blocks.end[-1]) + 1 if req.blocks is not None else 1
+            plan = dict(plan, readout=self._scored_rows(req, seqs, plan, scored, earliest))
+        # a pass that reads many rows runs its last layer whole, a few rows are pruned to
+        prune = self.prune_last and (scored is None or len(set(plan['readout'])) <= MAX_PRUNED_ROWS)
         slots = {kk: max(plan['cap'][kk], 1) for kk in 'gs'}
         if self.kv8 and pools is not None:
             slots.update((KINDS[kind], pool.slots) for kind, pool in zip(self.types, pools))
@@ -627,9 +628,10 @@ class LeanGemma4:
                 out[-1].update(top_ids=host[3][i], top_logprobs=host[4][i])
         return out
 
-    def _scored_rows(self, req, seqs, plan, scored):
+    def _scored_rows(self, req, seqs, plan, scored, earliest=1):
         """The (step, row) of every row that predicts a scored token, in the order of `seqs` and their tokens; fills
-        `scored` with each sequence's first scored token. The row of token t predicts token t + 1."""
+        `scored` with each sequence's first scored token. The row of token t predicts token t + 1. `earliest`: the first
+        token that may be scored (behind the image blocks of a request with images)."""
         place = {}
         for k, st in enumerate(plan['steps']):
             place.update((int(o), (k, r)) for r, o in enumerate(st['own']))
@@ -639,8 +641,11 @@ class LeanGemma4:
             first = scored[i]
             if first is None:  # the first token from which on every predecessor is computed in this pass
                 first = len(path)
-                while first > 1 and path[first - 2] in place:
+                while first > earliest and path[first - 2] in place:
                     first -= 1
+            if 1 <= first < min(earliest, len(path)):
+                raise ValueError(f'sequence {b} has tokens to score from {earliest} on, not from {first}: up to there it '
+                                 f'holds images, whose tokens attend to their whole block')
             if not 1 <= first <= len(path):
                 raise ValueError(f'sequence {b} has tokens 1..{len(path) - 1} to score, not from {first}')
             missing = next((t for t in range(first, len(path)) if path[t - 1] not in place), None)
@@ -657,10 +662,12 @@ class LeanGemma4:
     def token_logprobs(self, req, seqs, start=None, top=0, available=None):
         """Log-probabilities of the sequences' own tokens, each given the ones before it, in one pass over `seqs` of
         `req` (computing what `run` would compute). `start`: per sequence the first token scored (at least 1; None, or
-        None for a sequence: the first one from which on this pass computes every predecessor). Returns per sequence a
-        dict of arrays over the tokens start..len-1: `tokens`, `logprob`, `lse`, `entropy` and, with `top` > 0,
-        `top_ids`, `top_logprobs`; and `start`. Tokens that sequences share are computed once. ValueError for a token
-        whose predecessor an earlier pass computed (kept K/V hold no hidden states)."""
+        None for a sequence: the first one from which on this pass computes every predecessor). Of a request with images
+        only tokens behind the last block are scored: the rows of a block attend to all of it, so they predict nothing from
+        the tokens before alone; an earlier `start` is a ValueError. Returns per sequence a dict of arrays over the tokens
+        start..len-1: `tokens`, `logprob`, `lse`, `entropy` and, with `top` > 0, `top_ids`, `top_logprobs`; and `start`.
+        Tokens that sequences share are computed once. ValueError for a token whose predecessor an earlier pass computed
+        (kept K/V hold no hidden states)."""
         self._check_scoring(req, seqs, top)
         scored = list(start) if start is not None else [None] * len(seqs)
         if len(scored) != len(seqs):

@@ -223,3 +223,37 @@ def test_scoring_over_image_blocks(state):  # noqa: F811
     got = m.token_logprobs(req, seqs, start=[after] * len(seqs))
     want = m.label_logprobs(m.prepare(c['seqs'], c['label_ids'], images=images_of(state, c)), seqs)
     assert all(np.isfinite(g['logprob']).all() and np.isfinite(w['lse']) for g, w in zip(got, want))
+
+
+@pytest.mark.parametrize('name', ['tiny-images', 'tiny-images-steps'])
+@pytest.mark.parametrize('kv_cache', ['bf16', 'e4m3'])
+def test_with_images_the_text_behind_them_is_scored(state, monkeypatch, name, kv_cache):  # noqa: F811
+    """Without a start scoring begins behind the last block; its values are those of the truncated sequences' readouts,
+    with the last layer run for the scored rows only or for all."""
+    import morj_b200.lean_core as lc
+    c = CASES[name]
+    make = lambda **kw: engine(state, kv_cache=kv_cache, **kw)
+    m = make(single_max=c['single_max'], step_tokens=c['step_tokens'])
+    images, seqs = images_of(state, c), list(range(len(c['seqs'])))
+    got = []
+    for pruned in (10**9, 0):
+        monkeypatch.setattr(lc, 'MAX_PRUNED_ROWS', pruned)
+        req = m.prepare(c['seqs'], c['label_ids'], images=images)
+        got.append(m.token_logprobs(req, seqs, top=2))
+    end = int(req.blocks.end[-1])
+    for b, g, whole in zip(seqs, *got):
+        s = req.blocks.seqs[b]
+        assert g['start'] == whole['start'] == end + 1 and g['tokens'].tolist() == s[end + 1:]
+        assert m.image_id not in g['tokens'].tolist()
+        assert np.abs(np.exp(g['logprob']) - np.exp(whole['logprob'])).max() <= TOL
+        for t in (end + 1, len(s) - 1):
+            alone = make()
+            r = alone.prepare([c['seqs'][b][:len(c['seqs'][b]) - (len(s) - t)]], [[s[t]]], images=images)
+            assert r.blocks.seqs[0] == s[:t]
+            one = alone.label_logprobs(r, [0])[0]
+            assert abs(np.exp(one['logprob'][0]) - np.exp(g['logprob'][t - g['start']])) <= TOL
+            assert abs(one['lse'] - g['lse'][t - g['start']]) <= 0.05
+            assert abs(one['entropy'] - g['entropy'][t - g['start']]) <= 0.05
+    for start in (1, end):
+        with pytest.raises(ValueError, match=f'from {end + 1} on, not from {start}'):
+            m.token_logprobs(req, seqs, start=[start] * len(seqs))

@@ -43,3 +43,19 @@ def test_without_a_start_scoring_begins_behind_the_rows_of_earlier_passes():
 def test_refusals(steps, scored, match):
     with pytest.raises(ValueError, match=match):
         rows(steps, scored=scored)
+
+
+def test_with_images_scoring_begins_behind_the_last_block():
+    plan = dict(steps=[dict(own=[0, 1, 2, 3, 4, 5, 6, 7, 8])])
+    for given, want in [((None, None), [3, 3]), ((3, 5), [3, 5]), ((5, None), [5, 3])]:
+        scored = list(given)
+        got = LeanGemma4._scored_rows(None, REQ, [0, 1], plan, scored, earliest=3)
+        assert scored == want
+        assert got == [(0, o) for path, first in zip(([0, 1, 2, 3, 4, 5], [0, 1, 2, 3, 6, 7]), want)
+                       for o in path[first - 1:5]]
+    for start in (1, 2):
+        with pytest.raises(ValueError, match=f'from 3 on, not from {start}: up to there it holds images'):
+            LeanGemma4._scored_rows(None, REQ, [0], plan, [start], earliest=3)
+    # sequences that end with their images have no token to score
+    with pytest.raises(ValueError, match='no token to score'):
+        LeanGemma4._scored_rows(None, REQ, [0, 1], plan, [None, None], earliest=7)
