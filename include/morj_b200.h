@@ -186,8 +186,9 @@ int morj_label_head(const void* x, long long ld_x, const int* seq_row, const int
  * logprobs[i, j] = z at targets[i, j] - lse[i] ([n, n_targets]; target -1: 0), entropy[i] = -sum_v p log p, and the
  * `top` largest logits' ids and log-probabilities ([n, top], larger first, the lower id first among equal logits; at
  * most MORJ_MAX_TOP). All outputs FP32 / int32; lse and entropy may be NULL. The [n, vocab] logits are never stored.
- * A target outside [-1, vocab) sets the device error word (0x301) and gives NaN. A row with a NaN gives NaN; NaN and
- * -infinity are no alternatives (top id -1 and NaN where none is left). H % 8 == 0, ld % 8 == 0; h, w and workspace
+ * A target outside [-1, vocab) sets the device error word (0x301) and gives NaN. A row with a NaN among its z, or
+ * +infinity, gives NaN; z = -infinity has probability 0 and takes no part in the entropy. NaN and -infinity logits are no
+ * alternatives (top id -1 and NaN where none is left). H % 8 == 0, ld % 8 == 0; h, w and workspace
  * 16-byte aligned.
  * workspace: morj_token_logprobs_workspace bytes of the caller's, overwritten; calls that may overlap on the device must
  * not share it. Rows are taken 2048 at a time, w is read once for each such group. */

@@ -238,6 +238,13 @@ MORJ_DEV float fast_exp2(float x) {
   return y;
 }
 
+// maximum that keeps a NaN
+MORJ_DEV float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+
 // Shared-memory matrix descriptor for a 128-byte-swizzled tile whose 8-row groups are 1024 bytes apart
 // (K-major operand, or MN-major operand with `lbo` = distance between 64-element column groups).
 MORJ_DEV uint64_t sw128_desc(uint32_t saddr, uint32_t lbo_bytes = 16) {

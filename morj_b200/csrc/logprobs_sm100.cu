@@ -100,7 +100,8 @@ MORJ_DEV void fold(const uint32_t (&r)[32], int valid, float c, float inv_c, flo
 #pragma unroll
   for (int i = 0; i < 32; ++i) {
     const float l = __uint_as_float(r[i]);
-    const float u = (CAP == 0 ? l : CAP == 1 ? cap_near(l, c, inv_c) : cap(l, c, inv_c)) - shift;
+    float u = (CAP == 0 ? l : CAP == 1 ? cap_near(l, c, inv_c) : cap(l, c, inv_c)) - shift;
+    if (CAP == 0) u = max_nan(u, -1e30f);  // (a logit of -infinity: exp 0, and 0 in t; a softcap leaves none)
     const float e = fast_exp2(u * LOG2E);
     if (i < valid) {
       s4[i & 3] += e;

@@ -271,3 +271,36 @@ def test_refusals():
     empty = token_logprobs(h[:0], w, t[:0], top=2)
     assert empty.lse.shape == (0,) and empty.top_ids.shape == (0, 2)
     assert np.isfinite(token_logprobs(h, w, t[:, :0].contiguous()).lse.cpu().numpy()).all()
+
+
+@pytest.mark.parametrize('V', [50, 300, 9001])
+def test_logits_of_minus_infinity_have_no_probability(V):
+    """Vocabulary rows masked by -infinity in a column where every h is 1: their probability is 0, and so is their part of
+    the entropy (p log p -> 0)."""
+    g = torch.Generator(device=DEV).manual_seed(V)
+    h, w = grid(g, 5, 64, V, like=5.0)
+    h[:, 7] = 1
+    masked = torch.arange(V, device=DEV) % 3 == 1
+    masked[:32] = True  # (the whole first group of a tile)
+    w[masked, 7] = float('-inf')
+    assert not masked.all()
+    live = torch.nonzero(~masked)[:, 0]
+    t = torch.stack([live[:5], live[-5:], masked.nonzero()[:5, 0]], 1).to(torch.int32)
+    top = min(8, len(live))
+    got = token_logprobs(h, w, t, top=top, softcap=0.0)
+    l = h.double() @ w[live].double().T  # the definition over the rows that are left
+    lse = torch.logsumexp(l, 1)
+    lp = l - lse[:, None]
+    d = 2.0 ** -15
+    assert ((got.lse.double() - lse).abs() <= d + lse.abs() * 2.0 ** -23).all()
+    spread = (lp.exp() * (l.amax(1, keepdim=True) - l)).sum(1)
+    assert ((got.entropy.double() + (lp.exp() * lp).sum(1)).abs() <= 2 * d * (1 + spread)).all()
+    order = torch.sort(l, dim=1, descending=True, stable=True).indices[:, :top]
+    assert torch.equal(got.top_ids.long(), live[order])
+    place = torch.searchsorted(live, t[:, :2].long())
+    assert ((got.logprob[:, :2].double() - lp.gather(1, place)).abs() <= 2 * d + lp.abs().max() * 2.0 ** -22).all()
+    assert (got.logprob[:, 2] == float('-inf')).all()
+    # all masked: nothing is left
+    w[:, 7] = float('-inf')
+    got = token_logprobs(h, w, t, top=1, softcap=0.0)
+    assert (got.lse == float('-inf')).all() and (got.top_ids == -1).all() and torch.isnan(got.top_logprobs).all()
