@@ -158,6 +158,17 @@ def store(pool, k, v, plan):
                  pool.slots, s)
 
 
+def attention_workspace_bound(slots, heads, head_dim, sms=None):
+    """Workspace bytes that no attention call whose segments list at most `slots` distinct slots (page size 1) exceeds on
+    a GPU of `sms` SMs (default this one's): every slot expanded, and the partial units of tiles cut until two (few rows:
+    three) CTAs an SM are busy, eight units (one) a part."""
+    if sms is None:
+        sms = torch.cuda.get_device_properties(torch.cuda.current_device()).multi_processor_count
+    counts = nat.KV8_COUNTS()
+    counts[2], counts[6] = -(-(8 * 2 + 3) * sms // heads), slots
+    return nat.kv8_attention_workspace(counts, heads, head_dim)
+
+
 class AttentionPlan:
     """A call's key lists and work list on the device (arguments as `morj_tree_attention`'s tables: host integers)."""
 

@@ -165,6 +165,7 @@ class _Tables:
 
 class LeanGemma4:
     kv8 = False  # K/V pools in 8 bits (`kv_cache='e4m3'`)
+    sms = 148    # SMs of the device
 
     def __init__(self, model_dir, device='cuda', workspace_mb=512, retain_budget_gb=10.0, single_max=16384,
                  step_tokens=8192, *, tp_group=None, tp_comm='peer', kv_cache='bf16'):
@@ -287,6 +288,8 @@ class LeanGemma4:
         self.h2d_bytes = 0
         self.launches = 0
         self.trace = None
+        if self.device.type == 'cuda':
+            self.sms = torch.cuda.get_device_properties(self.device).multi_processor_count
         # split-tile workspace of the pair GEMM kernel, registered for every stream the model launches on
         self.gemm_ws = nat.GemmWorkspace(self.device) if self.device.type == 'cuda' else None
         if tp_group is not None and tp_comm == 'peer':
@@ -324,6 +327,7 @@ class LeanGemma4:
         if not retain:
             return False, False
         room = (self.free_bytes if available is None else available) - min(tokens, self.single_max) * self.act_bytes
+        room -= max(self._attention_bytes(kind, tokens) for kind in self.geom)
         whole = tokens * self.kv_bytes <= min(self.retain_budget, room)
         return whole, not whole
 
@@ -358,6 +362,17 @@ class LeanGemma4:
         if self.kv8:
             return 2 * (slots * hk * d + -(-slots // kv8.BLOCK) * hk * 4)
         return 4 * slots * hk * d
+
+    def _attention_bytes(self, kind, slots):
+        """Device bytes an attention call of a layer of `kind` over at most `slots` slots may take beside its inputs and
+        outputs: the workspace of 8-bit pools."""
+        return kv8.attention_workspace_bound(slots, *self.geom[kind], sms=self.sms) if self.kv8 else 0
+
+    def _vocab_bytes(self, rows, top):
+        """(bytes held from the first step on, bytes at the end) of reading `rows` rows under the whole vocabulary: their
+        residual rows; the gathered and the normed copy, the operator's workspace and outputs (with a target a row)."""
+        from .logprobs import workspace_bytes
+        return 2 * rows * self.hidden, 4 * rows * self.hidden + workspace_bytes(rows, top) + 4 * rows * (3 + 2 * top)
 
     def _kv_pool(self, kind, slots):
         """One layer's K/V pool of `slots` rows for a layer of `kind`: a (K, V) pair, or a `kv8.KV8Pool`. With POISON
@@ -435,16 +450,24 @@ class LeanGemma4:
         return s
 
     # ---- pass -----------------------------------------------------------------------------------------------------
-    def _pass_bytes(self, plan, persistent):
+    def _pass_bytes(self, plan, persistent, vocab=(0, 0)):
         """Device bytes a planned pass needs: its largest step's activations, plus every layer's pools when they live
-        for the whole pass (pinned requests, and multi-step passes of requests not kept whole)."""
+        for the whole pass (pinned requests, and multi-step passes of requests not kept whole). 8-bit pools: and the
+        largest attention call's workspace (the staged K/V rows lie within `act_bytes`, whose formula counts the QKV rows
+        that the fused projection never writes). `vocab` (`_vocab_bytes`): and what a readout under the whole vocabulary
+        takes, the second part when the steps' activations are free again."""
         largest = max(len(st['tokens']) for st in plan['steps'])
         pools = sum(self._pool_bytes(t, plan['cap'][KINDS[t]]) for t in self.types)
-        return (pools if persistent else 0) + largest * self.act_bytes
+        step = largest * self.act_bytes
+        if self.kv8:
+            step += max(self._attention_bytes(t, min(len(st['kv_indices_' + KINDS[t]]), plan['cap'][KINDS[t]]))
+                        for st in plan['steps'] for t in set(self.types))
+        return (pools if persistent else 0) + vocab[0] + max(step, vocab[1])
 
-    def plan(self, req, seqs, available=None):
+    def plan(self, req, seqs, available=None, vocab=None):
         """The planning half of `run` (`lean_core.py:497-529`): the nodes to compute, the head's tree offsets, the
-        pinned offsets, and a plan whose memory fits `available` (default `free_bytes`).
+        pinned offsets, and a plan whose memory fits `available` (default `free_bytes`). `vocab`: (rows, alternatives) of
+        a readout under the whole vocabulary, whose memory is to fit as well.
 
         Fitting: the whole pass as one step first; then in steps of `step_tokens` (so a pass's sliding-window slots
         are reused as it moves on); then steps halved down to 512 tokens, below which the request does not fit and
@@ -459,13 +482,15 @@ class LeanGemma4:
             later = [b for b in range(req.n_real) if b not in req.read and b not in set(seqs)]
             pinned = tree.pinned_for(cached | set(need), later, self.window)
         budget = self.free_bytes if available is None else available
+        if vocab is not None:  # (no more rows than tokens computed)
+            vocab = self._vocab_bytes(min(vocab[0], sum(tree.span(n) for n in need)), vocab[1])
         single, step = self.single_max, self.step_tokens
         while True:
             plan = tree.plan_pass(need, seqs, self.window, single, step, req.retain,
                                   prealloc=() if req.retain else head, initial=req.tables, pinned=pinned,
                                   bidir=req.bidir)
             one_step = len(plan['steps']) == 1
-            cost = self._pass_bytes(plan, req.pinned or (not one_step and not req.retain))
+            cost = self._pass_bytes(plan, req.pinned or (not one_step and not req.retain), vocab or (0, 0))
             if cost <= budget:
                 return need, head, pinned, plan
             if step <= 512:
@@ -492,13 +517,18 @@ class LeanGemma4:
             self._copy_head(pools, plan['slot_of'], head)
         return pools
 
-    def prepare_pass(self, req, seqs, available=None, scored=None):
+    def prepare_pass(self, req, seqs, available=None, scored=None, top=None):
         """Host half of `run`: plan (with the memory fit), the pools the pass writes, and every step's tables uploaded
         to the device. The result can be executed any number of times (`execute_pass`); each execution recomputes
         the same nodes into the same slots. `scored` (`token_logprobs`): per sequence its first scored token, or None;
-        the pass then reads the rows that predict them instead of the sequences' last rows."""
+        the pass then reads the rows that predict them instead of the sequences' last rows. `top`: the alternatives of a
+        readout under the whole vocabulary, None for the label head."""
         t0 = time.perf_counter()
-        need, head, pinned, plan = self.plan(req, seqs, available)
+        vocab = None
+        if top is not None:
+            rows = len(seqs) if scored is None else sum(len(req.tree.seqs[b]) - (s or 1) for b, s in zip(seqs, scored))
+            vocab = (max(rows, 0), top)
+        need, head, pinned, plan = self.plan(req, seqs, available, vocab)
         pools = self._pass_pools(req, plan, head)
         labels = [req.label_ids[b] for b in seqs]
         if any(len(ids) > MAX_LABELS for ids in labels):
@@ -613,7 +643,7 @@ class LeanGemma4:
         self._check_scoring(req, seqs, top)
         for b in seqs:
             self._check_ids(req.label_ids[b])
-        p = self.prepare_pass(req, seqs, available)
+        p = self.prepare_pass(req, seqs, available, top=top)
         targets = np.full((len(seqs), max(len(ids) for ids in p['labels'])), -1, np.int32)
         for row, ids in zip(targets, p['labels']):
             row[:len(ids)] = ids
@@ -674,7 +704,7 @@ class LeanGemma4:
             raise ValueError(f'{len(scored)} starts for {len(seqs)} sequences')
         for b in seqs:
             self._check_ids(req.tree.seqs[b])
-        p = self.prepare_pass(req, seqs, available, scored=scored)
+        p = self.prepare_pass(req, seqs, available, scored=scored, top=top)
         row_of = {place: j for j, place in enumerate(sorted(set(p['plan']['readout'])))}
         index = np.asarray([row_of[place] for place in p['plan']['readout']], np.int64)
         tokens = [np.asarray(req.tree.seqs[b])[first:] for b, first in zip(seqs, scored)]
