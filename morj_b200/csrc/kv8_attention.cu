@@ -1335,8 +1335,11 @@ extern "C" int morj_tree_attention_kv8_work(const int* qo_indptr_host, const int
     for (int s = 0; s < n_segments; ++s) {
       const int n_pages = kv_indptr_host[s + 1] - kv_indptr_host[s];
       const int last = kv_last_page_len_host ? kv_last_page_len_host[s] : page_size;
-      const long long kv = page_size == 1 || n_pages == 0 ? n_pages : (long long)(n_pages - 1) * page_size + last;
-      if (kv < 0 || kv > INT_MAX)
+      if (last < 0 || last > page_size)  // (more would be keys past the segment's list)
+        return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8_work: the last page of segment %d holds %d of %d slots", s,
+                         last, page_size);
+      const long long kv = n_pages == 0 ? 0 : (long long)(n_pages - 1) * page_size + last;
+      if (kv > INT_MAX)
         return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8_work: segment %d has %lld keys", s, kv);
       kv_len[s] = (int)kv;
       const int n = (qo_indptr_host[s + 1] - qo_indptr_host[s]) * G;

@@ -354,3 +354,16 @@ def test_host_indices_that_are_not_whole_numbers_are_refused():
         kv8.AttentionPlan([0, 1], [0, 2], np.array([0.0, 1.0]), 4, 2, 64, device='cpu')
     work, blocks = nat.kv8_store_work(np.array([70, 3], np.uint64), 128)
     assert blocks == 2 and work[6:].tolist() == [3, 1, 70, 0]
+
+
+def test_a_last_page_holds_from_none_to_all_of_its_slots():
+    # (more would list keys past the segment's pages: reads past the list)
+    for page, last in [(16, 17), (16, -1), (1, 2), (1, -1)]:
+        with pytest.raises(ValueError, match='the last page of segment 1 holds'):
+            nat.kv8_attention_work([0, 1, 2], [0, 2, 4], range(4), 0, 4, 2, 0, page, [page, last])
+    for page in (1, 16):
+        for last in (0, 1):
+            work, counts = nat.kv8_attention_work([0, 1], [0, 3], range(3), 0, 4, 2, 0, page, [last])
+            assert counts[0] == 1 and work[11] == 2 * page + last == work[3]
+    work, _ = nat.kv8_attention_work([0, 1], [0, 0], [], 0, 4, 2, 0, 16, [0])
+    assert work[11] == 0
