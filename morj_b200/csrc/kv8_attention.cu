@@ -1316,8 +1316,8 @@ extern "C" int morj_tree_attention_kv8_work(const int* qo_indptr_host, const int
   const int G = hq / hk;
   try {
     for (int s = 0; s < n_segments; ++s) {
-      const long long rows = (long long)(qo_indptr_host[s + 1] - qo_indptr_host[s]) * G;
-      if (rows < 0 || rows > (1 << 30) || kv_indptr_host[s] < 0 || kv_indptr_host[s + 1] < kv_indptr_host[s])
+      const long long rows = ((long long)qo_indptr_host[s + 1] - qo_indptr_host[s]) * G;
+      if (qo_indptr_host[s] < 0 || rows < 0 || rows > (1 << 30) || kv_indptr_host[s] < 0 || kv_indptr_host[s + 1] < kv_indptr_host[s])
         return set_error(MORJ_ERR_ARG, "morj_tree_attention_kv8_work: segment %d's tables are out of order", s);
     }
     std::vector<Item> tiles, rows, joins;

@@ -367,3 +367,12 @@ def test_a_last_page_holds_from_none_to_all_of_its_slots():
             assert counts[0] == 1 and work[11] == 2 * page + last == work[3]
     work, _ = nat.kv8_attention_work([0, 1], [0, 0], [], 0, 4, 2, 0, 16, [0])
     assert work[11] == 0
+
+
+def test_queries_in_front_of_the_first_row_are_refused():
+    # (their rows would be read and written in front of q and out)
+    for qo in ([-3, 2], [-2**31, 2**31 - 1], [0, -1]):
+        with pytest.raises(ValueError, match='out of order'):
+            nat.kv8_attention_work(qo, [0, 4], range(4), 0, 4, 2, 0)
+    work, counts = nat.kv8_attention_work([3, 5], [0, 4], range(4), 0, 4, 2, 0)
+    assert counts[9] == 5 and work[8] == 3
