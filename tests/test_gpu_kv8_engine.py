@@ -257,3 +257,31 @@ def test_with_images_the_text_behind_them_is_scored(state, monkeypatch, name, kv
     for start in (1, end):
         with pytest.raises(ValueError, match=f'from {end + 1} on, not from {start}'):
             m.token_logprobs(req, seqs, start=[start] * len(seqs))
+
+
+@pytest.mark.parametrize('kv_cache', ['bf16', 'e4m3'])
+def test_scoring_through_the_tensor_parallel_path(state, monkeypatch, tmp_path, kv_cache):  # noqa: F811
+    """A group of one rank takes the peer exchange's path (partials, reductions, waits; all on one stream): the same
+    probabilities and scores, with the last layer run for a few rows and for all of them (where the last site returns the
+    residual rows)."""
+    import torch.distributed as dist
+    import morj_b200.lean_core as lc
+    c = CASES['tiny-nested']
+    seqs = list(range(len(c['seqs'])))
+    plain = engine(state, kv_cache=kv_cache)
+    want = plain.run(plain.prepare(c['seqs'], c['label_ids']), seqs)
+    scores = plain.token_logprobs(plain.prepare(c['seqs'], c['label_ids']), seqs, top=2)
+    dist.init_process_group('gloo', init_method=f'file://{tmp_path}/store', world_size=1, rank=0)
+    try:
+        m = engine(state, kv_cache=kv_cache, tp_group=dist.group.WORLD, single_max=1024, step_tokens=1024)
+        assert m.peer is not None
+        for pruned in (10**9, 0):
+            monkeypatch.setattr(lc, 'MAX_PRUNED_ROWS', pruned)
+            assert np.abs(flat(m.run(m.prepare(c['seqs'], c['label_ids']), seqs)) - flat(want)).max() <= TOL
+            for g, w in zip(m.token_logprobs(m.prepare(c['seqs'], c['label_ids']), seqs, top=2), scores):
+                assert g['start'] == w['start']
+                assert np.abs(np.exp(g['logprob']) - np.exp(w['logprob'])).max() <= TOL
+                assert np.abs(g['entropy'] - w['entropy']).max() <= 0.05
+        m.peer.close()
+    finally:
+        dist.destroy_process_group()
