@@ -245,7 +245,7 @@ int morj_kv8_gather(const void* codes, const float* scale, int pool_slots, const
  * are first expanded to 16 bits in `workspace`, once per call. Long key lists of few tiles are cut into parts, whose
  * partial results go through `workspace` and are joined in a fixed order.
  * morj_tree_attention_kv8_workspace (host function): the bytes a call with these counts needs (4 per code pair of the
- * expanded pages, plus the parts; the caller's, 256-byte aligned; calls that may overlap on the device must not share
+ * expanded pages, plus the parts; the caller's, 16-byte aligned; calls that may overlap on the device must not share
  * it). `work`: the device copy of the list (16-byte aligned); `counts`: the host array; kv_indices, n_bidir, hq, hk,
  * page_size and window as the list was made for. */
 #define MORJ_KV8_COUNTS 12

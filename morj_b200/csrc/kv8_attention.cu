@@ -31,7 +31,13 @@ constexpr int WARPS = 4;
 constexpr int STEP = 32;             // keys a warp of rows_kernel takes at a time
 constexpr int T_ROWS = 128;           // rows of a tile_kernel tile
 constexpr int BN = 64;                // keys it takes at a time
-constexpr int FEW_ROWS = 16;         // segments of at most this many rows go to rows_kernel
+// Segments of at most this many rows go to rows_kernel, which reads a segment's codes once per 16 rows; the others to
+// tile_kernel, behind the expansion. Both ways, 16 heads of 128, us (rows, tiles): one segment of 18 rows over 4,096 /
+// 16,384 / 65,536 keys 18, 27 / 40, 72 / 123, 270, of 64 rows 26, 29 / 72, 73 / 247, 267, of 126 rows 41, 29 / 131, 74 / 482,
+// 266; eight segments of 18 rows over 16,384 keys each 359, 637, over the same 16,384 keys 355, 265, of 126 rows 879, 599 and
+// 872, 210. So 17 to about 64 rows over keys of their own would be better off here, and are not sent: the rule goes by rows
+// alone, and over shared keys the tiles win from two 16-row tiles on.
+constexpr int FEW_ROWS = 16;
 // ... and all segments of a call, 16 rows at a time, whose 16-row tiles see at most this many keys together (times the KV
 // heads) in at most one CTA per resident place: one launch in place of two and no expansion. 1 to 8 segments of 32 to
 // 2,048 rows, heads of 64 and 128, both ways: 6 to 16 us against 9 to 22 up to it, level on the whole at twice as many,
@@ -134,8 +140,9 @@ MORJ_DEV float row_scale(float amax) {
 // 16-byte units XOR-swizzled by the key, so both products read their fragments without bank conflicts: mma.m16n8k16
 // leaves the order of the head dimension (q . k) and of the output columns (P V) free, and each lane takes 32 (16)
 // consecutive codes of a K row and 16 (8) of a V row for D = 128 (64).
-// Measured: 64 single queries over 1 to 8,048 keys of 16 heads of 128, 786 MB, 130 us = 6.05 TB/s (0.92 of the measured
-// copy), 9 readout rows of 1,560 keys 19 us (latency: page entry -> codes -> five groups a warp -> join). Not kept: the
+// Measured: 64 single queries over 1 to 8,048 keys of 16 heads of 128, 786 MB, 122 us back to back = 6.4 TB/s (0.98 of the
+// measured copy), 143 with cold caches; 9 readout rows of 1,560 keys 16 us back to back, 22 alone (latency: page entry ->
+// codes -> five groups a warp -> join). Not kept: the
 // codes of K straight into an e4m3 mma against queries split in two codes (167 against 148 us at the time).
 // ---------------------------------------------------------------------------------------------------------------
 constexpr int R_STAGES = 2;
@@ -554,8 +561,8 @@ __global__ void __launch_bounds__(WARPS * 32, 3)
 // queries are BF16), V as FP16(code * scale / ref) with the head's largest scale among them, so that probabilities can be
 // FP16 too (11 bits). That is exact while the head's scales lie within 2^15 of one another (the smallest code is 2^-9, the
 // smallest FP16 2^-24). Where they do not, V is expanded as its codes, and tile_kernel takes each key's scale into its
-// probability, relative to the largest one its tile has met, so that what other segments hold moves no bit of a segment's
-// result. A key is used by every 128-row tile that sees it:
+// probability, relative to the largest one its tile has met, so that what other segments hold costs a segment no precision.
+// A key is used by every 128-row tile that sees it:
 // expanding costs 3 bytes of traffic per code once (35.7 M codes, the 8,704 tokens of a 16-head layer, K and V), where
 // converting in the tile loaders (built and measured) cost each tile the conversion, the address arithmetic and the
 // instruction cache: 130 us on the op-level tree (2048 + 8 x 64) against 73 now.
@@ -669,9 +676,13 @@ __global__ void __launch_bounds__(E_THREADS, 12) expand_kernel(const Args a, con
 //               O / l or the part's (maximum, sum, O), staged through shared memory to store whole rows
 // The pipeline is tree_attention_kernel's (S and P double-buffered in TMEM, a K buffer free once its S is complete, a V
 // buffer once its P V is, two CTAs per SM); what it lacks there is the parts of a key range and rows that see nothing.
-// Bound by the chain of a 64-key chunk, P stored -> P V and the next S issued -> S seen -> softmax, 1,600 cycles of which
-// two are under way per CTA: 51.8 GFLOP (2048 + 8 x 64 rows, 32 heads of 128) in 63 of the call's 73 us = 820 TFLOP/s.
-// The MMAs themselves need 640 cycles a chunk (N = 64 reads shared memory for 48 of them per 16-deep step, not 32).
+// Bound by the softmax of a chunk, which one warpgroup takes through its steps in turn while the chunk's MMAs wait for it.
+// Clocks read in the softmax warps (which cost 5-8% themselves), 8 x 64 rows on 8,192 keys: 1,700 cycles a chunk, of which
+// 820 for the exponentials with sum and packing, 260 for mask and maximum (460 at the ragged chunks of a window), 415 waiting
+// for S, 115 for the rescale's vote and the rare rescale, 100 for TMEM loads and stores. Two CTAs share an SM, so one chunk
+// every 850 cycles, where the MMAs need 640 (N = 64 reads shared memory for 48 of them per 16-deep step, not 32). On
+// top come 10,000 cycles to a CTA's first S and 7,500 to store its O, of 128,000, and here only 256 CTAs for 296 places.
+// 51.8 GFLOP (2048 + 8 x 64 rows, 32 heads of 128) in a call of 72 us back to back = 720 TFLOP/s with the expansion.
 // Measured and not kept: the MMAs by a whole warp with one lane's predicate, or elected (30-60% slower), P handed over in
 // halves (1-3% slower), keys cut further to even out the CTAs (5% slower, the joins cost more).
 // ---------------------------------------------------------------------------------------------------------------

@@ -15,9 +15,11 @@
 // is cut to its top ones. (A sorted list per row in shared memory cost 1.0 ms of 2.1 on 540 rows with 5 alternatives: one
 // of 32 rows inserting holds up the warp.)
 //
-// Bound by the tensor cores or, for few rows, by reading w: 2,040 x 262,144 x 5,376 (5.75 TFLOP) 4.45-4.6 ms = 1,250-1,290
-// TFLOP/s under the power cap, 540 rows (five row blocks of 128, the last with 28) 1.30 ms = 1,170, 9 rows (2.82 GB)
-// 0.457 ms = 6.2 TB/s. 1 row of 4,096 logits, 17 us, is latency: three dependent steps in two launches.
+// Bound by the tensor cores or, for few rows, by reading w (262,144 x 5,376). The SM clock, and with it the first two, depends
+// on the box and on what ran before (the power cap): 2,040 rows (5.75 TFLOP) 4.45-4.9 ms = 1,170-1,290 TFLOP/s, 540 rows
+// (five row blocks of 128, the last with 28) 1.30-1.55 ms = 980-1,170, 9 rows (2.82 GB) 0.457-0.469 ms = 6.0-6.2 TB/s back
+// to back, 0.50 with cold caches. 1 row of 4,096 logits, 13 us back to back, 18 alone, is latency: three dependent steps in
+// two launches.
 //
 // One CTA per SM: warp 0 TMA producer, warp 1 MMA issuer (tcgen05, M = 128, N = 256, two TMEM accumulators), warps 2-5
 // epilogue (thread = row). Row blocks are the fast tile index: the CTAs in flight share a few vocabulary tiles, so w
@@ -63,7 +65,8 @@ MORJ_DEV float below(unsigned o) {
   return __uint_as_float(p & 0x80000000u ? p & 0x7fffffffu : ~p);
 }
 
-// z = c tanh(l / c). Near 0 tanh's series, elsewhere 1 - 2 / (1 + e^2x): relative error of a few 2^-24 on both sides.
+// z = c tanh(l / c). Near 0 tanh's series, a few 2^-24 of z; elsewhere 1 - 2 / (1 + e^2x), whose error (ex2.approx,
+// rcp.approx, the rounded argument) is absolute, about 2^-22 c: a few parts in 2^22 of z right above c / 4.
 MORJ_DEV float cap_near(float l, float c, float inv_c) {  // |l| <= c / 4
   const float x = l * inv_c, x2 = x * x;
   const float p = fmaf(x2, fmaf(x2, fmaf(x2, fmaf(x2, 62.f / 2835.f, -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
@@ -666,7 +669,7 @@ extern "C" int morj_token_logprobs(const void* h, long long ld_h, int n, const v
     CUtensorMap mh;
     if ((st = make_map(&mh, static_cast<const __nv_bfloat16*>(h) + (size_t)r0 * ld_h, rows, H, ld_h, box))) return st;
     // Wide tiles where there are enough of them for most SMs, else four times as many narrow ones: the epilogue's passes
-    // over a tile's columns are what a small call waits for (1 row, 4096 x 256: 18 against 25 us).
+    // over a tile's columns are what a small call waits for (1 row, 4096 x 256, alone: 18 against 25 us).
     const int blocks = (rows + BM - 1) / BM, wide = (vocab + BN_WIDE - 1) / BN_WIDE;
     const int bn = (long long)blocks * wide * 2 > num_sms() ? BN_WIDE : BN_NARROW;
     const long long tiles = (long long)blocks * ((vocab + bn - 1) / bn);

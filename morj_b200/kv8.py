@@ -110,7 +110,8 @@ class KV8Pool:
         return 2 * (self.k.numel() + 4 * self.k_scale.numel())
 
     def rows(self, slots):
-        """The K and V rows of pool slots `slots` (int32, on the pool's device) as BF16 [n, heads, head_dim]."""
+        """The K and V rows of pool slots `slots` (int32, on the pool's device) as BF16 [n, heads, head_dim]. A slot outside
+        the pool sets the device error word, and its row is left as it was allocated."""
         if slots.dtype != torch.int32 or slots.dim() != 1 or not slots.is_contiguous() or slots.device != self.device:
             raise ValueError('slots must be a contiguous int32 vector on the pool\'s device')
         out = []
