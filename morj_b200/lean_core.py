@@ -482,8 +482,8 @@ class LeanGemma4:
             later = [b for b in range(req.n_real) if b not in req.read and b not in set(seqs)]
             pinned = tree.pinned_for(cached | set(need), later, self.window)
         budget = self.free_bytes if available is None else available
-        if vocab is not None:  # (no more rows than tokens computed)
-            vocab = self._vocab_bytes(min(vocab[0], sum(tree.span(n) for n in need)), vocab[1])
+        if vocab is not None:  # (no more rows than tokens computed, or one a sequence asked for)
+            vocab = self._vocab_bytes(min(vocab[0], max(len(seqs), sum(tree.span(n) for n in need))), vocab[1])
         single, step = self.single_max, self.step_tokens
         while True:
             plan = tree.plan_pass(need, seqs, self.window, single, step, req.retain,

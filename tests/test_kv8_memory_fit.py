@@ -114,6 +114,15 @@ def test_a_readout_under_the_whole_vocabulary_is_part_of_the_fit(use8):
         assert asked.pop() == want
 
 
+def test_a_sequence_asked_for_many_times_is_read_as_often():
+    req = Request(Tree([[1, 2, 3]]), [[0]], False, [])
+    m = model(kv8=False, act_bytes=10)
+    need = 2 * 500 * m.hidden + 4 * 500 * m.hidden + logprobs_workspace(500, 4)
+    with pytest.raises(MemoryError):
+        m.plan(req, [0] * 500, available=need, vocab=(500, 4))
+    m.plan(req, [0] * 500, available=need + 2**16, vocab=(500, 4))
+
+
 def test_retained_8_bit_requests_leave_room_for_the_workspace():
     m = model(act_bytes=1000)
     pools, act = 3000 * m.kv_bytes, 3000 * m.act_bytes
