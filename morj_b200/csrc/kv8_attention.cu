@@ -682,7 +682,7 @@ __global__ void __launch_bounds__(E_THREADS, 12) expand_kernel(const Args a, con
 // for S, 115 for the rescale's vote and the rare rescale, 100 for TMEM loads and stores. Two CTAs share an SM, so one chunk
 // every 850 cycles, where the MMAs need 640 (N = 64 reads shared memory for 48 of them per 16-deep step, not 32). On
 // top come 10,000 cycles to a CTA's first S and 7,500 to store its O, of 128,000, and here only 256 CTAs for 296 places.
-// 51.8 GFLOP (2048 + 8 x 64 rows, 32 heads of 128) in a call of 72 us back to back = 720 TFLOP/s with the expansion.
+// 51.8 GFLOP (2048 + 8 x 64 rows, 32 heads of 128) in a call of 71 us back to back = 725 TFLOP/s with the expansion.
 // Measured and not kept: the MMAs by a whole warp with one lane's predicate, or elected (30-60% slower), P handed over in
 // halves (1-3% slower), keys cut further to even out the CTAs (5% slower, the joins cost more).
 // ---------------------------------------------------------------------------------------------------------------
@@ -866,7 +866,7 @@ MORJ_DEV bool softmax_chunks(const Args& a, int h, const int2* pages, const int*
   }
   return true;
 }
-// (A call of its own costs the usual walk 1.5%; inlined, its code and registers cost it 3-6%. Static, so that it keeps to its
+// (A call of its own costs the usual walk 0.7%; inlined, its code and registers cost it 3-6%. Static, so that it keeps to its
 // callers' 128 registers.)
 template <int D>
 static __device__ __noinline__ bool softmax_chunks_apart(const Args& a, int h, const int2* pages, const int* places,
@@ -1030,10 +1030,17 @@ __global__ void __launch_bounds__(T_THREADS, 2)
       visible(it.q_len, it.kv_len, bidir, a.window, qi, &lo, &hi);
       lo = max(lo, it.t0), hi = min(hi, t_stop - 1);
     }
-    const ChunkSide side{t_lane, s_full, p_full, pv_done, t_begin, it.t0, t_stop, n_chunks, lo, hi, a.scale_log2, abort};
     float m_used = -INFINITY, l_run = 0.f;
-    const bool ok = apart ? softmax_chunks_apart<D>(a, h, pages, list + it.kv_base, n_slots, side, m_used, l_run, vr)
-                          : softmax_chunks<D, false>(a, h, nullptr, nullptr, 0, side, m_used, l_run, vr);
+    bool ok;
+    if (!apart) {
+      const ChunkSide side{t_lane, s_full, p_full, pv_done, t_begin, it.t0, t_stop, n_chunks, lo, hi, a.scale_log2, abort};
+      ok = softmax_chunks<D, false>(a, h, nullptr, nullptr, 0, side, m_used, l_run, vr);
+    } else {  // (numbers of its own: those of the usual walk stay in registers)
+      const ChunkSide side{t_lane, s_full, p_full, pv_done, t_begin, it.t0, t_stop, n_chunks, lo, hi, a.scale_log2, abort};
+      float m = -INFINITY, l = 0.f, v = 0.f;
+      ok = softmax_chunks_apart<D>(a, h, pages, list + it.kv_base, n_slots, side, m, l, v);
+      m_used = m, l_run = l, vr = v;
+    }
     if (ok && (n_chunks == 0 || warp_wait(pv_done + 8 * ((n_chunks - 1) & 1), ((n_chunks - 1) >> 1) & 1, abort))) {
       tc_fence_after();
       // A finished row: O / l times V's reference; a part: (maximum, sum, O in units of the values). The warp's 32 rows
